@@ -1,0 +1,248 @@
+"""Rotary positions on q and k, forward and backward, on MI355X (gfx950).
+
+``rotary_plan`` holds a model's frequencies; ``rotary`` turns q and k (in one
+launch) by the angles of their tokens' positions, ahead of ``attention`` or of
+a ``Cache4``; ``rotary_`` does it in place.  Pair i of a head at position p is
+turned by ``p * plan.frequencies[i]`` radians and scaled by ``plan.amplitude``:
+
+==================  =========================================================
+``layout``          pairs of the first R = ``rotary_dim`` values of a head
+==================  =========================================================
+``"half"``          (x[i], x[i + R/2])
+``"interleaved"``   (x[2i], x[2i + 1])
+==================  =========================================================
+
+Values from R on are copied.  Angles are reduced in 64 bits, so positions may
+be as large as a text gets; each output is rounded once.  All arithmetic runs in
+``lib/librsfa.so`` (``rsfa_rotary`` in ``include/rsfa.h``), on the current
+stream of the tensors' device; there is no other path.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _native
+from .flash_attention_forward import _raise_for
+
+__all__ = ["RotaryPlan", "rotary_plan", "rotary", "rotary_"]
+
+_DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16, torch.float32: _native.DTYPE_F32}
+_LAYOUTS = ("half", "interleaved")
+
+
+class RotaryPlan:
+    """Frequencies (float64, radians a position, [R/2], on the CPU), amplitude and layout."""
+
+    def __init__(self, frequencies, layout="half", amplitude=1.0):
+        f = torch.as_tensor(frequencies, dtype=torch.float64).detach().cpu().contiguous().clone()
+        if f.dim() != 1 or f.numel() < 1 or not bool(torch.isfinite(f).all()):
+            raise ValueError("frequencies must be a vector of finite numbers, one for each pair")
+        if layout not in _LAYOUTS:
+            raise ValueError(f"layout must be one of {_LAYOUTS}; got {layout!r}")
+        if not math.isfinite(amplitude):
+            raise ValueError("amplitude must be finite")
+        self.frequencies = f
+        self.layout = layout
+        self.amplitude = float(amplitude)
+        self.rotary_dim = 2 * f.numel()
+        self._turns = {}
+
+    def turns(self, device):
+        """Turns a position of each pair, on `device`."""
+        t = self._turns.get(device)
+        if t is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("call plan.turns(device) (or rotary) once before capturing a graph")
+            t = (self.frequencies / (2.0 * math.pi)).to(device)
+            # (other streams may use it at once)
+            torch.cuda.current_stream(device).synchronize()
+            self._turns[device] = t
+        return t
+
+
+def rotary_plan(rotary_dim, *, base=10000.0, layout="half", scaling=None, factor=1.0, original_length=None,
+                low=1.0, high=32.0, amplitude=1.0):
+    """A ``RotaryPlan`` of frequencies base^(-2i/R), scaled for long contexts:
+
+    ``scaling=None``: as they are.  ``"linear"``: divided by ``factor``.  ``"ntk"``: the base times
+    factor^(R/(R-2)), which divides the slowest frequency by ``factor`` and keeps
+    the fastest.  ``"by_parts"``: pairs that turn less than ``low`` times within
+    ``original_length`` positions are divided by ``factor``, those that turn more than
+    ``high`` times kept, with a linear ramp between.  ``amplitude`` scales the
+    turned values (by_parts plans often take 0.1 ln(factor) + 1).
+    """
+    R = int(rotary_dim)
+    if R != rotary_dim or R < 2 or R % 2:
+        raise ValueError(f"rotary_dim must be an even number of at least 2; got {rotary_dim}")
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError("base must be positive")
+    if not (factor > 0 and math.isfinite(factor)):
+        raise ValueError("factor must be positive")
+    if scaling not in (None, "linear", "ntk", "by_parts"):
+        raise ValueError(f"scaling must be None, 'linear', 'ntk' or 'by_parts'; got {scaling!r}")
+    if scaling == "ntk":
+        if R == 2:
+            raise ValueError("ntk scaling needs rotary_dim of at least 4")
+        base = base * factor ** (R / (R - 2.0))
+    f = base ** (-2.0 * torch.arange(R // 2, dtype=torch.float64) / R)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "by_parts":
+        if original_length is None or original_length < 1 or not low < high:
+            raise ValueError("by_parts scaling needs original_length >= 1 and low < high")
+        turns = original_length * f / (2.0 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        f = (1.0 - keep) * f / factor + keep * f
+    return RotaryPlan(f, layout, amplitude)
+
+
+def _check(x, name):
+    if x.dim() != 4:
+        raise ValueError(f"{name} must be 4-D [Z, H, N, D]; got {tuple(x.shape)}")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {x.dtype}; float16, bfloat16 and float32 are supported")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor")
+
+
+def _like(x):
+    """An output for x: in x's layout where that is dense, or contiguous."""
+    y = torch.empty_like(x)
+    return y if y.stride(3) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _launch(xs, ys, positions, plan, inverse):
+    """ys[i] = xs[i] turned; xs: one or two tensors that passed the checks."""
+    x = xs[0]
+    Z, _, N, D = x.shape
+    args = _native.RotaryArgs()
+    args.struct_size = ctypes.sizeof(_native.RotaryArgs)
+    args.dtype = _DTYPES[x.dtype]
+    args.z, args.n, args.head_dim, args.rotary_dim = Z, N, D, plan.rotary_dim
+    for i, (a, b) in enumerate(zip(xs, ys)):
+        args.x[i], args.y[i] = a.data_ptr(), b.data_ptr()
+        args.heads[i] = a.shape[1]
+        args.x_stride[i][:] = a.stride()
+        args.y_stride[i][:] = b.stride()
+    flags = (_native.ROTARY_INTERLEAVED if plan.layout == "interleaved" else 0) | (
+        _native.ROTARY_INVERSE if inverse else 0)
+    if isinstance(positions, int):
+        args.start = positions
+    else:
+        args.positions = positions.data_ptr()
+        if positions.dim() == 2:
+            st = positions.stride()
+            args.pos_stride[:] = (st[0] if positions.shape[0] > 1 else 0, st[1])
+        else:
+            args.pos_stride[:] = (0, positions.stride(0))
+        if positions.dtype == torch.int64:
+            flags |= _native.ROTARY_POS64
+    args.turns = plan.turns(x.device).data_ptr()
+    args.amplitude = plan.amplitude
+    args.flags = flags
+    dev = x.device.index
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch.cuda.current_device():
+        st = _native.lib().rsfa_rotary(ctypes.byref(args), stream)
+    else:
+        with torch.cuda.device(dev):
+            st = _native.lib().rsfa_rotary(ctypes.byref(args), stream)
+    _raise_for(st)
+
+
+def _unit(x):
+    return x if x.stride(3) == 1 else x.contiguous()
+
+
+class _Rotary(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, positions, plan):
+        ctx.plan, ctx.positions, ctx.pair = plan, positions, k is not None
+        # positions may be changed by the program before the backward pass
+        if not isinstance(positions, int):
+            ctx.positions = None
+            ctx.save_for_backward(positions)
+        return _forward(q, k, positions, plan, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        positions = ctx.positions if ctx.positions is not None else ctx.saved_tensors[0]
+        need = [g is not None and n for g, n in zip(grads, ctx.needs_input_grad)]
+        xs = [g for g, n in zip(grads, need) if n]
+        out = [None, None, None, None]
+        if xs:
+            ys = _forward(xs[0], xs[1] if len(xs) > 1 else None, positions, ctx.plan, True)
+            ys = list(ys) if isinstance(ys, tuple) else [ys]
+            for i, n in enumerate(need):
+                if n:
+                    out[i] = ys.pop(0)
+        return tuple(out)
+
+
+def _forward(q, k, positions, plan, inverse):
+    xs = [_unit(q)] if k is None else [_unit(q), _unit(k)]
+    ys = [_like(x) for x in xs]
+    if xs[0].shape[0] and xs[0].shape[2]:
+        xs_, ys_ = zip(*[(x, y) for x, y in zip(xs, ys) if x.numel()]) if any(x.numel() for x in xs) else ((), ())
+        if xs_:
+            _launch(xs_, ys_, positions, plan, inverse)
+    return ys[0] if k is None else tuple(ys)
+
+
+def _checked(q, k, positions, plan):
+    if not isinstance(plan, RotaryPlan):
+        raise TypeError("plan must be a RotaryPlan (rotary_plan(...))")
+    _check(q, "q")
+    if k is not None:
+        _check(k, "k")
+        if k.dtype != q.dtype or k.device != q.device:
+            raise TypeError("q and k must have one dtype and device")
+        if k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]:
+            raise ValueError(f"q and k must share Z, N and D; got {tuple(q.shape)} and {tuple(k.shape)}")
+    if plan.rotary_dim > q.shape[3]:
+        raise ValueError(f"the plan turns {plan.rotary_dim} values of a head; the head dim is {q.shape[3]}")
+    if isinstance(positions, bool) or not isinstance(positions, (int, torch.Tensor)):
+        raise TypeError("positions must be an int (the first token's) or an int32/int64 tensor [N] or [Z, N]")
+    if isinstance(positions, torch.Tensor):
+        Z, N = q.shape[0], q.shape[2]
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"positions must be int32 or int64; got {positions.dtype}")
+        if positions.device != q.device:
+            raise ValueError("positions must be on q's device")
+        if tuple(positions.shape) not in ((N,), (Z, N), (1, N)):
+            raise ValueError(f"positions must be [N] or [Z, N]; got {tuple(positions.shape)}")
+
+
+def rotary(q, k, positions, plan):
+    """(q', k') turned by their positions; ``k=None``: q' alone.
+
+    q [Z, Hq, N, D] and k [Z, Hk, N, D] (float16, bfloat16 or float32, any
+    strides); ``positions``: the first token's position (an int), or a tensor [N]
+    or [Z, N] of int32 or int64.  Differentiable in q and k: the gradient is the
+    same turn backwards.
+    """
+    _checked(q, k, positions, plan)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, positions, plan)
+    return _forward(q, k, positions, plan, False)
+
+
+def rotary_(q, k, positions, plan):
+    """``rotary`` in place (inference); the values beyond ``rotary_dim`` are not touched."""
+    _checked(q, k, positions, plan)
+    for x in (q, k):
+        if x is None:
+            continue
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("rotary_ works in place and keeps no gradient; use rotary")
+        if x.stride(3) != 1 and x.shape[3] > 1:
+            raise ValueError("rotary_ needs a unit stride in the head dim")
+        if any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
+            raise ValueError("rotary_ cannot write to an expanded tensor")
+    xs = [x for x in (q, k) if x is not None and x.numel()]
+    if xs:
+        _launch(xs, xs, positions, plan, False)
+    return q if k is None else (q, k)

@@ -514,7 +514,15 @@ const char* rsfa_strerror(int status) {
             return "the problem needs more workspace (split state) than the no-allocation "
                    "entry point's fixed buffer (RSFA_NOALLOC_WORKSPACE_BYTES)";
         case RSFA_E_WORKSPACE:
-            return "workspace missing or smaller than rsfa_split_workspace_bytes() (causal split mode)";
+            return "workspace missing or smaller than rsfa_split_workspace_bytes() (causal split mode), or than "
+                   "a cache call's own";
+        case RSFA_E_ROTARY: return "rotary_dim must be even, at least 2 and at most head_dim";
+        case RSFA_E_CACHE:
+            return "a 4-bit cache needs head_dim 32, 64, 128 or 256, sizes of at least 1, rows within 32-bit "
+                   "counts, and query heads that are a multiple of its heads";
+        case RSFA_E_BUDGET:
+            return "claim and evict need 0 <= recent + sinks <= budget <= capacity and n >= 1; evict a target of "
+                   "the cache's shape with room for the budget";
         default: return "unknown rsfa status";
     }
 }

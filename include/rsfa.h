@@ -23,6 +23,9 @@
  *   rsfa_strerror             -> (no counterpart: the reference raises Python
  *                                exceptions; codes map to them in the wrapper)
  *
+ * rsfa_rotary and rsfa_cache4_* (below) have no counterpart in the reference:
+ * they are what a program that serves with the operator runs around it.
+ *
  * Conventions
  *   - All tensor pointers are device pointers owned by the caller; the library
  *     never frees them.  Strides are in elements.  The last (head-dim) stride
@@ -61,14 +64,18 @@ typedef enum rsfa_status {
     RSFA_E_LAUNCH    = -8,  /* kernel launch failed                             */
     RSFA_E_ABI       = -9,  /* struct_size does not match this library          */
     RSFA_E_WORKSPACE = -10, /* split mode without a large enough workspace       */
-    RSFA_E_SCRATCH   = -11  /* rsfa_attention_fwd_noalloc: the problem needs
+    RSFA_E_SCRATCH   = -11, /* rsfa_attention_fwd_noalloc: the problem needs
                                more workspace than RSFA_NOALLOC_WORKSPACE_BYTES */
+    RSFA_E_ROTARY    = -12, /* rsfa_rotary: rotary_dim odd, < 2 or > head_dim   */
+    RSFA_E_CACHE     = -13, /* a cache or a call on one is out of its range: see
+                               rsfa_cache4                                      */
+    RSFA_E_BUDGET    = -14  /* claim / evict: budget, recent, sinks or n         */
 } rsfa_status;
 
 typedef enum rsfa_dtype {
     RSFA_DTYPE_F16  = 0,         /* q, k, v, o float16                         */
     RSFA_DTYPE_BF16 = 1,         /* q, k, v, o bfloat16                        */
-    RSFA_DTYPE_F16_V8E5M2 = 2    /* q, k, o float16; v float8 e5m2 (OCP: sign,
+    RSFA_DTYPE_F16_V8E5M2 = 2,   /* q, k, o float16; v float8 e5m2 (OCP: sign,
                                     5 exponent bits, bias 15, 2 mantissa bits).
                                     P is rounded to e5m2 for P.V and the row
                                     sums add the unrounded P, as the reference's
@@ -76,6 +83,7 @@ typedef enum rsfa_dtype {
                                     kernels read V's bytes and run P.V on the
                                     e5m2 MFMA at every head dim (no
                                     workspace) */
+    RSFA_DTYPE_F32 = 3           /* float32: rsfa_rotary only                   */
 } rsfa_dtype;
 
 /* flags (bit set) */
@@ -201,6 +209,161 @@ int rsfa_resolve_tiling(int64_t head_dim, int32_t causal, int32_t dtype,
 /* Number of compute units of `device` (-1 = current device); replaces
  * get_num_compute_cores (19-21).  Negative rsfa_status on error. */
 int rsfa_get_num_compute_cores(int device);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions.
+ *
+ * The first rotary_dim values of every head are R/2 pairs (R = rotary_dim):
+ * (x_i, x_(i+R/2)), or with RSFA_ROTARY_INTERLEAVED (x_2i, x_(2i+1)).  Pair i
+ * of the token at position p is turned by the angle 2 pi p turns[i] and scaled
+ * by `amplitude`; the other values are copied.  RSFA_ROTARY_INVERSE turns
+ * back (and scales by `amplitude` all the same): the gradient of the forward
+ * call.  One or two tensors (q and k) of one dtype in one launch; y[i] may be
+ * x[i] with the same strides (in place), but not overlap it otherwise.
+ * Strides are in elements, the last one 1; any alignment that the element
+ * type has (16-byte rows take wide loads).  Angles are reduced in 64 bits:
+ * their error is below 2^-52 of the angle and 2^-25 of a turn.
+ * ------------------------------------------------------------------------ */
+#define RSFA_ROTARY_INTERLEAVED 0x1u
+#define RSFA_ROTARY_INVERSE     0x2u
+#define RSFA_ROTARY_POS64       0x4u /* positions are int64 instead of int32 */
+
+typedef struct rsfa_rotary_args {
+    uint32_t      struct_size;    /* = sizeof(rsfa_rotary_args)                */
+    int32_t       dtype;          /* RSFA_DTYPE_F16, _BF16 or _F32             */
+    const void   *x[2];           /* [Z, heads[i], N, D]; x[1] may be NULL     */
+    void         *y[2];
+    int64_t       z, n, head_dim, rotary_dim;
+    int64_t       heads[2];
+    int64_t       x_stride[2][4]; /* element strides of dims (Z, H, N, D)      */
+    int64_t       y_stride[2][4];
+    const void   *positions;      /* device, or NULL: token n is at start + n  */
+    int64_t       pos_stride[2];  /* of dims (Z, N) of positions, in elements  */
+    int64_t       start;
+    const double *turns;          /* device, [rotary_dim / 2]: turns a position */
+    float         amplitude;
+    uint32_t      flags;          /* RSFA_ROTARY_*                              */
+} rsfa_rotary_args;
+
+int rsfa_rotary(const rsfa_rotary_args *args, void *stream);
+
+/* ------------------------------------------------------------------------
+ * A key/value cache held in 4 bits.
+ *
+ * A row (one token's key or value of one head) is head_dim / 2 bytes of codes
+ * and head_dim / 32 scale bytes.  Each 32 values share a scale byte b, which
+ * stands for 2^(b - 127); 255 makes the block NaN.  A code is a sign bit (8) and
+ * the index of 0, 0.5, 1, 1.5, 2, 3, 4, 6; byte j of a row holds value 2j in its low
+ * and value 2j + 1 in its high bits (the e2m1 elements and e8m0 scales of the
+ * OCP microscaling formats).  Written rows take the smallest scale of
+ * which no value of the block is more than 7, within the exponents -23 .. 13
+ * (float16) or -125 .. 125 (bfloat16), whose values all exist in the type:
+ * values are rounded to the nearest code, ties to the even index, and end at 6
+ * scales; a block that holds an infinity or a NaN is stored as NaN.
+ *
+ * Sequences and heads are [z, h]; each has `capacity` slots, whose rows lie
+ * densely: slot s of (z, h) is at z * stride[0] + h * stride[1] + s * row, with
+ * strides in elements of the buffer.  code_stride is that of k_codes and
+ * v_codes, scale_stride of both scale buffers, slot_stride of positions and
+ * weights.  Code buffers are 16-byte aligned with strides that are multiples
+ * of 16; scale buffers aligned to head_dim / 32 bytes, with strides that are
+ * multiples of it.
+ *
+ * Lengths say how many slots of a sequence are in use: `lengths` (device,
+ * int32 [z]) or, where it is NULL, `length` for all.  Values outside
+ * [0, capacity] are taken as its ends by the kernels.
+ * ------------------------------------------------------------------------ */
+typedef struct rsfa_cache4 {
+    uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+    int32_t *positions; /* position of each slot's token                       */
+    float   *weights;   /* accumulated attention weight of each slot, or NULL   */
+    int64_t  z, h, capacity, head_dim; /* head_dim: 32, 64, 128 or 256          */
+    int64_t  code_stride[2], scale_stride[2], slot_stride[2];
+    int32_t  dtype;     /* RSFA_DTYPE_F16 or _BF16: of the rows written and read */
+    int32_t  reserved;  /* 0 */
+} rsfa_cache4;
+
+/* append: writes the rows k, v [z, h, t, head_dim].  Token i of sequence z goes
+ * to slot lengths[z] + i, or with `slots` (device, int32 [z, h, t], dense) to
+ * slots[z, h, i]; tokens i >= counts[z] (device, int32 [z], or NULL) and
+ * slots outside [0, capacity) are left out; where `slots` names a slot twice
+ * the last token has it.  The slot's position becomes pos_start[z] + i (NULL:
+ * lengths[z] + i), its weight 0.
+ * read: the values of slots start[z] + i (NULL: start0 + i), or slots[z, h, i],
+ * into k, v; rows outside [0, capacity) read as 0. */
+typedef struct rsfa_cache4_rows_args {
+    uint32_t       struct_size; /* = sizeof(rsfa_cache4_rows_args)             */
+    uint32_t       reserved;    /* 0 */
+    rsfa_cache4    cache;
+    void          *k, *v;       /* either may be NULL in a read                */
+    int64_t        t;
+    int64_t        k_stride[4], v_stride[4]; /* elements; rows 16-byte aligned */
+    const int32_t *lengths;     /* append: the lengths; read: the first slots   */
+    int64_t        length;
+    const int32_t *slots;
+    const int32_t *counts;      /* append only */
+    const int32_t *pos_start;   /* append only */
+} rsfa_cache4_rows_args;
+
+int rsfa_cache4_append(const rsfa_cache4_rows_args *args, void *stream);
+int rsfa_cache4_read(const rsfa_cache4_rows_args *args, void *stream);
+
+/* attend: o = softmax(q k^T sm_scale) v over the slots in use; query head i
+ * reads key head i / (heads / cache.h).  With `causal` query token i of sequence
+ * z sees the slots whose position is at most pos_start[z] + i (NULL:
+ * length - count + i, with the sequence's count of tokens).  Rows i >= counts[z],
+ * and rows that see no slot, give 0 (lse -inf).  With `accumulate` the weights
+ * of the slots grow by the softmax weights that all rows of the call gave them.
+ * Lengths above max_length (0: the capacity) are taken as max_length.
+ * Workspace: rsfa_cache4_attend_workspace_bytes of the same arguments (its
+ * contents need not outlive the call's kernels). */
+typedef struct rsfa_cache4_attend_args {
+    uint32_t       struct_size; /* = sizeof(rsfa_cache4_attend_args)           */
+    int32_t        causal;
+    rsfa_cache4    cache;
+    const void    *q;           /* [z, heads, t, head_dim], the cache's dtype  */
+    void          *o;
+    float         *lse;         /* [z, heads, t], dense, or NULL               */
+    int64_t        heads, t;
+    int64_t        q_stride[4], o_stride[4];
+    const int32_t *lengths;
+    int64_t        length, max_length;
+    const int32_t *counts, *pos_start;
+    float          sm_scale;
+    int32_t        accumulate;
+    void          *workspace;   /* 16-byte aligned */
+    uint64_t       workspace_bytes;
+} rsfa_cache4_attend_args;
+
+int rsfa_cache4_attend(const rsfa_cache4_attend_args *args, void *stream);
+uint64_t rsfa_cache4_attend_workspace_bytes(const rsfa_cache4_attend_args *args);
+
+/* Eviction by accumulated weight.  A slot in use is protected when its position
+ * is less than `sinks` or among the last `recent` up to the sequence and head's
+ * largest.  Slots go in order of their weight, the lowest first, ties by the
+ * lowest slot (a NaN weight counts as the largest; -0 as 0).
+ * claim: out [z, h, n] (int32, dense): the slots for each sequence's next n
+ * tokens: those from lengths[z] up to `budget`, then the unprotected slots that
+ * go first, in order of slot; -1 where there is none.
+ * evict: copies to `into` (same z, h, head_dim and dtype; not the same memory) the
+ * slots that stay when the first max(0, lengths[z] - budget) go (protected ones
+ * after all others), in order of slot, to its slots 0, 1, ...; other slots of `into`
+ * keep what they hold.  Workspace: z * h * budget int32. */
+typedef struct rsfa_cache4_evict_args {
+    uint32_t       struct_size; /* = sizeof(rsfa_cache4_evict_args)            */
+    uint32_t       reserved;    /* 0 */
+    rsfa_cache4    cache;
+    rsfa_cache4    into;        /* evict only                                  */
+    const int32_t *lengths;
+    int64_t        length;
+    int64_t        n;           /* claim only                                  */
+    int64_t        budget, recent, sinks;
+    int32_t       *out;         /* claim: the slots; evict: the workspace      */
+    uint64_t       out_bytes;
+} rsfa_cache4_evict_args;
+
+int rsfa_cache4_claim(const rsfa_cache4_evict_args *args, void *stream);
+int rsfa_cache4_evict(const rsfa_cache4_evict_args *args, void *stream);
 
 /* Static string for a status code. */
 const char *rsfa_strerror(int status);
