@@ -22,6 +22,9 @@
 // only moves when a score passes it by SLACK (log2 units), as the weights then
 // stay below 2^SLACK and the final division takes the factor out; the row
 // sum adds the weights before they are rounded to the cache's type for P V.
+#include <cfloat>
+#include <type_traits>
+
 #include "cache4.hpp"
 
 using namespace rsfa4;
@@ -69,6 +72,8 @@ __device__ __forceinline__ float scale_bits(uint32_t w, int byte) {
     return __uint_as_float(__builtin_amdgcn_alignbit(w, w, (8 * byte + 9) & 31));
 }
 
+typedef u32x4 u32x4_u __attribute__((aligned(4)));  // loads need the alignment of a dword
+
 template <int BYTES>
 struct Bytes;
 template <> struct Bytes<1> { typedef uint8_t type; };
@@ -76,7 +81,7 @@ template <> struct Bytes<2> { typedef uint16_t type; };
 template <> struct Bytes<4> { typedef uint32_t type; };
 
 // A wave's raw K and V tile of 32 keys.
-template <int D>
+template <int D, bool CAUSAL>
 struct Raw {
     static constexpr int KW = D / 32;             // dwords of K codes a lane has of a key
     static constexpr int VW = D >= 128 ? D / 128 : 1;  // dwords of V codes a lane has of a key
@@ -84,21 +89,27 @@ struct Raw {
     uint32_t ks[2];                               // scale bytes of the lane's K values (byte 0, 1 at D = 256)
     uint32_t v[8][VW];
     uint32_t vs[8];                               // D >= 128: the dword of the key's scale bytes that has the lane's
+    int pos[CAUSAL ? 8 : 1];                      // positions of the lane's V keys (which are its S^T rows)
 };
 
-template <int D>
+template <int D, bool CAUSAL>
 struct Loader {
     const uint8_t *kc, *ks, *vc, *vs;  // of the sequence and head
-    int lane, col, grp;
+    const int32_t* pos;
+    int col, grp;
 
+    // `tile` is uniform: the loads take a scalar base, a lane's offset and constants.
     // Slots past `last` read slot `last` (TAIL) or are known to exist.
     template <bool TAIL>
-    __device__ __forceinline__ void load(Raw<D>& r, int tile, int last) const {
+    __device__ __forceinline__ void load(Raw<D, CAUSAL>& r, int tile, int last) const {
+        const uint8_t *kb = kc + (int64_t)tile * (D / 2), *ksb = ks + (int64_t)tile * (D / 32);
+        const uint8_t *vb = vc + (int64_t)tile * (D / 2), *vsb = vs + (int64_t)tile * (D / 32);
+        const int32_t* pb = pos + tile;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            int key = tile + 16 * h + col;
-            if (TAIL) key = min(key, last);
-            const uint8_t* p = kc + (int64_t)key * (D / 2) + grp * (D / 8);
+            uint32_t key = 16 * h + col;
+            if (TAIL) key = min(key, (uint32_t)(last - tile));
+            const uint8_t* p = kb + (key * (D / 2) + grp * (D / 8));
             if constexpr (D == 32) {
                 r.k[h][0] = *(const uint32_t*)p;
             } else if constexpr (D == 64) {
@@ -112,24 +123,39 @@ struct Loader {
                     for (int j = 0; j < 4; ++j) r.k[h][4 * i + j] = w[j];
                 }
             }
-            const uint8_t* s = ks + (int64_t)key * (D / 32);
-            if constexpr (D == 256) r.ks[h] = *(const uint16_t*)(s + 2 * grp);
-            else r.ks[h] = s[grp * (D / 4) / 32];
+            const uint8_t* s = ksb + (key * (D / 32) + (D == 256 ? 2 * grp : grp * (D / 4) / 32));
+            if constexpr (D == 256) r.ks[h] = *(const uint16_t*)s;
+            else r.ks[h] = *s;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            int key = tile + 16 * (j / 4) + 4 * grp + j % 4;
-            if (TAIL) key = min(key, last);
-            const uint8_t* p = vc + (int64_t)key * (D / 2) + col * (D / 32);
+            uint32_t key = 4 * grp + (16 * (j / 4) + j % 4);
+            if (TAIL) key = min(key, (uint32_t)(last - tile));
+            const uint8_t* p = vb + (key * (D / 2) + col * (D / 32));
             if constexpr (D == 256) {
                 const u32x2 w = *(const u32x2*)p;
                 r.v[j][0] = w[0], r.v[j][1] = w[1];
             } else {
                 r.v[j][0] = *(const typename Bytes<D / 32>::type*)p;
             }
-            const uint8_t* s = vs + (int64_t)key * (D / 32);
-            if constexpr (D == 256) r.vs[j] = *(const uint32_t*)(s + (col / 8) * 4);
-            else r.vs[j] = *(const typename Bytes<D / 32>::type*)s;
+            const uint8_t* s = vsb + (key * (D / 32) + (D == 256 ? (col / 8) * 4 : 0));
+            if constexpr (D == 256) r.vs[j] = *(const uint32_t*)s;
+            else if constexpr (D == 128 && !TAIL) {
+                if (j % 4 == 0) {  // four keys' scales lie together
+                    const u32x4_u w = *(const u32x4_u*)s;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) r.vs[j + i] = w[i];
+                }
+            } else r.vs[j] = *(const typename Bytes<D / 32>::type*)s;
+            if constexpr (CAUSAL && !TAIL) {
+                if (j % 4 == 0) {
+                    const u32x4_u w = *(const u32x4_u*)(pb + key);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) r.pos[j + i] = (int)w[i];
+                }
+            } else if constexpr (CAUSAL) {
+                r.pos[j] = pb[key];
+            }
         }
     }
     // The byte of vs[] that scales the lane's V values.
@@ -138,53 +164,55 @@ struct Loader {
     }
 };
 
-// NB blocks of 16 rows a wave; RW of the workgroup's four waves take rows of
-// their own, the others share their rows' keys.
-template <class T, int D, int NB, int RW>
-struct Geometry {
-    static constexpr int KWAVES = 4 / RW;
-    static constexpr int ROWS = RW * NB * 16;
-};
-
-template <class T, int D, int NB, int RW, bool CAUSAL>
+// Few rows (NB blocks of 16): the four waves of a workgroup take every fourth key
+// tile of its part of the slots and add up what they have at the end.  CAUSAL hides
+// keys in every tile; otherwise only the last, partial tile does.
+template <class T, int D, int NB, bool CAUSAL>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
-    typedef Geometry<T, D, NB, RW> G;
     typedef typename T::x8 x8;
     typedef typename T::elem elem;
     constexpr int DT = D / 16;  // 16-row tiles of O^T
     constexpr int QS = D / 32;  // k steps of S^T
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int WAVES = 4, STEP = TILE * WAVES;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
-    const int rw = wave / G::KWAVES, kw = wave % G::KWAVES;
-    const int bh = blockIdx.x % p.bh;  // with a multiple of 8, a head's row tiles meet in one XCD's L2
-    const int tile_id = blockIdx.x / p.bh;
+    const int bh = blockIdx.x;
     const int split = blockIdx.y;
     const int z = bh / (int)p.c.h, h = bh - z * (int)p.c.h;
-    const int len = length_of(p.lengths, p.length, z, p.most);
+    const int len = __builtin_amdgcn_readfirstlane(length_of(p.lengths, p.length, z, p.most));
     const int count = p.counts ? max(0, min(p.counts[z], p.t)) : p.t;
-    const int row0 = tile_id * G::ROWS + rw * NB * 16;
 
-    Loader<D> ld;
+    Loader<D, CAUSAL> ld;
     {
         const int64_t c = z * p.c.code_stride[0] + h * p.c.code_stride[1];
         const int64_t s = z * p.c.scale_stride[0] + h * p.c.scale_stride[1];
         ld.kc = p.c.k_codes + c, ld.vc = p.c.v_codes + c;
         ld.ks = p.c.k_scales + s, ld.vs = p.c.v_scales + s;
-        ld.lane = lane, ld.col = col, ld.grp = grp;
+        ld.pos = p.c.positions + z * p.c.slot_stride[0] + h * p.c.slot_stride[1];
+        ld.col = col, ld.grp = grp;
     }
-    const int32_t* pos = p.c.positions + z * p.c.slot_stride[0] + h * p.c.slot_stride[1];
+
+    // this part's slots, a whole number of steps but for the last part's
+    const int chunk = ((len + p.splits - 1) / p.splits + STEP - 1) / STEP * STEP;
+    const int64_t start64 = (int64_t)chunk * split;
+    const int start = (int)(start64 < len ? start64 : len);
+    const int end = min(start + chunk, len);
+    // whole tiles of this wave, and whether the partial one is its own
+    const int whole = (end - start) / TILE;
+    const int turns = whole > wave ? (whole - wave + WAVES - 1) / WAVES : 0;
+    const bool tail = (end - start) % TILE != 0 && whole % WAVES == wave;
+
+    Raw<D, CAUSAL> cur, next;
+    if (turns) ld.template load<false>(cur, start + TILE * wave, 0);
 
     // Q^T and the rows' positions
     x8 q[NB][QS];
     int qpos[NB];
-    int least = 0x7fffffff, greatest = -0x7fffffff - 1;  // of the wave's valid rows' positions
-    bool any_row = false;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        const int row = row0 + 16 * b + col;
+        const int row = 16 * b + col;
         const int tok = row / p.group, head = row - tok * p.group;
         const bool valid = tok < count;  // (row < rows follows)
-        any_row |= valid;
         u32x4 w[QS] = {};
         if (valid) {
             const elem* src = (const elem*)p.q + z * p.qs[0] + (int64_t)(h * p.group + head) * p.qs[1] + tok * p.qs[2] + grp * (D / 4);
@@ -200,14 +228,6 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
         if (CAUSAL) {
             const int64_t at = (p.pos_start ? (int64_t)p.pos_start[z] : (int64_t)len - count) + tok;
             qpos[b] = (int)(at > 0x7fffffff ? 0x7fffffff : at);
-            if (valid) least = min(least, qpos[b]), greatest = max(greatest, qpos[b]);
-        }
-    }
-    if (CAUSAL) {
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            least = min(least, __shfl_xor(least, d));
-            greatest = max(greatest, __shfl_xor(greatest, d));
         }
     }
 
@@ -220,45 +240,12 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[b][d] = (f32x4){0, 0, 0, 0};
     }
-
-    // this split's keys, a whole number of tiles for every wave but the last's
-    const int step = TILE * G::KWAVES;
-    const int chunk = ((len + p.splits - 1) / p.splits + step - 1) / step * step;
-    const int64_t start64 = (int64_t)chunk * split;
-    const int start = (int)(start64 < len ? start64 : len);
-    const int end = min(start + chunk, len);
     const int vbyte = ld.v_byte();
 
-    auto compute = [&](const Raw<D>& r, int tile) {
-        // hidden keys: past the end, or (causal) of a later position than a row's
-        int kpos[8];
-        bool masked = tile + TILE > end;
-        if (CAUSAL) {
-            int far = -0x7fffffff - 1, near = 0x7fffffff;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = tile + 16 * (j / 4) + 4 * grp + j % 4;
-                kpos[j] = pos[min(key, len - 1)];
-                far = max(far, kpos[j]);
-                near = min(near, kpos[j]);
-            }
-            masked |= __any(far > least);
-            if (!__any(near <= greatest)) {
-                if (p.scores) {  // no row sees the tile: its scores all the same are read
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const int row = row0 + 16 * b + col;
-                        if (row < p.rows)
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const int key = tile + 16 * (j / 4) + 4 * grp + j % 4;
-                                if (key < end) p.scores[((int64_t)bh * p.rows + row) * p.most + key] = -INFINITY;
-                            }
-                    }
-                }
-                return;
-            }
-        }
+    // One tile.  MASKED: some of its keys may be hidden from some row, past the end
+    // (TAIL) or (causal) of a later position than the row's.
+    auto compute = [&](const Raw<D, CAUSAL>& r, int tile, auto tail_) {
+        constexpr bool TAIL = decltype(tail_)::value, MASKED = CAUSAL || TAIL;
         f32x4 s[NB][2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -283,21 +270,21 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
             visible[b] = 0xff;
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = s[b][j / 4][j % 4] * p.scale;
-            if (masked) {
+            if constexpr (MASKED) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int key = tile + 16 * (j / 4) + 4 * grp + j % 4;
-                    const bool hidden = key >= end || (CAUSAL && kpos[j] > qpos[b]);
+                    const bool hidden = (TAIL && key >= end) || (CAUSAL && r.pos[j] > qpos[b]);
                     if (hidden) x[j] = -INFINITY, visible[b] &= ~(1u << j);
                 }
             }
             if (p.scores) {
-                const int row = row0 + 16 * b + col;
+                const int row = 16 * b + col;
                 if (row < p.rows) {
                     float* dst = p.scores + ((int64_t)bh * p.rows + row) * p.most + tile + 4 * grp;
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (!masked || tile + 16 * (j / 4) + 4 * grp + j % 4 < end) dst[16 * (j / 4) + j % 4] = x[j];
+                        if (!TAIL || tile + 16 * (j / 4) + 4 * grp + j % 4 < end) dst[16 * (j / 4) + j % 4] = x[j];
                 }
             }
             float top = x[0];
@@ -324,7 +311,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
         float sc[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) sc[j] = scale_bits(r.vs[j], vbyte);
-        if (masked) {
+        if constexpr (MASKED) {
             uint32_t bad = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -332,9 +319,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
             if (__any(bad != 0)) {
                 // lane l's O^T values are rows 4 (l / 16) + r of each tile: dims
                 // (4 (l / 16) + r) D/16 + d, whose block is that of a lane with col = 4 (l / 16) + r
-#pragma unroll
                 for (int b = 0; b < NB; ++b)
-#pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         bool hit = false;
                         for (int g = 0; g < 4; ++g) {
@@ -342,9 +327,13 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
                             const uint32_t there = __shfl((int)bad, 16 * g + 4 * grp + i);
                             hit |= (vis & there) != 0;
                         }
-                        if (hit)
 #pragma unroll
-                            for (int d = 0; d < DT; ++d) acc[b][d][i] = __builtin_nanf("");
+                        for (int bb = 0; bb < NB; ++bb)
+#pragma unroll
+                            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                                for (int ii = 0; ii < 4; ++ii)
+                                    if (hit && bb == b && ii == i) acc[bb][d][ii] = __builtin_nanf("");
                     }
             }
         }
@@ -374,80 +363,69 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
         }
     };
 
-    // (a wave whose rows are all invalid still takes part in the exchange below)
-    if (__any(any_row)) {
-        int tile = start + TILE * kw;
-        if (tile < end) {
-            Raw<D> cur, next;
-            if (tile + TILE <= len) ld.template load<false>(cur, tile, 0);
-            else ld.template load<true>(cur, tile, len - 1);
-            for (;;) {
-                const int after = tile + step;
-                if (after < end) {
-                    if (after + TILE <= len) ld.template load<false>(next, after, 0);
-                    else ld.template load<true>(next, after, len - 1);
-                }
-                compute(cur, tile);
-                if (after >= end) break;
-                cur = next;
-                tile = after;
-            }
-        }
+    for (int i = 0; i < turns; ++i) {
+        const int tile = start + TILE * (wave + WAVES * i);
+        if (i + 1 < turns) ld.template load<false>(next, tile + STEP, 0);
+        compute(cur, tile, std::false_type());
+        cur = next;
     }
+    if (tail) {
+        const int tile = start + TILE * whole;
+        ld.template load<true>(cur, tile, len - 1);
+        compute(cur, tile, std::true_type());
+    }
+
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         l[b] += __shfl_xor(l[b], 16);
         l[b] += __shfl_xor(l[b], 32);
         // rows past the count are empty (their q was taken as 0)
-        if ((row0 + 16 * b + col) / p.group >= count) m[b] = NEVER, l[b] = 0.0f;
+        if ((16 * b + col) / p.group >= count) m[b] = NEVER, l[b] = 0.0f;
     }
-
-    if constexpr (G::KWAVES > 1) {
-        // the waves that share rows add up their parts, through LDS
-        constexpr int PITCH = D + 4;  // dwords of a row: 16-lane columns meet no bank twice
-        __shared__ float2 ml[4][NB * 16];
-        __shared__ float part[RW][NB * 16][PITCH];
+    // the waves add up what they have, through LDS
+    constexpr int PITCH = D + 4;
+    __shared__ float2 ml[WAVES][NB * 16];
+    __shared__ float part[NB * 16][PITCH];
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-            if (grp == 0) ml[wave][16 * b + col] = make_float2(m[b], l[b]);
-        __syncthreads();
-        float f[NB];
+    for (int b = 0; b < NB; ++b)
+        if (grp == 0) ml[wave][16 * b + col] = make_float2(m[b], l[b]);
+    __syncthreads();
+    float f[NB];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            float mm = NEVER, ll = 0.0f;
-            for (int k = 0; k < G::KWAVES; ++k) mm = fmaxf(mm, ml[rw * G::KWAVES + k][16 * b + col].x);
-            for (int k = 0; k < G::KWAVES; ++k) {
-                const float2 v = ml[rw * G::KWAVES + k][16 * b + col];
-                ll += v.y * __builtin_amdgcn_exp2f(v.x - mm);
-            }
-            f[b] = __builtin_amdgcn_exp2f(m[b] - mm);
-            m[b] = mm;
-            l[b] = ll;
+    for (int b = 0; b < NB; ++b) {
+        float mm = NEVER, ll = 0.0f;
+        for (int k = 0; k < WAVES; ++k) mm = fmaxf(mm, ml[k][16 * b + col].x);
+        for (int k = 0; k < WAVES; ++k) {
+            const float2 v = ml[k][16 * b + col];
+            ll += v.y * __builtin_amdgcn_exp2f(v.x - mm);
         }
-        for (int k = G::KWAVES - 1; k >= 0; --k) {
-            if (kw == k) {
+        f[b] = __builtin_amdgcn_exp2f(m[b] - mm);
+        m[b] = mm;
+        l[b] = ll;
+    }
+    for (int k = WAVES - 1; k >= 0; --k) {
+        if (wave == k) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float* at = &part[rw][16 * b + col][(4 * grp + i) * DT];
+                for (int i = 0; i < 4; ++i) {
+                    float* at = &part[16 * b + col][(4 * grp + i) * DT];
 #pragma unroll
-                        for (int d = 0; d < DT; ++d) {
-                            float v = acc[b][d][i] * f[b];
-                            if (k < G::KWAVES - 1) v += at[d];
-                            if (k > 0) at[d] = v;
-                            else acc[b][d][i] = v;
-                        }
+                    for (int d = 0; d < DT; ++d) {
+                        float v = acc[b][d][i] * f[b];
+                        if (k < WAVES - 1) v += at[d];
+                        if (k > 0) at[d] = v;
+                        else acc[b][d][i] = v;
                     }
-            }
-            __syncthreads();
+                }
         }
-        if (kw != 0) return;
+        __syncthreads();
     }
+    if (wave != 0) return;
 
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        const int row = row0 + 16 * b + col;
+        const int row = 16 * b + col;
         if (row >= p.rows) continue;
         const int tok = row / p.group, head = row - tok * p.group;
         if (p.splits > 1) {
@@ -483,39 +461,357 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
     }
 }
 
-// Sum of a row's parts: one wave a row.
-template <class T, int D>
-__global__ void __launch_bounds__(256) join_kernel(AttendParams p) {
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // bh * rows + row
-    const int lane = threadIdx.x & 63;
-    const int64_t all = (int64_t)p.bh * p.rows;
-    if (id >= all) return;
-    const int bh = (int)(id / p.rows), row = (int)(id - (int64_t)bh * p.rows);
-    float m = NEVER;
-    for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, p.part_ml[s * all + id].x);
+// Many rows: each of the workgroup's four waves has 32 rows of its own, and all
+// share the key tile.  Its codes are converted once per workgroup and kept in LDS as
+// the operands of v_mfma_f32_32x32x16 themselves: fragment f is 64 lanes of 16 bytes,
+// so that writes and reads are linear.  Of the two buffers one is computed with while
+// the next tile is converted into the other, from codes loaded a tile ahead.
+//   S^T = K Q^T  A: lane l has the key l % 32 and 8 values a step of the D/2 that
+//                start at (l / 32) * D/2, so a fragment is one dword of codes.
+//   O^T = V^T P^T  S^T leaves lane l the row l % 32 and the keys 8 a + 4 (l / 32) + b;
+//                step s takes k = 8 (l / 32) + j as key 16 s + 8 (j / 4) + 4 (l / 32) + j % 4.
+//                A: lane l has these keys of the value (l % 32) * D/32 + t in fragment t.
+template <int D>
+struct Many {
+    static constexpr int KEYS = D == 256 ? 32 : 64;  // of a tile: its fragments take 32 KB at D = 128, 256
+    static constexpr int KF = KEYS / 32 * (D / 16) / 4;  // K fragments a wave converts
+    static constexpr int VF = KEYS / 16 * (D / 32) / 4;  // V fragments
+    static constexpr int KFRAGS = 4 * KF, FRAGS = 4 * (KF + VF);
+    static constexpr int PER_BLOCK = 4 / (KEYS / 32);    // waves that share a block of 32 keys' K
+    static constexpr int ROWS = 128;
+};
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32(F16::x8 a, F16::x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(BF16::x8 a, BF16::x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+template <class T, int D, bool CAUSAL>
+__global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
+    typedef Many<D> M;
+    typedef typename T::x8 x8;
+    typedef typename T::elem elem;
+    constexpr int QS = D / 16, DT = D / 32, KEYS = M::KEYS, SB = KEYS / 32;
+    __shared__ u32x4 frag[2][M::FRAGS][64];
+    __shared__ int kpos[2][CAUSAL ? KEYS : 1];
+    __shared__ int spoiled[2][4];  // a wave's V codes of the tile hold a NaN block
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int bh = blockIdx.x % p.bh;  // with a multiple of 8, a head's row tiles meet in one XCD's L2
+    const int z = bh / (int)p.c.h, h = bh - z * (int)p.c.h;
+    const int len = __builtin_amdgcn_readfirstlane(length_of(p.lengths, p.length, z, p.most));
+    const int count = p.counts ? max(0, min(p.counts[z], p.t)) : p.t;
+    const int row = blockIdx.x / p.bh * M::ROWS + 32 * wave + col;
+    const int tok = row / p.group, head = row - tok * p.group;
+    const bool valid = tok < count;  // (row < rows follows)
+    const int64_t cb = z * p.c.code_stride[0] + h * p.c.code_stride[1];
+    const int64_t sb = z * p.c.scale_stride[0] + h * p.c.scale_stride[1];
+    const uint8_t *kc = p.c.k_codes + cb, *vc = p.c.v_codes + cb, *ks = p.c.k_scales + sb, *vs = p.c.v_scales + sb;
+    const int32_t* pos = p.c.positions + z * p.c.slot_stride[0] + h * p.c.slot_stride[1];
+
+    const int chunk = ((len + p.splits - 1) / p.splits + KEYS - 1) / KEYS * KEYS;
+    const int64_t start64 = (int64_t)chunk * blockIdx.y;
+    const int start = (int)(start64 < len ? start64 : len);
+    const int end = min(start + chunk, len);
+
+    // Q^T
+    x8 q[QS];
+    int qpos = -0x7fffffff - 1, least = 0x7fffffff, greatest = -0x7fffffff - 1;
+    {
+        u32x4 w[QS] = {};
+        if (valid) {
+            const elem* src = (const elem*)p.q + z * p.qs[0] + (int64_t)(h * p.group + head) * p.qs[1] + tok * p.qs[2] + half * (D / 2);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    constexpr int W = D >= 64 ? D / 64 : 1;
-    float o[W] = {};
-    float l = 0.0f;
-    const bool mine = lane * W < D;
-    for (int s = 0; s < p.splits; ++s) {
-        const float2 v = p.part_ml[s * all + id];
-        if (v.y == 0.0f) continue;  // no slot in this part
-        const float f = __builtin_amdgcn_exp2f(v.x - m);
-        l += v.y * f;
-        if (mine)
+            for (int i = 0; i < QS; ++i) w[i] = *(const u32x4*)(src + 8 * i);
+        }
 #pragma unroll
-            for (int i = 0; i < W; ++i) o[i] += p.part_o[(s * all + id) * D + lane * W + i] * f;
+        for (int i = 0; i < QS; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[i][j] ^= p.neg;
+            q[i] = __builtin_bit_cast(x8, w[i]);
+        }
+        if (CAUSAL) {
+            const int64_t at = (p.pos_start ? (int64_t)p.pos_start[z] : (int64_t)len - count) + tok;
+            if (valid) least = greatest = qpos = (int)(at > 0x7fffffff ? 0x7fffffff : at);
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                least = min(least, __shfl_xor(least, d));
+                greatest = max(greatest, __shfl_xor(greatest, d));
+            }
+        }
+    }
+
+    // this wave's part of a tile's conversion
+    struct {
+        uint32_t k[M::KF], ks;
+        uint32_t v[8], vs[8];
+        int pos;
+    } raw;
+    const int kblock = wave / M::PER_BLOCK, kpart = wave % M::PER_BLOCK;
+    const int vstep = D == 256 ? wave / 2 : wave, vpart = D == 256 ? wave % 2 : 0;
+    // V codes of a lane: D/64 bytes of a key (D = 256: of its half of them; D = 32: half a byte)
+    const uint32_t koff = half * (D / 4) + kpart * (4 * M::KF);
+    const uint32_t ksoff = (half * (D / 2) + kpart * (8 * M::KF)) / 32;
+    const uint32_t voff = D == 32 ? col / 2 : D == 256 ? col * 4 + vpart * 2 : col * (D / 64);
+    const uint32_t vsoff = D == 256 ? (col / 16) * 4 : 0;
+    const int vbyte = D == 256 ? (col / 4) & 3 : D == 128 ? col / 8 : D == 64 ? col / 16 : 0;
+    auto load = [&](int tile) {
+        const uint32_t last = len - 1 - tile;  // keys past the length repeat the last
+        const uint8_t* kb = kc + (int64_t)tile * (D / 2);
+        const uint8_t* vb = vc + (int64_t)tile * (D / 2);
+        {
+            const uint32_t key = min((uint32_t)(32 * kblock + col), last);
+            const uint8_t* src = kb + (key * (D / 2) + koff);
+            if constexpr (M::KF == 4) {
+                const u32x4 w = *(const u32x4*)src;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw.k[i] = w[i];
+            } else if constexpr (M::KF == 2) {
+                const u32x2 w = *(const u32x2*)src;
+                raw.k[0] = w[0], raw.k[1] = w[1];
+            } else {
+                raw.k[0] = *(const uint32_t*)src;
+            }
+            raw.ks = (ks + (int64_t)tile * (D / 32))[key * (D / 32) + ksoff];
+        }
+        const uint8_t* vsb = vs + (int64_t)tile * (D / 32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t key = min((uint32_t)(16 * vstep + 8 * (j / 4) + 4 * half + j % 4), last);
+            const uint8_t* src = vb + (key * (D / 2) + voff);
+            if constexpr (D >= 128) raw.v[j] = *(const uint16_t*)src;
+            else raw.v[j] = *src;
+            const uint8_t* s = vsb + (key * (D / 32) + vsoff);
+            raw.vs[j] = *(const typename Bytes<D == 256 ? 4 : D / 32>::type*)s;
+        }
+        if (CAUSAL && threadIdx.x < KEYS) raw.pos = pos[tile + min((uint32_t)threadIdx.x, last)];
+    };
+    auto convert = [&](int buf) {
+        const float ksc = scale_bits(raw.ks, 0);
+#pragma unroll
+        for (int i = 0; i < M::KF; ++i) {
+            const uint32_t w = raw.k[i];
+            frag[buf][wave * M::KF + i][lane] = (u32x4){T::template cvt<0>(w, ksc), T::template cvt<1>(w, ksc),
+                                                         T::template cvt<2>(w, ksc), T::template cvt<3>(w, ksc)};
+        }
+        // a NaN block of V is converted as 0, and noted: it must reach only rows that see its key
+        float sc[8];
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            sc[j] = scale_bits(raw.vs[j], vbyte);
+            bad |= (__float_as_uint(sc[j]) & 0x7f800000u) == 0x7f800000u;
+        }
+        const bool any = __any(bad);
+        if (__builtin_expect(any, 0)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if ((__float_as_uint(sc[j]) & 0x7f800000u) == 0x7f800000u) sc[j] = 0.0f;
+        }
+        if (lane == 0) spoiled[buf][wave] = any;
+#pragma unroll
+        for (int pr = 0; pr < (M::VF + 1) / 2; ++pr) {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = pr == 0 ? T::template cvt<0>(raw.v[j], sc[j]) : T::template cvt<1>(raw.v[j], sc[j]);
+            const uint32_t lo = D == 32 && (col & 1) ? 0x07060302u : 0x05040100u;
+            u32x4 even, odd;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                even[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], lo);
+                odd[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
+            }
+            frag[buf][M::KFRAGS + wave * M::VF + 2 * pr][lane] = even;
+            if (M::VF > 1) frag[buf][M::KFRAGS + wave * M::VF + 2 * pr + 1][lane] = odd;
+        }
+        if (CAUSAL && threadIdx.x < KEYS) kpos[buf][threadIdx.x] = raw.pos;
+    };
+
+    f32x16 acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
+    float m = NEVER, l = 0.0f;
+
+    auto compute = [&](int buf, int tile) {
+        bool masked = tile + KEYS > end;
+        if (CAUSAL) {
+            const int kp = kpos[buf][lane & (KEYS - 1)];
+            masked |= __any(kp > least);
+            if (!__any(kp <= greatest)) return;
+        }
+        f32x16 s[SB];
+#pragma unroll
+        for (int b = 0; b < SB; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < QS; ++i) s[b] = mfma32(__builtin_bit_cast(x8, frag[buf][b * QS + i][lane]), q[i], s[b]);
+        }
+        if (__builtin_expect(masked, 0)) {
+#pragma unroll
+            for (int b = 0; b < SB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+                    bool hidden = tile + key >= end;
+                    if (CAUSAL) hidden |= kpos[buf][key] > qpos;
+                    if (hidden) s[b][r] = -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < SB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+        top *= p.scale;
+        if (__any(top > m + SLACK)) {
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float now = fmaxf(m, top);
+            const float f = __builtin_amdgcn_exp2f(m - now);
+            m = now;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= f;
+        }
+        x8 pb[2 * SB];
+#pragma unroll
+        for (int b = 0; b < SB; ++b)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * t + j], p.scale, -m));
+                l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+                pb[2 * b + t] = __builtin_bit_cast(x8, (u32x4){pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])});
+            }
+#pragma unroll
+        for (int k = 0; k < 2 * SB; ++k)
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                acc[d] = mfma32(__builtin_bit_cast(x8, frag[buf][M::KFRAGS + k * DT + d][lane]), pb[k], acc[d]);
+        if (__builtin_expect(spoiled[buf][0] | spoiled[buf][1] | spoiled[buf][2] | spoiled[buf][3], 0)) {
+            // NaN blocks of V, into the rows that see them: register r holds the values
+            // D/32 (8 (r / 4) + 4 half + r % 4) + d, which lie in one block
+            uint32_t hit = 0;
+            for (int k = 0; k < KEYS && tile + k < end; ++k) {
+                bool sees = true;
+                if (CAUSAL) sees = kpos[buf][k] <= qpos;
+                if (!sees) continue;
+                for (int r = 0; r < 16; ++r) {
+                    const int i = 8 * (r / 4) + 4 * half + r % 4;
+                    if (vs[(int64_t)(tile + k) * (D / 32) + i * D / 1024] == 255) hit |= 1u << r;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (hit & (1u << r))
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[d][r] = __builtin_nanf("");
+        }
+    };
+
+    if (start < end) {
+        load(start);
+        convert(0);
+        if (start + KEYS < end) load(start + KEYS);
+        int buf = 0;
+        for (int tile = start; tile < end; tile += KEYS, buf ^= 1) {
+            __syncthreads();  // this tile is in LDS, and nobody reads the other buffer any more
+            if (tile + KEYS < end) convert(buf ^ 1);
+            if (tile + 2 * KEYS < end) load(tile + 2 * KEYS);
+            compute(buf, tile);
+        }
+    }
+    l += __shfl_xor(l, 32);
+    if (!valid) m = NEVER, l = 0.0f;  // past the count (q was taken as 0)
+    if (row >= p.rows) return;
+    if (p.splits > 1) {
+        const int64_t at = ((int64_t)blockIdx.y * p.bh + bh) * p.rows + row;
+        if (half == 0) p.part_ml[at] = make_float2(m, l);
+        float* dst = p.part_o + at * D;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dst[(8 * (r / 4) + 4 * half + r % 4) * DT + d] = acc[d][r];
+        return;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int64_t hq = h * p.group + head;
+    elem* dst = (elem*)p.o + z * p.os[0] + hq * p.os[1] + tok * p.os[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        elem* at = dst + (8 * (r / 4) + 4 * half + r % 4) * DT;
+        if constexpr (DT == 1) {
+            *at = (elem)(l == 0.0f ? 0.0f : acc[0][r] * inv);
+        } else {
+#pragma unroll
+            for (int d = 0; d < DT; d += 2)
+                ((uint32_t*)at)[d / 2] = l == 0.0f ? 0u : pack2<T>(acc[d][r] * inv, acc[d + 1][r] * inv);
+        }
+    }
+    if (half == 0) {
+        const float lse2 = l == 0.0f ? -INFINITY : m + __builtin_amdgcn_logf(l);
+        if (p.lse) p.lse[(z * (int64_t)p.heads + hq) * p.t + tok] = lse2 * LN2;
+        if (p.row_lse) p.row_lse[(int64_t)bh * p.rows + row] = lse2;
+    }
+}
+
+// Sum of a row's parts: D / 4 lanes hold a row, four values each, and `pp` such
+// groups of a workgroup take every pp-th part of it, so that the loads of a row's
+// parts do not wait for each other.
+template <class T, int D>
+__global__ void __launch_bounds__(256) join_kernel(AttendParams p, int pp) {
+    constexpr int G = D / 4, GROUPS = 256 / G;
+    __shared__ f32x4 part[256];
+    __shared__ float2 ml[GROUPS];
+    const int lane = threadIdx.x % G, grp = threadIdx.x / G;
+    const int64_t all = (int64_t)p.bh * p.rows;
+    const int64_t id = (int64_t)blockIdx.x * (GROUPS / pp) + grp / pp;  // bh * rows + row
+    float m = NEVER, l = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    if (id < all) {
+#pragma unroll 4
+        for (int s = grp % pp; s < p.splits; s += pp) {
+            const float2 v = p.part_ml[s * all + id];
+            const f32x4 x = *(const f32x4*)(p.part_o + (s * all + id) * D + 4 * lane);
+            if (v.y == 0.0f) continue;  // no slot in this part
+            const float now = fmaxf(m, v.x);
+            const float f = __builtin_amdgcn_exp2f(m - now), g = __builtin_amdgcn_exp2f(v.x - now);
+            m = now;
+            l = l * f + v.y * g;
+            o = o * f + x * g;
+        }
+    }
+    if (pp > 1) {
+        part[threadIdx.x] = o;
+        if (lane == 0) ml[grp] = make_float2(m, l);
+        __syncthreads();
+        if (grp % pp != 0 || id >= all) return;
+        for (int i = 1; i < pp; ++i) {
+            const float2 v = ml[grp + i];
+            if (v.y == 0.0f) continue;
+            const float now = fmaxf(m, v.x);
+            const float f = __builtin_amdgcn_exp2f(m - now), g = __builtin_amdgcn_exp2f(v.x - now);
+            m = now;
+            l = l * f + v.y * g;
+            o = o * f + part[threadIdx.x + i * G] * g;
+        }
+    } else if (id >= all) {
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int bh = (int)(id / p.rows), row = (int)(id - (int64_t)bh * p.rows);
     const int z = bh / (int)p.c.h, h = bh - z * (int)p.c.h;
     const int tok = row / p.group, head = row - tok * p.group;
     const int64_t hq = h * p.group + head;
-    typename T::elem* dst = (typename T::elem*)p.o + z * p.os[0] + hq * p.os[1] + tok * p.os[2] + lane * W;
-    if (mine)
-#pragma unroll
-        for (int i = 0; i < W; ++i) dst[i] = (typename T::elem)(o[i] * inv);
+    typename T::elem* dst = (typename T::elem*)p.o + z * p.os[0] + hq * p.os[1] + tok * p.os[2] + 4 * lane;
+    *(u32x2*)dst = (u32x2){pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
     if (lane == 0) {
         const float lse2 = l == 0.0f ? -INFINITY : m + __builtin_amdgcn_logf(l);
         if (p.lse) p.lse[(z * (int64_t)p.heads + hq) * p.t + tok] = lse2 * LN2;
@@ -661,27 +957,26 @@ __global__ void __launch_bounds__(256, 2) weights_kernel(AttendParams p) {
 // Host
 // ---------------------------------------------------------------------------
 struct Plan {
-    int nb, rw;        // blocks of 16 rows a wave, waves with rows of their own
+    bool few;          // attend_kernel, with nb blocks of 16 rows
+    int nb;
     int tiles, splits;
     bool scores;       // weights from stored scores
     uint64_t part_o, part_ml, scores_at, row_lse, bytes;  // offsets into the workspace
 };
 
-// Rows up to 32 share their keys among the four waves of a workgroup; more give
-// each wave 32 rows of its own.
 Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
     Plan p{};
     const int64_t group = a->heads / a->cache.h, rows = group * a->t;
     const int64_t bh = a->cache.z * a->cache.h;
     const int64_t most = a->max_length > 0 && a->max_length < a->cache.capacity ? a->max_length : a->cache.capacity;
     const bool few = rows <= 16 || (rows <= 32 && a->cache.head_dim <= 128);
-    p.nb = rows <= 16 || (!few && a->cache.head_dim == 256) ? 1 : 2;
-    p.rw = few ? 1 : 4;
-    const int per = p.rw * p.nb * 16;
-    p.tiles = (int)((rows + per - 1) / per);
+    p.few = few;
+    p.nb = rows <= 16 ? 1 : 2;
+    p.tiles = few ? 1 : (int)((rows + 127) / 128);
     // enough workgroups for the chip, of at least four steps each
-    const int64_t step = TILE * (4 / p.rw);
-    const int64_t want = (4 * (int64_t)cus + bh * p.tiles - 1) / (bh * p.tiles);
+    const int64_t step = few ? 4 * TILE : 64;
+    const int64_t full = few ? 4 * (int64_t)cus : 2 * (int64_t)cus;
+    const int64_t want = (full + bh * p.tiles - 1) / (bh * p.tiles);
     const int64_t able = (most + 4 * step - 1) / (4 * step);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, able), 256));
     p.scores = a->accumulate && few;
@@ -710,13 +1005,12 @@ int cus_of_current_device() {
 
 template <class T, int D, bool CAUSAL>
 const void* attend_fn(const Plan& p) {
-    if (p.rw == 1) {
+    if (p.few) {
         if constexpr (D <= 128)
-            if (p.nb == 2) return (const void*)&attend_kernel<T, D, 2, 1, CAUSAL>;
-        return (const void*)&attend_kernel<T, D, 1, 1, CAUSAL>;
+            if (p.nb == 2) return (const void*)&attend_kernel<T, D, 2, CAUSAL>;
+        return (const void*)&attend_kernel<T, D, 1, CAUSAL>;
     }
-    if constexpr (D <= 128) return (const void*)&attend_kernel<T, D, 2, 4, CAUSAL>;
-    else return (const void*)&attend_kernel<T, D, 1, 4, CAUSAL>;
+    return (const void*)&attend_many_kernel<T, D, CAUSAL>;
 }
 
 struct Functions {
@@ -784,7 +1078,8 @@ int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
     p.most = (int32_t)(a->max_length > 0 && a->max_length < a->cache.capacity ? a->max_length : a->cache.capacity);
     p.bh = (int32_t)(a->cache.z * a->cache.h);
     p.splits = plan.splits;
-    p.scale = __builtin_fabsf(a->sm_scale) * LOG2E;
+    // (a scale of 0 would make a hidden score -inf * 0; at FLT_MIN the others still have weights of 1)
+    p.scale = std::max(__builtin_fabsf(a->sm_scale) * LOG2E, FLT_MIN);
     p.neg = a->sm_scale < 0.0f ? 0x80008000u : 0u;
     char* ws = (char*)a->workspace;
     if (plan.splits > 1) {
@@ -805,7 +1100,12 @@ int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
         return RSFA_E_LAUNCH;
     if (plan.splits > 1) {
         const int64_t rows = (int64_t)p.bh * p.rows;
-        if (hipLaunchKernel(fn.join, dim3((unsigned)((rows + 3) / 4)), dim3(256), args, 0, (hipStream_t)stream) != hipSuccess)
+        const int groups = 256 / (int)(a->cache.head_dim / 4);
+        int pp = 1;
+        while (pp < groups && pp < plan.splits) pp *= 2;
+        void* join_args[] = {&p, &pp};
+        const int64_t per = groups / pp;
+        if (hipLaunchKernel(fn.join, dim3((unsigned)((rows + per - 1) / per)), dim3(256), join_args, 0, (hipStream_t)stream) != hipSuccess)
             return RSFA_E_LAUNCH;
     }
     if (a->accumulate) {
