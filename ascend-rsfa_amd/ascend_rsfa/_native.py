@@ -191,7 +191,8 @@ class Cache4EvictArgs(ctypes.Structure):
         ("recent", ctypes.c_int64),
         ("sinks", ctypes.c_int64),
         ("out", ctypes.c_void_p),
-        ("out_bytes", ctypes.c_uint64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
     ]
 
 
@@ -210,6 +211,7 @@ SIGNATURES = {
     "rsfa_cache4_attend_workspace_bytes": (ctypes.c_uint64, [ctypes.POINTER(Cache4AttendArgs)]),
     "rsfa_cache4_claim": (ctypes.c_int, [ctypes.POINTER(Cache4EvictArgs), ctypes.c_void_p]),
     "rsfa_cache4_evict": (ctypes.c_int, [ctypes.POINTER(Cache4EvictArgs), ctypes.c_void_p]),
+    "rsfa_cache4_evict_workspace_bytes": (ctypes.c_uint64, [ctypes.POINTER(Cache4EvictArgs), _I32]),
     "rsfa_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "rsfa_abi_version": (ctypes.c_int, []),
 }

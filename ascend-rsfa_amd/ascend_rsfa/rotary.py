@@ -19,6 +19,7 @@ stream of the tensors' device; there is no other path.
 """
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -29,6 +30,22 @@ __all__ = ["RotaryPlan", "rotary_plan", "rotary", "rotary_"]
 
 _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16, torch.float32: _native.DTYPE_F32}
 _LAYOUTS = ("half", "interleaved")
+
+# A call's argument struct is joined from parts that its tensors' shapes settle, kept with
+# the plan, and packed addresses.
+_X, _Z, _POS, _POS_STRIDE, _START, _TURNS = (
+    getattr(_native.RotaryArgs, f).offset for f in ("x", "z", "positions", "pos_stride", "start", "turns"))
+_XY, _ONE, _NUMBER = struct.Struct("=4Q"), struct.Struct("=Q"), struct.Struct("=q")
+assert _Z - _X == _XY.size and _POS_STRIDE - _POS == _ONE.size and _TURNS - _START == _NUMBER.size
+_FUNCTION = None
+
+
+def _function():
+    """rsfa_rotary, taking its argument struct's bytes."""
+    global _FUNCTION
+    if _FUNCTION is None:
+        _FUNCTION = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)(("rsfa_rotary", _native.lib()))
+    return _FUNCTION
 
 
 class RotaryPlan:
@@ -47,6 +64,7 @@ class RotaryPlan:
         self.amplitude = float(amplitude)
         self.rotary_dim = 2 * f.numel()
         self._turns = {}
+        self._kept = {}
 
     def turns(self, device):
         """Turns a position of each pair, on `device`."""
@@ -112,8 +130,14 @@ def _like(x):
     return y if y.stride(3) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
-def _launch(xs, ys, positions, plan, inverse):
-    """ys[i] = xs[i] turned; xs: one or two tensors that passed the checks."""
+def _key(q, k, positions, inverse):
+    """What a call's argument struct depends on, but for addresses."""
+    return (q.shape, q.stride(), q.dtype, q.device, None if k is None else (k.shape, k.stride(), k.dtype, k.device),
+            None if isinstance(positions, int) else (positions.shape, positions.stride(), positions.dtype, positions.device),
+            inverse)
+
+
+def _parts(xs, ys, positions, plan, inverse):
     x = xs[0]
     Z, _, N, D = x.shape
     args = _native.RotaryArgs()
@@ -121,33 +145,37 @@ def _launch(xs, ys, positions, plan, inverse):
     args.dtype = _DTYPES[x.dtype]
     args.z, args.n, args.head_dim, args.rotary_dim = Z, N, D, plan.rotary_dim
     for i, (a, b) in enumerate(zip(xs, ys)):
-        args.x[i], args.y[i] = a.data_ptr(), b.data_ptr()
         args.heads[i] = a.shape[1]
         args.x_stride[i][:] = a.stride()
         args.y_stride[i][:] = b.stride()
     flags = (_native.ROTARY_INTERLEAVED if plan.layout == "interleaved" else 0) | (
         _native.ROTARY_INVERSE if inverse else 0)
-    if isinstance(positions, int):
-        args.start = positions
-    else:
-        args.positions = positions.data_ptr()
-        if positions.dim() == 2:
-            st = positions.stride()
-            args.pos_stride[:] = (st[0] if positions.shape[0] > 1 else 0, st[1])
-        else:
-            args.pos_stride[:] = (0, positions.stride(0))
+    if not isinstance(positions, int):
+        st = positions.stride()
+        args.pos_stride[:] = (st[0] if positions.dim() == 2 and positions.shape[0] > 1 else 0, st[-1])
         if positions.dtype == torch.int64:
             flags |= _native.ROTARY_POS64
     args.turns = plan.turns(x.device).data_ptr()
     args.amplitude = plan.amplitude
     args.flags = flags
-    dev = x.device.index
+    b = bytes(args)
+    return b[:_X], b[_Z:_POS], b[_POS_STRIDE:_START], b[_TURNS:]
+
+
+def _launch(parts, xs, ys, positions):
+    """ys[i] = xs[i] turned; xs: one or two tensors."""
+    head, sizes, strides, tail = parts
+    two = len(xs) > 1
+    start = isinstance(positions, int)
+    args = b"".join((head, _XY.pack(xs[0].data_ptr(), xs[1].data_ptr() if two else 0, ys[0].data_ptr(), ys[1].data_ptr() if two else 0),
+                     sizes, _ONE.pack(0 if start else positions.data_ptr()), strides, _NUMBER.pack(positions if start else 0), tail))
+    dev = xs[0].device.index
     stream = torch._C._cuda_getCurrentRawStream(dev)
     if dev == torch.cuda.current_device():
-        st = _native.lib().rsfa_rotary(ctypes.byref(args), stream)
+        st = _function()(args, stream)
     else:
         with torch.cuda.device(dev):
-            st = _native.lib().rsfa_rotary(ctypes.byref(args), stream)
+            st = _function()(args, stream)
     _raise_for(st)
 
 
@@ -183,12 +211,29 @@ class _Rotary(torch.autograd.Function):
 
 
 def _forward(q, k, positions, plan, inverse):
+    key = _key(q, k, positions, inverse)
+    parts = plan._kept.get(key)
+    if parts is not None:  # (tensors of this key were taken as they are)
+        y = torch.empty_like(q)
+        if k is None:
+            _launch(parts, (q,), (y,), positions)
+            return y
+        w = torch.empty_like(k)
+        _launch(parts, (q, k), (y, w), positions)
+        return y, w
+    _checked(q, k, positions, plan)
     xs = [_unit(q)] if k is None else [_unit(q), _unit(k)]
     ys = [_like(x) for x in xs]
-    if xs[0].shape[0] and xs[0].shape[2]:
-        xs_, ys_ = zip(*[(x, y) for x, y in zip(xs, ys) if x.numel()]) if any(x.numel() for x in xs) else ((), ())
-        if xs_:
-            _launch(xs_, ys_, positions, plan, inverse)
+    some = [(x, y) for x, y in zip(xs, ys) if x.numel()]
+    if some:
+        parts = _parts([x for x, _ in some], [y for _, y in some], positions, plan, inverse)
+        # kept where q and k go in as they are and empty_like gives their outputs
+        if len(some) == len(xs) and xs[0] is q and xs[-1] is (q if k is None else k) and all(
+                y.stride() == torch.empty_like(x, device="meta").stride() for x, y in some):
+            if len(plan._kept) > 1024:
+                plan._kept.clear()
+            plan._kept[key] = parts
+        _launch(parts, [x for x, _ in some], [y for _, y in some], positions)
     return ys[0] if k is None else tuple(ys)
 
 
@@ -206,6 +251,8 @@ def _checked(q, k, positions, plan):
         raise ValueError(f"the plan turns {plan.rotary_dim} values of a head; the head dim is {q.shape[3]}")
     if isinstance(positions, bool) or not isinstance(positions, (int, torch.Tensor)):
         raise TypeError("positions must be an int (the first token's) or an int32/int64 tensor [N] or [Z, N]")
+    if isinstance(positions, int) and abs(positions) >= 1 << 53:
+        raise ValueError("positions must be below 2^53")
     if isinstance(positions, torch.Tensor):
         Z, N = q.shape[0], q.shape[2]
         if positions.dtype not in (torch.int32, torch.int64):
@@ -224,7 +271,12 @@ def rotary(q, k, positions, plan):
     or [Z, N] of int32 or int64.  Differentiable in q and k: the gradient is the
     same turn backwards.
     """
-    _checked(q, k, positions, plan)
+    if not isinstance(plan, RotaryPlan):
+        raise TypeError("plan must be a RotaryPlan (rotary_plan(...))")
+    if isinstance(positions, bool) or not isinstance(positions, (int, torch.Tensor)):
+        raise TypeError("positions must be an int (the first token's) or an int32/int64 tensor [N] or [Z, N]")
+    if isinstance(positions, int) and abs(positions) >= 1 << 53:
+        raise ValueError("positions must be below 2^53")
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _Rotary.apply(q, k, positions, plan)
     return _forward(q, k, positions, plan, False)
@@ -244,5 +296,5 @@ def rotary_(q, k, positions, plan):
             raise ValueError("rotary_ cannot write to an expanded tensor")
     xs = [x for x in (q, k) if x is not None and x.numel()]
     if xs:
-        _launch(xs, xs, positions, plan, False)
+        _launch(_parts(xs, xs, positions, plan, False), xs, xs, positions)
     return q if k is None else (q, k)

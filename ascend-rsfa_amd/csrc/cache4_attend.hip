@@ -57,7 +57,8 @@ struct AttendParams {
     float* part_o;             // [splits][bh][rows][D] (splits > 1)
     float2* part_ml;           // [splits][bh][rows]: maximum (log2 units), sum
     float* scores;             // [bh][rows][most]: scores in log2 units, or null
-    float* row_lse;            // [bh][rows]: log2 of the row's sum of exp2 (weights of many rows)
+    float* row_lse;            // [bh][rows]: log2 of the row's sum of exp2 (for the weights)
+    float* part_w;             // [parts][bh][most]: sums of parts of the rows, or null
 };
 
 template <class T>
@@ -833,124 +834,190 @@ __global__ void __launch_bounds__(256) add_weights_kernel(AttendParams p) {
         float sum = 0.0f;
         for (int r = 0; r < rows; ++r) {
             const float lse2 = p.row_lse[(int64_t)bh * p.rows + r];
-            // (a row that sees no slot has -inf)
-            if (lse2 != -INFINITY) sum += __builtin_amdgcn_exp2f(p.scores[((int64_t)bh * p.rows + r) * p.most + slot] - lse2);
+            const float x = p.scores[((int64_t)bh * p.rows + r) * p.most + slot];
+            // a slot that the row does not see has -inf (and a row that sees none: in all)
+            sum += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - lse2);
         }
         w[slot] += sum;
     }
 }
 
-// Weights of many rows: the scores are computed again, now that the rows' sums
-// are known.  A workgroup holds 64 keys in registers, each wave all of them,
-// and its waves take every fourth block of 16 rows.
+// Weights of many rows: the scores are computed again, now that the rows' sums are
+// known.  Each of the workgroup's four waves holds keys of its own as operands
+// of the 32 x 32 MFMA (64 registers at D = 128, 256); blocks of 32 rows of Q pass by
+// in LDS, as operands too, two buffers of them.  A workgroup takes the row blocks
+// blockIdx.y, blockIdx.y + gridDim.y, ...
+template <int D>
+struct Weigh {
+    static constexpr int KEYS = D == 256 ? 32 : 64;  // of a wave
+    static constexpr int WG_KEYS = 4 * KEYS;
+};
+
 template <class T, int D, bool CAUSAL>
 __global__ void __launch_bounds__(256, 2) weights_kernel(AttendParams p) {
-    constexpr int KT = 4;  // tiles of 16 keys
-    constexpr int QS = D / 32;
     typedef typename T::x8 x8;
     typedef typename T::elem elem;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int col = lane & 15, grp = lane >> 4;
+    constexpr int QS = D / 16, KEYS = Weigh<D>::KEYS, SB = KEYS / 32;
+    constexpr int QF = (QS + 3) / 4;  // fragments of Q a wave brings
+    __shared__ u32x4 frag[2][QS][64];
+    __shared__ int kpos[CAUSAL ? 4 * KEYS : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
     const int bh = blockIdx.x % p.bh;
     const int z = bh / (int)p.c.h, h = bh - z * (int)p.c.h;
-    const int len = length_of(p.lengths, p.length, z, p.most);
+    const int len = __builtin_amdgcn_readfirstlane(length_of(p.lengths, p.length, z, p.most));
     const int count = p.counts ? max(0, min(p.counts[z], p.t)) : p.t;
-    const int64_t tile = (int64_t)(blockIdx.x / p.bh) * (16 * KT);
-    if (tile >= len) return;
+    const int rows = count * p.group;
+    const int64_t wg_tile = (int64_t)(blockIdx.x / p.bh) * Weigh<D>::WG_KEYS;
+    if (wg_tile >= len) return;
+    const int tile = (int)wg_tile + KEYS * wave;  // (may lie past the length: its keys repeat the last)
     const uint8_t* kc = p.c.k_codes + z * p.c.code_stride[0] + h * p.c.code_stride[1];
     const uint8_t* ks = p.c.k_scales + z * p.c.scale_stride[0] + h * p.c.scale_stride[1];
     const int32_t* pos = p.c.positions + z * p.c.slot_stride[0] + h * p.c.slot_stride[1];
-    x8 k[KT][QS];
-    int kpos[CAUSAL ? KT : 1][4];
-    int far = -0x7fffffff - 1, near = 0x7fffffff;
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-        const int key = (int)min(tile + 16 * t + col, (int64_t)len - 1);
-        const uint8_t* s = ks + (int64_t)key * (D / 32);
-        uint32_t sw;
-        if constexpr (D == 256) sw = *(const uint16_t*)(s + 2 * grp);
-        else sw = s[grp * (D / 4) / 32];
-        const float sc0 = scale_bits(sw, 0), sc1 = scale_bits(sw, 1);
-#pragma unroll
-        for (int i = 0; i < QS; ++i) {
-            const uint32_t w = *(const uint32_t*)(kc + (int64_t)key * (D / 2) + grp * (D / 8) + 4 * i);
-            const float sc = D == 256 && i >= 4 ? sc1 : sc0;
-            const u32x4 kv = {T::template cvt<0>(w, sc), T::template cvt<1>(w, sc), T::template cvt<2>(w, sc),
-                              T::template cvt<3>(w, sc)};
-            k[t][i] = __builtin_bit_cast(x8, kv);
-        }
-        if (CAUSAL)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int v = pos[min(tile + 16 * t + 4 * grp + r, (int64_t)len - 1)];
-                kpos[t][r] = v;
-                far = max(far, v);
-                near = min(near, v);
-            }
-    }
+    int far = -0x7fffffff - 1, near = 0x7fffffff;  // positions of the wave's keys
     if (CAUSAL) {
+        const int v = pos[min(tile + (lane & (KEYS - 1)), len - 1)];
+        kpos[KEYS * wave + (lane & (KEYS - 1))] = v;
+        far = near = v;
 #pragma unroll
-        for (int d = 16; d < 64; d <<= 1) {
+        for (int d = 1; d < 64; d <<= 1) {
             far = max(far, __shfl_xor(far, d));
             near = min(near, __shfl_xor(near, d));
         }
     }
-    float sum[KT][4] = {};
-    const int64_t first = CAUSAL ? (p.pos_start ? (int64_t)p.pos_start[z] : (int64_t)len - count) : 0;
-    const int rows = count * p.group;
-    for (int row0 = 16 * wave; row0 < rows; row0 += 64) {
-        const int row = row0 + col;
-        const int tok = min(row, rows - 1) / p.group, head = min(row, rows - 1) - tok * p.group;
-        int qpos = 0;
-        bool masked = row0 + 16 > rows;
-        if (CAUSAL) {
-            const int64_t at = first + tok;
-            qpos = (int)(at > 0x7fffffff ? 0x7fffffff : at);
-            // the block's rows have positions that grow with the row
-            const int64_t lo = first + row0 / p.group, hi = first + (min(row0 + 16, rows) - 1) / p.group;
-            if (near > hi) continue;
-            masked |= far > lo;
-        }
-        const float lse2 = row < rows ? p.row_lse[(int64_t)bh * p.rows + row] : -INFINITY;
-        masked |= __any(lse2 == -INFINITY);
-        const elem* src = (const elem*)p.q + z * p.qs[0] + (int64_t)(h * p.group + head) * p.qs[1] + tok * p.qs[2] + grp * (D / 4);
-        x8 q[QS];
+    x8 k[SB][QS];
+#pragma unroll
+    for (int b = 0; b < SB; ++b) {
+        const int key = min(tile + 32 * b + col, len - 1);
+        const uint8_t* src = kc + (int64_t)key * (D / 2) + half * (D / 4);
+        const uint8_t* s = ks + (int64_t)key * (D / 32);
 #pragma unroll
         for (int i = 0; i < QS; ++i) {
-            u32x4 w = *(const u32x4*)(src + 8 * i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] ^= p.neg;
-            q[i] = __builtin_bit_cast(x8, w);
+            const uint32_t w = *(const uint32_t*)(src + 4 * i);
+            const float sc = scale_bits(s[(half * (D / 2) + 8 * i) / 32], 0);
+            const u32x4 kv = {T::template cvt<0>(w, sc), T::template cvt<1>(w, sc), T::template cvt<2>(w, sc),
+                              T::template cvt<3>(w, sc)};
+            k[b][i] = __builtin_bit_cast(x8, kv);
         }
+    }
+    const int64_t first = CAUSAL ? (p.pos_start ? (int64_t)p.pos_start[z] : (int64_t)len - count) : 0;
+    const elem* qb = (const elem*)p.q + z * p.qs[0] + (int64_t)h * p.group * p.qs[1];
+    u32x4 raw[QF];
+    float lse_next = 0.0f;
+    auto load = [&](int row0) {
+        const int row = row0 + col, at = min(row, rows - 1);
+        const int tok = at / p.group, head = at - tok * p.group;
+        const elem* src = qb + head * p.qs[1] + tok * p.qs[2] + half * (D / 2);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            f32x4 s = {0, 0, 0, 0};
+        for (int i = 0; i < QF; ++i)
+            if (QS >= 4 || wave < QS) {
+                raw[i] = *(const u32x4*)(src + 8 * (wave * QF + i));
+                if (row >= rows) raw[i] = (u32x4){0, 0, 0, 0};
+            }
+        // rows past the last and rows that see no slot: exp2 of -inf
+        lse_next = row < rows ? p.row_lse[(int64_t)bh * p.rows + row] : INFINITY;
+        if (lse_next == -INFINITY) lse_next = INFINITY;
+    };
+    auto store = [&](int buf) {
 #pragma unroll
-            for (int i = 0; i < QS; ++i) s = T::mfma(k[t][i], q[i], s);
+        for (int i = 0; i < QF; ++i)
+            if (QS >= 4 || wave < QS) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float x = __builtin_amdgcn_exp2f(s[r] * p.scale - lse2);
-                if (masked) x = lse2 == -INFINITY || (CAUSAL && kpos[t][r] > qpos) ? 0.0f : x;
-                sum[t][r] += x;
+                for (int j = 0; j < 4; ++j) raw[i][j] ^= p.neg;
+                frag[buf][wave * QF + i][lane] = raw[i];
+            }
+    };
+    float sum[SB][16];
+#pragma unroll
+    for (int b = 0; b < SB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[b][r] = 0.0f;
+
+    const int step = 32 * gridDim.y;
+    int row0 = 32 * blockIdx.y;
+    if (row0 < rows) {
+        load(row0);
+        store(0);
+        float lse2 = lse_next;
+        if (row0 + step < rows) load(row0 + step);
+        int buf = 0;
+        for (; row0 < rows; row0 += step, buf ^= 1) {
+            __syncthreads();
+            const float lse_now = lse2;
+            if (row0 + step < rows) {
+                store(buf ^ 1);
+                lse2 = lse_next;
+            }
+            if (row0 + 2 * step < rows) load(row0 + 2 * step);
+            bool masked = __any(lse_now == INFINITY);
+            int qpos = 0;
+            if (CAUSAL) {
+                // the block's rows have positions that grow with the row
+                const int64_t lo = first + row0 / p.group, hi = first + (min(row0 + 32, rows) - 1) / p.group;
+                if (near > hi) continue;
+                masked |= far > lo;
+                if (masked) {
+                    const int64_t at = first + min(row0 + col, rows - 1) / p.group;
+                    qpos = (int)(at > 0x7fffffff ? 0x7fffffff : at);
+                }
+            }
+            f32x16 s[SB];
+#pragma unroll
+            for (int b = 0; b < SB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < QS; ++i) {
+                const x8 q = __builtin_bit_cast(x8, frag[buf][i][lane]);
+#pragma unroll
+                for (int b = 0; b < SB; ++b) s[b] = mfma32(k[b][i], q, s[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < SB; ++b) {
+                if (__builtin_expect(masked, 0)) {
+                    // (chosen after the exponential: a row whose sum is NaN adds nothing to slots it does not see)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        bool hidden = lse_now == INFINITY;
+                        if (CAUSAL) hidden |= kpos[KEYS * wave + 32 * b + 8 * (r / 4) + 4 * half + r % 4] > qpos;
+                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], p.scale, -lse_now));
+                        sum[b][r] += hidden ? 0.0f : x;
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        sum[b][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], p.scale, -lse_now));
+                }
             }
         }
     }
-    __shared__ float total[4][16 * KT];
+    float* out = p.part_w ? p.part_w + ((int64_t)blockIdx.y * p.bh + bh) * p.most
+                          : p.c.weights + z * p.c.slot_stride[0] + h * p.c.slot_stride[1];
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
+    for (int b = 0; b < SB; ++b)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float v = sum[t][r];
+        for (int r = 0; r < 16; ++r) {
+            float v = sum[b][r];
 #pragma unroll
-            for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
-            if (col == 0) total[wave][16 * t + 4 * grp + r] = v;
+            for (int d = 1; d < 32; d <<= 1) v += __shfl_xor(v, d);
+            const int key = tile + 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+            if (col == 0 && key < len) {
+                if (p.part_w) out[key] = v;
+                else out[key] += v;
+            }
         }
-    __syncthreads();
-    const int i = threadIdx.x;
-    if (i < 16 * KT && tile + i < len) {
-        float* w = p.c.weights + z * p.c.slot_stride[0] + h * p.c.slot_stride[1];
-        w[tile + i] += (total[0][i] + total[1][i]) + (total[2][i] + total[3][i]);
-    }
+}
+
+// The sums of weights_kernel's parts, where the rows were split.
+__global__ void __launch_bounds__(256) join_weights_kernel(AttendParams p, int parts) {
+    const int bh = blockIdx.x % p.bh;
+    const int z = bh / (int)p.c.h, h = bh - z * (int)p.c.h;
+    const int64_t slot = (int64_t)(blockIdx.x / p.bh) * 256 + threadIdx.x;
+    if (slot >= length_of(p.lengths, p.length, z, p.most)) return;
+    float v = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) v += p.part_w[((int64_t)i * p.bh + bh) * p.most + slot];
+    p.c.weights[z * p.c.slot_stride[0] + h * p.c.slot_stride[1] + slot] += v;
 }
 
 // ---------------------------------------------------------------------------
@@ -961,6 +1028,8 @@ struct Plan {
     int nb;
     int tiles, splits;
     bool scores;       // weights from stored scores
+    int weight_tiles, weight_parts;
+    uint64_t part_w;
     uint64_t part_o, part_ml, scores_at, row_lse, bytes;  // offsets into the workspace
 };
 
@@ -992,6 +1061,14 @@ Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
     }
     if (a->accumulate) p.row_lse = take((uint64_t)bh * rows * 4);
     if (p.scores) p.scores_at = take((uint64_t)bh * rows * most * 4);
+    const int wg_keys = p.scores ? 1024 : a->cache.head_dim == 256 ? Weigh<256>::WG_KEYS : Weigh<128>::WG_KEYS;
+    p.weight_tiles = (int)((most + wg_keys - 1) / wg_keys);
+    p.weight_parts = 1;
+    if (a->accumulate && !p.scores) {
+        const int64_t fill = (2 * (int64_t)cus + bh * p.weight_tiles - 1) / (bh * p.weight_tiles);
+        p.weight_parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(fill, rows / 128), 64));
+        if (p.weight_parts > 1) p.part_w = take((uint64_t)p.weight_parts * bh * most * 4);
+    }
     p.bytes = at;
     return p;
 }
@@ -1092,9 +1169,9 @@ int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
     const Functions fn = a->cache.dtype == RSFA_DTYPE_BF16 ? functions<BF16>(plan, causal, a->cache.head_dim)
                                                            : functions<F16>(plan, causal, a->cache.head_dim);
     const int64_t grid = (int64_t)p.bh * plan.tiles;
-    const int64_t slots = plan.scores ? 1024 : 64;
-    const int64_t weight_grid = (int64_t)p.bh * ((p.most + slots - 1) / slots);
-    if (grid > 0x7fffffff || (a->accumulate && weight_grid > 0x7fffffff)) return RSFA_E_CACHE;
+    const int64_t weight_grid = (int64_t)p.bh * plan.weight_tiles;
+    const int64_t join_grid = (int64_t)p.bh * ((p.most + 255) / 256);
+    if (grid > 0x7fffffff || (a->accumulate && join_grid > 0x7fffffff)) return RSFA_E_CACHE;
     void* args[] = {&p};
     if (hipLaunchKernel(fn.attend, dim3((unsigned)grid, (unsigned)plan.splits), dim3(256), args, 0, (hipStream_t)stream) != hipSuccess)
         return RSFA_E_LAUNCH;
@@ -1110,8 +1187,15 @@ int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
     }
     if (a->accumulate) {
         const void* f = plan.scores ? (const void*)&add_weights_kernel : fn.weights;
-        if (hipLaunchKernel(f, dim3((unsigned)weight_grid), dim3(256), args, 0, (hipStream_t)stream) != hipSuccess)
+        if (plan.weight_parts > 1) p.part_w = (float*)(ws + plan.part_w);
+        if (hipLaunchKernel(f, dim3((unsigned)weight_grid, (unsigned)plan.weight_parts), dim3(256), args, 0, (hipStream_t)stream) != hipSuccess)
             return RSFA_E_LAUNCH;
+        if (plan.weight_parts > 1) {
+            int parts = plan.weight_parts;
+            void* join_args[] = {&p, &parts};
+            if (hipLaunchKernel((const void*)&join_weights_kernel, dim3((unsigned)join_grid), dim3(256), join_args, 0, (hipStream_t)stream) != hipSuccess)
+                return RSFA_E_LAUNCH;
+        }
     }
     return RSFA_OK;
 }

@@ -348,7 +348,9 @@ uint64_t rsfa_cache4_attend_workspace_bytes(const rsfa_cache4_attend_args *args)
  * evict: copies to `into` (same z, h, head_dim and dtype; not the same memory) the
  * slots that stay when the first max(0, lengths[z] - budget) go (protected ones
  * after all others), in order of slot, to its slots 0, 1, ...; other slots of `into`
- * keep what they hold.  Workspace: z * h * budget int32. */
+ * keep what they hold.
+ * Workspace: rsfa_cache4_evict_workspace_bytes of the same arguments (evict: 1
+ * for evict, 0 for claim; 0 bytes for claims in caches of up to 8192 slots). */
 typedef struct rsfa_cache4_evict_args {
     uint32_t       struct_size; /* = sizeof(rsfa_cache4_evict_args)            */
     uint32_t       reserved;    /* 0 */
@@ -358,12 +360,14 @@ typedef struct rsfa_cache4_evict_args {
     int64_t        length;
     int64_t        n;           /* claim only                                  */
     int64_t        budget, recent, sinks;
-    int32_t       *out;         /* claim: the slots; evict: the workspace      */
-    uint64_t       out_bytes;
+    int32_t       *out;         /* claim only: the slots                       */
+    void          *workspace;   /* 16-byte aligned */
+    uint64_t       workspace_bytes;
 } rsfa_cache4_evict_args;
 
 int rsfa_cache4_claim(const rsfa_cache4_evict_args *args, void *stream);
 int rsfa_cache4_evict(const rsfa_cache4_evict_args *args, void *stream);
+uint64_t rsfa_cache4_evict_workspace_bytes(const rsfa_cache4_evict_args *args, int32_t evict);
 
 /* Static string for a status code. */
 const char *rsfa_strerror(int status);

@@ -101,6 +101,7 @@ def attend(q, k, v, lengths, scale, positions=None, first=None, counts=None):
                 hidden = torch.zeros((t, n), dtype=torch.bool, device=q.device)
             m = torch.logsumexp(s, -1)
             p = torch.where(torch.isinf(m)[..., None] & (m < 0)[..., None], torch.zeros_like(s), torch.exp(s - m[..., None]))
+            p = p.masked_fill(hidden, 0.0)
             # a hidden row's values never reach a query, whatever they are
             for i in range(t):
                 seen = ~hidden[i]

@@ -311,8 +311,10 @@ def test_non_finite_rows_reach_only_the_queries_that_see_them(D, T):
     # a NaN block of V and of K among the last tokens: seen by the later queries only
     cache.v_scales[0, 0, 100 - (T + 1) // 2, D // 32 - 1] = 255
     cache.k_scales[0, 1, 100 - (T + 1) // 2, 0] = 255
+    cache.positions[:, :, 5:9] = 1000  # seen by no query
     before = cache.weights.clone()
     got = cache.attend(q, 100, True, 0.1, accumulate=True, return_lse=True)
+    assert torch.equal(cache.weights[:, :, 5:9], before[:, :, 5:9])
     o = got[0]
     seen = T - (T + 1) // 2  # the first query token that sees it
     assert torch.isnan(o[0, :2, seen:, D - 32:]).all() and torch.isfinite(o[0, :2, :, :D - 32]).all()
@@ -427,7 +429,7 @@ def _weights(shape, seed, kind):
 
 
 @pytest.mark.parametrize("kind", ["spread", "ties", "zeros", "odd"])
-@pytest.mark.parametrize("C", [1, 5, 64, 2048, 2100, 9000])
+@pytest.mark.parametrize("C", [1, 5, 64, 2048, 2100, 8192, 8193, 40000])
 def test_claim_matches_the_definition(C, kind):
     Z, H = 3, 2
     cache = Cache4(Z, H, C, 32)

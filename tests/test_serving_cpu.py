@@ -15,7 +15,7 @@ def test_struct_layouts():
     assert ctypes.sizeof(_native.Cache4) == 48 + 32 + 48 + 8
     assert ctypes.sizeof(_native.Cache4RowsArgs) == 8 + 136 + 24 + 64 + 40
     assert ctypes.sizeof(_native.Cache4AttendArgs) == 8 + 136 + 24 + 16 + 64 + 24 + 16 + 8 + 16
-    assert ctypes.sizeof(_native.Cache4EvictArgs) == 8 + 272 + 16 + 32 + 16
+    assert ctypes.sizeof(_native.Cache4EvictArgs) == 8 + 272 + 16 + 32 + 24
 
 
 def test_strerror_covers_the_new_codes():
@@ -153,7 +153,7 @@ def _evict(cache=None, into=None, **over):
     a.cache = cache if cache is not None else _cache()
     a.into = into if into is not None else _cache(capacity=16)
     a.length, a.n, a.budget, a.recent, a.sinks = 40, 4, 16, 4, 2
-    a.out, a.out_bytes = 0x1000, 1 << 20
+    a.out, a.workspace, a.workspace_bytes = 0x1000, 0x1000, 1 << 20
     for k, v in over.items():
         setattr(a, k, v)
     return a
@@ -207,7 +207,17 @@ def test_cache_calls_abi_refusals():
         assert e(_cache(weights=None)) == _native.E_NULL
         assert e(budget=0) == e(budget=41) == e(recent=-1) == e(sinks=-1) == _native.E_BUDGET
         assert e(recent=15) == e(recent=1 << 62) == e(sinks=1 << 62) == _native.E_BUDGET
-        assert e(out=0x1002) == _native.E_ALIGN and e(out_bytes=8) == _native.E_WORKSPACE
+        assert e(out=0x1002) == _native.E_ALIGN
     assert lib.rsfa_cache4_claim(ctypes.byref(_evict(n=0)), None) == _native.E_BUDGET
+    need = lib.rsfa_cache4_evict_workspace_bytes(ctypes.byref(_evict()), 1)
+    assert need >= 2 * 3 * 16 * 4 and lib.rsfa_cache4_evict_workspace_bytes(ctypes.byref(_evict()), 0) == 0
+    assert lib.rsfa_cache4_evict_workspace_bytes(ctypes.byref(_evict(budget=0)), 1) == 0
+    long = {"capacity": 9000, "code_stride": (ctypes.c_int64 * 2)(3 * 9000 * 64, 9000 * 64)}
+    assert lib.rsfa_cache4_evict_workspace_bytes(ctypes.byref(_evict(_cache(**long))), 0) > 0
+    assert lib.rsfa_cache4_claim(ctypes.byref(_evict(out=None)), None) == _native.E_NULL
+    for make, fn in ((lambda **k: _evict(**k), lib.rsfa_cache4_evict), (lambda **k: _evict(_cache(**long), **k), lib.rsfa_cache4_claim)):
+        for over in ({"workspace": None}, {"workspace_bytes": 8}):
+            assert fn(ctypes.byref(make(**over)), None) == _native.E_WORKSPACE
+        assert fn(ctypes.byref(make(workspace=0x1008)), None) == _native.E_ALIGN
     for over in ({"z": 1}, {"h": 2}, {"head_dim": 64}, {"dtype": 1}, {"capacity": 15}):
         assert lib.rsfa_cache4_evict(ctypes.byref(_evict(into=_cache(**{"capacity": 16, **over}))), None) == _native.E_BUDGET
