@@ -74,6 +74,7 @@ __device__ __forceinline__ float scale_bits(uint32_t w, int byte) {
 }
 
 typedef u32x4 u32x4_u __attribute__((aligned(4)));  // loads need the alignment of a dword
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
 
 template <int BYTES>
 struct Bytes;
@@ -429,9 +430,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
         const int row = 16 * b + col;
         if (row >= p.rows) continue;
         const int tok = row / p.group, head = row - tok * p.group;
+        const int64_t at = ((int64_t)split * p.bh + bh) * p.rows + row;
+        if (grp == 0 && p.part_ml) p.part_ml[at] = make_float2(m[b], l[b]);
         if (p.splits > 1) {
-            const int64_t at = ((int64_t)split * p.bh + bh) * p.rows + row;
-            if (grp == 0) p.part_ml[at] = make_float2(m[b], l[b]);
             float* dst = p.part_o + at * D;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -767,26 +768,35 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
 // groups of a workgroup take every pp-th part of it, so that the loads of a row's
 // parts do not wait for each other.
 template <class T, int D>
-__global__ void __launch_bounds__(256) join_kernel(AttendParams p, int pp) {
+__device__ __forceinline__ void join_rows(const AttendParams& p, int pp, int block) {
     constexpr int G = D / 4, GROUPS = 256 / G;
     __shared__ f32x4 part[256];
     __shared__ float2 ml[GROUPS];
     const int lane = threadIdx.x % G, grp = threadIdx.x / G;
     const int64_t all = (int64_t)p.bh * p.rows;
-    const int64_t id = (int64_t)blockIdx.x * (GROUPS / pp) + grp / pp;  // bh * rows + row
+    const int64_t id = (int64_t)block * (GROUPS / pp) + grp / pp;  // bh * rows + row
     float m = NEVER, l = 0.0f;
     f32x4 o = {0, 0, 0, 0};
     if (id < all) {
-#pragma unroll 4
-        for (int s = grp % pp; s < p.splits; s += pp) {
-            const float2 v = p.part_ml[s * all + id];
-            const f32x4 x = *(const f32x4*)(p.part_o + (s * all + id) * D + 4 * lane);
-            if (v.y == 0.0f) continue;  // no slot in this part
-            const float now = fmaxf(m, v.x);
-            const float f = __builtin_amdgcn_exp2f(m - now), g = __builtin_amdgcn_exp2f(v.x - now);
-            m = now;
-            l = l * f + v.y * g;
-            o = o * f + x * g;
+        constexpr int U = 8;  // parts whose loads are under way together
+        for (int s0 = grp % pp; s0 < p.splits; s0 += U * pp) {
+            float2 v[U];
+            f32x4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int s = min(s0 + u * pp, p.splits - 1);
+                v[u] = p.part_ml[s * all + id];
+                x[u] = *(const f32x4*)(p.part_o + (s * all + id) * D + 4 * lane);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (s0 + u * pp >= p.splits || v[u].y == 0.0f) continue;  // (0: no slot in this part)
+                const float now = fmaxf(m, v[u].x);
+                const float f = __builtin_amdgcn_exp2f(m - now), g = __builtin_amdgcn_exp2f(v[u].x - now);
+                m = now;
+                l = l * f + v[u].y * g;
+                o = o * f + x[u] * g;
+            }
         }
     }
     if (pp > 1) {
@@ -820,26 +830,71 @@ __global__ void __launch_bounds__(256) join_kernel(AttendParams p, int pp) {
     }
 }
 
-// Weights of few rows: from their scores and sums.  A thread takes four slots.
-__global__ void __launch_bounds__(256) add_weights_kernel(AttendParams p) {
-    const int bh = blockIdx.x % p.bh;
+// Weights of up to 32 rows, from their scores and their parts' sums; a thread takes
+// four slots, a workgroup 1024.
+__device__ __forceinline__ void add_weights(const AttendParams& p, int block) {
+    __shared__ float sums[32];
+    const int bh = block % p.bh;
     const int z = bh / (int)p.c.h, h = bh - z * (int)p.c.h;
     const int len = length_of(p.lengths, p.length, z, p.most);
     const int count = p.counts ? max(0, min(p.counts[z], p.t)) : p.t;
     const int rows = count * p.group;
-    float* w = p.c.weights + z * p.c.slot_stride[0] + h * p.c.slot_stride[1];
-    for (int i = 0; i < 4; ++i) {
-        const int64_t slot = (int64_t)(blockIdx.x / p.bh) * 1024 + 256 * i + threadIdx.x;
-        if (slot >= len) return;
-        float sum = 0.0f;
-        for (int r = 0; r < rows; ++r) {
-            const float lse2 = p.row_lse[(int64_t)bh * p.rows + r];
-            const float x = p.scores[((int64_t)bh * p.rows + r) * p.most + slot];
-            // a slot that the row does not see has -inf (and a row that sees none: in all)
-            sum += x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - lse2);
+    const int64_t first = (int64_t)(block / p.bh) * 1024;
+    if (first >= len) return;
+    {
+        // eight lanes a row: log2 of its sum
+        const int row = threadIdx.x / 8;
+        const int64_t all = (int64_t)p.bh * p.rows, id = (int64_t)bh * p.rows + row;
+        float m = NEVER, l = 0.0f;
+        if (row < rows) {
+            for (int s = threadIdx.x % 8; s < p.splits; s += 8) {
+                const float2 v = p.part_ml[s * all + id];
+                if (v.y == 0.0f) continue;
+                const float now = fmaxf(m, v.x);
+                l = l * __builtin_amdgcn_exp2f(m - now) + v.y * __builtin_amdgcn_exp2f(v.x - now);
+                m = now;
+            }
         }
-        w[slot] += sum;
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) {
+            const float m2 = __shfl_xor(m, d), l2 = __shfl_xor(l, d);
+            const float now = fmaxf(m, m2);
+            l = l * __builtin_amdgcn_exp2f(m - now) + l2 * __builtin_amdgcn_exp2f(m2 - now);
+            m = now;
+        }
+        if (threadIdx.x % 8 == 0) sums[row] = l == 0.0f ? -INFINITY : m + __builtin_amdgcn_logf(l);
     }
+    __syncthreads();
+    const int64_t slot = first + 4 * threadIdx.x;
+    if (slot >= len) return;
+    float* w = p.c.weights + z * p.c.slot_stride[0] + h * p.c.slot_stride[1] + slot;
+    const float* x = p.scores + (int64_t)bh * p.rows * p.most + slot;
+    // a slot that the row does not see has a score of -inf (and a row that sees none: in all)
+    auto weight = [](float s, float sum) { return s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - sum); };
+    if (slot + 4 <= len) {
+        f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r) {
+            const f32x4 s = *(const f32x4_u*)(x + (int64_t)r * p.most);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] += weight(s[i], sums[r]);
+        }
+        *(f32x4_u*)w = *(const f32x4_u*)w + sum;
+    } else {
+        for (int i = 0; slot + i < len; ++i) {
+            float sum = 0.0f;
+            for (int r = 0; r < rows; ++r) sum += weight(x[(int64_t)r * p.most + i], sums[r]);
+            w[i] += sum;
+        }
+    }
+}
+
+// What follows attend_kernel or attend_many_kernel: the first join_blocks workgroups
+// join parts, the others add weights.
+template <class T, int D>
+__global__ void __launch_bounds__(256) finish_kernel(AttendParams p, int pp, int join_blocks) {
+    if ((int)blockIdx.x < join_blocks) join_rows<T, D>(p, pp, blockIdx.x);
+    else add_weights(p, blockIdx.x - join_blocks);
 }
 
 // Weights of many rows: the scores are computed again, now that the rows' sums are
@@ -1042,9 +1097,12 @@ Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
     p.few = few;
     p.nb = rows <= 16 ? 1 : 2;
     p.tiles = few ? 1 : (int)((rows + 127) / 128);
-    // enough workgroups for the chip, of at least four steps each
+    // Enough workgroups for the chip, of at least four steps each.  Few rows: eight
+    // workgroups a CU even out lengths (64 sequences of 1024 to 4096 slots 46.6 -> 44.9 us
+    // against four); fewer steps each cost more in joining them (one sequence of
+    // 32768 slots: 13.1, 16.4 with two steps each, 22.9 with one).
     const int64_t step = few ? 4 * TILE : 64;
-    const int64_t full = few ? 4 * (int64_t)cus : 2 * (int64_t)cus;
+    const int64_t full = (few ? 8 : 2) * (int64_t)cus;
     const int64_t want = (full + bh * p.tiles - 1) / (bh * p.tiles);
     const int64_t able = (most + 4 * step - 1) / (4 * step);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, able), 256));
@@ -1055,11 +1113,9 @@ Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
         at += (n + 255) / 256 * 256;
         return here;
     };
-    if (p.splits > 1) {
-        p.part_o = take((uint64_t)p.splits * bh * rows * a->cache.head_dim * 4);
-        p.part_ml = take((uint64_t)p.splits * bh * rows * 8);
-    }
-    if (a->accumulate) p.row_lse = take((uint64_t)bh * rows * 4);
+    if (p.splits > 1) p.part_o = take((uint64_t)p.splits * bh * rows * a->cache.head_dim * 4);
+    if (p.splits > 1 || p.scores) p.part_ml = take((uint64_t)p.splits * bh * rows * 8);
+    if (a->accumulate && !p.scores) p.row_lse = take((uint64_t)bh * rows * 4);
     if (p.scores) p.scores_at = take((uint64_t)bh * rows * most * 4);
     const int wg_keys = p.scores ? 1024 : a->cache.head_dim == 256 ? Weigh<256>::WG_KEYS : Weigh<128>::WG_KEYS;
     p.weight_tiles = (int)((most + wg_keys - 1) / wg_keys);
@@ -1091,12 +1147,12 @@ const void* attend_fn(const Plan& p) {
 }
 
 struct Functions {
-    const void *attend, *join, *weights;
+    const void *attend, *finish, *weights;
 };
 
 template <class T, int D>
 Functions functions(const Plan& p, bool causal) {
-    return {causal ? attend_fn<T, D, true>(p) : attend_fn<T, D, false>(p), (const void*)&join_kernel<T, D>,
+    return {causal ? attend_fn<T, D, true>(p) : attend_fn<T, D, false>(p), (const void*)&finish_kernel<T, D>,
             causal ? (const void*)&weights_kernel<T, D, true> : (const void*)&weights_kernel<T, D, false>};
 }
 
@@ -1159,11 +1215,9 @@ int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
     p.scale = std::max(__builtin_fabsf(a->sm_scale) * LOG2E, FLT_MIN);
     p.neg = a->sm_scale < 0.0f ? 0x80008000u : 0u;
     char* ws = (char*)a->workspace;
-    if (plan.splits > 1) {
-        p.part_o = (float*)(ws + plan.part_o);
-        p.part_ml = (float2*)(ws + plan.part_ml);
-    }
-    if (a->accumulate) p.row_lse = (float*)(ws + plan.row_lse);
+    if (plan.splits > 1) p.part_o = (float*)(ws + plan.part_o);
+    if (plan.splits > 1 || plan.scores) p.part_ml = (float2*)(ws + plan.part_ml);
+    if (a->accumulate && !plan.scores) p.row_lse = (float*)(ws + plan.row_lse);
     if (plan.scores) p.scores = (float*)(ws + plan.scores_at);
     const bool causal = a->causal != 0;
     const Functions fn = a->cache.dtype == RSFA_DTYPE_BF16 ? functions<BF16>(plan, causal, a->cache.head_dim)
@@ -1175,20 +1229,22 @@ int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
     void* args[] = {&p};
     if (hipLaunchKernel(fn.attend, dim3((unsigned)grid, (unsigned)plan.splits), dim3(256), args, 0, (hipStream_t)stream) != hipSuccess)
         return RSFA_E_LAUNCH;
-    if (plan.splits > 1) {
+    if (plan.splits > 1 || plan.scores) {
         const int64_t rows = (int64_t)p.bh * p.rows;
         const int groups = 256 / (int)(a->cache.head_dim / 4);
         int pp = 1;
-        while (pp < groups && pp < plan.splits) pp *= 2;
-        void* join_args[] = {&p, &pp};
+        while (pp < groups && pp * 8 < plan.splits) pp *= 2;
         const int64_t per = groups / pp;
-        if (hipLaunchKernel(fn.join, dim3((unsigned)((rows + per - 1) / per)), dim3(256), join_args, 0, (hipStream_t)stream) != hipSuccess)
+        int join_blocks = plan.splits > 1 ? (int)((rows + per - 1) / per) : 0;
+        const int64_t blocks = join_blocks + (plan.scores ? weight_grid : 0);
+        if (blocks > 0x7fffffff) return RSFA_E_CACHE;
+        void* finish_args[] = {&p, &pp, &join_blocks};
+        if (hipLaunchKernel(fn.finish, dim3((unsigned)blocks), dim3(256), finish_args, 0, (hipStream_t)stream) != hipSuccess)
             return RSFA_E_LAUNCH;
     }
-    if (a->accumulate) {
-        const void* f = plan.scores ? (const void*)&add_weights_kernel : fn.weights;
+    if (a->accumulate && !plan.scores) {
         if (plan.weight_parts > 1) p.part_w = (float*)(ws + plan.part_w);
-        if (hipLaunchKernel(f, dim3((unsigned)weight_grid, (unsigned)plan.weight_parts), dim3(256), args, 0, (hipStream_t)stream) != hipSuccess)
+        if (hipLaunchKernel(fn.weights, dim3((unsigned)weight_grid, (unsigned)plan.weight_parts), dim3(256), args, 0, (hipStream_t)stream) != hipSuccess)
             return RSFA_E_LAUNCH;
         if (plan.weight_parts > 1) {
             int parts = plan.weight_parts;

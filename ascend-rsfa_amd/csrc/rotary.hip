@@ -5,8 +5,8 @@
 //
 // What bounds it: memory; every value is read and written once.  The angles come from the positions and the
 // R/2 frequencies in the kernel, so no table of cosines is read; a thread
-// turns the same pairs of all its heads, so an angle is computed once per
-// `heads_per_thread` heads.  The reduction of p * turns[i] to a fraction of a
+// turns the same pairs of a few heads, so an angle is computed once for
+// them.  The reduction of p * turns[i] to a fraction of a
 // turn is in 64 bits (at p = 2^20 a 32-bit product is off by 2^-4 turns); the
 // sine and cosine of the fraction, the products and sums are in 32 bits, and each
 // output is rounded to its type once.
@@ -35,6 +35,7 @@ struct RotaryParams {
     int32_t rotary, dim;    // R, D
     int32_t pair_units, copy_units;  // threads of a token that turn pairs / copy the rest of the head
     int32_t hpt;            // heads per thread
+    uint32_t groups;        // of hpt heads
 };
 
 template <class E, int V>
@@ -52,13 +53,17 @@ __device__ __forceinline__ void angle(double p, double f, float amp, bool invers
     c *= amp;
 }
 
-// A unit of a token is V pairs (or 2 V values that are copied), one thread's
-// work on each of its heads: two loads and two stores of V elements.
+// A unit of a token is V pairs, or 2 V values that are copied: one thread's work on
+// each of its heads, two loads and two stores of V elements.  Its two chunks lie R/2
+// apart (half the copied values apart) in either layout, so that neighbouring lanes
+// load neighbouring chunks; interleaved pairs with V > 1 lie inside a chunk.
 template <class E, int V, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryParams p) {
     typedef Vec<E, V> Chunk;
+    constexpr bool INSIDE = INTERLEAVED && V > 1;
     const int units = p.pair_units + p.copy_units;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint32_t block = blockIdx.x / p.groups, hg = blockIdx.x - block * p.groups;
+    const int64_t id = (int64_t)block * 256 + threadIdx.x;
     const int64_t token = id / units;
     if (token >= p.tokens) return;
     const int u = (int)(id - token * units);
@@ -68,21 +73,24 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryParams p) {
     bool two = true;
     float c[V], s[V];
     if (turns) {
-        a = INTERLEAVED ? 2 * V * u : V * u;
-        b = INTERLEAVED ? a + V : a + p.half;
+        a = INTERLEAVED && V == 1 ? 2 * u : V * u;
+        b = INTERLEAVED && V == 1 ? a + 1 : a + p.half;
         int64_t pos = p.start + n;
         if (p.positions) {
             const int64_t at = z * p.ps[0] + n * p.ps[1];
             pos = p.pos64 ? ((const int64_t*)p.positions)[at] : (int64_t)((const int32_t*)p.positions)[at];
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) angle((double)pos, p.turns[V * u + i], p.amplitude, p.inverse != 0, s[i], c[i]);
+        for (int i = 0; i < V; ++i) {
+            const int pair = INSIDE ? (i < V / 2 ? a / 2 + i : b / 2 + i - V / 2) : V * u + i;
+            angle((double)pos, p.turns[pair], p.amplitude, p.inverse != 0, s[i], c[i]);
+        }
     } else {
-        a = p.rotary + 2 * V * (u - p.pair_units);
-        b = a + V;
+        a = p.rotary + V * (u - p.pair_units);
+        b = a + V * p.copy_units;
         two = b < p.dim;
     }
-    const int first = (int)blockIdx.y * p.hpt;
+    const int first = (int)hg * p.hpt;
     const int last = min(first + p.hpt, p.heads[0] + p.heads[1]);
 #pragma unroll 4
     for (int h = first; h < last; ++h) {
@@ -93,23 +101,20 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryParams p) {
         Chunk lo = *(const Chunk*)(x + a), hi = lo;
         if (two) hi = *(const Chunk*)(x + b);
         if (turns) {
-            if (INTERLEAVED) {
-                // values 0 .. 2V-1 are lo then hi: pair i is values 2i, 2i + 1
+            auto turn = [](E& eu, E& ew, float cos, float sin) {
+                const float fu = (float)eu, fw = (float)ew;
+                eu = (E)(fu * cos - fw * sin);
+                ew = (E)(fw * cos + fu * sin);
+            };
+            if constexpr (INSIDE) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    E& eu = 2 * i < V ? lo.v[(2 * i) % V] : hi.v[(2 * i) % V];
-                    E& ew = 2 * i + 1 < V ? lo.v[(2 * i + 1) % V] : hi.v[(2 * i + 1) % V];
-                    const float fu = (float)eu, fw = (float)ew;
-                    eu = (E)(fu * c[i] - fw * s[i]);
-                    ew = (E)(fw * c[i] + fu * s[i]);
+                for (int i = 0; i < V / 2; ++i) {
+                    turn(lo.v[2 * i], lo.v[2 * i + 1], c[i], s[i]);
+                    turn(hi.v[2 * i], hi.v[2 * i + 1], c[V / 2 + i], s[V / 2 + i]);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float fu = (float)lo.v[i], fw = (float)hi.v[i];
-                    lo.v[i] = (E)(fu * c[i] - fw * s[i]);
-                    hi.v[i] = (E)(fw * c[i] + fu * s[i]);
-                }
+                for (int i = 0; i < V; ++i) turn(lo.v[i], hi.v[i], c[i], s[i]);
             }
         }
         *(Chunk*)(y + a) = lo;
@@ -181,18 +186,24 @@ extern "C" int rsfa_rotary(const rsfa_rotary_args* a, void* stream) {
     const int64_t threads = p.tokens * (p.pair_units + p.copy_units);
     const int64_t blocks = (threads + 255) / 256;
     if (blocks > 0x7fffffff) return RSFA_E_SHAPE;
-    // heads a thread takes one after another: all of them (the angles are then
-    // computed once) unless the grid would not fill the chip
-    int64_t hpt = all;
+    // Heads that a thread takes one after another, with the same angles: few, so that
+    // the workgroups of a token's heads, which are neighbours in the grid, pass over memory
+    // side by side (8 x 4093 tokens of 32 heads, bf16, [Z, N, H, D], forward and backward,
+    // with 2, 4, 8, 16, 32 heads: 222, 224, 230, 270, 287 us; 4096 tokens in [Z, H, N, D]
+    // forward 94, 99, 103; float32, 4 x 2048 tokens of 20 heads 19.8, 14.5, 15.1); without
+    // wide loads, where the angles cost more, eight (2, 4, 8: 45, 38, 34).
+    int64_t hpt = std::min<int64_t>(all, V > 1 ? 4 : 8);
     while (hpt > 1 && blocks * ((all + hpt - 1) / hpt) < 2048) hpt = (hpt + 1) / 2;
-    if ((all + hpt - 1) / hpt > 65535) hpt = (all + 65534) / 65535;
     p.hpt = (int32_t)hpt;
+    p.groups = (uint32_t)((all + hpt - 1) / hpt);
+    const int64_t grid = blocks * p.groups;
+    if (grid > 0x7fffffff) return RSFA_E_SHAPE;
     const bool il = a->flags & RSFA_ROTARY_INTERLEAVED;
     const void* fn = a->dtype == RSFA_DTYPE_F32    ? (V > 1 ? pick<float, 4>(il) : pick<float, 1>(il))
                      : a->dtype == RSFA_DTYPE_BF16 ? (V > 1 ? pick<__bf16, 8>(il) : pick<__bf16, 1>(il))
                                                    : (V > 1 ? pick<_Float16, 8>(il) : pick<_Float16, 1>(il));
     void* args[] = {&p};
-    if (hipLaunchKernel(fn, dim3((unsigned)blocks, (unsigned)((all + hpt - 1) / hpt)), dim3(256), args, 0,
+    if (hipLaunchKernel(fn, dim3((unsigned)grid), dim3(256), args, 0,
                         (hipStream_t)stream) != hipSuccess)
         return RSFA_E_LAUNCH;
     return RSFA_OK;
