@@ -20,6 +20,7 @@ struct RowsParams {
     const int32_t *lengths, *slots, *counts, *pos_start;
     int64_t length;
     uint32_t t, h, rows;  // rows = Z * H * T
+    uint32_t blocks;      // append, several rows a thread: blocks of a head's tokens
 };
 
 struct Row {
@@ -72,23 +73,35 @@ __global__ void __launch_bounds__(256) append_kernel(RowsParams p) {
     constexpr int LANES = D / 8, PER_BLOCK = 256 / LANES;
     typedef typename T::x8 x8;
     const int lane = threadIdx.x % LANES;
-    const uint32_t first = blockIdx.x * (PER_BLOCK * EACH) + threadIdx.x / LANES;
     const int v = blockIdx.y;
     Row w[EACH];
+    uint32_t rows[EACH];
     x8 in[EACH];
+    if constexpr (EACH > 1) {
+        // a block of tokens of one head; the heads of the same tokens are neighbours in the
+        // grid, as [Z, T, H, D] tensors have them in memory
+        const uint32_t rest = blockIdx.x / p.h;
+        const uint32_t z = rest / p.blocks, h = blockIdx.x - rest * p.h;
+        const uint32_t t0 = (rest - z * p.blocks) * (PER_BLOCK * EACH) + threadIdx.x / LANES;
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        const uint32_t r = min(first + e * PER_BLOCK, p.rows - 1);
-        w[e] = row_of(p, r);
-        in[e] = *(const x8*)((const typename T::elem*)p.src[v] + w[e].z * p.st[v][0] + w[e].h * p.st[v][1] + w[e].t * p.st[v][2] + 8 * lane);
+        for (int e = 0; e < EACH; ++e) {
+            w[e].z = (int)z, w[e].h = (int)h, w[e].t = t0 + e * PER_BLOCK;
+            rows[e] = w[e].t < p.t ? (z * p.h + h) * p.t + w[e].t : p.rows;
+        }
+    } else {
+        rows[0] = blockIdx.x * PER_BLOCK + threadIdx.x / LANES;
+        w[0] = row_of(p, min(rows[0], p.rows - 1));
     }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+        in[e] = *(const x8*)((const typename T::elem*)p.src[v] + w[e].z * p.st[v][0] + w[e].h * p.st[v][1] +
+                             min(w[e].t, p.t - 1) * p.st[v][2] + 8 * lane);
     uint8_t* cb = v ? p.c.v_codes : p.c.k_codes;
     uint8_t* sb = v ? p.c.v_scales : p.c.k_scales;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-        const uint32_t r = first + e * PER_BLOCK;
-        if (r >= p.rows) return;  // whole blocks of four lanes leave together
-        const int64_t slot = target(p, w[e], r);
+        if (rows[e] >= p.rows) return;  // whole blocks of four lanes leave together
+        const int64_t slot = target(p, w[e], rows[e]);
         if (slot < 0) continue;
         float x[8];
         // (bits order as magnitudes do, infinities and NaN above all others)
@@ -192,9 +205,14 @@ int rows_launch(const rsfa_cache4_rows_args* a, bool read, void* stream) {
     p.t = (uint32_t)a->t, p.h = (uint32_t)a->cache.h, p.rows = (uint32_t)rows;
     // four rows a thread once one each would be over eight workgroups on each of 256 CUs
     const int64_t one = 256 / (a->cache.head_dim / 8);
-    const bool four = rows > 2048 * one;
+    // (append: where a head's tokens fill a block of four rows a thread)
+    const bool four = rows > 2048 * one && (read || a->t >= 4 * one);
     const int64_t per = four ? 4 * one : one;
-    const int64_t blocks = (rows + per - 1) / per;
+    int64_t blocks = (rows + per - 1) / per;
+    if (four && !read) {
+        p.blocks = (uint32_t)((a->t + per - 1) / per);
+        blocks = a->cache.z * a->cache.h * p.blocks;
+    }
     const int64_t d = a->cache.head_dim;
     const void* fn = a->cache.dtype == RSFA_DTYPE_BF16 ? (four ? pick<BF16, 4>(read, d) : pick<BF16, 1>(read, d))
                                                        : (four ? pick<F16, 4>(read, d) : pick<F16, 1>(read, d));
