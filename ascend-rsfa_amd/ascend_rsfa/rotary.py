@@ -18,6 +18,7 @@ be as large as a text gets; each output is rounded once.  All arithmetic runs in
 stream of the tensors' device; there is no other path.
 """
 import ctypes
+import functools
 import math
 import struct
 
@@ -79,6 +80,7 @@ class RotaryPlan:
         return t
 
 
+@functools.lru_cache(maxsize=64)  # (plans are constants: the same arguments give the same one)
 def rotary_plan(rotary_dim, *, base=10000.0, layout="half", scaling=None, factor=1.0, original_length=None,
                 low=1.0, high=32.0, amplitude=1.0):
     """A ``RotaryPlan`` of frequencies base^(-2i/R), scaled for long contexts:
@@ -186,28 +188,34 @@ def _unit(x):
 class _Rotary(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, positions, plan):
-        ctx.plan, ctx.positions, ctx.pair = plan, positions, k is not None
+    def forward(ctx, q, k, positions, plan, inverse):
+        ctx.plan, ctx.positions, ctx.inverse = plan, positions, inverse
         # positions may be changed by the program before the backward pass
         if not isinstance(positions, int):
             ctx.positions = None
             ctx.save_for_backward(positions)
-        return _forward(q, k, positions, plan, False)
+        return _forward(q, k, positions, plan, inverse)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, *grads):
-        positions = ctx.positions if ctx.positions is not None else ctx.saved_tensors[0]
-        need = [g is not None and n for g, n in zip(grads, ctx.needs_input_grad)]
-        xs = [g for g, n in zip(grads, need) if n]
-        out = [None, None, None, None]
-        if xs:
-            ys = _forward(xs[0], xs[1] if len(xs) > 1 else None, positions, ctx.plan, True)
-            ys = list(ys) if isinstance(ys, tuple) else [ys]
-            for i, n in enumerate(need):
-                if n:
-                    out[i] = ys.pop(0)
-        return tuple(out)
+    def backward(ctx, gq, gk=None):
+        positions = ctx.saved_tensors[0] if ctx.positions is None else ctx.positions
+        if not ctx.needs_input_grad[0]:
+            gq = None
+        if not ctx.needs_input_grad[1]:
+            gk = None
+        if gq is not None and gk is not None:
+            gq, gk = _turn(gq, gk, positions, ctx.plan, not ctx.inverse)
+        elif gq is not None:
+            gq = _turn(gq, None, positions, ctx.plan, not ctx.inverse)
+        elif gk is not None:
+            gk = _turn(gk, None, positions, ctx.plan, not ctx.inverse)
+        return gq, gk, None, None, None
+
+
+def _turn(q, k, positions, plan, inverse):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, positions, plan, inverse)
+    return _forward(q, k, positions, plan, inverse)
 
 
 def _forward(q, k, positions, plan, inverse):
@@ -277,9 +285,7 @@ def rotary(q, k, positions, plan):
         raise TypeError("positions must be an int (the first token's) or an int32/int64 tensor [N] or [Z, N]")
     if isinstance(positions, int) and abs(positions) >= 1 << 53:
         raise ValueError("positions must be below 2^53")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(q, k, positions, plan)
-    return _forward(q, k, positions, plan, False)
+    return _turn(q, k, positions, plan, False)
 
 
 def rotary_(q, k, positions, plan):

@@ -38,6 +38,7 @@ constexpr float SLACK = 8.0f;
 // that a hidden score's exp2(-inf - m) is 0 and not NaN.
 constexpr float NEVER = -3.0e38f;
 constexpr int TILE = 32;  // keys of a wave's step
+constexpr int NAN_OR_INF = 0x207;  // class mask: an exponent of all ones, as a scale byte of 255 gives
 
 struct AttendParams {
     rsfa_cache4 c;
@@ -178,7 +179,8 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
     constexpr int WAVES = 4, STEP = TILE * WAVES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
-    const int bh = blockIdx.x;
+    const int bh = blockIdx.x % p.bh;  // with a multiple of 8, a head's row tiles meet in one XCD's L2
+    const int row0 = blockIdx.x / p.bh * (NB * 16);
     const int split = blockIdx.y;
     const int z = bh / (int)p.c.h, h = bh - z * (int)p.c.h;
     const int len = __builtin_amdgcn_readfirstlane(length_of(p.lengths, p.length, z, p.most));
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
     int qpos[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        const int row = 16 * b + col;
+        const int row = row0 + 16 * b + col;
         const int tok = row / p.group, head = row - tok * p.group;
         const bool valid = tok < count;  // (row < rows follows)
         u32x4 w[QS] = {};
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
                 }
             }
             if (p.scores) {
-                const int row = 16 * b + col;
+                const int row = row0 + 16 * b + col;
                 if (row < p.rows) {
                     float* dst = p.scores + ((int64_t)bh * p.rows + row) * p.most + tile + 4 * grp;
 #pragma unroll
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
             uint32_t bad = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if ((__float_as_uint(sc[j]) & 0x7f800000u) == 0x7f800000u) bad |= 1u << j, sc[j] = 0.0f;
+                if (__builtin_amdgcn_classf(sc[j], NAN_OR_INF)) bad |= 1u << j, sc[j] = 0.0f;
             if (__any(bad != 0)) {
                 // lane l's O^T values are rows 4 (l / 16) + r of each tile: dims
                 // (4 (l / 16) + r) D/16 + d, whose block is that of a lane with col = 4 (l / 16) + r
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
         l[b] += __shfl_xor(l[b], 16);
         l[b] += __shfl_xor(l[b], 32);
         // rows past the count are empty (their q was taken as 0)
-        if ((16 * b + col) / p.group >= count) m[b] = NEVER, l[b] = 0.0f;
+        if ((row0 + 16 * b + col) / p.group >= count) m[b] = NEVER, l[b] = 0.0f;
     }
     // the waves add up what they have, through LDS
     constexpr int PITCH = D + 4;
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
 
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        const int row = 16 * b + col;
+        const int row = row0 + 16 * b + col;
         if (row >= p.rows) continue;
         const int tok = row / p.group, head = row - tok * p.group;
         const int64_t at = ((int64_t)split * p.bh + bh) * p.rows + row;
@@ -561,12 +563,15 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
     const uint32_t voff = D == 32 ? col / 2 : D == 256 ? col * 4 + vpart * 2 : col * (D / 64);
     const uint32_t vsoff = D == 256 ? (col / 16) * 4 : 0;
     const int vbyte = D == 256 ? (col / 4) & 3 : D == 128 ? col / 8 : D == 64 ? col / 16 : 0;
-    auto load = [&](int tile) {
-        const uint32_t last = len - 1 - tile;  // keys past the length repeat the last
+    auto load_tile = [&](int tile, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        // keys past the length repeat the last (without a check the addresses are constants apart)
+        const uint32_t last = len - 1 - tile;
+        auto inside = [&](uint32_t key) { return WHOLE ? key : min(key, last); };
         const uint8_t* kb = kc + (int64_t)tile * (D / 2);
         const uint8_t* vb = vc + (int64_t)tile * (D / 2);
         {
-            const uint32_t key = min((uint32_t)(32 * kblock + col), last);
+            const uint32_t key = inside(32 * kblock + col);
             const uint8_t* src = kb + (key * (D / 2) + koff);
             if constexpr (M::KF == 4) {
                 const u32x4 w = *(const u32x4*)src;
@@ -583,14 +588,26 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
         const uint8_t* vsb = vs + (int64_t)tile * (D / 32);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const uint32_t key = min((uint32_t)(16 * vstep + 8 * (j / 4) + 4 * half + j % 4), last);
+            const uint32_t key = inside(16 * vstep + 4 * half + (8 * (j / 4) + j % 4));
             const uint8_t* src = vb + (key * (D / 2) + voff);
             if constexpr (D >= 128) raw.v[j] = *(const uint16_t*)src;
             else raw.v[j] = *src;
             const uint8_t* s = vsb + (key * (D / 32) + vsoff);
-            raw.vs[j] = *(const typename Bytes<D == 256 ? 4 : D / 32>::type*)s;
+            if constexpr (D == 128 && WHOLE) {
+                if (j % 4 == 0) {  // four keys' scales lie together
+                    const u32x4_u w = *(const u32x4_u*)s;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) raw.vs[j + i] = w[i];
+                }
+            } else {
+                raw.vs[j] = *(const typename Bytes<D == 256 ? 4 : D / 32>::type*)s;
+            }
         }
-        if (CAUSAL && threadIdx.x < KEYS) raw.pos = pos[tile + min((uint32_t)threadIdx.x, last)];
+        if (CAUSAL && threadIdx.x < KEYS) raw.pos = pos[tile + inside(threadIdx.x)];
+    };
+    auto load = [&](int tile) {
+        if (tile + KEYS <= len) load_tile(tile, std::true_type());
+        else load_tile(tile, std::false_type());
     };
     auto convert = [&](int buf) {
         const float ksc = scale_bits(raw.ks, 0);
@@ -606,13 +623,13 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             sc[j] = scale_bits(raw.vs[j], vbyte);
-            bad |= (__float_as_uint(sc[j]) & 0x7f800000u) == 0x7f800000u;
+            bad |= __builtin_amdgcn_classf(sc[j], NAN_OR_INF);
         }
         const bool any = __any(bad);
         if (__builtin_expect(any, 0)) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if ((__float_as_uint(sc[j]) & 0x7f800000u) == 0x7f800000u) sc[j] = 0.0f;
+                if (__builtin_amdgcn_classf(sc[j], NAN_OR_INF)) sc[j] = 0.0f;
         }
         if (lane == 0) spoiled[buf][wave] = any;
 #pragma unroll
@@ -649,12 +666,13 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
         }
         f32x16 s[SB];
 #pragma unroll
-        for (int b = 0; b < SB; ++b) {
+        for (int b = 0; b < SB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < QS; ++i) s[b] = mfma32(__builtin_bit_cast(x8, frag[buf][b * QS + i][lane]), q[i], s[b]);
-        }
+        for (int i = 0; i < QS; ++i)
+#pragma unroll
+            for (int b = 0; b < SB; ++b) s[b] = mfma32(__builtin_bit_cast(x8, frag[buf][b * QS + i][lane]), q[i], s[b]);
         if (__builtin_expect(masked, 0)) {
 #pragma unroll
             for (int b = 0; b < SB; ++b)
@@ -959,10 +977,14 @@ __global__ void __launch_bounds__(256, 2) weights_kernel(AttendParams p) {
     const elem* qb = (const elem*)p.q + z * p.qs[0] + (int64_t)h * p.group * p.qs[1];
     u32x4 raw[QF];
     float lse_next = 0.0f;
+    // the row of a lane in the next block to be loaded, as token and head of the group
+    const int step = 32 * gridDim.y, step_tok = step / p.group, step_head = step - step_tok * p.group;
+    int tok = (32 * (int)blockIdx.y + col) / p.group, head = 32 * (int)blockIdx.y + col - tok * p.group;
+    int tok_next = 0;
     auto load = [&](int row0) {
-        const int row = row0 + col, at = min(row, rows - 1);
-        const int tok = at / p.group, head = at - tok * p.group;
-        const elem* src = qb + head * p.qs[1] + tok * p.qs[2] + half * (D / 2);
+        const int row = row0 + col;
+        tok_next = min(tok, count - 1);
+        const elem* src = qb + head * p.qs[1] + tok_next * p.qs[2] + half * (D / 2);
 #pragma unroll
         for (int i = 0; i < QF; ++i)
             if (QS >= 4 || wave < QS) {
@@ -972,6 +994,9 @@ __global__ void __launch_bounds__(256, 2) weights_kernel(AttendParams p) {
         // rows past the last and rows that see no slot: exp2 of -inf
         lse_next = row < rows ? p.row_lse[(int64_t)bh * p.rows + row] : INFINITY;
         if (lse_next == -INFINITY) lse_next = INFINITY;
+        tok += step_tok;
+        head += step_head;
+        if (head >= p.group) head -= p.group, ++tok;
     };
     auto store = [&](int buf) {
 #pragma unroll
@@ -988,61 +1013,73 @@ __global__ void __launch_bounds__(256, 2) weights_kernel(AttendParams p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) sum[b][r] = 0.0f;
 
-    const int step = 32 * gridDim.y;
+    auto scores = [&](int buf, int b) {
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < QS; ++i) s = mfma32(k[b][i], __builtin_bit_cast(x8, frag[buf][i][lane]), s);
+        return s;
+    };
+
     int row0 = 32 * blockIdx.y;
     if (row0 < rows) {
         load(row0);
         store(0);
         float lse2 = lse_next;
+        int tok2 = tok_next;
         if (row0 + step < rows) load(row0 + step);
         int buf = 0;
         for (; row0 < rows; row0 += step, buf ^= 1) {
             __syncthreads();
             const float lse_now = lse2;
+            const int tok_now = tok2;
             if (row0 + step < rows) {
                 store(buf ^ 1);
                 lse2 = lse_next;
+                tok2 = tok_next;
             }
             if (row0 + 2 * step < rows) load(row0 + 2 * step);
             bool masked = __any(lse_now == INFINITY);
             int qpos = 0;
             if (CAUSAL) {
                 // the block's rows have positions that grow with the row
-                const int64_t lo = first + row0 / p.group, hi = first + (min(row0 + 32, rows) - 1) / p.group;
+                const int64_t lo = first + __builtin_amdgcn_readfirstlane(tok_now), hi = first + __builtin_amdgcn_readlane(tok_now, 31);
                 if (near > hi) continue;
                 masked |= far > lo;
-                if (masked) {
-                    const int64_t at = first + min(row0 + col, rows - 1) / p.group;
-                    qpos = (int)(at > 0x7fffffff ? 0x7fffffff : at);
-                }
+                const int64_t at = first + tok_now;
+                qpos = (int)(at > 0x7fffffff ? 0x7fffffff : at);
             }
-            f32x16 s[SB];
+            if (__builtin_expect(masked, 0)) {
 #pragma unroll
-            for (int b = 0; b < SB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < QS; ++i) {
-                const x8 q = __builtin_bit_cast(x8, frag[buf][i][lane]);
-#pragma unroll
-                for (int b = 0; b < SB; ++b) s[b] = mfma32(k[b][i], q, s[b]);
-            }
-#pragma unroll
-            for (int b = 0; b < SB; ++b) {
-                if (__builtin_expect(masked, 0)) {
+                for (int b = 0; b < SB; ++b) {
+                    const f32x16 s = scores(buf, b);
                     // (chosen after the exponential: a row whose sum is NaN adds nothing to slots it does not see)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         bool hidden = lse_now == INFINITY;
                         if (CAUSAL) hidden |= kpos[KEYS * wave + 32 * b + 8 * (r / 4) + 4 * half + r % 4] > qpos;
-                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], p.scale, -lse_now));
+                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.scale, -lse_now));
                         sum[b][r] += hidden ? 0.0f : x;
                     }
-                } else {
+                }
+            } else {
+                f32x16 s[SB];
+#pragma unroll
+                for (int b = 0; b < SB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < QS; ++i) {
+                    const x8 q = __builtin_bit_cast(x8, frag[buf][i][lane]);
+#pragma unroll
+                    for (int b = 0; b < SB; ++b) s[b] = mfma32(k[b][i], q, s[b]);
+                }
+#pragma unroll
+                for (int b = 0; b < SB; ++b)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         sum[b][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], p.scale, -lse_now));
-                }
             }
         }
     }
@@ -1093,10 +1130,14 @@ Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
     const int64_t group = a->heads / a->cache.h, rows = group * a->t;
     const int64_t bh = a->cache.z * a->cache.h;
     const int64_t most = a->max_length > 0 && a->max_length < a->cache.capacity ? a->max_length : a->cache.capacity;
-    const bool few = rows <= 16 || (rows <= 32 && a->cache.head_dim <= 128);
+    // (32 heads of 8192 slots, bf16, causal, few and many rows' kernel: 40 rows at D = 64
+    // 23.9 and 21.6 us, at 128 30.1 and 28.2, at 256 52 and 55; 64 rows 26.4 and 23.9, 31.9 and
+    // 30.6, 68 and 60; 24 rows at D = 256 37 and 53)
+    const bool few = rows <= 32;
     p.few = few;
-    p.nb = rows <= 16 ? 1 : 2;
-    p.tiles = few ? 1 : (int)((rows + 127) / 128);
+    p.nb = rows <= 16 || a->cache.head_dim == 256 ? 1 : 2;
+    const int64_t tile_rows = few ? 16 * p.nb : 128;
+    p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
     // Enough workgroups for the chip, of at least four steps each.  Few rows: eight
     // workgroups a CU even out lengths (64 sequences of 1024 to 4096 slots 46.6 -> 44.9 us
     // against four); fewer steps each cost more in joining them (one sequence of
@@ -1106,7 +1147,7 @@ Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
     const int64_t want = (full + bh * p.tiles - 1) / (bh * p.tiles);
     const int64_t able = (most + 4 * step - 1) / (4 * step);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, able), 256));
-    p.scores = a->accumulate && few;
+    p.scores = a->accumulate && rows <= 32;
     uint64_t at = 0;
     auto take = [&](uint64_t n) {
         const uint64_t here = at;

@@ -239,10 +239,10 @@ __device__ __forceinline__ void write_rest(const EvictParams& p, int32_t* out, i
     }
 }
 
-// A row of up to 8 * THREADS slots: wave w holds slots [w * 512, w * 512 + 512).
-template <int THREADS>
+// A row of up to KPT * THREADS slots: wave w holds slots [w * 64 KPT, (w + 1) * 64 KPT).
+template <int THREADS, int KPT>
 __global__ void __launch_bounds__(THREADS) select_kernel(EvictParams p) {
-    constexpr int WAVES = THREADS / 64, KPT = 8;
+    constexpr int WAVES = THREADS / 64;
     __shared__ Shared<THREADS> sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Row r = row_of(p, blockIdx.x);
@@ -719,9 +719,13 @@ int evict_launch(const rsfa_cache4_evict_args* a, bool evict, void* stream) {
         return hipLaunchKernel(fn, grid, dim3((unsigned)threads), args, 0, (hipStream_t)stream) == hipSuccess;
     };
     if (!plan.parts) {
-        const bool small = a->cache.capacity <= 2048;
-        if (!launch(small ? (const void*)&select_kernel<256> : (const void*)&select_kernel<1024>, dim3((unsigned)bh), small ? 256 : 1024))
-            return RSFA_E_LAUNCH;
+        // eight slots a thread (4096 slots of 64 rows, with the copy: 14.9 us, 18.2 with 16 or 32 a thread)
+        const int64_t c = a->cache.capacity;
+        const void* fn = (const void*)&select_kernel<1024, 8>;
+        int threads = 1024;
+        if (c <= 2048) fn = (const void*)&select_kernel<256, 8>, threads = 256;
+        else if (c <= 4096) fn = (const void*)&select_kernel<512, 8>, threads = 512;
+        if (!launch(fn, dim3((unsigned)bh), threads)) return RSFA_E_LAUNCH;
     } else {
         const dim3 grid((unsigned)bh, (unsigned)plan.parts);
         if (!launch((const void*)&survey_kernel, grid, PART_THREADS) || !launch((const void*)&histogram_kernel, grid, PART_THREADS) ||

@@ -125,6 +125,16 @@ def test_gradients(layout, dtype):
         torch.autograd.grad(yq, q, gq)
 
 
+def test_gradients_of_gradients():
+    # linear: the gradient of <d, grad> in the output gradient is the forward turn of d
+    q = _inputs(1, 2, 1, 5, 64, torch.float32, "bhsd", 3)[0].requires_grad_()
+    plan = _plan(64, "half")
+    g, d = (torch.randn_like(q).requires_grad_() for _ in range(2))
+    dq, = torch.autograd.grad(R.rotary(q, None, 9, plan), q, g, create_graph=True)
+    dg, = torch.autograd.grad(dq, g, d)
+    _check(dg, d, torch.arange(9, 14).cuda(), plan)
+
+
 def test_gradient_against_differences():
     # float32, directional: (f(x + h d) - f(x - h d)) / 2h of f = <g, rotary(x)>; f is linear, so h may be
     # large: the difference's error is that of the two sums, 2 * 24 * 2^-24 * sum |g||y| / 2h, at h = 8
