@@ -76,6 +76,9 @@ __device__ __forceinline__ float scale_bits(uint32_t w, int byte) {
 
 typedef u32x4 u32x4_u __attribute__((aligned(4)));  // loads need the alignment of a dword
 typedef f32x4 f32x4_u __attribute__((aligned(4)));
+// scale rows of two bytes and of one
+typedef u32x2 u32x2_u __attribute__((aligned(2)));
+typedef uint32_t u32_u __attribute__((aligned(1)));
 
 template <int BYTES>
 struct Bytes;
@@ -91,7 +94,8 @@ struct Raw {
     uint32_t k[2][KW];
     uint32_t ks[2];                               // scale bytes of the lane's K values (byte 0, 1 at D = 256)
     uint32_t v[8][VW];
-    uint32_t vs[8];                               // D >= 128: the dword of the key's scale bytes that has the lane's
+    static constexpr int SW = D >= 128 ? 1 : 128 / D;  // V keys whose scale bytes share a dword
+    uint32_t vs[8 / SW];                          // those bytes (D = 256: the half of a key's that has the lane's)
     int pos[CAUSAL ? 8 : 1];                      // positions of the lane's V keys (which are its S^T rows)
 };
 
@@ -141,15 +145,26 @@ struct Loader {
             } else {
                 r.v[j][0] = *(const typename Bytes<D / 32>::type*)p;
             }
+            // (four keys' scales lie together)
             const uint8_t* s = vsb + (key * (D / 32) + (D == 256 ? (col / 8) * 4 : 0));
-            if constexpr (D == 256) r.vs[j] = *(const uint32_t*)s;
-            else if constexpr (D == 128 && !TAIL) {
-                if (j % 4 == 0) {  // four keys' scales lie together
+            if constexpr (D == 256) {
+                r.vs[j] = *(const uint32_t*)s;
+            } else if constexpr (TAIL) {
+                const uint32_t w = *(const typename Bytes<D / 32>::type*)s;
+                constexpr int SW = Raw<D, CAUSAL>::SW;
+                r.vs[j / SW] = j % SW ? r.vs[j / SW] | w << (32 / SW * (j % SW)) : w;
+            } else if (j % 4 == 0) {
+                if constexpr (D == 128) {
                     const u32x4_u w = *(const u32x4_u*)s;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) r.vs[j + i] = w[i];
+                } else if constexpr (D == 64) {
+                    const u32x2_u w = *(const u32x2_u*)s;
+                    r.vs[j / 2] = w[0], r.vs[j / 2 + 1] = w[1];
+                } else {
+                    r.vs[j / 4] = *(const u32_u*)s;
                 }
-            } else r.vs[j] = *(const typename Bytes<D / 32>::type*)s;
+            }
             if constexpr (CAUSAL && !TAIL) {
                 if (j % 4 == 0) {
                     const u32x4_u w = *(const u32x4_u*)(pb + key);
@@ -314,7 +329,10 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
         // must not reach it (0 * NaN): it is scaled as 0 and put into the rows that see it
         float sc[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sc[j] = scale_bits(r.vs[j], vbyte);
+        for (int j = 0; j < 8; ++j) {
+            constexpr int SW = Raw<D, CAUSAL>::SW;
+            sc[j] = scale_bits(r.vs[j / SW], 4 / SW * (j % SW) + vbyte);
+        }
         if constexpr (MASKED) {
             uint32_t bad = 0;
 #pragma unroll
@@ -606,7 +624,9 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
         if (CAUSAL && threadIdx.x < KEYS) raw.pos = pos[tile + inside(threadIdx.x)];
     };
     auto load = [&](int tile) {
-        if (tile + KEYS <= len) load_tile(tile, std::true_type());
+        // (at D = 256 the second path's registers spill: 256 rows of 32 x 8192 slots 113 -> 259 us; one wave a
+        // SIMD instead of two, without spills: 158)
+        if (D != 256 && tile + KEYS <= len) load_tile(tile, std::true_type());
         else load_tile(tile, std::false_type());
     };
     auto convert = [&](int buf) {
