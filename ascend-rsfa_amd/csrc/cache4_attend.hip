@@ -404,82 +404,59 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
         // rows past the count are empty (their q was taken as 0)
         if ((row0 + 16 * b + col) / p.group >= count) m[b] = NEVER, l[b] = 0.0f;
     }
-    // the waves add up what they have, through LDS
-    constexpr int PITCH = D + 4;
-    __shared__ float2 ml[WAVES][NB * 16];
-    __shared__ float part[NB * 16][PITCH];
+    // the waves add up what they have, through LDS: each leaves its sums, scaled to the
+    // rows' common maximum, and every thread adds E values of a row
+    constexpr int ROWS = NB * 16, E = ROWS * D / 256, PITCH = D + 4;
+    __shared__ float2 ml[WAVES][ROWS];
+    __shared__ float part[WAVES][ROWS][PITCH];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
         if (grp == 0) ml[wave][16 * b + col] = make_float2(m[b], l[b]);
     __syncthreads();
-    float f[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        float mm = NEVER, ll = 0.0f;
+        float mm = NEVER;
+#pragma unroll
         for (int k = 0; k < WAVES; ++k) mm = fmaxf(mm, ml[k][16 * b + col].x);
-        for (int k = 0; k < WAVES; ++k) {
-            const float2 v = ml[k][16 * b + col];
-            ll += v.y * __builtin_amdgcn_exp2f(v.x - mm);
-        }
-        f[b] = __builtin_amdgcn_exp2f(m[b] - mm);
-        m[b] = mm;
-        l[b] = ll;
-    }
-    for (int k = WAVES - 1; k >= 0; --k) {
-        if (wave == k) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float* at = &part[16 * b + col][(4 * grp + i) * DT];
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        float v = acc[b][d][i] * f[b];
-                        if (k < WAVES - 1) v += at[d];
-                        if (k > 0) at[d] = v;
-                        else acc[b][d][i] = v;
-                    }
-                }
-        }
-        __syncthreads();
-    }
-    if (wave != 0) return;
-
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int row = row0 + 16 * b + col;
-        if (row >= p.rows) continue;
-        const int tok = row / p.group, head = row - tok * p.group;
-        const int64_t at = ((int64_t)split * p.bh + bh) * p.rows + row;
-        if (grp == 0 && p.part_ml) p.part_ml[at] = make_float2(m[b], l[b]);
-        if (p.splits > 1) {
-            float* dst = p.part_o + at * D;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int d = 0; d < DT; d += 2)
-                    *(float2*)(dst + (4 * grp + i) * DT + d) = make_float2(acc[b][d][i], acc[b][d + 1][i]);
-            continue;
-        }
-        // (a NaN sum is a row whose scores are NaN)
-        const float inv = l[b] == 0.0f ? 0.0f : 1.0f / l[b];
-        const int64_t hq = h * p.group + head;
-        elem* dst = (elem*)p.o + z * p.os[0] + hq * p.os[1] + tok * p.os[2];
+        const float f = __builtin_amdgcn_exp2f(m[b] - mm);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t w[DT / 2];
+            float* at = &part[wave][16 * b + col][(4 * grp + i) * DT];
 #pragma unroll
-            for (int d = 0; d < DT; d += 2)
-                w[d / 2] = l[b] == 0.0f ? 0u : pack2<T>(acc[b][d][i] * inv, acc[b][d + 1][i] * inv);
-            elem* at = dst + (4 * grp + i) * DT;
+            for (int d = 0; d < DT; ++d) at[d] = acc[b][d][i] * f;
+        }
+    }
+    __syncthreads();
+    const int r = threadIdx.x / (D / E), d0 = threadIdx.x % (D / E) * E;
+    const int row = row0 + r;
+    if (row >= p.rows) return;
+    float mm = NEVER, ll = 0.0f;
 #pragma unroll
-            for (int d = 0; d < DT / 2; ++d) ((uint32_t*)at)[d] = w[d];
-        }
-        if (grp == 0) {
-            const float lse2 = l[b] == 0.0f ? -INFINITY : m[b] + __builtin_amdgcn_logf(l[b]);
-            if (p.lse) p.lse[(z * (int64_t)p.heads + hq) * p.t + tok] = lse2 * LN2;
-            if (p.row_lse) p.row_lse[(int64_t)bh * p.rows + row] = lse2;
-        }
+    for (int k = 0; k < WAVES; ++k) mm = fmaxf(mm, ml[k][r].x);
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) ll += ml[k][r].y * __builtin_amdgcn_exp2f(ml[k][r].x - mm);
+    float sum[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] = (part[0][r][d0 + e] + part[1][r][d0 + e]) + (part[2][r][d0 + e] + part[3][r][d0 + e]);
+    const int64_t at = ((int64_t)split * p.bh + bh) * p.rows + row;
+    if (d0 == 0 && p.part_ml) p.part_ml[at] = make_float2(mm, ll);
+    if (p.splits > 1) {
+        float* dst = p.part_o + at * D + d0;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) *(float2*)(dst + e) = make_float2(sum[e], sum[e + 1]);
+        return;
+    }
+    // (a NaN sum is a row whose scores are NaN)
+    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+    const int tok = row / p.group, head = row - tok * p.group;
+    const int64_t hq = h * p.group + head;
+    uint32_t* dst = (uint32_t*)((elem*)p.o + z * p.os[0] + hq * p.os[1] + tok * p.os[2] + d0);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) dst[e / 2] = ll == 0.0f ? 0u : pack2<T>(sum[e] * inv, sum[e + 1] * inv);
+    if (d0 == 0) {
+        const float lse2 = ll == 0.0f ? -INFINITY : mm + __builtin_amdgcn_logf(ll);
+        if (p.lse) p.lse[(z * (int64_t)p.heads + hq) * p.t + tok] = lse2 * LN2;
+        if (p.row_lse) p.row_lse[(int64_t)bh * p.rows + row] = lse2;
     }
 }
 
