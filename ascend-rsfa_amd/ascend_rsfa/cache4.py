@@ -22,7 +22,9 @@ says how many of a call's T tokens a sequence has, in a padded batch.
 
 All arithmetic runs in ``lib/librsfa.so`` (``rsfa_cache4_*`` in ``include/rsfa.h``),
 enqueued on the current stream of the cache's device; there is no other path.
-No gradients: the cache is for inference.
+Calls that write a cache (append, attend with ``accumulate``, evict into it) and
+others on the same cache must run one after another: on one stream, or ordered by
+events.  No gradients: the cache is for inference.
 """
 import ctypes
 import math
@@ -65,6 +67,37 @@ def _function(name):
 
 def _is_int(x):
     return isinstance(x, int) and not isinstance(x, bool)
+
+
+def _span(t):
+    """First and last byte of a tensor's memory."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + last * t.element_size() + t.element_size()
+
+
+def _meet(a, b):
+    """Whether two buffers [Z, H, C, ...] of rows share memory (sequences and heads of
+    one may lie between those of the other)."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    starts = []  # of each sequence and head's rows
+    for i, t in enumerate((a, b)):
+        size = t[0, 0].numel() * t.element_size()
+        starts += [(t.data_ptr() + (z * t.stride(0) + h * t.stride(1)) * t.element_size(), size, i)
+                   for z in range(t.shape[0]) for h in range(t.shape[1])]
+    starts.sort()
+    ends = [0, 0]
+    for at, size, i in starts:
+        if at < ends[1 - i]:
+            return True
+        ends[i] = max(ends[i], at + size)
+    return False
+
+
+def _no_gradient(*tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("a Cache4 keeps no gradients: call it under torch.no_grad()")
 
 
 class Cache4:
@@ -147,6 +180,7 @@ class Cache4:
         c.dtype = _DTYPES[dtype]
         self._c = c
         self._z = torch.Size((Z,))
+        self._spans = [(t, *_span(t)) for _, t, _, _ in named]
         self._kept = {}
 
     def _keep(self, key, parts):
@@ -221,6 +255,7 @@ class Cache4:
         Not written: tokens ``i >= counts[z]`` and slots outside the cache
         (-1, say).  A slot that ``slots`` names twice holds the last of its tokens.
         """
+        _no_gradient(k, v)
         key = ("append", k.shape, v.shape, k.stride(), v.stride(), k.dtype, v.dtype, k.device, v.device)
         parts = self._kept.get(key)
         if parts is None or (k.data_ptr() | v.data_ptr()) & 15:
@@ -285,8 +320,11 @@ class Cache4:
         its softmax weights over all tokens and the query heads of its group.
         ``max_length``: a bound on the lengths (longer ones are cut to it), which
         sizes the call's workspace and its division of the work; the capacity without one.
+        (With ``accumulate`` and at most 32 rows a key head, tokens times group, the workspace
+        holds 4 bytes for each row and slot, up to 4 GiB.)
         ``lse``: the natural logarithm of each row's sum of exponentials, float32 [Z, Hq, T].
         """
+        _no_gradient(q)
         key = ("attend", q.shape, q.stride(), q.dtype, q.device, bool(causal), None if out is None else out.stride())
         parts = self._kept.get(key)
         if parts is None or out is not None or q.data_ptr() & 15:
@@ -301,6 +339,10 @@ class Cache4:
                 o = out
                 if o.shape != q.shape or o.dtype != q.dtype or o.device != q.device or not _meets_contract(o):
                     raise ValueError("out must match q's shape, dtype and device and have a unit-stride head dim")
+                if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
+                    raise ValueError("out is expanded: its rows must not share memory")
+                if o.numel() and _meet(o, q):
+                    raise ValueError("out must not share memory with q")
             args = _native.Cache4AttendArgs()
             args.struct_size = ctypes.sizeof(args)
             args.cache, args.causal = self._c, int(bool(causal))
@@ -405,6 +447,7 @@ class Cache4:
         if (into.Z, into.H, into.head_dim, into.dtype, into.device) != (
                 self.Z, self.H, self.head_dim, self.dtype, self.device):
             raise ValueError("into must have this cache's sequences, heads, head_dim, dtype and device")
-        if into.k_codes.data_ptr() == self.k_codes.data_ptr():
-            raise ValueError("into must be another cache")
+        for (a, a0, a1), (b, b0, b1) in zip(self._spans, into._spans):
+            if a0 < b1 and b0 < a1 and _meet(a, b):
+                raise ValueError("into must not share memory with this cache")
         self._evict_call("rsfa_cache4_evict", into, lengths, 1, into.capacity if budget is None else budget, recent, sinks, 0)

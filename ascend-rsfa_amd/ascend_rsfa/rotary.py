@@ -301,6 +301,8 @@ def rotary_(q, k, positions, plan):
         if any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
             raise ValueError("rotary_ cannot write to an expanded tensor")
     xs = [x for x in (q, k) if x is not None and x.numel()]
+    if len(xs) == 2 and q.data_ptr() == k.data_ptr():
+        raise ValueError("q and k must not share memory")
     if xs:
         _launch(_parts(xs, xs, positions, plan, False), xs, xs, positions)
     return q if k is None else (q, k)

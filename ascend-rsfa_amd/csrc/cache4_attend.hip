@@ -1144,7 +1144,9 @@ Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
     const int64_t want = (full + bh * p.tiles - 1) / (bh * p.tiles);
     const int64_t able = (most + 4 * step - 1) / (4 * step);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, able), 256));
-    p.scores = a->accumulate && rows <= 32;
+    // (computing the scores again instead, one token of 16 x 8 x 8192 slots at most, D = 128: 4
+    // rows 28 and 97 us, 32 rows 73 and 121; the workspace that they take is kept below 4 GiB)
+    p.scores = a->accumulate && rows <= 32 && (uint64_t)bh * rows * most < (uint64_t(1) << 30);
     uint64_t at = 0;
     auto take = [&](uint64_t n) {
         const uint64_t here = at;

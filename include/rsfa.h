@@ -259,7 +259,8 @@ int rsfa_rotary(const rsfa_rotary_args *args, void *stream);
  * which no value of the block is more than 7, within the exponents -23 .. 13
  * (float16) or -125 .. 125 (bfloat16), whose values all exist in the type:
  * values are rounded to the nearest code, ties to the even index, and end at 6
- * scales; a block that holds an infinity or a NaN is stored as NaN.
+ * scales; a block that holds an infinity or a NaN is stored as NaN.  Scale
+ * bytes of slots in use are expected to be of that range, or 255.
  *
  * Sequences and heads are [z, h]; each has `capacity` slots, whose rows lie
  * densely: slot s of (z, h) is at z * stride[0] + h * stride[1] + s * row, with
@@ -314,7 +315,8 @@ int rsfa_cache4_read(const rsfa_cache4_rows_args *args, void *stream);
  * length - count + i, with the sequence's count of tokens).  Rows i >= counts[z],
  * and rows that see no slot, give 0 (lse -inf).  With `accumulate` the weights
  * of the slots grow by the softmax weights that all rows of the call gave them.
- * Lengths above max_length (0: the capacity) are taken as max_length.
+ * Lengths above max_length (0: the capacity) are taken as max_length.  o must not
+ * overlap q; calls that accumulate into one cache must not overlap in time.
  * Workspace: rsfa_cache4_attend_workspace_bytes of the same arguments (its
  * contents need not outlive the call's kernels). */
 typedef struct rsfa_cache4_attend_args {
@@ -345,7 +347,7 @@ uint64_t rsfa_cache4_attend_workspace_bytes(const rsfa_cache4_attend_args *args)
  * claim: out [z, h, n] (int32, dense): the slots for each sequence's next n
  * tokens: those from lengths[z] up to `budget`, then the unprotected slots that
  * go first, in order of slot; -1 where there is none.
- * evict: copies to `into` (same z, h, head_dim and dtype; not the same memory) the
+ * evict: copies to `into` (same z, h, head_dim and dtype; no memory in common) the
  * slots that stay when the first max(0, lengths[z] - budget) go (protected ones
  * after all others), in order of slot, to its slots 0, 1, ...; other slots of `into`
  * keep what they hold.

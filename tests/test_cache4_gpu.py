@@ -198,6 +198,38 @@ def test_append_counts_slots_and_edges():
     _same(cache, want)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_append_of_many_rows(D):
+    # blocks of four rows a thread: counts, slots and lengths that end inside of a block
+    Z, H, T = 3, 7, 128 * 256 * 8 // D // 7
+    k = _randn((Z, T, H, D), 1, BF16).transpose(1, 2)
+    v = _randn((Z, H, T, D), 2, BF16)
+    packed = dict(zip(("k_codes", "k_scales", "v_codes", "v_scales"), (*S.quantise(k, BF16), *S.quantise(v, BF16))))
+    for use_slots in (False, True):
+        cache = _filled(Z, H, T + 50, D, BF16, 7)
+        want = {n: getattr(cache, n).clone() for n in (*packed, "positions", "weights")}
+        counts, at = [T, 0, T // 2 + 3], [50, 7, 80]
+        slots = None
+        if use_slots:
+            slots = torch.rand((Z, H, T + 50), generator=torch.Generator().manual_seed(3)).argsort(-1)[..., :T].int().cuda()
+        for z in range(Z):
+            n = min(counts[z], T + 50 - at[z]) if slots is None else counts[z]
+            i = torch.arange(n).cuda()
+            for h in range(H):
+                s = at[z] + i if slots is None else slots[z, h, :n].long()
+                for name, rows in packed.items():
+                    want[name][z, h, s] = rows[z, h, :n]
+                want["positions"][z, h, s] = (at[z] + i).int()
+                want["weights"][z, h, s] = 0.0
+        cache.append(k, v, _ints(at), counts=_ints(counts), slots=slots)
+        _same(cache, want)
+        rk, _ = cache.read(_ints(at), T)
+        full = S.values(cache.k_codes, cache.k_scales)
+        for z in range(Z):
+            n = min(T, T + 50 - at[z])
+            assert torch.equal(rk[z, :, :n].double(), full[z, :, at[z]:at[z] + n]) and (rk[z, :, n:] == 0).all()
+
+
 def test_non_finite_blocks_are_stored_as_nan():
     cache = Cache4(1, 1, 4, 64, BF16)
     k = _randn((1, 1, 4, 64), 1, BF16)
@@ -472,6 +504,20 @@ def test_evict_matches_the_definition(C, D, kind):
                                t.view(torch.int32) if n == "weights" else t), n
 
 
+def test_evict_between_layers_of_one_buffer():
+    # two caches whose sequences alternate in memory share none of it
+    big = {n: torch.zeros((3, 2, 2, 20) + ((32,) if "codes" in n else (2,) if "scales" in n else ()), dtype=t).cuda() for n, t in (
+        ("k_codes", torch.uint8), ("k_scales", torch.uint8), ("v_codes", torch.uint8), ("v_scales", torch.uint8),
+        ("positions", torch.int32), ("weights", torch.float32))}
+    a, b = (Cache4.from_buffers(**{n: t[:, i] for n, t in big.items()}) for i in range(2))
+    k = _randn((3, 2, 20, 64), 1, F16)
+    a.append(k, k, 0)
+    a.weights.copy_(_randn((3, 2, 20), 2))
+    kept = S.evict(a.weights.cpu(), a.positions.cpu(), [20] * 3, 6)
+    a.evict(b, 20, budget=6)
+    assert b.positions[..., :6].tolist() == kept and (b.positions[..., 6:] == 0).all()
+
+
 def test_protected_slots_beyond_the_budget_go_by_slot():
     cache = _filled(1, 1, 12, 32, F16, 3)
     cache.positions.fill_(5)  # all of one position: all among the most recent
@@ -608,7 +654,10 @@ def test_refusals():
                 lambda: bare.attend(q, n, False, 1.0, accumulate=True), lambda: bare.claim(4, 1), lambda: bare.evict(cache, 4),
                 lambda: cache.claim(n, 0), lambda: cache.claim(n, 1, budget=17), lambda: cache.claim(n, 1, budget=0),
                 lambda: cache.claim(n, 1, recent=10, sinks=7), lambda: cache.claim(n, 1, recent=-1), lambda: cache.claim(17, 1),
-                lambda: cache.evict(cache, n), lambda: cache.evict(Cache4(2, 2, 8, 64, BF16), n),
+                lambda: cache.evict(cache, n), lambda: cache.evict(Cache4.from_buffers(**{
+                    x: getattr(cache, x)[:, :, :8] for x in ("k_codes", "k_scales", "v_codes", "v_scales", "positions", "weights")}), n),
+                lambda: cache.attend(q, n, False, 1.0, out=q), lambda: cache.attend(q, n, False, 1.0, out=q[:, :1].expand(2, 4, 4, 64)),
+                lambda: cache.evict(Cache4(2, 2, 8, 64, BF16), n),
                 lambda: cache.evict(Cache4(2, 2, 8, 32, F16), n), lambda: cache.evict(Cache4(1, 2, 8, 64, F16), n),
                 lambda: cache.evict(Cache4(2, 2, 8, 64, F16), n, budget=9), lambda: cache.evict(Cache4(2, 2, 8, 64, F16), n, recent=9)):
         with pytest.raises(ValueError):
@@ -617,6 +666,11 @@ def test_refusals():
                 lambda: cache.append(k, k, n.long()), lambda: cache.attend(q, n[:1], False, 1.0),
                 lambda: cache.attend(q, n, False, 1.0, counts=[4, 4]), lambda: cache.append(k, k, 1.5), lambda: cache.evict(None, n)):
         with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: cache.attend(q.clone().requires_grad_(), n, False, 1.0), lambda: cache.append(k.clone().requires_grad_(), k, 0)):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            bad()
+        with torch.no_grad():
             bad()
     b = {x: getattr(cache, x) for x in ("k_codes", "k_scales", "v_codes", "v_scales", "positions", "weights")}
     for over in ({"k_codes": b["k_codes"][..., :24]}, {"k_scales": b["k_scales"].float()}, {"v_codes": b["v_codes"].cpu()},

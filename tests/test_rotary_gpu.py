@@ -248,5 +248,9 @@ def test_refusals():
         R.rotary(x, None, 0, None)
     with pytest.raises(ValueError):
         R.rotary_(x.expand(2, 2, 3, 64), None, 0, plan)
+    with pytest.raises(ValueError):
+        R.rotary_(x, x, 0, plan)
+    with pytest.raises(ValueError):
+        R.rotary(x, None, 1 << 53, plan)
     with pytest.raises(RuntimeError):
         R.rotary_(x.clone().requires_grad_(), None, 0, plan)
