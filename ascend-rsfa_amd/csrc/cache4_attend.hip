@@ -185,6 +185,14 @@ struct Loader {
 // Few rows (NB blocks of 16): the four waves of a workgroup take every fourth key
 // tile of its part of the slots and add up what they have at the end.  CAUSAL hides
 // keys in every tile; otherwise only the last, partial tile does.
+// Bound by memory: D/2 + D/32 bytes of K and as many of V a slot.  The loop holds
+// one tile while the next is loaded (26 registers at D = 128), with a scalar base and
+// constant offsets; with the checks for a partial tile inside of it, and the mask as a
+// second path, it took 250 registers and spilled.  One token of 32 heads, 8 key
+// heads: 64 sequences of 1024 to 4096 slots, D = 128, bf16, scores kept for the weights:
+// 36 us, 5.6 TB/s of codes, scales and scores; 32 x 8192 slots at D = 64, 128, 256: 30.8, 50, 109 us
+// (5.2 TB/s would be 27.6, 55, 110); one sequence of 32768 slots 9.6 us where the codes'
+// bytes are 6.9: the launch and the first loads.
 template <class T, int D, int NB, bool CAUSAL>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
     typedef typename T::x8 x8;
@@ -470,6 +478,12 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
 //   O^T = V^T P^T  S^T leaves lane l the row l % 32 and the keys 8 a + 4 (l / 32) + b;
 //                step s takes k = 8 (l / 32) + j as key 16 s + 8 (j / 4) + 4 (l / 32) + j % 4.
 //                A: lane l has these keys of the value (l % 32) * D/32 + t in fragment t.
+// Bound by the matrix and the vector units together: a chunk of 2048 tokens, 32 heads,
+// over 16384 slots of 8 key heads, D = 128, bf16, causal: 545 to 615 us, 840 to 945 TFLOP/s,
+// the MFMAs busy 38 % and vector instructions issuing 48 % of the cycles.  (Direct
+// operands without LDS, 32 rows a wave: 1107 us.  Halves of a tile whose softmax and
+// products alternate: 805.  Raised wave priority around the products: 582 against 559; LDS
+// reads two to eight MFMAs ahead: the same.)
 template <int D>
 struct Many {
     static constexpr int KEYS = D == 256 ? 32 : 64;  // of a tile: its fragments take 32 KB at D = 128, 256
@@ -781,7 +795,7 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
 
 // Sum of a row's parts: D / 4 lanes hold a row, four values each, and `pp` such
 // groups of a workgroup take every pp-th part of it, so that the loads of a row's
-// parts do not wait for each other.
+// parts do not wait for each other (64 parts of 32 rows: 3.9 us, one after another 41).
 template <class T, int D>
 __device__ __forceinline__ void join_rows(const AttendParams& p, int pp, int block) {
     constexpr int G = D / 4, GROUPS = 256 / G;
@@ -917,6 +931,8 @@ __global__ void __launch_bounds__(256) finish_kernel(AttendParams p, int pp, int
 // of the 32 x 32 MFMA (64 registers at D = 128, 256); blocks of 32 rows of Q pass by
 // in LDS, as operands too, two buffers of them.  A workgroup takes the row blocks
 // blockIdx.y, blockIdx.y + gridDim.y, ...
+// Bound as attend_many_kernel is, with half its products and all of its exponentials: 375 to
+// 430 us for the chunk above.  (16 x 16 tiles with Q from global memory: 492.)
 template <int D>
 struct Weigh {
     static constexpr int KEYS = D == 256 ? 32 : 64;  // of a wave
