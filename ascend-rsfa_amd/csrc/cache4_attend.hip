@@ -927,26 +927,36 @@ __global__ void __launch_bounds__(256) finish_kernel(AttendParams p, int pp, int
 }
 
 // Weights of many rows: the scores are computed again, now that the rows' sums are
-// known.  Each of the workgroup's four waves holds keys of its own as operands
-// of the 32 x 32 MFMA (64 registers at D = 128, 256); blocks of 32 rows of Q pass by
-// in LDS, as operands too, two buffers of them.  A workgroup takes the row blocks
+// known.  Each wave holds 32 keys of its own as operands of the 32 x 32 MFMA (32
+// registers at D = 128, 64 at 256); blocks of 32 rows of Q pass by in LDS, as operands
+// too, two buffers of ROW_BLOCKS blocks.  A workgroup takes the groups of row blocks
 // blockIdx.y, blockIdx.y + gridDim.y, ...
-// Bound as attend_many_kernel is, with half its products and all of its exponentials: 375 to
-// 430 us for the chunk above.  (16 x 16 tiles with Q from global memory: 492.)
+// Bound as attend_many_kernel is, with half its products and all of its exponentials: 265
+// us of the chunk above (the call 840).  Up to D = 128 a wave keeps to 128 registers, so
+// that four waves of a SIMD hide each other's products and exponentials; with 64
+// keys, two waves: the call 864.  Row blocks between barriers, one, two, three, four: 861,
+// 843, 840, 848 at D = 128, 346, 336, 329, 329 at D = 64.  D = 256 (1024 rows a
+// head, 16384 slots) does not fit four waves: 536 us spilled, 513 with two; one row block
+// 548, two 514, four, which leave room for one workgroup, 666.  (16 x 16 tiles with Q from
+// global memory: 492 of the chunk.)
 template <int D>
 struct Weigh {
-    static constexpr int KEYS = D == 256 ? 32 : 64;  // of a wave
-    static constexpr int WG_KEYS = 4 * KEYS;
+    static constexpr int KEYS = 32;  // of a wave
+    static constexpr int WAVES = D == 256 ? 4 : 8;
+    static constexpr int OCCUPANCY = D == 256 ? 2 : 4;  // waves of a SIMD
+    static constexpr int ROW_BLOCKS = D == 256 ? 2 : 3;
+    static constexpr int WG_KEYS = WAVES * KEYS;
 };
 
 template <class T, int D, bool CAUSAL>
-__global__ void __launch_bounds__(256, 2) weights_kernel(AttendParams p) {
+__global__ void __launch_bounds__(64 * Weigh<D>::WAVES, Weigh<D>::OCCUPANCY) weights_kernel(AttendParams p) {
     typedef typename T::x8 x8;
     typedef typename T::elem elem;
-    constexpr int QS = D / 16, KEYS = Weigh<D>::KEYS, SB = KEYS / 32;
-    constexpr int QF = (QS + 3) / 4;  // fragments of Q a wave brings
-    __shared__ u32x4 frag[2][QS][64];
-    __shared__ int kpos[CAUSAL ? 4 * KEYS : 1];
+    constexpr int QS = D / 16, KEYS = Weigh<D>::KEYS;
+    constexpr int WAVES = Weigh<D>::WAVES, QF = (QS + WAVES - 1) / WAVES;  // fragments of Q a wave brings
+    constexpr int RB = Weigh<D>::ROW_BLOCKS;
+    __shared__ u32x4 frag[2][RB][QS][64];
+    __shared__ int kpos[CAUSAL ? WAVES * KEYS : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int bh = blockIdx.x % p.bh;
@@ -971,10 +981,9 @@ __global__ void __launch_bounds__(256, 2) weights_kernel(AttendParams p) {
             near = min(near, __shfl_xor(near, d));
         }
     }
-    x8 k[SB][QS];
-#pragma unroll
-    for (int b = 0; b < SB; ++b) {
-        const int key = min(tile + 32 * b + col, len - 1);
+    x8 k[QS];
+    {
+        const int key = min(tile + col, len - 1);
         const uint8_t* src = kc + (int64_t)key * (D / 2) + half * (D / 4);
         const uint8_t* s = ks + (int64_t)key * (D / 32);
 #pragma unroll
@@ -983,134 +992,119 @@ __global__ void __launch_bounds__(256, 2) weights_kernel(AttendParams p) {
             const float sc = scale_bits(s[(half * (D / 2) + 8 * i) / 32], 0);
             const u32x4 kv = {T::template cvt<0>(w, sc), T::template cvt<1>(w, sc), T::template cvt<2>(w, sc),
                               T::template cvt<3>(w, sc)};
-            k[b][i] = __builtin_bit_cast(x8, kv);
+            k[i] = __builtin_bit_cast(x8, kv);
         }
     }
     const int64_t first = CAUSAL ? (p.pos_start ? (int64_t)p.pos_start[z] : (int64_t)len - count) : 0;
     const elem* qb = (const elem*)p.q + z * p.qs[0] + (int64_t)h * p.group * p.qs[1];
-    u32x4 raw[QF];
-    float lse_next = 0.0f;
+    const float scale = p.neg ? -p.scale : p.scale;
+    u32x4 raw[RB][QF];
+    float lse_next[RB];
+    int tok_next[RB];
     // the row of a lane in the next block to be loaded, as token and head of the group
-    const int step = 32 * gridDim.y, step_tok = step / p.group, step_head = step - step_tok * p.group;
-    int tok = (32 * (int)blockIdx.y + col) / p.group, head = 32 * (int)blockIdx.y + col - tok * p.group;
-    int tok_next = 0;
+    const int step = 32 * RB * gridDim.y;
+    const int more_tok = 32 / p.group, more_head = 32 - more_tok * p.group;  // a block of rows further
+    const int step_tok = (step - 32 * (RB - 1)) / p.group, step_head = step - 32 * (RB - 1) - step_tok * p.group;
+    int tok = (32 * RB * (int)blockIdx.y + col) / p.group, head = 32 * RB * (int)blockIdx.y + col - tok * p.group;
     auto load = [&](int row0) {
-        const int row = row0 + col;
-        tok_next = min(tok, count - 1);
-        const elem* src = qb + head * p.qs[1] + tok_next * p.qs[2] + half * (D / 2);
 #pragma unroll
-        for (int i = 0; i < QF; ++i)
-            if (QS >= 4 || wave < QS) {
-                raw[i] = *(const u32x4*)(src + 8 * (wave * QF + i));
-                if (row >= rows) raw[i] = (u32x4){0, 0, 0, 0};
-            }
-        // rows past the last and rows that see no slot: exp2 of -inf
-        lse_next = row < rows ? p.row_lse[(int64_t)bh * p.rows + row] : INFINITY;
-        if (lse_next == -INFINITY) lse_next = INFINITY;
-        tok += step_tok;
-        head += step_head;
-        if (head >= p.group) head -= p.group, ++tok;
+        for (int g = 0; g < RB; ++g) {
+            const int row = row0 + 32 * g + col;
+            tok_next[g] = min(tok, count - 1);
+            const elem* src = qb + head * p.qs[1] + tok_next[g] * p.qs[2] + half * (D / 2);
+#pragma unroll
+            for (int i = 0; i < QF; ++i)
+                if (QS >= WAVES || wave < QS) raw[g][i] = *(const u32x4*)(src + 8 * (wave * QF + i));
+            // rows past the last and rows that see no slot are hidden below
+            lse_next[g] = row < rows ? p.row_lse[(int64_t)bh * p.rows + row] : INFINITY;
+            if (lse_next[g] == -INFINITY) lse_next[g] = INFINITY;
+            tok += g < RB - 1 ? more_tok : step_tok;
+            head += g < RB - 1 ? more_head : step_head;
+            if (head >= p.group) head -= p.group, ++tok;
+        }
     };
     auto store = [&](int buf) {
 #pragma unroll
-        for (int i = 0; i < QF; ++i)
-            if (QS >= 4 || wave < QS) {
+        for (int g = 0; g < RB; ++g)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) raw[i][j] ^= p.neg;
-                frag[buf][wave * QF + i][lane] = raw[i];
-            }
+            for (int i = 0; i < QF; ++i)
+                if (QS >= WAVES || wave < QS) frag[buf][g][wave * QF + i][lane] = raw[g][i];
     };
-    float sum[SB][16];
+    float sum[16];
 #pragma unroll
-    for (int b = 0; b < SB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum[b][r] = 0.0f;
+    for (int r = 0; r < 16; ++r) sum[r] = 0.0f;
 
-    auto scores = [&](int buf, int b) {
-        f32x16 s;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < QS; ++i) s = mfma32(k[b][i], __builtin_bit_cast(x8, frag[buf][i][lane]), s);
-        return s;
-    };
-
-    int row0 = 32 * blockIdx.y;
+    int row0 = 32 * RB * blockIdx.y;
     if (row0 < rows) {
         load(row0);
         store(0);
-        float lse2 = lse_next;
-        int tok2 = tok_next;
+        float lse2[RB];
+        int tok2[RB];
+#pragma unroll
+        for (int g = 0; g < RB; ++g) lse2[g] = lse_next[g], tok2[g] = tok_next[g];
         if (row0 + step < rows) load(row0 + step);
         int buf = 0;
         for (; row0 < rows; row0 += step, buf ^= 1) {
             __syncthreads();
-            const float lse_now = lse2;
-            const int tok_now = tok2;
+            float lse_now[RB];
+            int tok_now[RB];
+#pragma unroll
+            for (int g = 0; g < RB; ++g) lse_now[g] = lse2[g], tok_now[g] = tok2[g];
             if (row0 + step < rows) {
                 store(buf ^ 1);
-                lse2 = lse_next;
-                tok2 = tok_next;
+#pragma unroll
+                for (int g = 0; g < RB; ++g) lse2[g] = lse_next[g], tok2[g] = tok_next[g];
             }
             if (row0 + 2 * step < rows) load(row0 + 2 * step);
-            bool masked = __any(lse_now == INFINITY);
-            int qpos = 0;
-            if (CAUSAL) {
-                // the block's rows have positions that grow with the row
-                const int64_t lo = first + __builtin_amdgcn_readfirstlane(tok_now), hi = first + __builtin_amdgcn_readlane(tok_now, 31);
-                if (near > hi) continue;
-                masked |= far > lo;
-                const int64_t at = first + tok_now;
-                qpos = (int)(at > 0x7fffffff ? 0x7fffffff : at);
-            }
-            if (__builtin_expect(masked, 0)) {
 #pragma unroll
-                for (int b = 0; b < SB; ++b) {
-                    const f32x16 s = scores(buf, b);
+            for (int g = 0; g < RB; ++g) {
+                if (row0 + 32 * g >= rows) break;
+                bool masked = __any(lse_now[g] == INFINITY);
+                int qpos = 0;
+                if (CAUSAL) {
+                    // the block's rows have positions that grow with the row
+                    const int64_t lo = first + __builtin_amdgcn_readfirstlane(tok_now[g]);
+                    const int64_t hi = first + __builtin_amdgcn_readlane(tok_now[g], 31);
+                    if (near > hi) continue;
+                    masked |= far > lo;
+                    const int64_t at = first + tok_now[g];
+                    qpos = (int)(at > 0x7fffffff ? 0x7fffffff : at);
+                }
+                f32x16 s;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < QS; ++i) s = mfma32(k[i], __builtin_bit_cast(x8, frag[buf][g][i][lane]), s);
+                if (__builtin_expect(masked, 0)) {
                     // (chosen after the exponential: a row whose sum is NaN adds nothing to slots it does not see)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        bool hidden = lse_now == INFINITY;
-                        if (CAUSAL) hidden |= kpos[KEYS * wave + 32 * b + 8 * (r / 4) + 4 * half + r % 4] > qpos;
-                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.scale, -lse_now));
-                        sum[b][r] += hidden ? 0.0f : x;
+                        bool hidden = lse_now[g] == INFINITY;
+                        if (CAUSAL) hidden |= kpos[KEYS * wave + 8 * (r / 4) + 4 * half + r % 4] > qpos;
+                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale, -lse_now[g]));
+                        sum[r] += hidden ? 0.0f : x;
                     }
-                }
-            } else {
-                f32x16 s[SB];
-#pragma unroll
-                for (int b = 0; b < SB; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[b][r] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < QS; ++i) {
-                    const x8 q = __builtin_bit_cast(x8, frag[buf][i][lane]);
-#pragma unroll
-                    for (int b = 0; b < SB; ++b) s[b] = mfma32(k[b][i], q, s[b]);
-                }
-#pragma unroll
-                for (int b = 0; b < SB; ++b)
+                } else {
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        sum[b][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], p.scale, -lse_now));
+                        sum[r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale, -lse_now[g]));
+                }
             }
         }
     }
     float* out = p.part_w ? p.part_w + ((int64_t)blockIdx.y * p.bh + bh) * p.most
                           : p.c.weights + z * p.c.slot_stride[0] + h * p.c.slot_stride[1];
 #pragma unroll
-    for (int b = 0; b < SB; ++b)
+    for (int r = 0; r < 16; ++r) {
+        float v = sum[r];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float v = sum[b][r];
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) v += __shfl_xor(v, d);
-            const int key = tile + 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-            if (col == 0 && key < len) {
-                if (p.part_w) out[key] = v;
-                else out[key] += v;
-            }
+        for (int d = 1; d < 32; d <<= 1) v += __shfl_xor(v, d);
+        const int key = tile + 8 * (r / 4) + 4 * half + r % 4;
+        if (col == 0 && key < len) {
+            if (p.part_w) out[key] = v;
+            else out[key] += v;
         }
+    }
 }
 
 // The sums of weights_kernel's parts, where the rows were split.
@@ -1300,7 +1294,8 @@ int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
     }
     if (a->accumulate && !plan.scores) {
         if (plan.weight_parts > 1) p.part_w = (float*)(ws + plan.part_w);
-        if (hipLaunchKernel(fn.weights, dim3((unsigned)weight_grid, (unsigned)plan.weight_parts), dim3(256), args, 0, (hipStream_t)stream) != hipSuccess)
+        const int threads = 64 * (a->cache.head_dim == 256 ? Weigh<256>::WAVES : Weigh<128>::WAVES);
+        if (hipLaunchKernel(fn.weights, dim3((unsigned)weight_grid, (unsigned)plan.weight_parts), dim3(threads), args, 0, (hipStream_t)stream) != hipSuccess)
             return RSFA_E_LAUNCH;
         if (plan.weight_parts > 1) {
             int parts = plan.weight_parts;

@@ -373,6 +373,22 @@ def test_scales_and_score_sizes():
             _check_attend(cache, got, q, [64], 1.0)
 
 
+@pytest.mark.parametrize("group, T", [(1, 401), (5, 107), (3, 211), (40, 9)])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_weights_of_many_rows(D, group, T):
+    # rows in several parts, which end inside of a block; scales of either sign; fewer tokens than the batch's most
+    Z, H, C = 2, 1, 530
+    cache = _filled(Z, H, C, D, BF16, 3)
+    q = _randn((Z, T, group, D), 5, BF16).transpose(1, 2)
+    counts, lengths = [T, T // 2 + 1], [C, 413]
+    q[1, :, counts[1]:] = math.nan
+    for scale, causal in ((0.11, True), (-0.11, False), (-0.07, True), (0.0, False)):
+        before = cache.weights.clone()
+        got = cache.attend(q, _ints(lengths), causal, scale, counts=_ints(counts), accumulate=True, return_lse=True)
+        _check_attend(cache, got, q, lengths, scale, before, cache.positions if causal else None,
+                      [n - c for n, c in zip(lengths, counts)], counts)
+
+
 def test_overflowing_scores_are_nan_or_dominate_as_in_ieee():
     cache = Cache4(1, 1, 40, 64, BF16)
     k = torch.zeros((1, 1, 40, 64), dtype=BF16).cuda()
