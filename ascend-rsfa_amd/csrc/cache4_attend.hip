@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
     }
 }
 
-// Many rows: each of the workgroup's four waves has 32 rows of its own, and all
+// Many rows: each of the workgroup's W waves has 32 rows of its own, and all
 // share the key tile.  Its codes are converted once per workgroup and kept in LDS as
 // the operands of v_mfma_f32_32x32x16 themselves: fragment f is 64 lanes of 16 bytes,
 // so that writes and reads are linear.  Of the two buffers one is computed with while
@@ -478,20 +478,27 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
 //   O^T = V^T P^T  S^T leaves lane l the row l % 32 and the keys 8 a + 4 (l / 32) + b;
 //                step s takes k = 8 (l / 32) + j as key 16 s + 8 (j / 4) + 4 (l / 32) + j % 4.
 //                A: lane l has these keys of the value (l % 32) * D/32 + t in fragment t.
+// With eight waves a tile is computed with in two pieces; half of the waves convert their
+// part of the next tile before the first piece, half after it, so that the two waves of a SIMD
+// want the matrix unit at different times.
 // Bound by the matrix and the vector units together: a chunk of 2048 tokens, 32 heads,
-// over 16384 slots of 8 key heads, D = 128, bf16, causal: 545 to 615 us, 840 to 945 TFLOP/s,
-// the MFMAs busy 38 % and vector instructions issuing 48 % of the cycles.  (Direct
-// operands without LDS, 32 rows a wave: 1107 us.  Halves of a tile whose softmax and
-// products alternate: 805.  Raised wave priority around the products: 582 against 559; LDS
-// reads two to eight MFMAs ahead: the same.)
-template <int D>
+// over 16384 slots of 8 key heads, D = 128, bf16, causal: 490 us, 1050 TFLOP/s.  (Four waves,
+// which convert twice as often: 575; eight that convert together: 495, at D = 64 290
+// against 280 and at D = 256 494 against 459 of the whole call for 1024 tokens.  The two pieces in
+// a loop instead of code of their own: 40 us more.  Direct operands
+// without LDS, 32 rows a wave: 1107.  Halves of a tile whose softmax and products alternate,
+// raised wave priority around the products, LDS reads two to eight MFMAs ahead:
+// no gain with four waves.)
+template <int D, int W>
 struct Many {
-    static constexpr int KEYS = D == 256 ? 32 : 64;  // of a tile: its fragments take 32 KB at D = 128, 256
-    static constexpr int KF = KEYS / 32 * (D / 16) / 4;  // K fragments a wave converts
-    static constexpr int VF = KEYS / 16 * (D / 32) / 4;  // V fragments
-    static constexpr int KFRAGS = 4 * KF, FRAGS = 4 * (KF + VF);
-    static constexpr int PER_BLOCK = 4 / (KEYS / 32);    // waves that share a block of 32 keys' K
-    static constexpr int ROWS = 128;
+    static constexpr int PIECE = D == 256 ? 32 : 64;     // keys between two looks at the running maximum
+    static constexpr int PIECES = W / 4;
+    static constexpr int KEYS = PIECE * PIECES;          // of a tile: its fragments take 8 KB a wave at D = 128, 256
+    static constexpr int KF = KEYS / 32 * (D / 16) / W;  // K fragments a wave converts
+    static constexpr int VF = KEYS / 16 * (D / 32) / W;  // V fragments
+    static constexpr int KFRAGS = W * KF, FRAGS = W * (KF + VF);
+    static constexpr int PER_BLOCK = W / (KEYS / 32);    // waves that share a block of 32 keys' K
+    static constexpr int ROWS = 32 * W;
 };
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -503,15 +510,15 @@ __device__ __forceinline__ f32x16 mfma32(BF16::x8 a, BF16::x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-template <class T, int D, bool CAUSAL>
-__global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
-    typedef Many<D> M;
+template <class T, int D, bool CAUSAL, int W>
+__global__ void __launch_bounds__(64 * W, 2) attend_many_kernel(AttendParams p) {
+    typedef Many<D, W> M;
     typedef typename T::x8 x8;
     typedef typename T::elem elem;
-    constexpr int QS = D / 16, DT = D / 32, KEYS = M::KEYS, SB = KEYS / 32;
+    constexpr int QS = D / 16, DT = D / 32, KEYS = M::KEYS, PIECE = M::PIECE, SB = PIECE / 32;
     __shared__ u32x4 frag[2][M::FRAGS][64];
     __shared__ int kpos[2][CAUSAL ? KEYS : 1];
-    __shared__ int spoiled[2][4];  // a wave's V codes of the tile hold a NaN block
+    __shared__ int spoiled[2][W];  // a wave's V codes of the tile hold a NaN block
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int bh = blockIdx.x % p.bh;  // with a multiple of 8, a head's row tiles meet in one XCD's L2
@@ -668,10 +675,12 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
     float m = NEVER, l = 0.0f;
 
-    auto compute = [&](int buf, int tile) {
-        bool masked = tile + KEYS > end;
+    auto compute = [&](int buf, int tile, int piece) {
+        const int kb = piece * SB, vb = M::KFRAGS + piece * 2 * SB * DT, at = piece * PIECE;
+        tile += at;
+        bool masked = tile + PIECE > end;
         if (CAUSAL) {
-            const int kp = kpos[buf][lane & (KEYS - 1)];
+            const int kp = kpos[buf][at + (lane & (PIECE - 1))];
             masked |= __any(kp > least);
             if (!__any(kp <= greatest)) return;
         }
@@ -683,7 +692,7 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
 #pragma unroll
         for (int i = 0; i < QS; ++i)
 #pragma unroll
-            for (int b = 0; b < SB; ++b) s[b] = mfma32(__builtin_bit_cast(x8, frag[buf][b * QS + i][lane]), q[i], s[b]);
+            for (int b = 0; b < SB; ++b) s[b] = mfma32(__builtin_bit_cast(x8, frag[buf][(kb + b) * QS + i][lane]), q[i], s[b]);
         if (__builtin_expect(masked, 0)) {
 #pragma unroll
             for (int b = 0; b < SB; ++b)
@@ -691,7 +700,7 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
                 for (int r = 0; r < 16; ++r) {
                     const int key = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
                     bool hidden = tile + key >= end;
-                    if (CAUSAL) hidden |= kpos[buf][key] > qpos;
+                    if (CAUSAL) hidden |= kpos[buf][at + key] > qpos;
                     if (hidden) s[b][r] = -INFINITY;
                 }
         }
@@ -725,14 +734,17 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
         for (int k = 0; k < 2 * SB; ++k)
 #pragma unroll
             for (int d = 0; d < DT; ++d)
-                acc[d] = mfma32(__builtin_bit_cast(x8, frag[buf][M::KFRAGS + k * DT + d][lane]), pb[k], acc[d]);
-        if (__builtin_expect(spoiled[buf][0] | spoiled[buf][1] | spoiled[buf][2] | spoiled[buf][3], 0)) {
+                acc[d] = mfma32(__builtin_bit_cast(x8, frag[buf][vb + k * DT + d][lane]), pb[k], acc[d]);
+        int nan = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) nan |= spoiled[buf][w];
+        if (__builtin_expect(nan, 0)) {
             // NaN blocks of V, into the rows that see them: register r holds the values
             // D/32 (8 (r / 4) + 4 half + r % 4) + d, which lie in one block
             uint32_t hit = 0;
-            for (int k = 0; k < KEYS && tile + k < end; ++k) {
+            for (int k = 0; k < PIECE && tile + k < end; ++k) {
                 bool sees = true;
-                if (CAUSAL) sees = kpos[buf][k] <= qpos;
+                if (CAUSAL) sees = kpos[buf][at + k] <= qpos;
                 if (!sees) continue;
                 for (int r = 0; r < 16; ++r) {
                     const int i = 8 * (r / 4) + 4 * half + r % 4;
@@ -747,6 +759,7 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
         }
     };
 
+    const bool late = W > 4 && wave >= 4;
     if (start < end) {
         load(start);
         convert(0);
@@ -754,9 +767,13 @@ __global__ void __launch_bounds__(256, 2) attend_many_kernel(AttendParams p) {
         int buf = 0;
         for (int tile = start; tile < end; tile += KEYS, buf ^= 1) {
             __syncthreads();  // this tile is in LDS, and nobody reads the other buffer any more
+            if (late) compute(buf, tile, 0);
             if (tile + KEYS < end) convert(buf ^ 1);
             if (tile + 2 * KEYS < end) load(tile + 2 * KEYS);
-            compute(buf, tile);
+            if (!late) compute(buf, tile, 0);
+#pragma unroll
+            for (int i = 1; i < M::PIECES; ++i)
+                if (tile + i * PIECE < end) compute(buf, tile, i);
         }
     }
     l += __shfl_xor(l, 32);
@@ -1125,7 +1142,7 @@ __global__ void __launch_bounds__(256) join_weights_kernel(AttendParams p, int p
 struct Plan {
     bool few;          // attend_kernel, with nb blocks of 16 rows
     int nb;
-    int tiles, splits;
+    int waves, tiles, splits;
     bool scores;       // weights from stored scores
     int weight_tiles, weight_parts;
     uint64_t part_w;
@@ -1143,14 +1160,17 @@ Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
     const bool few = rows <= 32;
     p.few = few;
     p.nb = rows <= 16 || a->cache.head_dim == 256 ? 1 : 2;
-    const int64_t tile_rows = few ? 16 * p.nb : 128;
+    // (D = 256, four and eight waves: 128 rows of 32 heads of 8192 slots 83 and 91 us, 192 rows 108 and 97; below
+    // 256 eight are never slower: 64 rows at D = 128 31.6 and 30.7, 384 rows 93 and 71)
+    p.waves = few || (a->cache.head_dim == 256 && rows <= 128) ? 4 : 8;
+    const int64_t tile_rows = few ? 16 * p.nb : 32 * p.waves;
     p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
     // Enough workgroups for the chip, of at least four steps each.  Few rows: eight
     // workgroups a CU even out lengths (64 sequences of 1024 to 4096 slots 46.6 -> 44.9 us
     // against four); fewer steps each cost more in joining them (one sequence of
     // 32768 slots: 13.1, 16.4 with two steps each, 22.9 with one).
-    const int64_t step = few ? 4 * TILE : 64;
-    const int64_t full = (few ? 8 : 2) * (int64_t)cus;
+    const int64_t step = few ? 4 * TILE : 16 * p.waves;
+    const int64_t full = (few ? 8 : 8 / p.waves) * (int64_t)cus;
     const int64_t want = (full + bh * p.tiles - 1) / (bh * p.tiles);
     const int64_t able = (most + 4 * step - 1) / (4 * step);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, able), 256));
@@ -1193,7 +1213,9 @@ const void* attend_fn(const Plan& p) {
             if (p.nb == 2) return (const void*)&attend_kernel<T, D, 2, CAUSAL>;
         return (const void*)&attend_kernel<T, D, 1, CAUSAL>;
     }
-    return (const void*)&attend_many_kernel<T, D, CAUSAL>;
+    if constexpr (D == 256)
+        if (p.waves == 4) return (const void*)&attend_many_kernel<T, D, CAUSAL, 4>;
+    return (const void*)&attend_many_kernel<T, D, CAUSAL, 8>;
 }
 
 struct Functions {
@@ -1277,7 +1299,7 @@ int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
     const int64_t join_grid = (int64_t)p.bh * ((p.most + 255) / 256);
     if (grid > 0x7fffffff || (a->accumulate && join_grid > 0x7fffffff)) return RSFA_E_CACHE;
     void* args[] = {&p};
-    if (hipLaunchKernel(fn.attend, dim3((unsigned)grid, (unsigned)plan.splits), dim3(256), args, 0, (hipStream_t)stream) != hipSuccess)
+    if (hipLaunchKernel(fn.attend, dim3((unsigned)grid, (unsigned)plan.splits), dim3(64 * plan.waves), args, 0, (hipStream_t)stream) != hipSuccess)
         return RSFA_E_LAUNCH;
     if (plan.splits > 1 || plan.scores) {
         const int64_t rows = (int64_t)p.bh * p.rows;

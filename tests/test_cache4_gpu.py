@@ -294,7 +294,7 @@ def test_attend_matches_the_definition(shape, dtype, causal):
     _check_attend(cache, plain, q, lengths, scale, None, cache.positions if causal else None, first)
 
 
-@pytest.mark.parametrize("T", [1, 3, 9, 50])
+@pytest.mark.parametrize("T", [1, 3, 9, 50, 90])
 @pytest.mark.parametrize("D", [32, 64, 128, 256])
 def test_attend_masks_by_position(D, T):
     # positions in no order, some rows seeing nothing, some tiles seen by no row
@@ -327,7 +327,7 @@ def test_attend_with_counts_of_a_padded_batch(T):
             assert (got[0][z, :, counts[z]:] == 0).all() and (got[1][z, :, counts[z]:] == -math.inf).all()
 
 
-@pytest.mark.parametrize("T", [1, 4, 40])
+@pytest.mark.parametrize("T", [1, 4, 40, 97])
 @pytest.mark.parametrize("D", [32, 64, 128, 256])
 def test_non_finite_rows_reach_only_the_queries_that_see_them(D, T):
     Z, H, Hq, C = 1, 2, 4, 140
