@@ -5,16 +5,18 @@
 // of a row (a sequence and head) is found digit by digit, 2048 bins in LDS, from the
 // range that the row's keys span, so that the first digit already spreads them
 // (the leading bits of a float hardly differ within a row); once a bin holds at most
-// 256 keys, they are ranked directly, each against all.  Up to 8192 slots a workgroup does it for a row,
-// with the keys in registers; longer rows are cut into parts, whose workgroups
+// 256 keys, they are ranked directly, each against all.  Up to 32768 slots a workgroup does it for
+// a row, with the keys in registers; longer rows are cut into parts, whose workgroups
 // meet between four launches (survey, histogram, collect, choose).  The order of
 // atomics has no say in the result: they only count, and lists are only counted.
 // gather_kernel copies the slots that stay, 16 bytes of codes and the scale byte of
 // their block a lane.
 // Bound: reading 4 (weights) + 4 (positions, where some are protected) bytes a slot, and
 // 2 * (D/2 + D/32) + 8 bytes in and out of each slot that is copied.  In practice by
-// latency: one slot of 2048 for 256 rows 6 us; 4096 slots of 64 rows 10 (their bytes: 0.4);
-// 32768 of 32 rows 33 in four launches (one workgroup a row: 48), 65521 of 8 rows 37 (123).
+// latency: one slot of 2048 for 256 rows 6 us; 4096 slots of 64 rows 9.5 (their bytes: 0.4);
+// and by the instructions of one workgroup, some 0.75 us for every 1024 slots beyond 8192: 16384 slots of 32
+// rows 15 us, 32768 25, of 256 rows 18 and 32 (in four launches 32 and 33, 49 and 96);
+// 65521 of 8 rows 37 in four launches (64 keys a thread do not fit the registers: 123).
 // The copy of 65520 slots at D = 256 takes 9 us, 4 TB/s.
 #include "cache4.hpp"
 
@@ -169,8 +171,10 @@ __device__ __forceinline__ void search(Shared<THREADS>& sh, E&& each, uint32_t l
         for (int i = threadIdx.x; i < BINS; i += THREADS) sh.bins[i] = 0;
         if (threadIdx.x == 0) sh.listed = 0;
         __syncthreads();
-        auto inside = [&](uint32_t k, int w) { return k != PROTECTED && k >= base && (w == 32 || ((k - base) >> w) == 0); };
-        each([&](uint32_t k) { count_key(sh, inside(k, width), (k - base) >> shift, lane); });
+        // (the largest key bounds the bins too: protected ones lie above it, and keys below base wrap around)
+        auto last = [&](int w) { return min(high - base, w == 32 ? 0xffffffffu : (1u << w) - 1); };
+        uint32_t limit = last(width);
+        each([&](uint32_t k) { count_key(sh, k - base <= limit, (k - base) >> shift, lane); });
         __syncthreads();
         find_bin(sh, rest, lane, wave, [&](int i) { return sh.bins[i]; });
         base += sh.found[0] << shift;
@@ -178,8 +182,9 @@ __device__ __forceinline__ void search(Shared<THREADS>& sh, E&& each, uint32_t l
         width = shift;
         const uint32_t c = sh.found[2];
         if (width > 0 && c <= RANKED) {
+            limit = last(width);
             each([&](uint32_t k) {
-                if (inside(k, width)) sh.list[atomicAdd(&sh.listed, 1u)] = k;
+                if (k - base <= limit) sh.list[atomicAdd(&sh.listed, 1u)] = k;
             });
             __syncthreads();  // (found is read by all before it is written again)
             rank_listed(sh, c, rest, edge, ties);
@@ -196,23 +201,26 @@ __device__ __forceinline__ void search(Shared<THREADS>& sh, E&& each, uint32_t l
 struct Writer {
     const EvictParams& p;
     int32_t* out;
-    int64_t free, ties, gone, seen;
-    uint32_t edge;
-    int len, lane;
-    __device__ __forceinline__ void operator()(uint32_t k, int64_t i) {
-        const bool live = i < len;
-        const uint64_t lower = ((uint64_t)1 << lane) - 1;
+    uint32_t free, ties, gone, seen, edge;
+    int len;
+    static __device__ __forceinline__ uint32_t before(uint64_t mask, uint32_t base) {
+        return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, base));
+    }
+    __device__ __forceinline__ void operator()(uint32_t k, uint32_t i) {
+        const bool live = i < (uint32_t)len;
+        bool goes = live && k < edge;
         const uint64_t eq = __ballot(live && k == edge);
-        const bool goes = live && (k < edge || (k == edge && seen + __popcll(eq & lower) < ties));
+        if (eq) {
+            goes |= live && k == edge && before(eq, seen) < ties;
+            seen += __popcll(eq);
+        }
         const uint64_t who = __ballot(goes);
-        const int64_t rank = gone + __popcll(who & lower);
         if (p.evict) {
-            if (live && !goes) out[i - rank] = (int32_t)i;
+            if (live && !goes) out[i - before(who, gone)] = (int32_t)i;
         } else if (goes) {
-            out[free + rank] = (int32_t)i;
+            out[before(who, free + gone)] = (int32_t)i;
         }
         gone += __popcll(who);
-        seen += __popcll(eq);
     }
 };
 
@@ -252,19 +260,35 @@ __global__ void __launch_bounds__(THREADS) select_kernel(EvictParams p) {
     const int seg = wave * 64 * KPT;
     uint32_t held[KPT];
     {
-        int v[KPT];
-        float w[KPT];
+        // positions stay in registers too, up to 16 a thread; else they are read again (32768 slots of 32 rows, all
+        // kept: 36.4 us, spilled; read again: 31.4)
+        constexpr int U = KPT < 16 ? KPT : 16;
+        const int slot = seg + lane, last = max(r.len - 1, 0);  // (beyond: the last again, no branches)
+        int v[U];
+        auto positions = [&](int j0) {
 #pragma unroll
-        for (int j = 0; j < KPT; ++j) {
-            const int i = seg + 64 * j + lane;
-            v[j] = r.guarded && i < r.len ? r.pos[i] : -0x7fffffff - 1;
-            w[j] = i < r.len ? r.weights[i] : 0.0f;
+            for (int u = 0; u < U; ++u) {
+                v[u] = r.pos[min(slot + 64 * (j0 + u), last)];
+            }
+        };
+        if (r.guarded) positions(0);
+#pragma unroll
+        for (int j0 = 0; j0 < KPT; j0 += U) {
+            float w[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) w[u] = r.weights[min(slot + 64 * (j0 + u), last)];
+#pragma unroll
+            for (int u = 0; u < U; ++u) held[j0 + u] = slot + 64 * (j0 + u) < r.len ? key_of(w[u]) : PROTECTED;
         }
         int64_t old = 0x7fffffffll + 1;  // positions above it are protected
         if (p.recent > 0) {
             int top = v[0];
 #pragma unroll
-            for (int j = 1; j < KPT; ++j) top = max(top, v[j]);
+            for (int j0 = 0; j0 < KPT; j0 += U) {
+                if (j0) positions(j0);
+#pragma unroll
+                for (int u = 0; u < U; ++u) top = max(top, v[u]);
+            }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) top = max(top, __shfl_xor(top, d));
             if (lane == 0) sh.wave[3][wave] = (uint32_t)top;
@@ -272,10 +296,14 @@ __global__ void __launch_bounds__(THREADS) select_kernel(EvictParams p) {
             for (int i = 0; i < WAVES; ++i) top = max(top, (int)sh.wave[3][i]);
             old = (int64_t)top - p.recent;
         }
+        if (r.guarded) {
 #pragma unroll
-        for (int j = 0; j < KPT; ++j) {
-            const bool safe = r.guarded && ((int64_t)v[j] > old || (int64_t)v[j] < p.sinks);
-            held[j] = seg + 64 * j + lane >= r.len || safe ? PROTECTED : key_of(w[j]);
+            for (int j0 = 0; j0 < KPT; j0 += U) {
+                if (KPT > U) positions(j0);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if ((int64_t)v[u] > old || (int64_t)v[u] < p.sinks) held[j0 + u] = PROTECTED;
+            }
         }
     }
     auto each = [&](auto&& f) {
@@ -318,10 +346,14 @@ __global__ void __launch_bounds__(THREADS) select_kernel(EvictParams p) {
     }
 
     // ranks: counts of the waves before, then along the wave
+    // (asm: or the compiler keeps two masks a key, of the comparisons that it then need not
+    // repeat, and spills hundreds of scalar registers)
     uint32_t below = 0, same = 0;
+    int at = seg + lane;
+    asm("" : "+v"(at));
 #pragma unroll
     for (int j = 0; j < KPT; ++j) {
-        const bool live = seg + 64 * j + lane < r.len;
+        const bool live = at + 64 * j < r.len;
         below += __popcll(__ballot(live && held[j] < edge));
         same += __popcll(__ballot(live && held[j] == edge));
     }
@@ -331,9 +363,10 @@ __global__ void __launch_bounds__(THREADS) select_kernel(EvictParams p) {
     for (int w = 0; w < wave; ++w) gone += sh.wave[0][w], seen += sh.wave[1][w];
     gone += min(seen, ties);
     int32_t* out = p.out + (int64_t)r.bh * (p.evict ? p.budget : p.n);
-    Writer write{p, out, free, ties, gone, seen, edge, r.len, lane};
+    asm("" : "+v"(at), "+v"(edge));
+    Writer write{p, out, (uint32_t)free, (uint32_t)ties, (uint32_t)gone, (uint32_t)seen, edge, r.len};
 #pragma unroll
-    for (int j = 0; j < KPT; ++j) write(held[j], seg + 64 * j + lane);
+    for (int j = 0; j < KPT; ++j) write(held[j], (uint32_t)(at + 64 * j));
     if (!p.evict) write_rest(p, out, r.len, free, v, threadIdx.x, THREADS);
 }
 
@@ -400,7 +433,7 @@ __global__ void __launch_bounds__(PART_THREADS) survey_kernel(EvictParams p) {
 
 struct Range {
     int64_t old;  // positions above it are protected
-    uint32_t low;
+    uint32_t low, high;
     int shift;    // of the first digit
 };
 
@@ -417,7 +450,7 @@ __device__ __forceinline__ Range range_of(const EvictParams& p, int bh, int lane
         high = max(high, (uint32_t)__shfl_xor((int)high, d));
     }
     const int width = high <= low ? 0 : 32 - __clz((int)(high - low));
-    return {p.recent > 0 ? (int64_t)top - p.recent : 0x7fffffffll + 1, low, width > DIGIT ? width - DIGIT : 0};
+    return {p.recent > 0 ? (int64_t)top - p.recent : 0x7fffffffll + 1, low, high, width > DIGIT ? width - DIGIT : 0};
 }
 
 // The first digit's counts of the part's unprotected keys.
@@ -533,7 +566,7 @@ __global__ void __launch_bounds__(PART_THREADS) choose_kernel(EvictParams p) {
             auto each = [&](auto&& f) {
                 for (uint32_t i = 64 * wave; i < inside; i += PART_THREADS) f(i + lane < inside ? list[i + lane] : PROTECTED);
             };
-            search(sh, each, base, base + ((1u << g.shift) - 1), rest, lane, wave, edge, ties);
+            search(sh, each, base, base + min(g.high - base, (1u << g.shift) - 1), rest, lane, wave, edge, ties);
         }
         // of the parts before: keys below the edge, and equal to it
         uint32_t below = wave == 0 && lane < (int)blockIdx.y ? (uint32_t)n.x : 0, same = 0;
@@ -599,12 +632,12 @@ __global__ void __launch_bounds__(PART_THREADS) choose_kernel(EvictParams p) {
     for (int w = 0; w < wave; ++w) gone += sh.wave[0][w], seen += sh.wave[1][w];
     gone += min(seen, ties);
     int32_t* out = p.out + (int64_t)r.bh * (p.evict ? p.budget : p.n);
-    Writer write{p, out, free, ties, gone, seen, edge, r.len, lane};
+    Writer write{p, out, (uint32_t)free, (uint32_t)ties, (uint32_t)gone, (uint32_t)seen, edge, r.len};
     if (hold) {
 #pragma unroll
-        for (int j = 0; j < HELD; ++j) write(held[j], first + 64 * j + lane);
+        for (int j = 0; j < HELD; ++j) write(held[j], (uint32_t)(first + 64 * j + lane));
     } else {
-        each_of_part(p, r, g.old, lane, wave, [&](uint32_t k, int64_t i, int) { write(k, i); });
+        each_of_part(p, r, g.old, lane, wave, [&](uint32_t k, int64_t i, int) { write(k, (uint32_t)i); });
     }
     if (!p.evict) write_rest(p, out, r.len, free, v, (int64_t)blockIdx.y * PART_THREADS + threadIdx.x, (int64_t)p.parts * PART_THREADS);
 }
@@ -639,7 +672,7 @@ __global__ void __launch_bounds__(256) gather_kernel(EvictParams p) {
     }
 }
 
-constexpr int64_t WHOLE_ROW = 8192;  // slots that one workgroup chooses among
+constexpr int64_t WHOLE_ROW = 32768;  // slots that one workgroup chooses among
 
 // Parts of a row, and the workspace: 4096 slots a part, up to 32 parts of more.
 struct Plan {
@@ -722,12 +755,15 @@ int evict_launch(const rsfa_cache4_evict_args* a, bool evict, void* stream) {
         return hipLaunchKernel(fn, grid, dim3((unsigned)threads), args, 0, (hipStream_t)stream) == hipSuccess;
     };
     if (!plan.parts) {
-        // eight slots a thread (4096 slots of 64 rows, with the copy: 14.9 us, 18.2 with 16 or 32 a thread)
+        // eight slots a thread (4096 slots of 64 rows, with the copy: 13.8 us, 15.9 with 16), until that takes
+        // more than the largest workgroup
         const int64_t c = a->cache.capacity;
         const void* fn = (const void*)&select_kernel<1024, 8>;
         int threads = 1024;
         if (c <= 2048) fn = (const void*)&select_kernel<256, 8>, threads = 256;
         else if (c <= 4096) fn = (const void*)&select_kernel<512, 8>, threads = 512;
+        else if (c > 16384) fn = (const void*)&select_kernel<1024, 32>;
+        else if (c > 8192) fn = (const void*)&select_kernel<1024, 16>;
         if (!launch(fn, dim3((unsigned)bh), threads)) return RSFA_E_LAUNCH;
     } else {
         const dim3 grid((unsigned)bh, (unsigned)plan.parts);

@@ -477,7 +477,7 @@ def _weights(shape, seed, kind):
 
 
 @pytest.mark.parametrize("kind", ["spread", "ties", "zeros", "odd"])
-@pytest.mark.parametrize("C", [1, 5, 64, 2048, 2100, 8192, 8193, 40000])
+@pytest.mark.parametrize("C", [1, 5, 64, 2048, 2100, 8192, 8193, 16384, 16385, 32768, 32769, 40000, 140000])
 def test_claim_matches_the_definition(C, kind):
     Z, H = 3, 2
     cache = Cache4(Z, H, C, 32)
@@ -494,7 +494,8 @@ def test_claim_matches_the_definition(C, kind):
 
 
 @pytest.mark.parametrize("kind", ["spread", "ties", "zeros", "odd"])
-@pytest.mark.parametrize("C,D", [(1, 32), (70, 64), (700, 128), (3000, 256), (40000, 32), (66000, 32), (70000, 32)])
+@pytest.mark.parametrize("C,D", [(1, 32), (70, 64), (700, 128), (3000, 256), (20000, 64), (40000, 32), (66000, 32),
+                                 (70000, 32), (140000, 32)])
 def test_evict_matches_the_definition(C, D, kind):
     Z, H = (2, 2) if C < 10000 else (1, 2)
     cache = _filled(Z, H, C, D, F16, 3)
