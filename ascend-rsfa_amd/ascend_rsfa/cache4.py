@@ -95,6 +95,21 @@ def _meet(a, b):
     return False
 
 
+def _overlaps_itself(t):
+    """Whether sequences and heads of a buffer [Z, H, C, ...] share memory with each other."""
+    size = t[0, 0].numel()
+    outer = sorted((s, n) for s, n in zip(t.stride()[:2], t.shape[:2]) if n > 1)
+    need = size
+    for s, n in outer:
+        if s < need:
+            break
+        need = s * (n - 1) + need
+    else:
+        return False
+    starts = sorted(z * t.stride(0) + h * t.stride(1) for z in range(t.shape[0]) for h in range(t.shape[1]))
+    return any(b - a < size for a, b in zip(starts, starts[1:]))
+
+
 def _no_gradient(*tensors):
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("a Cache4 keeps no gradients: call it under torch.no_grad()")
@@ -157,8 +172,8 @@ class Cache4:
             row = shape[3] if len(shape) == 4 else 1
             if (C > 1 and st[2] != row) or (row > 1 and st[3] != 1):
                 raise ValueError(f"{name}: the rows of a sequence and head must lie densely")
-            if (Z > 1 and st[0] == 0) or (H > 1 and st[1] == 0):
-                raise ValueError(f"{name} is expanded: its sequences and heads must not share memory")
+            if _overlaps_itself(t):
+                raise ValueError(f"{name}: its sequences and heads must not share memory")
             strides.append(tuple(st[:2]))
         for a, b in ((0, 1), (2, 3)) + (((4, 5),) if weights is not None else ()):
             if strides[a] != strides[b]:
@@ -168,6 +183,11 @@ class Cache4:
         width = D // 32
         if any(s % width for s in strides[2]) or (ks.data_ptr() | vs.data_ptr()) % width:
             raise ValueError(f"scales must be {width}-byte aligned, with strides that are multiples of {width}")
+        spans = [(t, *_span(t)) for _, t, _, _ in named]
+        for i, (a, a0, a1) in enumerate(spans):
+            for j, (b, b0, b1) in enumerate(spans[:i]):
+                if a0 < b1 and b0 < a1 and _meet(a, b):
+                    raise ValueError(f"{named[j][0]} and {named[i][0]} must not share memory")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = kc, ks, vc, vs
         self.positions, self.weights, self.dtype = positions, weights, dtype
         self.Z, self.H, self.capacity, self.head_dim, self.device = Z, H, C, D, kc.device
@@ -180,7 +200,7 @@ class Cache4:
         c.dtype = _DTYPES[dtype]
         self._c = c
         self._z = torch.Size((Z,))
-        self._spans = [(t, *_span(t)) for _, t, _, _ in named]
+        self._spans = spans
         self._kept = {}
 
     def _keep(self, key, parts):
@@ -447,7 +467,8 @@ class Cache4:
         if (into.Z, into.H, into.head_dim, into.dtype, into.device) != (
                 self.Z, self.H, self.head_dim, self.dtype, self.device):
             raise ValueError("into must have this cache's sequences, heads, head_dim, dtype and device")
-        for (a, a0, a1), (b, b0, b1) in zip(self._spans, into._spans):
-            if a0 < b1 and b0 < a1 and _meet(a, b):
-                raise ValueError("into must not share memory with this cache")
+        for a, a0, a1 in self._spans:
+            for b, b0, b1 in into._spans:
+                if a0 < b1 and b0 < a1 and _meet(a, b):
+                    raise ValueError("into must not share memory with this cache")
         self._evict_call("rsfa_cache4_evict", into, lengths, 1, into.capacity if budget is None else budget, recent, sinks, 0)

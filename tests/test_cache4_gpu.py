@@ -653,6 +653,31 @@ def test_two_streams_at_once():
 
 
 # -- refusals -----------------------------------------------------------------
+def test_buffers_that_share_memory_are_refused():
+    def buffers(C=20):
+        return {n: torch.zeros((3, 2, C) + ((32,) if "codes" in n else (2,) if "scales" in n else ()), dtype=t).cuda() for n, t in (
+            ("k_codes", torch.uint8), ("k_scales", torch.uint8), ("v_codes", torch.uint8), ("v_scales", torch.uint8),
+            ("positions", torch.int32), ("weights", torch.float32))}
+
+    a, big = buffers(), buffers(40)
+    first, second = ({n: t[:, :, i:i + 20] for n, t in big.items()} for i in (0, 20))  # halves of one cache's slots
+    into, cache = Cache4.from_buffers(**second), Cache4.from_buffers(**first)
+    cache.evict(into, 20, budget=3)
+    swapped = dict(first, k_codes=second["v_codes"], v_codes=second["k_codes"])
+    for bad in (lambda: Cache4.from_buffers(**dict(a, v_codes=a["k_codes"])),
+                lambda: Cache4.from_buffers(**dict(a, weights=a["positions"].view(torch.float32))),
+                lambda: Cache4.from_buffers(**dict(a, k_scales=a["k_codes"].view(-1)[:240].view(3, 2, 20, 2))),
+                # heads 16 slots apart, of 20 each; sequences that meet the heads of the one before
+                lambda: Cache4.from_buffers(**{n: t.as_strided(t.shape, (64 * t[0, 0, 0].numel(), 16 * t[0, 0, 0].numel()) + t.stride()[2:])
+                                               for n, t in big.items()}),
+                lambda: Cache4.from_buffers(**{n: t.as_strided((3, 2) + t.shape[2:], (t.stride(1), t.stride(1)) + t.stride()[2:])
+                                               for n, t in a.items()}),
+                lambda: cache.evict(Cache4.from_buffers(**first), 20, budget=3),
+                lambda: into.evict(Cache4.from_buffers(**swapped), 20, budget=3)):
+        with pytest.raises(ValueError, match="share memory"):
+            bad()
+
+
 def test_refusals():
     cache = Cache4(2, 2, 16, 64, F16)
     bare = Cache4(2, 2, 16, 64, F16, weights=False)
