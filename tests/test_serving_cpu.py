@@ -212,12 +212,12 @@ def test_cache_calls_abi_refusals():
     need = lib.rsfa_cache4_evict_workspace_bytes(ctypes.byref(_evict()), 1)
     assert need >= 2 * 3 * 16 * 4 and lib.rsfa_cache4_evict_workspace_bytes(ctypes.byref(_evict()), 0) == 0
     assert lib.rsfa_cache4_evict_workspace_bytes(ctypes.byref(_evict(budget=0)), 1) == 0
-    long = {"capacity": 9000, "code_stride": (ctypes.c_int64 * 2)(3 * 9000 * 64, 9000 * 64)}
+    long = {"capacity": 40000, "code_stride": (ctypes.c_int64 * 2)(3 * 40000 * 64, 40000 * 64)}
     assert lib.rsfa_cache4_evict_workspace_bytes(ctypes.byref(_evict(_cache(**long))), 0) > 0
     assert lib.rsfa_cache4_claim(ctypes.byref(_evict(out=None)), None) == _native.E_NULL
     for make, fn in ((lambda **k: _evict(**k), lib.rsfa_cache4_evict), (lambda **k: _evict(_cache(**long), **k), lib.rsfa_cache4_claim)):
         for over in ({"workspace": None}, {"workspace_bytes": 8}):
             assert fn(ctypes.byref(make(**over)), None) == _native.E_WORKSPACE
-        assert fn(ctypes.byref(make(workspace=0x1008)), None) == _native.E_ALIGN
+        assert fn(ctypes.byref(make(workspace=0x1008, workspace_bytes=1 << 30)), None) == _native.E_ALIGN
     for over in ({"z": 1}, {"h": 2}, {"head_dim": 64}, {"dtype": 1}, {"capacity": 15}):
         assert lib.rsfa_cache4_evict(ctypes.byref(_evict(into=_cache(**{"capacity": 16, **over}))), None) == _native.E_BUDGET
