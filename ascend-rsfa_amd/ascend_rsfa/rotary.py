@@ -289,7 +289,8 @@ def rotary(q, k, positions, plan):
 
 
 def rotary_(q, k, positions, plan):
-    """``rotary`` in place (inference); the values beyond ``rotary_dim`` are not touched."""
+    """``rotary`` in place (inference); the values beyond ``rotary_dim`` are not touched.  q and k (parts of one
+    fused tensor, say) must not share elements."""
     _checked(q, k, positions, plan)
     for x in (q, k):
         if x is None:

@@ -482,10 +482,10 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
 // part of the next tile before the first piece, half after it, so that the two waves of a SIMD
 // want the matrix unit at different times.
 // Bound by the matrix and the vector units together: a chunk of 2048 tokens, 32 heads,
-// over 16384 slots of 8 key heads, D = 128, bf16, causal: 490 us, 1050 TFLOP/s.  (Four waves,
-// which convert twice as often: 575; eight that convert together: 495, at D = 64 290
-// against 280 and at D = 256 494 against 459 of the whole call for 1024 tokens.  The two pieces in
-// a loop instead of code of their own: 40 us more.  Direct operands
+// over 16384 slots of 8 key heads, D = 128, bf16, causal: 468 us, 1100 TFLOP/s.  (Four waves,
+// which convert twice as often: 75 us more; eight that convert together: 3, at D = 64 290
+// against 280 and at D = 256 494 against 459 of calls for 1024 tokens with weights.  The two
+// pieces in a loop instead of code of their own: 40 us more.  Direct operands
 // without LDS, 32 rows a wave: 1107.  Halves of a tile whose softmax and products alternate,
 // raised wave priority around the products, LDS reads two to eight MFMAs ahead:
 // no gain with four waves.)
@@ -948,11 +948,11 @@ __global__ void __launch_bounds__(256) finish_kernel(AttendParams p, int pp, int
 // registers at D = 128, 64 at 256); blocks of 32 rows of Q pass by in LDS, as operands
 // too, two buffers of ROW_BLOCKS blocks.  A workgroup takes the groups of row blocks
 // blockIdx.y, blockIdx.y + gridDim.y, ...
-// Bound as attend_many_kernel is, with half its products and all of its exponentials: 265
-// us of the chunk above (the call 840).  Up to D = 128 a wave keeps to 128 registers, so
+// Bound as attend_many_kernel is, with half its products and all of its exponentials: 300
+// us for the chunk above.  Up to D = 128 a wave keeps to 128 registers, so
 // that four waves of a SIMD hide each other's products and exponentials; with 64
-// keys, two waves: the call 864.  Row blocks between barriers, one, two, three, four: 861,
-// 843, 840, 848 at D = 128, 346, 336, 329, 329 at D = 64.  D = 256 (1024 rows a
+// keys, two waves: 24 us more.  Row blocks between barriers, one, two, three, four: the two
+// kernels 861, 843, 840, 848 at D = 128, 346, 336, 329, 329 at D = 64.  D = 256 (1024 rows a
 // head, 16384 slots) does not fit four waves: 536 us spilled, 513 with two; one row block
 // 548, two 514, four, which leave room for one workgroup, 666.  (16 x 16 tiles with Q from
 // global memory: 492 of the chunk.)
