@@ -948,8 +948,9 @@ __global__ void __launch_bounds__(256) finish_kernel(AttendParams p, int pp, int
 // registers at D = 128, 64 at 256); blocks of 32 rows of Q pass by in LDS, as operands
 // too, two buffers of ROW_BLOCKS blocks.  A workgroup takes the groups of row blocks
 // blockIdx.y, blockIdx.y + gridDim.y, ...
-// Bound as attend_many_kernel is, with half its products and all of its exponentials: 300
-// us for the chunk above.  Up to D = 128 a wave keeps to 128 registers, so
+// Bound as attend_many_kernel is, with half its products and all of its exponentials: 295
+// us for the chunk above, of which no part stands alone (in copies without it: loads of Q 56 less, seven of
+// eight products 94, exponentials 38).  Up to D = 128 a wave keeps to 128 registers, so
 // that four waves of a SIMD hide each other's products and exponentials; with 64
 // keys, two waves: 24 us more.  Row blocks between barriers, one, two, three, four: the two
 // kernels 861, 843, 840, 848 at D = 128, 346, 336, 329, 329 at D = 64.  D = 256 (1024 rows a
@@ -997,6 +998,8 @@ __global__ void __launch_bounds__(64 * Weigh<D>::WAVES, Weigh<D>::OCCUPANCY) wei
             far = max(far, __shfl_xor(far, d));
             near = min(near, __shfl_xor(near, d));
         }
+        far = __builtin_amdgcn_readfirstlane(far);
+        near = __builtin_amdgcn_readfirstlane(near);
     }
     x8 k[QS];
     {
@@ -1014,6 +1017,7 @@ __global__ void __launch_bounds__(64 * Weigh<D>::WAVES, Weigh<D>::OCCUPANCY) wei
     }
     const int64_t first = CAUSAL ? (p.pos_start ? (int64_t)p.pos_start[z] : (int64_t)len - count) : 0;
     const elem* qb = (const elem*)p.q + z * p.qs[0] + (int64_t)h * p.group * p.qs[1];
+    const float* lse = p.row_lse + (int64_t)bh * p.rows;
     const float scale = p.neg ? -p.scale : p.scale;
     u32x4 raw[RB][QF];
     float lse_next[RB];
@@ -1032,20 +1036,26 @@ __global__ void __launch_bounds__(64 * Weigh<D>::WAVES, Weigh<D>::OCCUPANCY) wei
 #pragma unroll
             for (int i = 0; i < QF; ++i)
                 if (QS >= WAVES || wave < QS) raw[g][i] = *(const u32x4*)(src + 8 * (wave * QF + i));
-            // rows past the last and rows that see no slot are hidden below
-            lse_next[g] = row < rows ? p.row_lse[(int64_t)bh * p.rows + row] : INFINITY;
-            if (lse_next[g] == -INFINITY) lse_next[g] = INFINITY;
+            lse_next[g] = lse[min(row, rows - 1)];
             tok += g < RB - 1 ? more_tok : step_tok;
             head += g < RB - 1 ? more_head : step_head;
             if (head >= p.group) head -= p.group, ++tok;
         }
     };
-    auto store = [&](int buf) {
+    float lse2[RB];
+    int tok2[RB];
+    // (what was loaded is first looked at here: a comparison where it is loaded waits for it, 462 us against 433
+    // for 1024 tokens at D = 256)
+    auto store = [&](int buf, int row0) {
 #pragma unroll
-        for (int g = 0; g < RB; ++g)
+        for (int g = 0; g < RB; ++g) {
+            // rows past the last and rows that see no slot are hidden below
+            lse2[g] = row0 + 32 * g + col < rows && lse_next[g] != -INFINITY ? lse_next[g] : INFINITY;
+            tok2[g] = tok_next[g];
 #pragma unroll
             for (int i = 0; i < QF; ++i)
                 if (QS >= WAVES || wave < QS) frag[buf][g][wave * QF + i][lane] = raw[g][i];
+        }
     };
     float sum[16];
 #pragma unroll
@@ -1054,11 +1064,7 @@ __global__ void __launch_bounds__(64 * Weigh<D>::WAVES, Weigh<D>::OCCUPANCY) wei
     int row0 = 32 * RB * blockIdx.y;
     if (row0 < rows) {
         load(row0);
-        store(0);
-        float lse2[RB];
-        int tok2[RB];
-#pragma unroll
-        for (int g = 0; g < RB; ++g) lse2[g] = lse_next[g], tok2[g] = tok_next[g];
+        store(0, row0);
         if (row0 + step < rows) load(row0 + step);
         int buf = 0;
         for (; row0 < rows; row0 += step, buf ^= 1) {
@@ -1067,11 +1073,7 @@ __global__ void __launch_bounds__(64 * Weigh<D>::WAVES, Weigh<D>::OCCUPANCY) wei
             int tok_now[RB];
 #pragma unroll
             for (int g = 0; g < RB; ++g) lse_now[g] = lse2[g], tok_now[g] = tok2[g];
-            if (row0 + step < rows) {
-                store(buf ^ 1);
-#pragma unroll
-                for (int g = 0; g < RB; ++g) lse2[g] = lse_next[g], tok2[g] = tok_next[g];
-            }
+            if (row0 + step < rows) store(buf ^ 1, row0 + step);
             if (row0 + 2 * step < rows) load(row0 + 2 * step);
 #pragma unroll
             for (int g = 0; g < RB; ++g) {
