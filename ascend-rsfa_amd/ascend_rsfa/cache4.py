@@ -32,7 +32,7 @@ import struct
 
 import torch
 
-from . import _native
+from . import _native, _overlap
 from .flash_attention_forward import _as_kernel_layout, _meets_contract, _raise_for
 
 __all__ = ["Cache4"]
@@ -67,47 +67,6 @@ def _function(name):
 
 def _is_int(x):
     return isinstance(x, int) and not isinstance(x, bool)
-
-
-def _span(t):
-    """First and last byte of a tensor's memory."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + last * t.element_size() + t.element_size()
-
-
-def _meet(a, b):
-    """Whether two buffers [Z, H, C, ...] of rows share memory (sequences and heads of
-    one may lie between those of the other)."""
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    if a1 <= b0 or b1 <= a0:
-        return False
-    starts = []  # of each sequence and head's rows
-    for i, t in enumerate((a, b)):
-        size = t[0, 0].numel() * t.element_size()
-        starts += [(t.data_ptr() + (z * t.stride(0) + h * t.stride(1)) * t.element_size(), size, i)
-                   for z in range(t.shape[0]) for h in range(t.shape[1])]
-    starts.sort()
-    ends = [0, 0]
-    for at, size, i in starts:
-        if at < ends[1 - i]:
-            return True
-        ends[i] = max(ends[i], at + size)
-    return False
-
-
-def _overlaps_itself(t):
-    """Whether sequences and heads of a buffer [Z, H, C, ...] share memory with each other."""
-    size = t[0, 0].numel()
-    outer = sorted((s, n) for s, n in zip(t.stride()[:2], t.shape[:2]) if n > 1)
-    need = size
-    for s, n in outer:
-        if s < need:
-            break
-        need = s * (n - 1) + need
-    else:
-        return False
-    starts = sorted(z * t.stride(0) + h * t.stride(1) for z in range(t.shape[0]) for h in range(t.shape[1]))
-    return any(b - a < size for a, b in zip(starts, starts[1:]))
 
 
 def _no_gradient(*tensors):
@@ -172,7 +131,7 @@ class Cache4:
             row = shape[3] if len(shape) == 4 else 1
             if (C > 1 and st[2] != row) or (row > 1 and st[3] != 1):
                 raise ValueError(f"{name}: the rows of a sequence and head must lie densely")
-            if _overlaps_itself(t):
+            if _overlap.meets_itself(t, t.dim() - 2):
                 raise ValueError(f"{name}: its sequences and heads must not share memory")
             strides.append(tuple(st[:2]))
         for a, b in ((0, 1), (2, 3)) + (((4, 5),) if weights is not None else ()):
@@ -183,10 +142,10 @@ class Cache4:
         width = D // 32
         if any(s % width for s in strides[2]) or (ks.data_ptr() | vs.data_ptr()) % width:
             raise ValueError(f"scales must be {width}-byte aligned, with strides that are multiples of {width}")
-        spans = [(t, *_span(t)) for _, t, _, _ in named]
+        spans = [(t, *_overlap.span(t)) for _, t, _, _ in named]
         for i, (a, a0, a1) in enumerate(spans):
             for j, (b, b0, b1) in enumerate(spans[:i]):
-                if a0 < b1 and b0 < a1 and _meet(a, b):
+                if a0 < b1 and b0 < a1 and _overlap.meet(a, b, a.dim() - 2, b.dim() - 2):
                     raise ValueError(f"{named[j][0]} and {named[i][0]} must not share memory")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = kc, ks, vc, vs
         self.positions, self.weights, self.dtype = positions, weights, dtype
@@ -359,9 +318,9 @@ class Cache4:
                 o = out
                 if o.shape != q.shape or o.dtype != q.dtype or o.device != q.device or not _meets_contract(o):
                     raise ValueError("out must match q's shape, dtype and device and have a unit-stride head dim")
-                if any(s == 0 and n > 1 for s, n in zip(o.stride(), o.shape)):
-                    raise ValueError("out is expanded: its rows must not share memory")
-                if o.numel() and _meet(o, q):
+                if o.numel() and _overlap.meets_itself(o):
+                    raise ValueError("the rows of out must not share memory")
+                if o.numel() and _overlap.meet(o, q):
                     raise ValueError("out must not share memory with q")
             args = _native.Cache4AttendArgs()
             args.struct_size = ctypes.sizeof(args)
@@ -469,6 +428,6 @@ class Cache4:
             raise ValueError("into must have this cache's sequences, heads, head_dim, dtype and device")
         for a, a0, a1 in self._spans:
             for b, b0, b1 in into._spans:
-                if a0 < b1 and b0 < a1 and _meet(a, b):
+                if a0 < b1 and b0 < a1 and _overlap.meet(a, b, a.dim() - 2, b.dim() - 2):
                     raise ValueError("into must not share memory with this cache")
         self._evict_call("rsfa_cache4_evict", into, lengths, 1, into.capacity if budget is None else budget, recent, sinks, 0)

@@ -428,6 +428,24 @@ def test_strides_of_caches_and_rows():
                        cache.attend(q[:, :1].expand(Z, 6, 2, D).contiguous(), C, False, 0.2)[:, 5])
 
 
+@pytest.mark.parametrize("T", [3, 60])
+def test_out_beside_q_in_one_buffer(T):
+    # heads of q and others' of out in one [Z, T, heads, D] buffer; out and q side by side in each row
+    cache = _filled(2, 4, 100, 128, BF16, 3)
+    heads = _randn((2, T, 24, 128), 5, BF16)
+    rows = _randn((2, 8, T, 256), 6, BF16)
+    for whole, q, out in ((heads, heads[:, :, :8].transpose(1, 2), heads[:, :, 16:].transpose(1, 2)),
+                          (rows, rows[..., :128], rows[..., 128:])):
+        want, before = cache.attend(q, 100, True, 0.1, accumulate=True), whole.clone()
+        got = cache.attend(q, 100, True, 0.1, accumulate=True, out=out)
+        assert got is out and torch.equal(out, want)
+        out.copy_((before[:, :, 16:].transpose(1, 2) if whole is heads else before[..., 128:]))
+        assert torch.equal(whole, before)  # nothing beside out was written
+    tokens = _randn((1, 48, 32, 128), 7, BF16)
+    with pytest.raises(ValueError, match="share memory"):  # tokens 16 .. 31 are both's
+        Cache4(1, 4, 64, 128, BF16).attend(tokens[:, :32].transpose(1, 2), 64, False, 1.0, out=tokens[:, 16:].transpose(1, 2))
+
+
 def test_a_cache_past_four_gibibytes():
     # 2^25 + 1000 slots of 128 code bytes: the last rows' offsets pass 32 bits
     C, D, last = (1 << 25) + 1000, 256, 500

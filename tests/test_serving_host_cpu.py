@@ -1,0 +1,78 @@
+"""What the serving operators do on the host around their launches, on CPU tensors with the launches replaced."""
+import random
+
+import pytest
+import torch
+
+from ascend_rsfa import _overlap, cache4
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+class Launches(list):
+    """Names of the entry points that a test's calls reach."""
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """Cache calls take CPU tensors, and end where their kernels would start."""
+    launches = Launches()
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    monkeypatch.setattr(cache4.Cache4, "_call", lambda self, name, args: launches.append(name))
+    monkeypatch.setattr(cache4.Cache4, "_on_device", lambda self, fn, *args: fn(*args))
+    return launches
+
+
+def _cache(Z=1, H=2, C=16, D=32, dtype=BF16, **more):
+    return cache4.Cache4(Z, H, C, D, dtype, device="cpu", **more)
+
+
+# -- tensors that share memory --------------------------------------------------
+def _bytes(t):
+    at = torch.tensor([t.data_ptr()])
+    for s, n in zip(t.stride(), t.shape):
+        at = (at[:, None] + s * t.element_size() * torch.arange(n)).flatten()
+    return (at[:, None] + torch.arange(t.element_size())).flatten().tolist()
+
+
+def test_shared_bytes_of_strided_tensors():
+    rng = random.Random(1)
+    memory = torch.zeros(4096, dtype=torch.uint8)
+    seen = set()
+    for _ in range(4000):
+        steps = [rng.choice((0, 1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64)) for _ in range(3)]
+        a, b = (memory.as_strided([rng.randint(1, 4) for _ in range(3)] + [rng.choice((1, 2, 4, 8))],
+                                  [rng.choice((x, x, rng.choice((0, 1, 3, 4, 8, 16, 32, 40, 64, 128)))) for x in steps] + [1],
+                                  rng.choice((0, 8, 16, 64, rng.randint(0, 200)))) for _ in range(2))
+        x, y = _bytes(a), _bytes(b)
+        want = bool(set(x) & set(y)), len(set(x)) < len(x)
+        assert (_overlap.meet(a, b), _overlap.meets_itself(a)) == want, (a.shape, a.stride(), b.shape, b.stride())
+        assert _overlap.span(a) == (min(x), max(x) + 1)
+        seen.add(want)
+    assert len(seen) == 4
+
+
+def test_out_beside_q_in_one_buffer(host):
+    cache = _cache(1, 4, 64, 128)
+    heads = torch.zeros((1, 24, 24, 128), dtype=BF16)  # [Z, T, heads, D]: heads of q, others', of out
+    q, out = heads[:, :, :8].transpose(1, 2), heads[:, :, 16:].transpose(1, 2)
+    assert cache.attend(q, 64, False, 1.0, out=out) is out
+    both = torch.zeros((1, 8, 24, 256), dtype=BF16)  # q and out side by side in each row
+    out = both[..., 128:]
+    assert cache.attend(both[..., :128], 64, False, 1.0, out=out) is out
+    assert len(host) == 2
+
+
+def test_out_that_meets_q_or_itself_is_refused(host):
+    cache = _cache(1, 4, 64, 128)
+    tokens = torch.zeros((1, 48, 32, 128), dtype=BF16)
+    q = tokens[:, :32].transpose(1, 2)
+    flat = torch.zeros(1 << 20, dtype=BF16)
+    for out in (tokens[:, 16:].transpose(1, 2),  # tokens 16 .. 31 are q's too
+                tokens[:, 31:32].transpose(1, 2).expand(1, 32, 32, 128),
+                tokens.view(-1)[8:].as_strided(q.shape, q.stride()),
+                flat.as_strided((1, 32, 32, 128), (0, 64, 4096, 1)),  # heads half a row apart
+                flat.as_strided((1, 32, 32, 128), (0, 128, 2048, 1))):  # tokens that meet the heads of others
+        with pytest.raises(ValueError, match="share memory"):
+            cache.attend(q, 64, False, 1.0, out=out)
+    assert not host
