@@ -24,7 +24,7 @@ import struct
 
 import torch
 
-from . import _native
+from . import _native, _overlap
 from .flash_attention_forward import _raise_for
 
 __all__ = ["RotaryPlan", "rotary_plan", "rotary", "rotary_"]
@@ -299,10 +299,10 @@ def rotary_(q, k, positions, plan):
             raise RuntimeError("rotary_ works in place and keeps no gradient; use rotary")
         if x.stride(3) != 1 and x.shape[3] > 1:
             raise ValueError("rotary_ needs a unit stride in the head dim")
-        if any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
-            raise ValueError("rotary_ cannot write to an expanded tensor")
+        if x.numel() and _overlap.meets_itself(x):
+            raise ValueError("rotary_ cannot write to a tensor whose rows share memory, as an expanded one's do")
     xs = [x for x in (q, k) if x is not None and x.numel()]
-    if len(xs) == 2 and q.data_ptr() == k.data_ptr():
+    if len(xs) == 2 and _overlap.meet(q, k):
         raise ValueError("q and k must not share memory")
     if xs:
         _launch(_parts(xs, xs, positions, plan, False), xs, xs, positions)

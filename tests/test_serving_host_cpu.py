@@ -4,7 +4,7 @@ import random
 import pytest
 import torch
 
-from ascend_rsfa import _overlap, cache4
+from ascend_rsfa import _overlap, cache4, rotary
 
 F16, BF16 = torch.float16, torch.bfloat16
 
@@ -15,11 +15,13 @@ class Launches(list):
 
 @pytest.fixture
 def host(monkeypatch):
-    """Cache calls take CPU tensors, and end where their kernels would start."""
+    """The operators take CPU tensors, and end where their kernels would start."""
     launches = Launches()
     monkeypatch.setattr(torch.Tensor, "is_cuda", True)
     monkeypatch.setattr(cache4.Cache4, "_call", lambda self, name, args: launches.append(name))
     monkeypatch.setattr(cache4.Cache4, "_on_device", lambda self, fn, *args: fn(*args))
+    monkeypatch.setattr(rotary, "_launch", lambda parts, xs, ys, positions: launches.append("rsfa_rotary"))
+    monkeypatch.setattr(rotary.RotaryPlan, "turns", lambda self, device: torch.zeros(self.rotary_dim // 2, dtype=torch.float64))
     return launches
 
 
@@ -76,3 +78,19 @@ def test_out_that_meets_q_or_itself_is_refused(host):
         with pytest.raises(ValueError, match="share memory"):
             cache.attend(q, 64, False, 1.0, out=out)
     assert not host
+
+
+def test_rotary_in_place_refuses_tensors_that_share_memory(host):
+    plan = rotary.RotaryPlan([1.0] * 16)
+    fused = torch.zeros((2, 9, 8, 32))  # [Z, N, heads of q, k and v, D]
+    part = lambda a, b: fused[:, :, a:b].transpose(1, 2)  # noqa: E731
+    rotary.rotary_(part(0, 4), part(4, 6), 0, plan)
+    rotary.rotary_(part(4, 6), part(0, 4), 0, plan)
+    assert len(host) == 2
+    flat = torch.zeros(4096)
+    for q, k in ((part(0, 4), part(3, 5)), (part(2, 4), part(0, 4)), (part(0, 4), part(0, 4)),
+                 (fused[:, :8].transpose(1, 2), fused[:, 1:].transpose(1, 2)),  # tokens 1 .. 7 are both's
+                 (flat.as_strided((1, 2, 9, 32), (0, 16, 64, 1)), None)):  # heads half a row apart
+        with pytest.raises(ValueError, match="share"):
+            rotary.rotary_(q, k, 0, plan)
+    assert len(host) == 2
