@@ -23,6 +23,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native, _overlap
 from .flash_attention_forward import _raise_for
@@ -194,7 +195,13 @@ class _Rotary(torch.autograd.Function):
         if not isinstance(positions, int):
             ctx.positions = None
             ctx.save_for_backward(positions)
+            ctx.save_for_forward(positions)
         return _forward(q, k, positions, plan, inverse)
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):  # linear: tangents turn as values do
+        positions = ctx.saved_tensors[0] if ctx.positions is None else ctx.positions
+        return _turn(tq, tk, positions, ctx.plan, ctx.inverse)
 
     @staticmethod
     def backward(ctx, gq, gk=None):
@@ -212,8 +219,14 @@ class _Rotary(torch.autograd.Function):
         return gq, gk, None, None, None
 
 
+def _has_tangent(*xs):
+    """Whether a tensor carries a derivative of forward mode (no grad mode hides it)."""
+    return forward_ad._current_level >= 0 and any(
+        x is not None and forward_ad.unpack_dual(x).tangent is not None for x in xs)
+
+
 def _turn(q, k, positions, plan, inverse):
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) or _has_tangent(q, k):
         return _Rotary.apply(q, k, positions, plan, inverse)
     return _forward(q, k, positions, plan, inverse)
 
@@ -276,8 +289,8 @@ def rotary(q, k, positions, plan):
 
     q [Z, Hq, N, D] and k [Z, Hk, N, D] (float16, bfloat16 or float32, any
     strides); ``positions``: the first token's position (an int), or a tensor [N]
-    or [Z, N] of int32 or int64.  Differentiable in q and k: the gradient is the
-    same turn backwards.
+    or [Z, N] of int32 or int64.  Differentiable in q and k, in reverse and in
+    forward mode: the gradient is the same turn backwards, a tangent turns as its value does.
     """
     if not isinstance(plan, RotaryPlan):
         raise TypeError("plan must be a RotaryPlan (rotary_plan(...))")
@@ -295,7 +308,7 @@ def rotary_(q, k, positions, plan):
     for x in (q, k):
         if x is None:
             continue
-        if x.requires_grad and torch.is_grad_enabled():
+        if (x.requires_grad and torch.is_grad_enabled()) or _has_tangent(x):
             raise RuntimeError("rotary_ works in place and keeps no gradient; use rotary")
         if x.stride(3) != 1 and x.shape[3] > 1:
             raise ValueError("rotary_ needs a unit stride in the head dim")

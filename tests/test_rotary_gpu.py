@@ -10,6 +10,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from ascend_rsfa import rotary as R
 from oracle import serving as S
@@ -133,6 +134,21 @@ def test_gradients_of_gradients():
     dq, = torch.autograd.grad(R.rotary(q, None, 9, plan), q, g, create_graph=True)
     dg, = torch.autograd.grad(dq, g, d)
     _check(dg, d, torch.arange(9, 14).cuda(), plan)
+
+
+def test_tangents():
+    q, k = _inputs(2, 3, 2, 9, 64, torch.float32, "bshd", 3)
+    tq, tk = _inputs(2, 3, 2, 9, 64, torch.float32, "bhsd", 4)
+    plan = _plan(48, "half", "ntk")
+    positions = torch.arange(9).cuda() * 1000
+    for inverse, turn in ((False, lambda a, b: R.rotary(a, b, positions, plan)), (True, lambda a, b: R._turn(a, b, positions, plan, True))):
+        with forward_ad.dual_level():
+            got = [forward_ad.unpack_dual(y) for y in turn(forward_ad.make_dual(q, tq), forward_ad.make_dual(k, tk))]
+            for y, x, t in zip(got, (q, k), (tq, tk)):
+                _check(y.primal, x, positions, plan, inverse)
+                _check(y.tangent, t, positions, plan, inverse)
+            with pytest.raises(RuntimeError, match="in place"):
+                R.rotary_(forward_ad.make_dual(q, tq), None, 0, plan)
 
 
 def test_gradient_against_differences():

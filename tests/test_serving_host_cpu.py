@@ -3,8 +3,10 @@ import random
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from ascend_rsfa import _overlap, cache4, rotary
+from oracle import serving as S
 
 F16, BF16 = torch.float16, torch.bfloat16
 
@@ -94,3 +96,46 @@ def test_rotary_in_place_refuses_tensors_that_share_memory(host):
         with pytest.raises(ValueError, match="share"):
             rotary.rotary_(q, k, 0, plan)
     assert len(host) == 2
+
+
+@pytest.fixture
+def turned(host, monkeypatch):
+    """rotary's values from the definition, which know nothing of derivatives, as the kernel's."""
+    def forward(q, k, positions, plan, inverse):
+        q, k = forward_ad.unpack_dual(q).primal, k if k is None else forward_ad.unpack_dual(k).primal
+        p = positions + torch.arange(q.shape[2]) if isinstance(positions, int) else positions
+        ys = tuple(S.rotary(x, p, plan.frequencies, plan.amplitude, plan.layout, inverse).to(x.dtype) for x in (q, k) if x is not None)
+        return ys[0] if k is None else ys
+
+    monkeypatch.setattr(rotary, "_forward", forward)
+
+
+@pytest.mark.parametrize("positions", [5, torch.tensor([4, 0, 9])])
+def test_rotary_in_forward_mode(turned, positions):
+    g = torch.Generator().manual_seed(3)
+    q, k, tq, tk, w = (torch.randn((1, 2, 3, 16), generator=g, dtype=torch.float64) for _ in range(5))
+    plan = rotary.RotaryPlan([0.3] * 4, amplitude=1.5)
+    want = rotary.rotary(tq, tk, positions, plan)
+    with forward_ad.dual_level():
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                a, b = rotary.rotary(forward_ad.make_dual(q, tq), forward_ad.make_dual(k, tk), positions, plan)
+                assert torch.equal(forward_ad.unpack_dual(a).tangent, want[0]) and torch.equal(forward_ad.unpack_dual(b).tangent, want[1])
+                # one of the two, and one alone
+                a, b = rotary.rotary(q, forward_ad.make_dual(k, tk), positions, plan)
+                assert torch.equal(forward_ad.unpack_dual(b).tangent, want[1])
+                assert not torch.count_nonzero(forward_ad.unpack_dual(a).tangent)
+                a = rotary.rotary(forward_ad.make_dual(q, tq), None, positions, plan)
+                assert torch.equal(forward_ad.unpack_dual(a).tangent, want[0])
+                assert forward_ad.unpack_dual(rotary.rotary(q, None, positions, plan)).tangent is None
+        # a tangent of a gradient, and a gradient of a tangent
+        x = q.clone().requires_grad_()
+        dx, = torch.autograd.grad(rotary.rotary(x, None, positions, plan), x, forward_ad.make_dual(w, tk))
+        back = rotary._turn(tk, None, positions, plan, True)
+        assert torch.equal(forward_ad.unpack_dual(dx).tangent, back)
+        t = tq.clone().requires_grad_()
+        a = forward_ad.unpack_dual(rotary.rotary(forward_ad.make_dual(q, t), None, positions, plan)).tangent
+        assert torch.equal(torch.autograd.grad(a, t, tk)[0], back)
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match="in place"):
+                rotary.rotary_(forward_ad.make_dual(q.float(), tq.float()), None, positions, plan)
