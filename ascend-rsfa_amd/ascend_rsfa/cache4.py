@@ -34,6 +34,7 @@ import torch
 
 from . import _native, _overlap
 from .flash_attention_forward import _as_kernel_layout, _meets_contract, _raise_for
+from .rotary import _has_tangent
 
 __all__ = ["Cache4"]
 
@@ -72,6 +73,8 @@ def _is_int(x):
 def _no_gradient(*tensors):
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("a Cache4 keeps no gradients: call it under torch.no_grad()")
+    if _has_tangent(*tensors):
+        raise RuntimeError("a Cache4 keeps no gradients, those of forward mode neither: call it with the tensors' primals")
 
 
 class Cache4:

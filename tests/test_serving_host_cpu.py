@@ -139,3 +139,20 @@ def test_rotary_in_forward_mode(turned, positions):
         for mode in (torch.enable_grad, torch.no_grad):
             with mode(), pytest.raises(RuntimeError, match="in place"):
                 rotary.rotary_(forward_ad.make_dual(q.float(), tq.float()), None, positions, plan)
+
+
+def test_cache_calls_refuse_tangents(host):
+    cache = _cache()
+    k, q = torch.zeros((1, 2, 3, 32), dtype=BF16), torch.zeros((1, 4, 3, 32), dtype=BF16)
+    with forward_ad.dual_level():
+        dual = lambda x: forward_ad.make_dual(x, torch.ones_like(x))  # noqa: E731
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                for bad in (lambda: cache.append(dual(k), k, 0), lambda: cache.append(k, dual(k), 0),
+                            lambda: cache.attend(dual(q), 3, False, 1.0)):
+                    with pytest.raises(RuntimeError, match="no gradients"):
+                        bad()
+        assert not host
+        cache.append(k, k, 0)
+        cache.attend(forward_ad.unpack_dual(dual(q)).primal, 3, False, 1.0)
+    assert len(host) == 2
