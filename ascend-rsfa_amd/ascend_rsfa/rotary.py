@@ -24,6 +24,7 @@ import struct
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _native, _overlap
 from .flash_attention_forward import _raise_for
@@ -319,4 +320,5 @@ def rotary_(q, k, positions, plan):
         raise ValueError("q and k must not share memory")
     if xs:
         _launch(_parts(xs, xs, positions, plan, False), xs, xs, positions)
+        increment_version(xs)  # (an earlier operation may have kept them for its gradient)
     return q if k is None else (q, k)

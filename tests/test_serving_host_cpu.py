@@ -156,3 +156,19 @@ def test_cache_calls_refuse_tangents(host):
         cache.append(k, k, 0)
         cache.attend(forward_ad.unpack_dual(dual(q)).primal, 3, False, 1.0)
     assert len(host) == 2
+
+
+def test_rotary_in_place_is_told_to_autograd(host):
+    plan = rotary.RotaryPlan([0.3] * 8)
+    fused = torch.randn((1, 4, 3, 32))
+    for which in range(2):
+        b = torch.randn((1, 4, 3, 32), requires_grad=True)
+        y = fused * b  # keeps fused for b's gradient
+        q, k = fused[:, :3], fused[:, 3:]
+        rotary.rotary_(q, None, 0, plan) if which else rotary.rotary_(torch.randn_like(q), k, 0, plan)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    with torch.inference_mode():
+        rotary.rotary_(torch.randn_like(q), None, 0, plan)
+    rotary.rotary_(torch.randn((1, 2, 0, 32)), None, 0, plan)
+    assert len(host) == 3
