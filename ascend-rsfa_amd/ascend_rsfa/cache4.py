@@ -31,6 +31,7 @@ import math
 import struct
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native, _overlap
 from .flash_attention_forward import _as_kernel_layout, _meets_contract, _raise_for
@@ -127,6 +128,8 @@ class Cache4:
         for name, t, shape, dt in named:
             if tuple(t.shape) != shape or t.dtype != dt:
                 raise ValueError(f"{name} must be {dt} {shape}; got {t.dtype} {tuple(t.shape)}")
+            if t.requires_grad:
+                raise ValueError(f"{name} must not require a gradient")
             if not t.is_cuda or t.device != kc.device:
                 raise ValueError(f"{name} must be a GPU tensor on the device of k_codes")
             # strides of dims of size 1 mean nothing
@@ -163,6 +166,7 @@ class Cache4:
         self._c = c
         self._z = torch.Size((Z,))
         self._spans = spans
+        self._buffers = tuple(t for _, t, _, _ in named)
         self._kept = {}
 
     def _keep(self, key, parts):
@@ -257,6 +261,7 @@ class Cache4:
         if T:
             self._call("rsfa_cache4_append", b"".join((parts[0], _ROWS_KV.pack(k.data_ptr(), v.data_ptr()), parts[1], _ROWS_TAIL.pack(
                 at, length, 0 if slots is None else slots.data_ptr(), counts, positions))))
+            increment_version(self._buffers)  # (an earlier operation may have kept them for its gradient)
 
     def read(self, start=0, count=None, *, slots=None):
         """(k, v): the values of slots ``start[z] .. start[z] + count - 1`` (an int or an
@@ -306,7 +311,7 @@ class Cache4:
         holds 4 bytes for each row and slot, up to 4 GiB.)
         ``lse``: the natural logarithm of each row's sum of exponentials, float32 [Z, Hq, T].
         """
-        _no_gradient(q)
+        _no_gradient(q) if out is None else _no_gradient(q, out)
         key = ("attend", q.shape, q.stride(), q.dtype, q.device, bool(causal), None if out is None else out.stride())
         parts = self._kept.get(key)
         if parts is None or out is not None or q.data_ptr() & 15:
@@ -366,6 +371,10 @@ class Cache4:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
         self._call("rsfa_cache4_attend", head + _AT_TAIL.pack(at, length, max_length, counts, positions, scale, accumulate,
                                                               ws.data_ptr() if nbytes else 0, nbytes))
+        if out is not None:
+            increment_version(out)
+        if accumulate:
+            increment_version(self.weights)
         return (o, lse) if return_lse else o
 
     # -- eviction -----------------------------------------------------------
@@ -434,3 +443,4 @@ class Cache4:
                 if a0 < b1 and b0 < a1 and _overlap.meet(a, b, a.dim() - 2, b.dim() - 2):
                     raise ValueError("into must not share memory with this cache")
         self._evict_call("rsfa_cache4_evict", into, lengths, 1, into.capacity if budget is None else budget, recent, sinks, 0)
+        increment_version(into._buffers)

@@ -172,3 +172,38 @@ def test_rotary_in_place_is_told_to_autograd(host):
         rotary.rotary_(torch.randn_like(q), None, 0, plan)
     rotary.rotary_(torch.randn((1, 2, 0, 32)), None, 0, plan)
     assert len(host) == 3
+
+
+def test_writes_of_cache_calls_are_told_to_autograd(host):
+    cache, into = _cache(), _cache(C=8)
+    k, q = torch.zeros((1, 2, 3, 32), dtype=BF16), torch.zeros((1, 4, 3, 32), dtype=BF16)
+    out = torch.zeros_like(q)
+    every = ("k_codes", "k_scales", "v_codes", "v_scales", "positions", "weights")
+
+    def versions():
+        return {**{n: getattr(cache, n)._version for n in every}, **{"into." + n: getattr(into, n)._version for n in every}, "out": out._version}
+
+    for call, written in ((lambda: cache.append(k, k, 0), every), (lambda: cache.attend(q, 3, False, 1.0), ()),
+                          (lambda: cache.attend(q, 3, False, 1.0, accumulate=True), ("weights",)),
+                          (lambda: cache.attend(q, 3, False, 1.0, out=out), ("out",)), (lambda: cache.read(0, 2), ()),
+                          (lambda: cache.claim(3, 2), ()), (lambda: cache.evict(into, 3), tuple("into." + n for n in every)),
+                          (lambda: cache.append(k[:, :, :0], k[:, :, :0], 0), ())):
+        before = versions()
+        call()
+        assert {n for n, v in versions().items() if v != before[n]} == set(written)
+    # as autograd sees it: weights and an out that an earlier product keeps
+    for kept, call in ((cache.weights, lambda: cache.attend(q, 3, False, 1.0, accumulate=True)),
+                       (out, lambda: cache.attend(q, 3, False, 1.0, out=out))):
+        y = kept * torch.ones_like(kept).requires_grad_()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        cache.attend(q, 3, False, 1.0, out=out.clone().requires_grad_())
+    b = {n: getattr(cache, n) for n in every}
+    with pytest.raises(ValueError, match="gradient"):
+        cache4.Cache4.from_buffers(**{**b, "weights": b["weights"].clone().requires_grad_()}, dtype=BF16)
+    with torch.inference_mode():
+        mine = _cache()
+        mine.append(k, k, 0)
+        mine.attend(q, 3, False, 1.0, accumulate=True)
