@@ -41,6 +41,8 @@ __all__ = ["Cache4"]
 
 _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16}
 _HEAD_DIMS = (32, 64, 128, 256)
+_FIXED = frozenset(("k_codes", "k_scales", "v_codes", "v_scales", "positions", "weights", "dtype", "Z", "H", "capacity",
+                    "head_dim", "device"))
 
 # A call's argument struct is joined from parts that its tensors' shapes settle,
 # kept per cache (`_kept`), and packed addresses: filling the struct field by
@@ -85,8 +87,19 @@ class Cache4:
     ``weights`` the cache keeps no attention weights (no accumulate, claim or evict).
     The buffers are attributes: k_codes, v_codes (uint8 [Z, H, capacity, D / 2]), k_scales,
     v_scales (uint8 [Z, H, capacity, D / 32]), positions (int32) and weights (float32,
-    both [Z, H, capacity]).
+    both [Z, H, capacity]).  Programs may write into them (``cache.weights.zero_()``), but
+    not put others in their places: the kernels hold their addresses.
     """
+
+    def __setattr__(self, name, value):
+        # (cache.weights *= 0.5 works in place, and assigns the same tensor)
+        if name in _FIXED and name in self.__dict__ and value is not self.__dict__[name]:
+            raise AttributeError(f"{name} of a Cache4 is fixed: the kernels hold the buffers' addresses and sizes "
+                                 f"(write into a buffer, as cache.weights.copy_(...), or take from_buffers)")
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{name} of a Cache4 is fixed")
 
     def __init__(self, Z, H, capacity, head_dim, dtype=torch.float16, device="cuda", weights=True):
         if head_dim not in _HEAD_DIMS:

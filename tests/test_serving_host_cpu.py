@@ -207,3 +207,24 @@ def test_writes_of_cache_calls_are_told_to_autograd(host):
         mine = _cache()
         mine.append(k, k, 0)
         mine.attend(q, 3, False, 1.0, accumulate=True)
+
+
+def test_buffers_and_sizes_of_a_cache_stay(host):
+    cache = _cache()
+    for name in ("k_codes", "k_scales", "v_codes", "v_scales", "positions", "weights"):
+        t = getattr(cache, name)
+        with pytest.raises(AttributeError, match="fixed"):
+            setattr(cache, name, torch.zeros_like(t))
+        with pytest.raises(AttributeError, match="fixed"):
+            delattr(cache, name)
+        assert getattr(cache, name) is t
+    for name, value in (("dtype", F16), ("Z", 2), ("H", 1), ("capacity", 8), ("head_dim", 64), ("device", torch.device("cuda:1"))):
+        with pytest.raises(AttributeError, match="fixed"):
+            setattr(cache, name, value)
+    with pytest.raises(AttributeError, match="fixed"):
+        _cache(weights=False).weights = cache.weights
+    w = cache.weights
+    cache.weights += 2.0
+    cache.weights *= 0.5
+    cache.weights[0, 0] = 4.0
+    assert cache.weights is w and w[0, 0].eq(4.0).all() and w[0, 1].eq(1.0).all()
