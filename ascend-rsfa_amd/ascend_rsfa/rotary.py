@@ -52,7 +52,10 @@ def _function():
 
 
 class RotaryPlan:
-    """Frequencies (float64, radians a position, [R/2], on the CPU), amplitude and layout."""
+    """Frequencies (float64, radians a position, [R/2], on the CPU), amplitude and layout.
+
+    A plan stays as it was made (rotary_plan gives one plan to all callers of the same
+    arguments): its attributes are read-only, ``frequencies`` is a copy."""
 
     def __init__(self, frequencies, layout="half", amplitude=1.0):
         f = torch.as_tensor(frequencies, dtype=torch.float64).detach().cpu().contiguous().clone()
@@ -62,12 +65,17 @@ class RotaryPlan:
             raise ValueError(f"layout must be one of {_LAYOUTS}; got {layout!r}")
         if not math.isfinite(amplitude):
             raise ValueError("amplitude must be finite")
-        self.frequencies = f
-        self.layout = layout
-        self.amplitude = float(amplitude)
-        self.rotary_dim = 2 * f.numel()
+        self._frequencies = f
+        self._layout = layout
+        self._amplitude = float(amplitude)
+        self._rotary_dim = 2 * f.numel()
         self._turns = {}
         self._kept = {}
+
+    frequencies = property(lambda self: self._frequencies.clone())
+    layout = property(lambda self: self._layout)
+    amplitude = property(lambda self: self._amplitude)
+    rotary_dim = property(lambda self: self._rotary_dim)
 
     def turns(self, device):
         """Turns a position of each pair, on `device`."""
@@ -75,7 +83,7 @@ class RotaryPlan:
         if t is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call plan.turns(device) (or rotary) once before capturing a graph")
-            t = (self.frequencies / (2.0 * math.pi)).to(device)
+            t = (self._frequencies / (2.0 * math.pi)).to(device)
             # (other streams may use it at once)
             torch.cuda.current_stream(device).synchronize()
             self._turns[device] = t

@@ -228,3 +228,20 @@ def test_buffers_and_sizes_of_a_cache_stay(host):
     cache.weights *= 0.5
     cache.weights[0, 0] = 4.0
     assert cache.weights is w and w[0, 0].eq(4.0).all() and w[0, 1].eq(1.0).all()
+
+
+def test_plans_stay_as_they_were_made():
+    plan = rotary.rotary_plan(16, base=50.0, layout="interleaved", amplitude=1.25)
+    f = plan.frequencies
+    for name, value in (("amplitude", 2.0), ("layout", "half"), ("frequencies", f * 2), ("rotary_dim", 8)):
+        with pytest.raises(AttributeError):
+            setattr(plan, name, value)
+    plan.frequencies.mul_(3.0)
+    f.zero_()
+    again = rotary.rotary_plan(16, base=50.0, layout="interleaved", amplitude=1.25)
+    assert (again.amplitude, again.layout, again.rotary_dim) == (1.25, "interleaved", 16)
+    assert torch.equal(again.frequencies, rotary.rotary_plan(16, base=50.0).frequencies) and again.frequencies[0] == 1.0
+    mine = torch.ones(4, dtype=torch.float64)
+    own = rotary.RotaryPlan(mine)
+    mine.zero_()
+    assert own.frequencies.eq(1.0).all()
