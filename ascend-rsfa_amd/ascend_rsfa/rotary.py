@@ -72,6 +72,9 @@ class RotaryPlan:
         self._turns = {}
         self._kept = {}
 
+    def __reduce__(self):  # (what is kept holds addresses of this process, of memory that a copy does not keep alive)
+        return type(self), (self.frequencies, self.layout, self.amplitude)
+
     frequencies = property(lambda self: self._frequencies.clone())
     layout = property(lambda self: self._layout)
     amplitude = property(lambda self: self._amplitude)

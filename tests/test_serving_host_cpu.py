@@ -1,4 +1,6 @@
 """What the serving operators do on the host around their launches, on CPU tensors with the launches replaced."""
+import copy
+import pickle
 import random
 
 import pytest
@@ -245,3 +247,20 @@ def test_plans_stay_as_they_were_made():
     own = rotary.RotaryPlan(mine)
     mine.zero_()
     assert own.frequencies.eq(1.0).all()
+
+
+def test_copies_of_plans_hold_no_addresses(host):
+    plan = rotary.RotaryPlan([0.5, 0.25], "interleaved", 1.5)
+    rotary.rotary(torch.zeros((1, 2, 3, 8)), None, 0, plan)
+    assert plan._kept
+    for other in (copy.deepcopy(plan), copy.copy(plan), pickle.loads(pickle.dumps(plan))):
+        assert not other._kept and not other._turns
+        assert torch.equal(other.frequencies, plan.frequencies) and (other.layout, other.amplitude) == ("interleaved", 1.5)
+
+
+def test_caches_are_not_pickled_or_copied_by_value(host):
+    cache = _cache()
+    cache.append(torch.zeros((1, 2, 3, 32), dtype=BF16), torch.zeros((1, 2, 3, 32), dtype=BF16), 0)
+    for bad in (lambda: pickle.dumps(cache), lambda: copy.deepcopy(cache)):
+        with pytest.raises(ValueError, match="cannot be pickled"):
+            bad()
