@@ -416,7 +416,7 @@ class Cache4:
         head, sizes = parts
         nbytes = sizes.get(budget)
         if nbytes is None:
-            args = _native.Cache4EvictArgs.from_buffer_copy(head + _EVICT_TAIL.pack(0, 0, n, budget, 0, 0, 0, 0, 0))
+            args = _native.Cache4EvictArgs.from_buffer_copy(head + _EVICT_TAIL.pack(0, 0, 1, budget, 0, 0, 0, 0, 0))
             nbytes = sizes[budget] = _native.lib().rsfa_cache4_evict_workspace_bytes(ctypes.byref(args), 0 if into is None else 1)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
         self._call(name, head + _EVICT_TAIL.pack(at, length, n, budget, recent, sinks, out, ws.data_ptr() if nbytes else 0, nbytes))
@@ -433,6 +433,8 @@ class Cache4:
         """
         if not _is_int(n) or n < 1:
             raise ValueError(f"n must be an int of at least 1; got {n!r}")
+        if n > 1 << 30:
+            raise ValueError(f"n must be at most 2^30; got {n}")
         slots = torch.empty((self.Z, self.H, n), dtype=torch.int32, device=self.device)
         self._evict_call("rsfa_cache4_claim", None, lengths, n, self.capacity if budget is None else budget, recent, sinks,
                          slots.data_ptr())

@@ -7,7 +7,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from ascend_rsfa import _overlap, cache4, rotary
+from ascend_rsfa import _native, _overlap, cache4, rotary
 from oracle import serving as S
 
 F16, BF16 = torch.float16, torch.bfloat16
@@ -264,3 +264,14 @@ def test_caches_are_not_pickled_or_copied_by_value(host):
     for bad in (lambda: pickle.dumps(cache), lambda: copy.deepcopy(cache)):
         with pytest.raises(ValueError, match="cannot be pickled"):
             bad()
+
+
+def test_a_refused_claim_leaves_nothing_behind(host, monkeypatch):
+    cache, sizes = _cache(1, 1, 40000), []
+    monkeypatch.setattr(cache4.Cache4, "_call", lambda self, name, args: sizes.append(
+        _native.Cache4EvictArgs.from_buffer_copy(args).workspace_bytes))
+    with pytest.raises(ValueError, match="n must"):
+        cache.claim(40000, (1 << 30) + 1, budget=100)
+    cache.claim(40000, 1, budget=100)
+    cache.claim(40000, 1 << 10, budget=100)
+    assert len(sizes) == 2 and sizes[0] == sizes[1] > 0
