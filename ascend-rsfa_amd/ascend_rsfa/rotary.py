@@ -81,7 +81,10 @@ class RotaryPlan:
     rotary_dim = property(lambda self: self._rotary_dim)
 
     def turns(self, device):
-        """Turns a position of each pair, on `device`."""
+        """Turns a position of each pair, on `device` ("cuda": the current one)."""
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         t = self._turns.get(device)
         if t is None:
             if torch.cuda.is_current_stream_capturing():

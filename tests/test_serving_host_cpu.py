@@ -275,3 +275,22 @@ def test_a_refused_claim_leaves_nothing_behind(host, monkeypatch):
     cache.claim(40000, 1, budget=100)
     cache.claim(40000, 1 << 10, budget=100)
     assert len(sizes) == 2 and sizes[0] == sizes[1] > 0
+
+
+def test_turns_of_the_current_device(monkeypatch):
+    class Stream:
+        def synchronize(self):
+            pass
+
+    capturing = []
+    monkeypatch.setattr(torch.Tensor, "to", lambda self, device: self)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: Stream())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: bool(capturing))
+    plan = rotary.RotaryPlan([0.5, 0.25])
+    t = plan.turns("cuda")
+    capturing.append(True)  # a graph's calls find what was asked for before
+    assert plan.turns(torch.device("cuda", 1)) is t and plan.turns("cuda:1") is t
+    for device in ("cuda:0", torch.device("cuda", 2)):
+        with pytest.raises(RuntimeError, match="before capturing"):
+            plan.turns(device)
