@@ -21,6 +21,7 @@ import ctypes
 import functools
 import math
 import struct
+import threading
 
 import torch
 from torch.autograd import forward_ad
@@ -42,6 +43,19 @@ _XY, _ONE, _NUMBER = struct.Struct("=4Q"), struct.Struct("=Q"), struct.Struct("=
 assert _Z - _X == _XY.size and _POS_STRIDE - _POS == _ONE.size and _TURNS - _START == _NUMBER.size
 _FUNCTION = None
 
+# Frequencies on devices whose plans are gone: launches on any stream may still read them, and freed
+# memory is given out again on the stream of the plan's first call. They wait for many, and then for the devices.
+_DEAD, _DEAD_MOST, _DEAD_LOCK = [], 256, threading.Lock()
+
+
+def _bury():
+    with _DEAD_LOCK:
+        n = len(_DEAD)
+        if n >= _DEAD_MOST:
+            for device in {t.device for t in _DEAD[:n]}:
+                torch.cuda.synchronize(device)
+            del _DEAD[:n]
+
 
 def _function():
     """rsfa_rotary, taking its argument struct's bytes."""
@@ -55,7 +69,8 @@ class RotaryPlan:
     """Frequencies (float64, radians a position, [R/2], on the CPU), amplitude and layout.
 
     A plan stays as it was made (rotary_plan gives one plan to all callers of the same
-    arguments): its attributes are read-only, ``frequencies`` is a copy."""
+    arguments): its attributes are read-only, ``frequencies`` is a copy.  Programs keep a plan
+    as long as a captured graph that uses it, as they keep the graph's tensors."""
 
     def __init__(self, frequencies, layout="half", amplitude=1.0):
         f = torch.as_tensor(frequencies, dtype=torch.float64).detach().cpu().contiguous().clone()
@@ -80,6 +95,9 @@ class RotaryPlan:
     amplitude = property(lambda self: self._amplitude)
     rotary_dim = property(lambda self: self._rotary_dim)
 
+    def __del__(self, dead=_DEAD):
+        dead.extend(self.__dict__.get("_turns", {}).values())
+
     def turns(self, device):
         """Turns a position of each pair, on `device` ("cuda": the current one)."""
         device = torch.device(device)
@@ -89,6 +107,7 @@ class RotaryPlan:
         if t is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call plan.turns(device) (or rotary) once before capturing a graph")
+            _bury()
             t = (self._frequencies / (2.0 * math.pi)).to(device)
             # (other streams may use it at once)
             torch.cuda.current_stream(device).synchronize()

@@ -2,6 +2,7 @@
 import copy
 import pickle
 import random
+import weakref
 
 import pytest
 import torch
@@ -277,7 +278,9 @@ def test_a_refused_claim_leaves_nothing_behind(host, monkeypatch):
     assert len(sizes) == 2 and sizes[0] == sizes[1] > 0
 
 
-def test_turns_of_the_current_device(monkeypatch):
+@pytest.fixture
+def device(monkeypatch):
+    """Plans prepare frequencies for a device that is not there; True in the list: under capture."""
     class Stream:
         def synchronize(self):
             pass
@@ -287,10 +290,29 @@ def test_turns_of_the_current_device(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device: Stream())
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: bool(capturing))
+    return capturing
+
+
+def test_turns_of_the_current_device(device):
+    capturing = device
     plan = rotary.RotaryPlan([0.5, 0.25])
     t = plan.turns("cuda")
     capturing.append(True)  # a graph's calls find what was asked for before
     assert plan.turns(torch.device("cuda", 1)) is t and plan.turns("cuda:1") is t
-    for device in ("cuda:0", torch.device("cuda", 2)):
+    for other in ("cuda:0", torch.device("cuda", 2)):
         with pytest.raises(RuntimeError, match="before capturing"):
-            plan.turns(device)
+            plan.turns(other)
+
+
+def test_frequencies_outlive_a_dropped_plan(device, monkeypatch):
+    waits, dead = [], []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device: waits.append([r() is not None for r in dead]))
+    for i in range(600):
+        plan = rotary.RotaryPlan([0.5, 0.25])
+        dead.append(weakref.ref(plan.turns("cuda")))
+        del plan
+        # launches on other streams may still read them: none is freed without a wait since its plan's end
+        alive = [r() is not None for r in dead]
+        last = len(waits[-1]) if waits else 0
+        assert all(alive[last:]) and sum(alive) <= 300
+    assert 2 <= len(waits) <= 4 and all(w[-1] for w in waits)
