@@ -12,6 +12,7 @@ append, read, claim and evict are exact.  attend's tolerances follow from what i
 """
 import math
 
+import long_rows
 import pytest
 import torch
 
@@ -292,6 +293,66 @@ def test_attend_matches_the_definition(shape, dtype, causal):
     # without weights, with a bound on the lengths: another division of the work
     plain = cache.attend(q.contiguous(), _ints(lengths), causal, scale, max_length=max(max(lengths), 1), return_lse=True)
     _check_attend(cache, plain, q, lengths, scale, None, cache.positions if causal else None, first)
+
+
+LONG = [
+    # query heads (of one key head), T, slots, length, D
+    (1, 1, 20000, 19999, 128), (4, 1, 16000, 16000, 64), (2, 1, 9000, 8130, 256), (1, 1, 4000, 3977, 32), (4, 8, 20000, 16385, 128),
+    (1, 32, 9000, 8999, 256), (5, 8, 20000, 19990, 128), (2, 60, 9000, 8190, 64), (1, 100, 9000, 8192, 256), (1, 100, 4000, 3977, 32),
+    (3, 150, 20000, 20000, 128), (2, 200, 9000, 8999, 256),
+]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("shape", LONG)
+def test_every_slot_of_a_long_row_counts(shape, dtype):
+    Hq, T, C, n, D = shape
+    print(f"long rows {shape} {dtype}", flush=True)
+    q = torch.zeros((1, Hq, T, D), dtype=dtype).cuda()
+    k = _randn((1, 1, C, D), 3, dtype)
+    for step in (1, 32, 512):
+        v = long_rows.marked(n, C, D, dtype, step)
+        cache = Cache4(1, 1, C, D, dtype)
+        cache.append(k, v.cuda(), 0)
+        for causal in (False, True):
+            cache.weights.zero_()
+            pos = _ints([n - 1])  # (causal: every token sees all slots in use)
+            o, lse = cache.attend(q, _ints([n]), causal, 1.0, positions=pos, accumulate=causal, return_lse=True)
+            assert long_rows.marks_hold(o.cpu(), n, v), (step, causal)
+            assert (lse.double() - math.log(n)).abs().max() <= 4 * 2.0 ** -23 * math.log(n)
+        want = Hq * T / n
+        assert (cache.weights[0, 0, :n].double() - want).abs().max() <= want * (Hq * T + 8) * 2.0 ** -23
+        assert not cache.weights[0, 0, n:].any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("shape", LONG)
+def test_peaks_in_every_part_of_a_long_row(shape, dtype):
+    Hq, T, C, n, D = shape
+    rows = min(Hq * T, D)
+    print(f"peaks {shape} {dtype}", flush=True)
+    # the ends, and slots all over the row: as many as there are rows, in several calls where those are few
+    spread = [0, n - 1, n - 2, 31, 32, 127, 128, 511, n // 32 * 32 - 1, n // 2] + [(i * 617 + 300) % n for i in range(64)]
+    spread = list(dict.fromkeys(spread))
+    for first in range(0, len(spread), D):
+        some = spread[first:first + D]
+        k, v, peaks = long_rows.peaks(some, n, C, D, dtype, first)
+        cache = Cache4(1, 1, C, D, dtype)
+        cache.append(k.cuda(), v.cuda(), 0)
+        assert torch.equal(cache.read()[1].cpu(), v)
+        for turn in range(0, len(some), rows):
+            slots = torch.tensor(some[turn:turn + rows])
+            # row i is token i // Hq, head i % Hq; rows without a peak of their own repeat the first ones'
+            at = torch.arange(Hq * T) % len(slots)
+            q = peaks[turn + at].reshape(T, Hq, D).transpose(0, 1)[None].cuda()
+            want = v[0, 0][slots[at]].reshape(T, Hq, D).transpose(0, 1)[None]
+            for causal in (False, True):
+                cache.weights.zero_()
+                o = cache.attend(q, n, causal, 1.0, positions=_ints([n - 1]), accumulate=True)
+                assert torch.equal(o.cpu(), want), causal
+                count = torch.zeros(C).index_add_(0, slots[at], torch.ones(Hq * T))
+                # (a peak's weight is 1 to 2^-16, the others' n e^-40 in all)
+                assert ((cache.weights[0, 0].cpu() - count).abs() <= count * 2.0 ** -16 + 2.0 ** -30).all()
 
 
 @pytest.mark.parametrize("T", [1, 3, 9, 50, 90])

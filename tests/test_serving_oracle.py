@@ -1,6 +1,8 @@
 """Known answers that pin the float64 definitions of the serving operators (oracle/serving.py)."""
 import math
 
+import long_rows
+import pytest
 import torch
 
 from oracle import serving as S
@@ -70,3 +72,40 @@ def test_eviction_known_answers():
     assert S.claim(w, pos, [8], 4, 8, recent=4, sinks=2)[0, 0].tolist() == [2, 3, -1, -1]
     assert S.evict(w, pos, [8], 3)[0][0] == [2, 6, 7]
     assert S.evict(w, pos, [8], 3, recent=2, sinks=1)[0][0] == [0, 6, 7]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_long_rows_show_what_is_lost(dtype):
+    # the values that the GPU tests of long rows expect follow from the definition, and a mistake in V alone shows
+    for n, D, C in ((19999, 128, 20000), (16000, 64, 16000), (8130, 256, 9000), (3977, 32, 4000)):
+        k, q = torch.zeros((1, 1, C, D), dtype=torch.float64), torch.zeros((1, 1, 1, D), dtype=torch.float64)
+        steps = {step: long_rows.marked(n, C, D, dtype, step) for step in (1, 32, 512)}
+
+        def holds(spoil):
+            found = []
+            for step, v in steps.items():
+                bad = v.double()
+                spoil(bad[0, 0])
+                found.append(long_rows.marks_hold(S.attend(q, k, bad, [n], 1.0)[0].to(dtype), n, v))
+            return all(found)
+
+        def shift(v):
+            v[512:1024] = v[513:1025].clone()
+
+        def twice(v):
+            v[64:96] += v[96:128]
+
+        def unseen(v):
+            v[n - 1] = 1.0
+
+        assert holds(lambda v: None)
+        one = (lambda v: v[5].zero_(), lambda v: v[n - 1].zero_(), unseen) if dtype == torch.float16 or n <= 2 ** 7 * D else ()
+        for spoil in (lambda v: v[:512].zero_(), lambda v: v[n // 2:n // 2 + 32].zero_(), lambda v: v[n - n % 32 - 32:].zero_(),
+                      lambda v: v[1024:1536].zero_(), shift, twice, *one):
+            assert not holds(spoil)
+        slots = [0, n - 1, n // 2, 31]
+        k, v, q = long_rows.peaks(slots, n, C, D, dtype, 1)
+        codes, scales = S.quantise(v, dtype)
+        assert torch.equal(S.values(codes, scales), v.double())
+        o = S.attend(q[None, None].double(), k.double(), v.double(), [n], 1.0)[0]
+        assert torch.equal(o[0, 0].to(dtype), v[0, 0, slots])
