@@ -314,7 +314,8 @@ class Cache4:
         slots whose position is at most ``positions[z] + i`` (int32 [Z]; None:
         ``lengths[z] - T + i``, with ``counts`` ``lengths[z] - counts[z] + i``, which is right
         while no slot has been evicted); otherwise all slots in use.  Tokens
-        ``i >= counts[z]``, and tokens that see no slot, give 0 (lse -inf).
+        ``i >= counts[z]``, and tokens that see no slot, give 0 (lse -inf); so do tokens whose
+        visible scores are all -inf (an infinite q), as hidden scores are.
 
         ``accumulate`` adds to each slot's weight the attention that it received: the sum of
         its softmax weights over all tokens and the query heads of its group.

@@ -313,7 +313,8 @@ int rsfa_cache4_read(const rsfa_cache4_rows_args *args, void *stream);
  * reads key head i / (heads / cache.h).  With `causal` query token i of sequence
  * z sees the slots whose position is at most pos_start[z] + i (NULL:
  * length - count + i, with the sequence's count of tokens).  Rows i >= counts[z],
- * and rows that see no slot, give 0 (lse -inf).  With `accumulate` the weights
+ * and rows that see no slot, give 0 (lse -inf); so do rows whose visible scores are
+ * all -inf (an infinite q), as hidden scores are.  With `accumulate` the weights
  * of the slots grow by the softmax weights that all rows of the call gave them.
  * Lengths above max_length (0: the capacity) are taken as max_length.  o must not
  * overlap q; calls that accumulate into one cache must not overlap in time.

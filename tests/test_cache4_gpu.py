@@ -464,6 +464,35 @@ def test_overflowing_scores_are_nan_or_dominate_as_in_ieee():
     assert torch.allclose(o[0, 0, 0].double(), want, rtol=0, atol=2.0 ** -8 * v.abs().max().item())
 
 
+@pytest.mark.parametrize("Hq, T, C", [(2, 1, 40), (2, 1, 5000), (4, 8, 700), (2, 60, 90), (2, 60, 5000)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_rows_whose_scores_are_all_minus_infinity_see_nothing(Hq, T, C, dtype):
+    # an infinite q: each visible score is -inf, which is how hidden ones enter the softmax
+    D = 64
+    cache = Cache4(1, 1, C, D, dtype)
+    k = _randn((1, 1, C, D), 1, dtype)
+    k[..., 0] = 4.0
+    cache.append(k, _randn((1, 1, C, D), 2, dtype), 0)
+    cache.weights.copy_(_randn((1, 1, C), 3).exp())
+    q = _randn((1, Hq, T, D), 5, dtype)
+    q[0, 0, 0] = 0.0
+    q[0, 0, 0, 0] = -math.inf
+    for causal, scale, n in ((False, 0.1, C), (True, 0.1, C - 3), (False, 1e-30, C - 3)):
+        before = cache.weights.clone()
+        got = cache.attend(q, n, causal, scale, accumulate=True, return_lse=True)
+        assert (got[0][0, 0, 0] == 0).all() and got[1][0, 0, 0] == -math.inf
+        first = cache.positions if causal else None
+        _check_attend(cache, got, q, [n], scale, None, first, [n - T])
+        _, _, ww, _, reach = S.attend(q, *_values(cache), [n], scale, first, [n - T])
+        tol = ww * (2 * reach[torch.isfinite(reach)].amax() * (D + 4) * 2.0 ** -24 + (n + 16 + Hq * T + 4) * 2.0 ** -23)
+        want = before.double() + ww
+        assert ((cache.weights.double() - want).abs() <= tol + want * 2.0 ** -23).all()
+    # +inf leaves inf - inf
+    q[0, 0, 0, 0] = math.inf
+    o, lse = cache.attend(q, C, False, 0.1, return_lse=True)
+    assert torch.isnan(o[0, 0, 0]).all() and torch.isnan(lse[0, 0, 0]) and torch.isfinite(o[0, 1:]).all()
+
+
 def test_strides_of_caches_and_rows():
     # a layer's part of buffers that all layers share, q with gaps, out given
     Z, H, C, D = 2, 3, 50, 64
