@@ -65,6 +65,12 @@ def _function():
     return _FUNCTION
 
 
+def _has_tangent(*xs):
+    """Whether a tensor carries a derivative of forward mode (no grad mode hides it)."""
+    return forward_ad._current_level >= 0 and any(
+        x is not None and forward_ad.unpack_dual(x).tangent is not None for x in xs)
+
+
 class RotaryPlan:
     """Frequencies (float64, radians a position, [R/2], on the CPU), amplitude and layout.
 
@@ -73,7 +79,10 @@ class RotaryPlan:
     as long as a captured graph that uses it, as they keep the graph's tensors."""
 
     def __init__(self, frequencies, layout="half", amplitude=1.0):
-        f = torch.as_tensor(frequencies, dtype=torch.float64).detach().cpu().contiguous().clone()
+        f = torch.as_tensor(frequencies, dtype=torch.float64)
+        if (f.requires_grad and torch.is_grad_enabled()) or _has_tangent(f):
+            raise RuntimeError("a plan's frequencies are constants: no gradient reaches them (detach them)")
+        f = f.detach().cpu().contiguous().clone()
         if f.dim() != 1 or f.numel() < 1 or not bool(torch.isfinite(f).all()):
             raise ValueError("frequencies must be a vector of finite numbers, one for each pair")
         if layout not in _LAYOUTS:
@@ -251,12 +260,6 @@ class _Rotary(torch.autograd.Function):
         elif gk is not None:
             gk = _turn(gk, None, positions, ctx.plan, not ctx.inverse)
         return gq, gk, None, None, None
-
-
-def _has_tangent(*xs):
-    """Whether a tensor carries a derivative of forward mode (no grad mode hides it)."""
-    return forward_ad._current_level >= 0 and any(
-        x is not None and forward_ad.unpack_dual(x).tangent is not None for x in xs)
 
 
 def _turn(q, k, positions, plan, inverse):

@@ -316,3 +316,15 @@ def test_frequencies_outlive_a_dropped_plan(device, monkeypatch):
         last = len(waits[-1]) if waits else 0
         assert all(alive[last:]) and sum(alive) <= 300
     assert 2 <= len(waits) <= 4 and all(w[-1] for w in waits)
+
+
+def test_plans_of_learned_frequencies_are_refused():
+    f = torch.tensor([0.5, 0.25], requires_grad=True)
+    for bad in (f, f * 2, torch.nn.Parameter(torch.ones(2, dtype=torch.float64))):
+        with pytest.raises(RuntimeError, match="constants"):
+            rotary.RotaryPlan(bad)
+    with forward_ad.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="constants"):
+        rotary.RotaryPlan(forward_ad.make_dual(f.detach(), torch.ones(2)))
+    with torch.no_grad():
+        assert rotary.RotaryPlan(f).frequencies.tolist() == [0.5, 0.25]
+    assert rotary.RotaryPlan(f.detach()).frequencies.tolist() == [0.5, 0.25]
