@@ -124,7 +124,6 @@ class RotaryPlan:
         return t
 
 
-@functools.lru_cache(maxsize=64)  # (plans are constants: the same arguments give the same one)
 def rotary_plan(rotary_dim, *, base=10000.0, layout="half", scaling=None, factor=1.0, original_length=None,
                 low=1.0, high=32.0, amplitude=1.0):
     """A ``RotaryPlan`` of frequencies base^(-2i/R), scaled for long contexts:
@@ -136,6 +135,14 @@ def rotary_plan(rotary_dim, *, base=10000.0, layout="half", scaling=None, factor
     ``high`` times kept, with a linear ramp between.  ``amplitude`` scales the
     turned values (by_parts plans often take 0.1 ln(factor) + 1).
     """
+    # (plans are constants: the same arguments give the same one; tensors and the like by what they hold now)
+    dim, *numbers = (x if x is None or type(x) in (int, float) else float(x)
+                     for x in (rotary_dim, base, factor, original_length, low, high, amplitude))
+    return _plan(dim, layout, scaling, *numbers)
+
+
+@functools.lru_cache(maxsize=64)
+def _plan(rotary_dim, layout, scaling, base, factor, original_length, low, high, amplitude):
     R = int(rotary_dim)
     if R != rotary_dim or R < 2 or R % 2:
         raise ValueError(f"rotary_dim must be an even number of at least 2; got {rotary_dim}")

@@ -328,3 +328,16 @@ def test_plans_of_learned_frequencies_are_refused():
     with torch.no_grad():
         assert rotary.RotaryPlan(f).frequencies.tolist() == [0.5, 0.25]
     assert rotary.RotaryPlan(f.detach()).frequencies.tolist() == [0.5, 0.25]
+
+
+def test_plans_of_arguments_that_change():
+    # a number in a tensor is taken when the plan is asked for
+    factor, base, dim = torch.tensor(2.0, dtype=torch.float64), torch.tensor(100.0), torch.tensor(8)
+    first = rotary.rotary_plan(dim, base=base, scaling="linear", factor=factor)
+    factor.fill_(4.0)
+    base.fill_(50.0)
+    dim.fill_(16)
+    second = rotary.rotary_plan(dim, base=base, scaling="linear", factor=factor)
+    assert torch.equal(first.frequencies, rotary.rotary_plan(8, base=100.0, scaling="linear", factor=2.0).frequencies)
+    assert torch.equal(second.frequencies, rotary.rotary_plan(16, base=50.0, scaling="linear", factor=4.0).frequencies)
+    assert rotary.rotary_plan(16, base=50) is rotary.rotary_plan(16, base=torch.tensor(50.0))
