@@ -32,9 +32,9 @@ def span(t):
 
 
 def _starts(at, dims):
-    x = torch.tensor([at], dtype=torch.int64)
+    x = torch.tensor([at], dtype=torch.int64, device="cpu")
     for s, n in dims:
-        x = (x[:, None] + s * torch.arange(n)).flatten()
+        x = (x[:, None] + s * torch.arange(n, device="cpu")).flatten()
     return x
 
 

@@ -79,10 +79,10 @@ class RotaryPlan:
     as long as a captured graph that uses it, as they keep the graph's tensors."""
 
     def __init__(self, frequencies, layout="half", amplitude=1.0):
-        f = torch.as_tensor(frequencies, dtype=torch.float64)
+        f = torch.as_tensor(frequencies, dtype=torch.float64, device="cpu")
         if (f.requires_grad and torch.is_grad_enabled()) or _has_tangent(f):
             raise RuntimeError("a plan's frequencies are constants: no gradient reaches them (detach them)")
-        f = f.detach().cpu().contiguous().clone()
+        f = f.detach().contiguous().clone()
         if f.dim() != 1 or f.numel() < 1 or not bool(torch.isfinite(f).all()):
             raise ValueError("frequencies must be a vector of finite numbers, one for each pair")
         if layout not in _LAYOUTS:
@@ -156,7 +156,7 @@ def _plan(rotary_dim, layout, scaling, base, factor, original_length, low, high,
         if R == 2:
             raise ValueError("ntk scaling needs rotary_dim of at least 4")
         base = base * factor ** (R / (R - 2.0))
-    f = base ** (-2.0 * torch.arange(R // 2, dtype=torch.float64) / R)
+    f = base ** (-2.0 * torch.arange(R // 2, dtype=torch.float64, device="cpu") / R)
     if scaling == "linear":
         f = f / factor
     elif scaling == "by_parts":

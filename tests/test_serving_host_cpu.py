@@ -341,3 +341,16 @@ def test_plans_of_arguments_that_change():
     assert torch.equal(first.frequencies, rotary.rotary_plan(8, base=100.0, scaling="linear", factor=2.0).frequencies)
     assert torch.equal(second.frequencies, rotary.rotary_plan(16, base=50.0, scaling="linear", factor=4.0).frequencies)
     assert rotary.rotary_plan(16, base=50) is rotary.rotary_plan(16, base=torch.tensor(50.0))
+
+
+def test_plans_and_checks_under_another_default_device():
+    want = rotary.rotary_plan(12, base=77.0).frequencies
+    a, b = torch.zeros(64).as_strided((1, 2, 3, 8), (0, 3, 5, 1)), torch.zeros(64).as_strided((1, 2, 3, 8), (0, 5, 3, 1))
+    assert (_overlap.meets_itself(a), _overlap.meet(a, b[..., :4])) == (True, False)
+    with torch.device("meta"):
+        rotary._plan.cache_clear()
+        assert torch.equal(rotary.rotary_plan(12, base=77.0).frequencies, want)
+        assert rotary.RotaryPlan([0.5, 0.25]).frequencies.tolist() == [0.5, 0.25]
+        for f in (_overlap._runs_overlap, _overlap._runs_meet):
+            f.cache_clear()
+        assert _overlap.meets_itself(a) and _overlap.meet(a, a.as_strided((1, 2, 3, 4), (0, 5, 3, 1), 1))
