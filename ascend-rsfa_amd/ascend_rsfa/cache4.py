@@ -24,7 +24,8 @@ All arithmetic runs in ``lib/librsfa.so`` (``rsfa_cache4_*`` in ``include/rsfa.h
 enqueued on the current stream of the cache's device; there is no other path.
 Calls that write a cache (append, attend with ``accumulate``, evict into it) and
 others on the same cache must run one after another: on one stream, or ordered by
-events.  No gradients: the cache is for inference.
+events.  No gradients, of either mode: the cache is for inference.  What a call writes has its
+version raised, as torch's in-place operators do.
 """
 import ctypes
 import math
@@ -315,7 +316,8 @@ class Cache4:
         ``lengths[z] - T + i``, with ``counts`` ``lengths[z] - counts[z] + i``, which is right
         while no slot has been evicted); otherwise all slots in use.  Tokens
         ``i >= counts[z]``, and tokens that see no slot, give 0 (lse -inf); so do tokens whose
-        visible scores are all -inf (an infinite q), as hidden scores are.
+        visible scores are all -inf (an infinite q), as hidden scores are.  Sums are in 32 bits;
+        softmax weights are rounded to the dtype for the product with v, as o is.
 
         ``accumulate`` adds to each slot's weight the attention that it received: the sum of
         its softmax weights over all tokens and the query heads of its group.

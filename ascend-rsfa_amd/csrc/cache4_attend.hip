@@ -20,8 +20,10 @@
 //                pairs of values and paired by key with v_perm_b32.
 // Statistics, sums and accumulators are in 32 bits.  The running maximum of a row
 // only moves when a score passes it by SLACK (log2 units), as the weights then
-// stay below 2^SLACK and the final division takes the factor out; the row
-// sum adds the weights before they are rounded to the cache's type for P V.
+// stay below 2^SLACK and the final division takes the factor out.  A weight is rounded to the
+// cache's type for P V, half a step at most, as the matrix unit takes 16-bit operands at sixteen times
+// the rate of 32-bit ones; the row sum, lse and the slots' weights take it unrounded.  (o is then about 1.35
+// times as far from 64 bits as with 32-bit weights, most of either distance being o's own rounding.)
 #include <cfloat>
 #include <type_traits>
 
@@ -189,10 +191,10 @@ struct Loader {
 // one tile while the next is loaded (26 registers at D = 128), with a scalar base and
 // constant offsets; with the checks for a partial tile inside of it, and the mask as a
 // second path, it took 250 registers and spilled.  One token of 32 heads, 8 key
-// heads: 64 sequences of 1024 to 4096 slots, D = 128, bf16, scores kept for the weights:
-// 36 us, 5.6 TB/s of codes, scales and scores; 32 x 8192 slots at D = 64, 128, 256: 30.8, 50, 109 us
-// (5.2 TB/s would be 27.6, 55, 110); one sequence of 32768 slots 9.6 us where the codes'
-// bytes are 6.9: the launch and the first loads.
+// heads, bf16, caches in turn so that none stays in the last-level cache: 64 sequences of 1024 to
+// 4096 slots, D = 128, scores kept for the weights: 47 us, 4.2 TB/s of codes, scales and scores (36 with one
+// cache); 32 x 8192 slots at D = 64, 128, 256: 39, 60, 114 us, 3.7, 4.7, 5.0 TB/s (32, 50, 114 with
+// one); one sequence of 32768 slots 10 us where the codes' bytes are 6.9: the launch and the first loads.
 template <class T, int D, int NB, bool CAUSAL>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
     typedef typename T::x8 x8;
@@ -482,9 +484,11 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
 // part of the next tile before the first piece, half after it, so that the two waves of a SIMD
 // want the matrix unit at different times.
 // Bound by the matrix and the vector units together: a chunk of 2048 tokens, 32 heads,
-// over 16384 slots of 8 key heads, D = 128, bf16, causal: 468 us, 1100 TFLOP/s.  (Four waves,
-// which convert twice as often: 75 us more; eight that convert together: 3, at D = 64 290
-// against 280 and at D = 256 494 against 459 of calls for 1024 tokens with weights.  The two
+// over 16384 slots of 8 key heads, D = 128, bf16, causal: 468 to 478 us, 1080 to 1100 TFLOP/s; at D = 64
+// 326 us, 790 TFLOP/s, where the vector unit is busy for 56 % of it and the matrix unit for 31 (45 and 45 at
+// D = 128).  (Four waves, which convert twice as often: 75 us more; eight that convert together: 3, and of calls for
+// 1024 tokens with weights at D = 64, two sequences of 32 heads, 8192 slots of 8, 290 against 280, at D = 256, 16
+// heads, 16384 slots of 4, 494 against 459.  The two
 // pieces in a loop instead of code of their own: 40 us more.  Direct operands
 // without LDS, 32 rows a wave: 1107.  Halves of a tile whose softmax and products alternate,
 // raised wave priority around the products, LDS reads two to eight MFMAs ahead:
@@ -948,13 +952,13 @@ __global__ void __launch_bounds__(256) finish_kernel(AttendParams p, int pp, int
 // registers at D = 128, 64 at 256); blocks of 32 rows of Q pass by in LDS, as operands
 // too, two buffers of ROW_BLOCKS blocks.  A workgroup takes the groups of row blocks
 // blockIdx.y, blockIdx.y + gridDim.y, ...
-// Bound as attend_many_kernel is, with half its products and all of its exponentials: 295
+// Bound as attend_many_kernel is, with half its products and all of its exponentials: 295 to 316
 // us for the chunk above, of which no part stands alone (in copies without it: loads of Q 56 less, seven of
 // eight products 94, exponentials 38).  Up to D = 128 a wave keeps to 128 registers, so
 // that four waves of a SIMD hide each other's products and exponentials; with 64
 // keys, two waves: 24 us more.  Row blocks between barriers, one, two, three, four: the two
-// kernels 861, 843, 840, 848 at D = 128, 346, 336, 329, 329 at D = 64.  D = 256 (1024 rows a
-// head, 16384 slots) does not fit four waves: 536 us spilled, 513 with two; one row block
+// kernels 861, 843, 840, 848 at D = 128, 346, 336, 329, 329 at D = 64.  D = 256 (1024 tokens of
+// 16 heads, 16384 slots of 4) does not fit four waves: 536 us spilled, 513 with two; one row block
 // 548, two 514, four, which leave room for one workgroup, 666.  (16 x 16 tiles with Q from
 // global memory: 492 of the chunk.)
 template <int D>
@@ -1045,7 +1049,7 @@ __global__ void __launch_bounds__(64 * Weigh<D>::WAVES, Weigh<D>::OCCUPANCY) wei
     float lse2[RB];
     int tok2[RB];
     // (what was loaded is first looked at here: a comparison where it is loaded waits for it, 462 us against 433
-    // for 1024 tokens at D = 256)
+    // for 1024 tokens of 16 heads, 16384 slots of 4, at D = 256)
     auto store = [&](int buf, int row0) {
 #pragma unroll
         for (int g = 0; g < RB; ++g) {
@@ -1156,14 +1160,14 @@ Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
     const int64_t group = a->heads / a->cache.h, rows = group * a->t;
     const int64_t bh = a->cache.z * a->cache.h;
     const int64_t most = a->max_length > 0 && a->max_length < a->cache.capacity ? a->max_length : a->cache.capacity;
-    // (32 heads of 8192 slots, bf16, causal, few and many rows' kernel: 40 rows at D = 64
-    // 23.9 and 21.6 us, at 128 30.1 and 28.2, at 256 52 and 55; 64 rows 26.4 and 23.9, 31.9 and
-    // 30.6, 68 and 60; 24 rows at D = 256 37 and 53)
+    // (32 key heads of 8192 slots, bf16, causal, caches in turn, few and many rows' kernel at D = 64, 128, 256: 32 rows 17
+    // and 26 us, 20 and 29, 38 and 55; 64 rows 24 and 27, 32 and 31, 63 and 66; 128 rows 36 and 31, 53 and 37, 94 and 92:
+    // up to 64 rows the few rows' kernel would still be ahead at D = 64 and 256)
     const bool few = rows <= 32;
     p.few = few;
     p.nb = rows <= 16 || a->cache.head_dim == 256 ? 1 : 2;
-    // (D = 256, four and eight waves: 128 rows of 32 heads of 8192 slots 83 and 91 us, 192 rows 108 and 97; below
-    // 256 eight are never slower: 64 rows at D = 128 31.6 and 30.7, 384 rows 93 and 71)
+    // (D = 256, four and eight waves: 128 rows of the same 92 and 96 us, 192 rows 115 and 107; below 256 they are
+    // the same within half a microsecond)
     p.waves = few || (a->cache.head_dim == 256 && rows <= 128) ? 4 : 8;
     const int64_t tile_rows = few ? 16 * p.nb : 32 * p.waves;
     p.tiles = (int)((rows + tile_rows - 1) / tile_rows);

@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(THREADS) select_kernel(EvictParams p) {
 constexpr int PART_THREADS = 256, PART_WAVES = 4, MAX_PARTS = 32;
 
 // f(key, slot) for the part's slots (the ends of rounds past the length among them, as
-// PROTECTED); a wave's are consecutive.  Without RECENT, recency protects nothing.
+// PROTECTED); a wave's are consecutive.  Positions above `old` are protected, and below the sinks.
 template <class F>
 __device__ __forceinline__ void each_of_part(const EvictParams& p, const Row& r, int64_t old, int lane, int wave, F&& f) {
     const int per = p.part / PART_WAVES;

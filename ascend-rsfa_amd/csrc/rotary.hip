@@ -43,7 +43,9 @@ struct alignas(sizeof(E) * V) Vec {
     E v[V];
 };
 
-// Sine and cosine of 2 pi p f, scaled.
+// Sine and cosine of 2 pi p f, scaled.  The fraction of a turn goes into them in 32 bits (2^-26 of a turn, 1.6 * 2^-24
+// radians at most): of the three types only float32 has steps as small, and 64-bit sines would take many
+// times the instructions.
 __device__ __forceinline__ void angle(double p, double f, float amp, bool inverse, float& s, float& c) {
     const double turn = p * f;
     float frac = (float)(turn - __builtin_rint(turn));

@@ -288,7 +288,7 @@ typedef struct rsfa_cache4 {
  * to slot lengths[z] + i, or with `slots` (device, int32 [z, h, t], dense) to
  * slots[z, h, i]; tokens i >= counts[z] (device, int32 [z], or NULL) and
  * slots outside [0, capacity) are left out; where `slots` names a slot twice
- * the last token has it.  The slot's position becomes pos_start[z] + i (NULL:
+ * the last token has it (more than 96 tokens take four launches for that).  The slot's position becomes pos_start[z] + i (NULL:
  * lengths[z] + i), its weight 0.
  * read: the values of slots start[z] + i (NULL: start0 + i), or slots[z, h, i],
  * into k, v; rows outside [0, capacity) read as 0. */
@@ -316,6 +316,8 @@ int rsfa_cache4_read(const rsfa_cache4_rows_args *args, void *stream);
  * and rows that see no slot, give 0 (lse -inf); so do rows whose visible scores are
  * all -inf (an infinite q), as hidden scores are.  With `accumulate` the weights
  * of the slots grow by the softmax weights that all rows of the call gave them.
+ * Scores, sums, lse and the slots' weights are in 32 bits; for the product with v a softmax
+ * weight is rounded to the cache's type (half a step), as o is.
  * Lengths above max_length (0: the capacity) are taken as max_length.  o must not
  * overlap q; calls that accumulate into one cache must not overlap in time.
  * Workspace: rsfa_cache4_attend_workspace_bytes of the same arguments (its
@@ -353,7 +355,7 @@ uint64_t rsfa_cache4_attend_workspace_bytes(const rsfa_cache4_attend_args *args)
  * after all others), in order of slot, to its slots 0, 1, ...; other slots of `into`
  * keep what they hold.
  * Workspace: rsfa_cache4_evict_workspace_bytes of the same arguments (evict: 1
- * for evict, 0 for claim; 0 bytes for claims in caches of up to 8192 slots). */
+ * for evict, 0 for claim; 0 bytes for claims in caches of up to 32768 slots). */
 typedef struct rsfa_cache4_evict_args {
     uint32_t       struct_size; /* = sizeof(rsfa_cache4_evict_args)            */
     uint32_t       reserved;    /* 0 */
