@@ -344,7 +344,7 @@ class Cache4:
                     raise ValueError("out must match q's shape, dtype and device and have a unit-stride head dim")
                 if o.numel() and _overlap.meets_itself(o):
                     raise ValueError("the rows of out must not share memory")
-                if o.numel() and _overlap.meet(o, q):
+                if o.numel() and _overlap.meet(o, q_):  # (a copy of q meets nothing)
                     raise ValueError("out must not share memory with q")
             args = _native.Cache4AttendArgs()
             args.struct_size = ctypes.sizeof(args)

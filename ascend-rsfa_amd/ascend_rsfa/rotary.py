@@ -67,7 +67,7 @@ def _function():
 
 def _has_tangent(*xs):
     """Whether a tensor carries a derivative of forward mode (no grad mode hides it)."""
-    return forward_ad._current_level >= 0 and any(
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
         x is not None and forward_ad.unpack_dual(x).tangent is not None for x in xs)
 
 
