@@ -239,6 +239,38 @@ def test_on_a_side_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(out, eager)), step
 
 
+def test_backward_in_a_graph():
+    # as torch asks of a captured backward pass: tried on a side stream first, no eager graph of the leaves alive
+    q, k = _inputs(2, 4, 2, 33, 64, torch.bfloat16, "bshd", 4)
+    gq, gk = _inputs(2, 4, 2, 33, 64, torch.bfloat16, "bhsd", 5)
+    plan = _plan(48, "half", "linear")
+    positions = torch.arange(33).cuda()
+    q.requires_grad_(), k.requires_grad_()
+
+    def step():
+        return torch.autograd.grad(R.rotary(q, k, positions, plan), (q, k), (gq, gk))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        dq, dk = step()
+    for start in (0, 7, 90000):
+        with torch.no_grad():
+            positions.copy_(torch.arange(33).cuda() + start)
+            gq.copy_(gq.flip(0))
+            gk.copy_(gk.flip(0))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(dq, gq, positions, plan, inverse=True)
+        _check(dk, gk, positions, plan, inverse=True)
+
+
 def test_refusals():
     plan = _plan(64, "half")
     x = torch.zeros((1, 2, 3, 64)).cuda().half()
