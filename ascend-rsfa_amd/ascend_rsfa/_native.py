@@ -27,6 +27,7 @@ E_SCRATCH = -11
 E_ROTARY = -12
 E_CACHE = -13
 E_BUDGET = -14
+E_DRAFT = -15
 
 # rsfa_dtype
 DTYPE_F16 = 0
@@ -48,6 +49,9 @@ ROTARY_POS64 = 0x4
 
 # rsfa_attention_fwd_noalloc's fixed workspace
 NOALLOC_WORKSPACE_BYTES = 16 << 20
+
+# most drafted tokens of a call
+DRAFT_TOKENS = 512
 
 # Every symbol include/rsfa.h declares, with (restype, argtypes).
 _I64 = ctypes.c_int64
@@ -196,6 +200,37 @@ class Cache4EvictArgs(ctypes.Structure):
     ]
 
 
+class DraftTreeArgs(ctypes.Structure):
+    """Mirror of struct rsfa_draft_tree_args."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("parents", ctypes.c_void_p),
+        ("parents_stride", ctypes.c_int64),
+        ("trees", ctypes.c_int64),
+        ("t", ctypes.c_int64),
+        ("bits", ctypes.c_void_p),
+        ("depths", ctypes.c_void_p),
+    ]
+
+
+class Cache4KeepArgs(ctypes.Structure):
+    """Mirror of struct rsfa_cache4_keep_args."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("cache", Cache4),
+        ("tokens", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("length", ctypes.c_int64),
+        ("counts", ctypes.c_void_p),
+        ("pos_start", ctypes.c_void_p),
+    ]
+
+
 SIGNATURES = {
     "rsfa_attention_fwd": (ctypes.c_int, [ctypes.POINTER(FwdArgs), ctypes.c_void_p]),
     "rsfa_attention_fwd_noalloc": (ctypes.c_int, [ctypes.POINTER(FwdArgs), ctypes.c_void_p]),
@@ -212,6 +247,9 @@ SIGNATURES = {
     "rsfa_cache4_claim": (ctypes.c_int, [ctypes.POINTER(Cache4EvictArgs), ctypes.c_void_p]),
     "rsfa_cache4_evict": (ctypes.c_int, [ctypes.POINTER(Cache4EvictArgs), ctypes.c_void_p]),
     "rsfa_cache4_evict_workspace_bytes": (ctypes.c_uint64, [ctypes.POINTER(Cache4EvictArgs), _I32]),
+    "rsfa_draft_tree": (ctypes.c_int, [ctypes.POINTER(DraftTreeArgs), ctypes.c_void_p]),
+    "rsfa_cache4_attend_tree": (ctypes.c_int, [ctypes.POINTER(Cache4AttendArgs), ctypes.c_void_p, _I64, ctypes.c_void_p]),
+    "rsfa_cache4_keep": (ctypes.c_int, [ctypes.POINTER(Cache4KeepArgs), ctypes.c_void_p]),
     "rsfa_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "rsfa_abi_version": (ctypes.c_int, []),
 }

@@ -11,6 +11,7 @@ for sequences [Z], key heads [H] and ``capacity`` slots each:
                 weight grows by the attention it received
 ``claim``       slots for the next tokens of a full cache: those of least weight
 ``evict``       copies the slots of most weight into a smaller cache
+``keep``        moves the rows of accepted drafted tokens to the end of their context
 ==============  ==================================================================
 
 How many slots of a sequence are in use is the caller's: every call takes
@@ -24,7 +25,7 @@ All arithmetic runs in ``lib/librsfa.so`` (``rsfa_cache4_*`` in ``include/rsfa.h
 enqueued on the current stream of the cache's device; there is no other path.
 Calls that write a cache (append, attend with ``accumulate``, evict into it) and
 others on the same cache must run one after another: on one stream, or ordered by
-events.  No gradients, of either mode: the cache is for inference.  What a call writes has its
+events; so does ``keep``.  No gradients, of either mode: the cache is for inference.  What a call writes has its
 version raised, as torch's in-place operators do.
 """
 import ctypes
@@ -35,6 +36,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _native, _overlap
+from .draft import DraftTree
 from .flash_attention_forward import _as_kernel_layout, _meets_contract, _raise_for
 from .rotary import _has_tangent
 
@@ -59,6 +61,9 @@ assert _AT_HEADS - _AT_Q == _AT_QO.size and ctypes.sizeof(_native.Cache4AttendAr
 _EVICT_LENGTHS = _native.Cache4EvictArgs.lengths.offset
 _EVICT_TAIL = struct.Struct("=QqqqqqQQQ")  # lengths, length, n, budget, recent, sinks, out, workspace, its bytes
 assert ctypes.sizeof(_native.Cache4EvictArgs) - _EVICT_LENGTHS == _EVICT_TAIL.size
+_KEEP_TOKENS = _native.Cache4KeepArgs.tokens.offset
+_KEEP_TAIL = struct.Struct("=QqQqQQ")  # tokens, n, lengths, length, counts, pos_start
+assert ctypes.sizeof(_native.Cache4KeepArgs) - _KEEP_TOKENS == _KEEP_TAIL.size
 _FUNCTIONS = {}
 
 
@@ -67,6 +72,14 @@ def _function(name):
     fn = _FUNCTIONS.get(name)
     if fn is None:
         fn = _FUNCTIONS[name] = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)((name, _native.lib()))
+    return fn
+
+
+def _tree_function():
+    fn = _FUNCTIONS.get("tree")
+    if fn is None:
+        fn = _FUNCTIONS["tree"] = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p)(
+            ("rsfa_cache4_attend_tree", _native.lib()))
     return fn
 
 
@@ -306,7 +319,7 @@ class Cache4:
 
     # -- attention ----------------------------------------------------------
     def attend(self, q, lengths, causal, sm_scale, *, positions=None, counts=None, accumulate=False,
-               return_lse=False, max_length=None, out=None):
+               return_lse=False, max_length=None, out=None, tree=None):
         """softmax(q k^T sm_scale) v over the slots in use: ``o``, or ``(o, lse)``.
 
         q [Z, Hq, T, D] in the cache's dtype, Hq a multiple of H: query head i reads key
@@ -326,6 +339,11 @@ class Cache4:
         (With ``accumulate`` and at most 32 rows a key head, tokens times group, the workspace
         holds 4 bytes for each row and slot, up to 4 GiB.)
         ``lse``: the natural logarithm of each row's sum of exponentials, float32 [Z, Hq, T].
+
+        ``tree`` (a ``DraftTree`` of T tokens, with ``causal``): the tokens are drafted ones, the last T
+        (``counts[z]``) slots in use.  Token i sees every slot before them, whatever its position, and
+        the drafted tokens that its row of the tree names; a token without context that sees none gives 0.
+        No ``positions``, no ``accumulate``: drafted tokens that are not accepted leave no weight.
         """
         _no_gradient(q) if out is None else _no_gradient(q, out)
         key = ("attend", q.shape, q.stride(), q.dtype, q.device, bool(causal), None if out is None else out.stride())
@@ -373,6 +391,8 @@ class Cache4:
         scale = float(sm_scale)
         if math.isnan(scale):
             raise ValueError("sm_scale is NaN")
+        if tree is not None:
+            self._check_tree(tree, q.shape[2], causal, positions, accumulate)
         if q.numel() == 0:
             return (o, lse) if return_lse else o
         accumulate = int(bool(accumulate))
@@ -385,13 +405,58 @@ class Cache4:
             if at:  # (an int's bound changes from call to call)
                 parts[2][max_length, accumulate] = nbytes
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
-        self._call("rsfa_cache4_attend", head + _AT_TAIL.pack(at, length, max_length, counts, positions, scale, accumulate,
-                                                              ws.data_ptr() if nbytes else 0, nbytes))
+        args = head + _AT_TAIL.pack(at, length, max_length, counts, positions, scale, accumulate, ws.data_ptr() if nbytes else 0, nbytes)
+        if tree is None:
+            self._call("rsfa_cache4_attend", args)
+        else:
+            _raise_for(self._on_device(_tree_function(), args, tree.bits.data_ptr(), tree.bits.stride(0) if tree.trees > 1 else 0,
+                                       torch._C._cuda_getCurrentRawStream(self.device.index)))
         if out is not None:
             increment_version(out)
         if accumulate:
             increment_version(self.weights)
         return (o, lse) if return_lse else o
+
+    def _check_tree(self, tree, T, causal, positions, accumulate):
+        if not isinstance(tree, DraftTree):
+            raise TypeError("tree must be a DraftTree")
+        if not causal or positions or accumulate:
+            raise ValueError("a tree goes with causal, without positions and accumulate")
+        if tree.tokens != T or tree.trees not in (1, self.Z):
+            raise ValueError(f"the tree must be of {T} tokens, one or {self.Z} of them; got {tree.trees} of {tree.tokens}")
+        if tree.bits.device != self.device:
+            raise ValueError("the tree must be on the cache's device")
+
+    # -- drafted tokens -----------------------------------------------------
+    def keep(self, tokens, lengths, *, counts=None, positions=None):
+        """Moves the rows of accepted drafted tokens to the end of their context.
+
+        ``tokens``: int32 [Z, n], n at most 512, the accepted ones in the order of their text;
+        ``counts`` (int32 [Z]): how many of them each sequence has (None: n).  ``lengths`` are those of the contexts,
+        so drafted token t lies in slot ``lengths[z] + t``.  Row j goes to slot ``lengths[z] + j`` of every
+        head, with its weight, and takes the position ``positions[z] + j`` (int32 [Z]; None: ``lengths[z] + j``).
+        All are read before one is written.  Tokens outside the cache (-1, say) leave slot
+        ``lengths[z] + j`` as it is, as do all j from ``counts[z]`` on."""
+        if not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != self.Z:
+            raise TypeError(f"tokens must be an int32 tensor [{self.Z}, n]")
+        if tokens.device != self.device:
+            raise ValueError("tokens must be on the cache's device")
+        n = tokens.shape[1]
+        if n > _native.DRAFT_TOKENS:
+            raise ValueError(f"at most {_native.DRAFT_TOKENS} drafted tokens; got {n}")
+        tokens = tokens.contiguous()
+        at, length = self._lengths(lengths)
+        counts, positions = self._vector(counts, "counts"), self._vector(positions, "positions")
+        if n == 0:
+            return
+        head = self._kept.get("keep")
+        if head is None:
+            args = _native.Cache4KeepArgs()
+            args.struct_size = ctypes.sizeof(args)
+            args.cache = self._c
+            head = self._keep("keep", bytes(args)[:_KEEP_TOKENS])
+        self._call("rsfa_cache4_keep", head + _KEEP_TAIL.pack(tokens.data_ptr(), n, at, length, counts, positions))
+        increment_version(self._buffers)
 
     # -- eviction -----------------------------------------------------------
     def _evict_call(self, name, into, lengths, n, budget, recent, sinks, out):

@@ -62,7 +62,23 @@ struct AttendParams {
     float* scores;             // [bh][rows][most]: scores in log2 units, or null
     float* row_lse;            // [bh][rows]: log2 of the row's sum of exp2 (for the weights)
     float* part_w;             // [parts][bh][most]: sums of parts of the rows, or null
+    const uint32_t* tree;      // MASK_TREE: [Z][t][tree_words]: the drafted tokens that a token sees
+    int64_t tree_sz;           // its stride of Z (0: one tree for all)
+    int32_t tree_words;
 };
+
+// What a row sees of the slots in use: all of them; those of a position up to its own; or those before the
+// call's drafted tokens, which are the last `count` slots in use, and of these the ones whose bit its token has.
+enum { MASK_NONE = 0, MASK_POSITION = 1, MASK_TREE = 2 };
+
+// The 32 slots whose first is the drafted token `first` (below 0: slots of the context, all seen), as a mask,
+// from the bits of a token.  A token past the bits' last word is seen by none.
+__device__ __forceinline__ uint32_t tree_mask(const uint32_t* bits, int words, int first) {
+    const int w = first >> 5;  // (rounds down)
+    const uint32_t lo = w < 0 ? 0xffffffffu : w < words ? bits[w] : 0u;
+    const uint32_t hi = w + 1 < 0 ? 0xffffffffu : w + 1 < words ? bits[w + 1] : 0u;
+    return __builtin_amdgcn_alignbit(hi, lo, first & 31);
+}
 
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -186,7 +202,8 @@ struct Loader {
 
 // Few rows (NB blocks of 16): the four waves of a workgroup take every fourth key
 // tile of its part of the slots and add up what they have at the end.  CAUSAL hides
-// keys in every tile; otherwise only the last, partial tile does.
+// keys in every tile; otherwise only the last, partial tile does, and a tree hides some of the drafted tokens: its
+// tiles from the first drafted token on take the masked path, the context's the other.
 // Bound by memory: D/2 + D/32 bytes of K and as many of V a slot.  The loop holds
 // one tile while the next is loaded (26 registers at D = 128), with a scalar base and
 // constant offsets; with the checks for a partial tile inside of it, and the mask as a
@@ -195,8 +212,9 @@ struct Loader {
 // 4096 slots, D = 128, scores kept for the weights: 47 us, 4.2 TB/s of codes, scales and scores (36 with one
 // cache); 32 x 8192 slots at D = 64, 128, 256: 39, 60, 114 us, 3.7, 4.7, 5.0 TB/s (32, 50, 114 with
 // one); one sequence of 32768 slots 10 us where the codes' bytes are 6.9: the launch and the first loads.
-template <class T, int D, int NB, bool CAUSAL>
+template <class T, int D, int NB, int MASK>
 __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
+    constexpr bool CAUSAL = MASK == MASK_POSITION, TREE = MASK == MASK_TREE;
     typedef typename T::x8 x8;
     typedef typename T::elem elem;
     constexpr int DT = D / 16;  // 16-row tiles of O^T
@@ -226,8 +244,9 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
     const int64_t start64 = (int64_t)chunk * split;
     const int start = (int)(start64 < len ? start64 : len);
     const int end = min(start + chunk, len);
-    // whole tiles of this wave, and whether the partial one is its own
-    const int whole = (end - start) / TILE;
+    // whole tiles of this wave (a tree: of the context), and whether the partial one is its own
+    const int context = len - count;  // (a tree: the slot of the first drafted token; below 0 it has none)
+    const int whole = (TREE ? max(0, min(end, context) - start) : end - start) / TILE;
     const int turns = whole > wave ? (whole - wave + WAVES - 1) / WAVES : 0;
     const bool tail = (end - start) % TILE != 0 && whole % WAVES == wave;
 
@@ -237,6 +256,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
     // Q^T and the rows' positions
     x8 q[NB][QS];
     int qpos[NB];
+    const uint32_t* bits[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int row = row0 + 16 * b + col;
@@ -258,6 +278,7 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
             const int64_t at = (p.pos_start ? (int64_t)p.pos_start[z] : (int64_t)len - count) + tok;
             qpos[b] = (int)(at > 0x7fffffff ? 0x7fffffff : at);
         }
+        if (TREE) bits[b] = p.tree + z * p.tree_sz + (int64_t)(valid ? tok : 0) * p.tree_words;
     }
 
     f32x4 acc[NB][DT];
@@ -300,10 +321,12 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = s[b][j / 4][j % 4] * p.scale;
             if constexpr (MASKED) {
+                uint32_t seen = 0;
+                if constexpr (TREE) seen = tree_mask(bits[b], p.tree_words, tile - context);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int key = tile + 16 * (j / 4) + 4 * grp + j % 4;
-                    const bool hidden = (TAIL && key >= end) || (CAUSAL && r.pos[j] > qpos[b]);
+                    const int at = 16 * (j / 4) + 4 * grp + j % 4, key = tile + at;
+                    const bool hidden = (TAIL && key >= end) || (CAUSAL && r.pos[j] > qpos[b]) || (TREE && !(seen >> at & 1));
                     if (hidden) x[j] = -INFINITY, visible[b] &= ~(1u << j);
                 }
             }
@@ -401,7 +424,12 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
         compute(cur, tile, std::false_type());
         cur = next;
     }
-    if (tail) {
+    if constexpr (TREE) {
+        for (int i = whole + (wave - whole % WAVES + WAVES) % WAVES; start + TILE * i < end; i += WAVES) {
+            ld.template load<true>(cur, start + TILE * i, len - 1);
+            compute(cur, start + TILE * i, std::true_type());
+        }
+    } else if (tail) {
         const int tile = start + TILE * whole;
         ld.template load<true>(cur, tile, len - 1);
         compute(cur, tile, std::true_type());
@@ -514,8 +542,9 @@ __device__ __forceinline__ f32x16 mfma32(BF16::x8 a, BF16::x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-template <class T, int D, bool CAUSAL, int W>
+template <class T, int D, int MASK, int W>
 __global__ void __launch_bounds__(64 * W, 2) attend_many_kernel(AttendParams p) {
+    constexpr bool CAUSAL = MASK == MASK_POSITION, TREE = MASK == MASK_TREE;
     typedef Many<D, W> M;
     typedef typename T::x8 x8;
     typedef typename T::elem elem;
@@ -568,6 +597,9 @@ __global__ void __launch_bounds__(64 * W, 2) attend_many_kernel(AttendParams p) 
             }
         }
     }
+
+    const int context = len - count;  // (a tree: the slot of the first drafted token)
+    const uint32_t* const bits = TREE ? p.tree + z * p.tree_sz + (int64_t)(valid ? tok : 0) * p.tree_words : nullptr;
 
     // this wave's part of a tile's conversion
     struct {
@@ -682,7 +714,7 @@ __global__ void __launch_bounds__(64 * W, 2) attend_many_kernel(AttendParams p) 
     auto compute = [&](int buf, int tile, int piece) {
         const int kb = piece * SB, vb = M::KFRAGS + piece * 2 * SB * DT, at = piece * PIECE;
         tile += at;
-        bool masked = tile + PIECE > end;
+        bool masked = tile + PIECE > (TREE ? min(end, context) : end);
         if (CAUSAL) {
             const int kp = kpos[buf][at + (lane & (PIECE - 1))];
             masked |= __any(kp > least);
@@ -699,14 +731,17 @@ __global__ void __launch_bounds__(64 * W, 2) attend_many_kernel(AttendParams p) 
             for (int b = 0; b < SB; ++b) s[b] = mfma32(__builtin_bit_cast(x8, frag[buf][(kb + b) * QS + i][lane]), q[i], s[b]);
         if (__builtin_expect(masked, 0)) {
 #pragma unroll
-            for (int b = 0; b < SB; ++b)
+            for (int b = 0; b < SB; ++b) {
+                const uint32_t seen = TREE ? tree_mask(bits, p.tree_words, tile + 32 * b - context) : 0u;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int key = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+                    const int sub = 8 * (r / 4) + 4 * half + r % 4, key = 32 * b + sub;
                     bool hidden = tile + key >= end;
                     if (CAUSAL) hidden |= kpos[buf][at + key] > qpos;
+                    if (TREE) hidden |= !(seen >> sub & 1);
                     if (hidden) s[b][r] = -INFINITY;
                 }
+            }
         }
         float top = s[0][0];
 #pragma unroll
@@ -749,6 +784,7 @@ __global__ void __launch_bounds__(64 * W, 2) attend_many_kernel(AttendParams p) 
             for (int k = 0; k < PIECE && tile + k < end; ++k) {
                 bool sees = true;
                 if (CAUSAL) sees = kpos[buf][at + k] <= qpos;
+                if (TREE) sees = tree_mask(bits, p.tree_words, tile + k - context) & 1;
                 if (!sees) continue;
                 for (int r = 0; r < 16; ++r) {
                     const int i = 8 * (r / 4) + 4 * half + r % 4;
@@ -1212,16 +1248,16 @@ int cus_of_current_device() {
     return n;
 }
 
-template <class T, int D, bool CAUSAL>
+template <class T, int D, int MASK>
 const void* attend_fn(const Plan& p) {
     if (p.few) {
         if constexpr (D <= 128)
-            if (p.nb == 2) return (const void*)&attend_kernel<T, D, 2, CAUSAL>;
-        return (const void*)&attend_kernel<T, D, 1, CAUSAL>;
+            if (p.nb == 2) return (const void*)&attend_kernel<T, D, 2, MASK>;
+        return (const void*)&attend_kernel<T, D, 1, MASK>;
     }
     if constexpr (D == 256)
-        if (p.waves == 4) return (const void*)&attend_many_kernel<T, D, CAUSAL, 4>;
-    return (const void*)&attend_many_kernel<T, D, CAUSAL, 8>;
+        if (p.waves == 4) return (const void*)&attend_many_kernel<T, D, MASK, 4>;
+    return (const void*)&attend_many_kernel<T, D, MASK, 8>;
 }
 
 struct Functions {
@@ -1229,18 +1265,21 @@ struct Functions {
 };
 
 template <class T, int D>
-Functions functions(const Plan& p, bool causal) {
-    return {causal ? attend_fn<T, D, true>(p) : attend_fn<T, D, false>(p), (const void*)&finish_kernel<T, D>,
-            causal ? (const void*)&weights_kernel<T, D, true> : (const void*)&weights_kernel<T, D, false>};
+Functions functions(const Plan& p, int mask) {
+    return {mask == MASK_TREE       ? attend_fn<T, D, MASK_TREE>(p)
+            : mask == MASK_POSITION ? attend_fn<T, D, MASK_POSITION>(p)
+                                    : attend_fn<T, D, MASK_NONE>(p),
+            (const void*)&finish_kernel<T, D>,
+            mask == MASK_POSITION ? (const void*)&weights_kernel<T, D, true> : (const void*)&weights_kernel<T, D, false>};
 }
 
 template <class T>
-Functions functions(const Plan& p, bool causal, int64_t d) {
+Functions functions(const Plan& p, int mask, int64_t d) {
     switch (d) {
-        case 32: return functions<T, 32>(p, causal);
-        case 64: return functions<T, 64>(p, causal);
-        case 128: return functions<T, 128>(p, causal);
-        default: return functions<T, 256>(p, causal);
+        case 32: return functions<T, 32>(p, mask);
+        case 64: return functions<T, 64>(p, mask);
+        case 128: return functions<T, 128>(p, mask);
+        default: return functions<T, 256>(p, mask);
     }
 }
 
@@ -1255,16 +1294,7 @@ int check_attend(const rsfa_cache4_attend_args* a) {
     return RSFA_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-uint64_t rsfa_cache4_attend_workspace_bytes(const rsfa_cache4_attend_args* a) {
-    if (check_attend(a) != RSFA_OK) return 0;
-    return make_plan(a, cus_of_current_device()).bytes;
-}
-
-int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
+int attend(const rsfa_cache4_attend_args* a, const int32_t* tree, int64_t tree_stride, int mask, void* stream) {
     int st = check_attend(a);
     if (st != RSFA_OK) return st;
     if (!a->q || !a->o) return RSFA_E_NULL;
@@ -1297,9 +1327,11 @@ int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
     if (plan.splits > 1 || plan.scores) p.part_ml = (float2*)(ws + plan.part_ml);
     if (a->accumulate && !plan.scores) p.row_lse = (float*)(ws + plan.row_lse);
     if (plan.scores) p.scores = (float*)(ws + plan.scores_at);
-    const bool causal = a->causal != 0;
-    const Functions fn = a->cache.dtype == RSFA_DTYPE_BF16 ? functions<BF16>(plan, causal, a->cache.head_dim)
-                                                           : functions<F16>(plan, causal, a->cache.head_dim);
+    p.tree = (const uint32_t*)tree;
+    p.tree_sz = tree_stride;
+    p.tree_words = (p.t + 31) / 32;
+    const Functions fn = a->cache.dtype == RSFA_DTYPE_BF16 ? functions<BF16>(plan, mask, a->cache.head_dim)
+                                                           : functions<F16>(plan, mask, a->cache.head_dim);
     const int64_t grid = (int64_t)p.bh * plan.tiles;
     const int64_t weight_grid = (int64_t)p.bh * plan.weight_tiles;
     const int64_t join_grid = (int64_t)p.bh * ((p.most + 255) / 256);
@@ -1333,6 +1365,27 @@ int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
         }
     }
     return RSFA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t rsfa_cache4_attend_workspace_bytes(const rsfa_cache4_attend_args* a) {
+    if (check_attend(a) != RSFA_OK) return 0;
+    return make_plan(a, cus_of_current_device()).bytes;
+}
+
+int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {
+    return attend(a, nullptr, 0, a && a->causal ? MASK_POSITION : MASK_NONE, stream);
+}
+
+int rsfa_cache4_attend_tree(const rsfa_cache4_attend_args* a, const int32_t* bits, int64_t bits_stride, void* stream) {
+    if (!a || !bits) return RSFA_E_NULL;
+    if (a->struct_size != sizeof(rsfa_cache4_attend_args)) return RSFA_E_ABI;
+    if ((uintptr_t)bits & 3) return RSFA_E_ALIGN;
+    if (a->accumulate || a->pos_start || a->t > RSFA_DRAFT_TOKENS || bits_stride < 0) return RSFA_E_DRAFT;
+    return attend(a, bits, bits_stride, MASK_TREE, stream);
 }
 
 }  // extern "C"

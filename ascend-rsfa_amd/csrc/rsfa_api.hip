@@ -523,6 +523,9 @@ const char* rsfa_strerror(int status) {
         case RSFA_E_BUDGET:
             return "claim and evict need 0 <= recent + sinks <= budget <= capacity and n >= 1; evict a target of "
                    "the cache's shape with room for the budget";
+        case RSFA_E_DRAFT:
+            return "drafted tokens: 1 to 512 (RSFA_DRAFT_TOKENS) of them; attention of a tree takes no accumulate "
+                   "and no first positions";
         default: return "unknown rsfa status";
     }
 }

@@ -69,7 +69,9 @@ typedef enum rsfa_status {
     RSFA_E_ROTARY    = -12, /* rsfa_rotary: rotary_dim odd, < 2 or > head_dim   */
     RSFA_E_CACHE     = -13, /* a cache or a call on one is out of its range: see
                                rsfa_cache4                                      */
-    RSFA_E_BUDGET    = -14  /* claim / evict: budget, recent, sinks or n         */
+    RSFA_E_BUDGET    = -14, /* claim / evict: budget, recent, sinks or n         */
+    RSFA_E_DRAFT     = -15  /* drafted tokens: more than RSFA_DRAFT_TOKENS, or
+                               an option that a tree does not go with           */
 } rsfa_status;
 
 typedef enum rsfa_dtype {
@@ -373,6 +375,57 @@ typedef struct rsfa_cache4_evict_args {
 int rsfa_cache4_claim(const rsfa_cache4_evict_args *args, void *stream);
 int rsfa_cache4_evict(const rsfa_cache4_evict_args *args, void *stream);
 uint64_t rsfa_cache4_evict_workspace_bytes(const rsfa_cache4_evict_args *args, int32_t evict);
+
+/* ------------------------------------------------------------------------
+ * Drafted tokens.
+ *
+ * A program that drafts appends t tokens that may follow each sequence's context to its cache,
+ * attends with all of them at once, and keeps those that it accepts.  The drafted tokens of a
+ * sequence are its last slots in use, in order; which of them a token sees is a row of
+ * (t + 31) / 32 words: token j where bit j % 32 of word j / 32 is set.
+ * ------------------------------------------------------------------------ */
+#define RSFA_DRAFT_TOKENS 512
+
+/* The rows of trees: token i sees itself and its ancestors.  parents[i] is an
+ * earlier token, or anything else: token i follows the context's last token.
+ * depths[i] counts the ancestors: the token's position is the context's
+ * length + depths[i]. */
+typedef struct rsfa_draft_tree_args {
+    uint32_t       struct_size; /* = sizeof(rsfa_draft_tree_args)              */
+    uint32_t       reserved;    /* 0 */
+    const int32_t *parents;     /* device, [trees, t], rows dense              */
+    int64_t        parents_stride;
+    int64_t        trees, t;    /* t: 1 .. RSFA_DRAFT_TOKENS                    */
+    int32_t       *bits;        /* device, [trees, t, (t + 31) / 32], dense     */
+    int32_t       *depths;      /* device, [trees, t], dense                   */
+} rsfa_draft_tree_args;
+
+int rsfa_draft_tree(const rsfa_draft_tree_args *args, void *stream);
+
+/* rsfa_cache4_attend over a context and drafted tokens: lengths count both, the
+ * t tokens (counts[z] of them) being the last slots in use.  Token i sees all slots before
+ * them, and drafted token j < counts[z] where row i of `bits` has it; positions and `causal`
+ * are not looked at.  `bits`: device, [t, words] for each sequence, bits_stride elements
+ * apart (0: one for all).  accumulate must be 0 and pos_start NULL. */
+int rsfa_cache4_attend_tree(const rsfa_cache4_attend_args *args, const int32_t *bits,
+                            int64_t bits_stride, void *stream);
+
+/* keep: row j < counts[z] (NULL: n) of drafted token tokens[z, j] goes from slot
+ * lengths[z] + tokens[z, j] to slot lengths[z] + j (lengths: the contexts), with its weight, and
+ * takes the position pos_start[z] + j (NULL: lengths[z] + j).  All rows are read before one is
+ * written.  Tokens below 0 or past the cache leave slot lengths[z] + j as it is. */
+typedef struct rsfa_cache4_keep_args {
+    uint32_t       struct_size; /* = sizeof(rsfa_cache4_keep_args)             */
+    uint32_t       reserved;    /* 0 */
+    rsfa_cache4    cache;
+    const int32_t *tokens;      /* device, [z, n], dense                       */
+    int64_t        n;           /* 1 .. RSFA_DRAFT_TOKENS                       */
+    const int32_t *lengths;
+    int64_t        length;
+    const int32_t *counts, *pos_start;
+} rsfa_cache4_keep_args;
+
+int rsfa_cache4_keep(const rsfa_cache4_keep_args *args, void *stream);
 
 /* Static string for a status code. */
 const char *rsfa_strerror(int status);

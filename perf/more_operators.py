@@ -323,7 +323,7 @@ def _run_tree(s):
     case, b, q = s["case"], s["buffers"], s["q"]
     if own:
         tree = s["tree"] if not case["dynamic"] else _framework()[2].draft_tree(s["parents"])
-        r = s["cache"].attend_tree(q, s["lengths"], tree, s["scale"], counts=s["counts"], return_lse=case["lse"])
+        r = s["cache"].attend(q, s["lengths"], True, s["scale"], counts=s["counts"], return_lse=case["lse"], tree=tree)
         return list(r) if case["lse"] else [r]
     Z, Hq, T, D = q.shape
     H, N = case["H"], case["N"]
