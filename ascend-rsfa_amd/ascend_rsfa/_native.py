@@ -28,6 +28,7 @@ E_ROTARY = -12
 E_CACHE = -13
 E_BUDGET = -14
 E_DRAFT = -15
+E_CROSS = -16
 
 # rsfa_dtype
 DTYPE_F16 = 0
@@ -200,6 +201,73 @@ class Cache4EvictArgs(ctypes.Structure):
     ]
 
 
+class CrossArgs(ctypes.Structure):
+    """Mirror of struct rsfa_cross_args."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("z", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("key_heads", ctypes.c_int64),
+        ("t", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 4),
+        ("k_stride", ctypes.c_int64 * 4),
+        ("v_stride", ctypes.c_int64 * 4),
+        ("o_stride", ctypes.c_int64 * 4),
+        ("lengths", ctypes.c_void_p),
+        ("sm_scale", ctypes.c_float),
+        ("reserved", ctypes.c_uint32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+class CrossBwdArgs(ctypes.Structure):
+    """Mirror of struct rsfa_cross_bwd_args."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("grad_o", ctypes.c_void_p),
+        ("grad_lse", ctypes.c_void_p),
+        ("grad_q", ctypes.c_void_p),
+        ("grad_k", ctypes.c_void_p),
+        ("grad_v", ctypes.c_void_p),
+        ("z", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("key_heads", ctypes.c_int64),
+        ("t", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 4),
+        ("k_stride", ctypes.c_int64 * 4),
+        ("v_stride", ctypes.c_int64 * 4),
+        ("o_stride", ctypes.c_int64 * 4),
+        ("grad_o_stride", ctypes.c_int64 * 4),
+        ("grad_q_stride", ctypes.c_int64 * 4),
+        ("grad_k_stride", ctypes.c_int64 * 4),
+        ("grad_v_stride", ctypes.c_int64 * 4),
+        ("lengths", ctypes.c_void_p),
+        ("sm_scale", ctypes.c_float),
+        ("reserved", ctypes.c_uint32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
 class DraftTreeArgs(ctypes.Structure):
     """Mirror of struct rsfa_draft_tree_args."""
 
@@ -247,6 +315,10 @@ SIGNATURES = {
     "rsfa_cache4_claim": (ctypes.c_int, [ctypes.POINTER(Cache4EvictArgs), ctypes.c_void_p]),
     "rsfa_cache4_evict": (ctypes.c_int, [ctypes.POINTER(Cache4EvictArgs), ctypes.c_void_p]),
     "rsfa_cache4_evict_workspace_bytes": (ctypes.c_uint64, [ctypes.POINTER(Cache4EvictArgs), _I32]),
+    "rsfa_cross_fwd": (ctypes.c_int, [ctypes.POINTER(CrossArgs), ctypes.c_void_p]),
+    "rsfa_cross_fwd_workspace_bytes": (ctypes.c_uint64, [ctypes.POINTER(CrossArgs)]),
+    "rsfa_cross_bwd": (ctypes.c_int, [ctypes.POINTER(CrossBwdArgs), ctypes.c_void_p]),
+    "rsfa_cross_bwd_workspace_bytes": (ctypes.c_uint64, [ctypes.POINTER(CrossBwdArgs)]),
     "rsfa_draft_tree": (ctypes.c_int, [ctypes.POINTER(DraftTreeArgs), ctypes.c_void_p]),
     "rsfa_cache4_attend_tree": (ctypes.c_int, [ctypes.POINTER(Cache4AttendArgs), ctypes.c_void_p, _I64, ctypes.c_void_p]),
     "rsfa_cache4_keep": (ctypes.c_int, [ctypes.POINTER(Cache4KeepArgs), ctypes.c_void_p]),

@@ -1,0 +1,186 @@
+"""Cross attention on MI355X (gfx950): queries over keys of another length, an encoder's states say.
+
+``cross_attention(q, k, v, sm_scale, lengths)`` is ``softmax(q k^T sm_scale) v`` without a mask
+but for the lengths of a padded batch.  A training step differentiates it; a decoding step calls it with one
+token or a few.
+
+All arithmetic runs in ``lib/librsfa.so`` (``rsfa_cross_*`` in ``include/rsfa.h``), enqueued on the
+current stream of the tensors' device; there is no other path.
+"""
+import ctypes
+import math
+import struct
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+from .flash_attention_forward import _as_kernel_layout, _meets_contract, _raise_for
+from .rotary import _has_tangent
+
+__all__ = ["cross_attention"]
+
+_DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16}
+_HEAD_DIMS = (32, 64, 128, 256)
+
+# The argument struct is joined from a part that the tensors' shapes settle, kept by them, and packed addresses.
+_SIZES, _LENGTHS, _PTRS = (getattr(_native.CrossArgs, f).offset for f in ("z", "lengths", "q"))
+_FWD_PTRS = struct.Struct("=5Q")  # q, k, v, o, lse
+_FWD_TAIL = struct.Struct("=QfIQQ")  # lengths, sm_scale, reserved, workspace, its bytes
+assert _SIZES - _PTRS == _FWD_PTRS.size and ctypes.sizeof(_native.CrossArgs) - _LENGTHS == _FWD_TAIL.size
+_PLANS = {}
+_FUNCTIONS = {}
+
+
+def _function(name):
+    """An entry point that takes its argument struct's bytes."""
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)((name, _native.lib()))
+    return fn
+
+
+def _on_device(device, fn, *args):
+    if device.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
+def _call(device, name, args):
+    _raise_for(_on_device(device, _function(name), args, torch._C._cuda_getCurrentRawStream(device.index)))
+
+
+def _empty_rows(t):
+    """An output like t, whose rows the kernels can write."""
+    o = torch.empty_like(t)
+    return o if _meets_contract(o) else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _forward(q, k, v, scale, lengths, want_lse):
+    """(o, lse or None) of checked tensors in the kernels' layout."""
+    o = _empty_rows(q)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
+    if o.numel() == 0:
+        return o, lse
+    if k.shape[2] == 0:
+        return o.zero_(), lse.fill_(-math.inf) if want_lse else None
+    key = (q.shape, k.shape, q.stride(), k.stride(), v.stride(), q.dtype, q.device)
+    plan = _PLANS.get(key)
+    if plan is None:
+        args = _native.CrossArgs()
+        args.struct_size, args.dtype = ctypes.sizeof(args), _DTYPES[q.dtype]
+        args.z, args.heads, args.t, args.head_dim = q.shape
+        args.key_heads, args.n = k.shape[1], k.shape[2]
+        for name, t in (("q_stride", q), ("k_stride", k), ("v_stride", v), ("o_stride", o)):
+            getattr(args, name)[:] = t.stride()
+        nbytes = _on_device(q.device, _native.lib().rsfa_cross_fwd_workspace_bytes, ctypes.byref(args))
+        b = bytes(args)
+        if len(_PLANS) > 4096:
+            _PLANS.clear()
+        plan = _PLANS[key] = (b[:_PTRS], b[_SIZES:_LENGTHS], nbytes)
+    head, sizes, nbytes = plan
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _call(q.device, "rsfa_cross_fwd", b"".join((
+        head, _FWD_PTRS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if want_lse else 0), sizes,
+        _FWD_TAIL.pack(0 if lengths is None else lengths.data_ptr(), scale, 0, ws.data_ptr() if nbytes else 0, nbytes))))
+    return o, lse
+
+
+def _backward(q, k, v, o, lse, go, glse, scale, lengths, needs):
+    """The gradients of q, k and v, those that ``needs`` names (None for the others)."""
+    grads = [_empty_rows(t) if need else None for t, need in zip((q, k, v), needs)]
+    if q.numel() == 0 or k.shape[2] == 0:
+        return [g if g is None else g.zero_() for g in grads]
+    go = torch.zeros_like(o) if go is None else _as_kernel_layout(go)
+    if glse is not None:
+        glse = glse.contiguous()
+    args = _native.CrossBwdArgs()
+    args.struct_size, args.dtype = ctypes.sizeof(args), _DTYPES[q.dtype]
+    args.z, args.heads, args.t, args.head_dim = q.shape
+    args.key_heads, args.n = k.shape[1], k.shape[2]
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("grad_o", go), ("grad_q", grads[0]), ("grad_k", grads[1]), ("grad_v", grads[2])):
+        if t is not None:
+            setattr(args, name, t.data_ptr())
+            getattr(args, name + "_stride")[:] = t.stride()
+    args.lse = lse.data_ptr()
+    args.grad_lse = None if glse is None else glse.data_ptr()
+    args.lengths = None if lengths is None else lengths.data_ptr()
+    args.sm_scale = scale
+    nbytes = _on_device(q.device, _native.lib().rsfa_cross_bwd_workspace_bytes, ctypes.byref(args))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
+    _raise_for(_on_device(q.device, _native.lib().rsfa_cross_bwd, ctypes.byref(args),
+                          torch._C._cuda_getCurrentRawStream(q.device.index)))
+    return grads
+
+
+def _check(q, k, v, sm_scale, lengths):
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q must be [Z, heads, T, D], k and v [Z, key heads, N, D]; got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    if q.shape[3] not in _HEAD_DIMS:
+        raise ValueError(f"the head dim must be one of {_HEAD_DIMS}; got {q.shape[3]}")
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"query heads ({q.shape[1]}) must be a multiple of the key heads ({k.shape[1]})")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError("q, k and v must have the same dtype")
+    if q.dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {q.dtype}; float16 and bfloat16 are supported")
+    if not q.is_cuda or not (q.device == k.device == v.device):
+        raise ValueError("q, k and v must be GPU tensors on one device")
+    if math.isnan(sm_scale):
+        raise ValueError("sm_scale is NaN")
+    if lengths is not None:
+        if not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or lengths.shape != q.shape[:1]:
+            raise TypeError(f"lengths must be an int32 tensor [{q.shape[0]}]")
+        if lengths.device != q.device:
+            raise ValueError("lengths must be on the device of q")
+
+
+class _CrossAttention(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, v, sm_scale, lengths):
+        o, lse = _forward(q, k, v, sm_scale, lengths, True)
+        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        ctx.sm_scale = sm_scale
+        ctx.set_materialize_grads(False)
+        return o, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go, glse):
+        q, k, v, o, lse, lengths = ctx.saved_tensors
+        if go is None and glse is None:
+            return None, None, None, None, None
+        return (*_backward(q, k, v, o, lse, go, glse, ctx.sm_scale, lengths, ctx.needs_input_grad[:3]), None, None)
+
+
+def cross_attention(q, k, v, sm_scale, lengths=None, *, return_lse=False):
+    """softmax(q k^T sm_scale) v: ``o``, or ``(o, lse)``.
+
+    q [Z, heads, T, D]; k, v [Z, key heads, N, D] of the same dtype, float16 or bfloat16; D is 32, 64, 128
+    or 256, heads a multiple of the key heads: query head i reads key head ``i // (heads // key heads)``.
+    Any strides (rows that are not 16-byte aligned with a unit last stride are copied first; strides of 0, as
+    ``expand`` gives them, are fine).  ``lengths`` (int32 [Z] on the GPU; None: N of all): the keys of each
+    sequence, its first ones; values outside [0, N] are taken as its ends, and what lies behind them is not read.  A
+    sequence without keys gives 0 (lse -inf).
+
+    Sums are in 32 bits; softmax weights are rounded to the dtype for the product with v, as o is.
+    ``lse``: the natural logarithm of each row's sum of exponentials, float32 [Z, heads, T].
+
+    Differentiable once in q, k and v, through o and lse; gradients do not change from call to call (no atomics).
+    For the gradients' products softmax weights and their gradients are rounded to the dtype.  Keys past a length
+    have gradients of 0.
+    """
+    sm_scale = float(sm_scale)
+    _check(q, k, v, sm_scale, lengths)
+    if lengths is not None:
+        lengths = lengths.contiguous()
+    q, k, v = (t if t.numel() == 0 else _as_kernel_layout(t) for t in (q, k, v))
+    if _has_tangent(q, k, v) or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        o, lse = _CrossAttention.apply(q, k, v, sm_scale, lengths)
+    else:
+        o, lse = _forward(q, k, v, sm_scale, lengths, return_lse)
+    return (o, lse) if return_lse else o

@@ -1,0 +1,494 @@
+// Cross attention, forward (rsfa_cross_fwd, declared in include/rsfa.h).
+//
+//   o = softmax(sm_scale q k^T) v,  q [Z, heads, T, D],  k, v [Z, key heads, N, D]
+//
+// Many query tokens run the forward kernel (fa_fwd_kernel.hpp, MODE_CROSS), a task being a block
+// of one query head's tokens; with too few tasks for the chip each takes a part of the keys.  Few
+// tokens run cross_few_kernel below, which packs the rows (tokens and query heads) that share a key
+// head and always has the keys in parts.  Parts are added up by join_kernel.
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#include "../../include/rsfa.h"
+#include "cross.hpp"
+#include "kernel_table.hpp"
+
+using namespace rsfa;
+
+namespace {
+
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
+// A running maximum of scores starts below every finite score, and finite: a hidden score's exp2(-inf - m) is 0.
+constexpr float NEVER = -3.0e38f;
+constexpr float SLACK = 8.0f;  // how far (log2 units) a score may pass the running maximum: weights stay below 2^8
+
+struct FewParams {
+    const void *q, *k, *v;
+    void* o;
+    float* lse;
+    int64_t q_st[3], k_st[3], v_st[3], o_st[3];  // element strides of (Z, heads, rows)
+    const int32_t* lengths;
+    int32_t heads, key_heads, group, t, n, bh;   // bh = Z * key heads
+    int32_t rows;                                // group * t: row = token * group + head of the group
+    int32_t splits;
+    float c;                                     // |sm_scale| * log2 e
+    uint32_t neg;                                // sign of sm_scale, as a mask for a pair of q's values
+    float* part_o;                               // [splits][Z * heads * t][D] (splits > 1)
+    float2* part_ml;                             // [splits][Z * heads * t]: maximum (log2 units), sum
+};
+
+// Few rows (NB blocks of 16): each wave of a workgroup takes every WAVES-th tile of 32 keys of its part,
+// and they add up what they have at the end.  A wave's tiles go from memory straight into LDS of its own,
+// two buffers, so that a tile is under way while one is computed with and no barrier is needed.  In LDS a tile
+// has the layout of the forward kernel (fa_fwd_kernel.hpp), whose rows and transposes are read without bank conflicts:
+//   S^T = K Q^T   (v_mfma 16x16x32) A: lane l has the key l % 16 and values 8 (l / 16) .. of a step of 32
+//   O^T = V^T P^T  S^T leaves lane l the row l % 16 and keys 16 t + 4 (l / 16) + r; step k = 8 (l / 16) + 4 t + r takes
+//                 them as they are, and A, two transposing reads a lane, has the same keys.
+// Bound by memory: 4 D bytes a key, whatever the rows.
+template <class T, int D, int NB>
+__global__ void __launch_bounds__(64 * Few<D>::WAVES, Few<D>::OCC) cross_few_kernel(FewParams p) {
+    typedef typename T::elem elem;
+    typedef typename T::x8 x8;
+    constexpr int WAVES = Few<D>::WAVES, KEYS = 32, STEP = KEYS * WAVES;
+    constexpr int QS = D / 32, DT = D / 16;
+    constexpr int BLK = 32 * D;          // bytes of 16 rows
+    constexpr int TILE = KEYS * D * 2;   // bytes of a K or V tile
+    constexpr int LOADS = TILE / 1024;   // direct loads of one
+    constexpr int ROWS = 16 * NB, PITCH = D + 4;
+    constexpr int BUFFERS = WAVES * 2 * 2 * TILE, SUMS = WAVES * ROWS * (PITCH * 4 + 8);
+    __shared__ __attribute__((aligned(1024))) char smem_raw[BUFFERS > SUMS ? BUFFERS : SUMS];
+    RSFA_LDS char* const smem = (RSFA_LDS char*)smem_raw;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const int bh = blockIdx.x % p.bh;  // with a multiple of 8, a head's row tiles meet in one XCD's L2
+    const int row0 = blockIdx.x / p.bh * ROWS;
+    const int z = bh / p.key_heads, h = bh - z * p.key_heads;
+    const int len = __builtin_amdgcn_readfirstlane(p.lengths ? max(0, min(p.lengths[z], p.n)) : p.n);
+    const int chunk = ((len + p.splits - 1) / p.splits + STEP - 1) / STEP * STEP;
+    const int64_t start64 = (int64_t)chunk * blockIdx.y;
+    const int start = (int)(start64 < len ? start64 : len);
+    const int end = min(start + chunk, len);
+
+    const elem* const kb = (const elem*)p.k + z * p.k_st[0] + h * p.k_st[1];
+    const elem* const vb = (const elem*)p.v + z * p.v_st[0] + h * p.v_st[1];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem + wave * (4 * TILE);  // buffer b: K at 2 b TILE, V behind
+    // lane i of a load fills chunk i % 4 of row i / 4 of a plane of 16 rows x 32 values
+    const int ld_row = lane >> 2, ld_col = ((lane & 3) ^ row_swz(ld_row)) * 8;
+    auto load = [&](int tile, int buf) {
+        const uint32_t dst = lds0 + buf * (2 * TILE);
+        const int last = len - 1 - tile;  // rows behind the last key repeat it
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int row = min(16 * b + ld_row, last);
+            const uint32_t ko = (uint32_t)((row * p.k_st[2] + ld_col) * 2), vo = (uint32_t)((row * p.v_st[2] + ld_col) * 2);
+            const elem *kt = kb + tile * p.k_st[2], *vt = vb + tile * p.v_st[2];
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) dma16(kt + 32 * i, ko, dst + b * BLK + i * 1024);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) dma16(vt + 32 * i, vo, dst + TILE + b * BLK + i * 1024);
+        }
+    };
+    const int tiles = (end - start + KEYS - 1) / KEYS;
+    const int turns = tiles > wave ? (tiles - wave + WAVES - 1) / WAVES : 0;
+
+    // Q^T (ahead of the tiles: the wait for it would wait for them)
+    x8 q[NB][QS];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int row = row0 + 16 * b + col;
+        const int tok = row / p.group, head = row - tok * p.group;
+        u32x4 w[QS] = {};
+        if (row < p.rows) {
+            const elem* src = (const elem*)p.q + z * p.q_st[0] + (int64_t)(h * p.group + head) * p.q_st[1] + tok * p.q_st[2] + 8 * grp;
+#pragma unroll
+            for (int i = 0; i < QS; ++i) w[i] = *(const u32x4*)(src + 32 * i);
+        }
+#pragma unroll
+        for (int i = 0; i < QS; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[i][j] ^= p.neg;
+            q[b][i] = __builtin_bit_cast(x8, w[i]);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < QS; ++i) asm volatile("" : "+v"(q[b][i]));
+    if (turns) load(start + KEYS * wave, 0);
+
+    f32x4 acc[NB][DT];
+    float m[NB], l[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        m[b] = NEVER;
+        l[b] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[b][d] = (f32x4){0, 0, 0, 0};
+    }
+    const uint32_t koff = col * 64 + (grp ^ row_swz(col)) * 16;
+    const int vrow = 4 * grp + (col >> 2);
+    uint32_t voff[2];  // even and odd blocks of 16 values
+#pragma unroll
+    for (int e = 0; e < 2; ++e) voff[e] = vrow * 64 + ((2 * e + ((col >> 1) & 1)) ^ row_swz(vrow)) * 16 + 8 * (col & 1);
+
+    auto compute = [&](int buf, int tile) {
+        const RSFA_LDS char* const kt = smem + wave * (4 * TILE) + buf * (2 * TILE);
+        const RSFA_LDS char* const vt = kt + TILE;
+        f32x4 s[NB][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) s[b][t] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < QS; ++i) {
+                const x8 a = *(const RSFA_LDS x8*)(kt + t * BLK + i * 1024 + koff);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) s[b][t] = mfma16(a, q[b][i], s[b][t]);
+            }
+        }
+        x8 pk[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = s[b][j / 4][j % 4] * p.c;
+            if (__builtin_expect(tile + KEYS > end, 0)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (tile + 16 * (j / 4) + 4 * grp + j % 4 >= end) x[j] = -INFINITY;
+            }
+            float top = x[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+            if (__any(top > m[b] + SLACK)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float now = fmaxf(m[b], top);
+                const float f = __builtin_amdgcn_exp2f(m[b] - now);
+                m[b] = now;
+                l[b] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[b][d] *= f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_exp2f(x[j] - m[b]);
+            l[b] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pk[b][j] = (elem)x[j];
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const RSFA_LDS char* const at = vt + (d / 2) * 1024 + voff[d & 1];
+            const i32x2 lo = __builtin_bit_cast(i32x2, T::tr_read(at));
+            const i32x2 hi = __builtin_bit_cast(i32x2, T::tr_read(at + BLK));
+            const x8 a = __builtin_bit_cast(x8, (i32x4){lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+            for (int b = 0; b < NB; ++b) acc[b][d] = mfma16(a, pk[b], acc[b][d]);
+        }
+    };
+
+    for (int i = 0; i < turns; ++i) {
+        const int tile = start + KEYS * (wave + WAVES * i);
+        // the other buffer's reads have all been used, as its products have been issued
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (i + 1 < turns) {
+            load(tile + STEP, (i + 1) & 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        compute(i & 1, tile);
+    }
+
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        l[b] += __shfl_xor(l[b], 16);
+        l[b] += __shfl_xor(l[b], 32);
+    }
+    // the waves add up what they have, through LDS: each leaves its sums, scaled to the rows' common
+    // maximum, and every thread adds E values of a row
+    constexpr int THREADS = 64 * WAVES, E = ROWS * D / THREADS;
+    __syncthreads();  // (the tiles' LDS is used again)
+    RSFA_LDS float2* const ml = (RSFA_LDS float2*)(smem + WAVES * ROWS * PITCH * 4);
+    RSFA_LDS float* const part = (RSFA_LDS float*)smem;
+    auto put = [&](RSFA_LDS float2* at, float2 v) { ((RSFA_LDS float*)at)[0] = v.x, ((RSFA_LDS float*)at)[1] = v.y; };
+    auto get = [&](const RSFA_LDS float2* at) { return make_float2(((const RSFA_LDS float*)at)[0], ((const RSFA_LDS float*)at)[1]); };
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+        if (grp == 0) put(ml + wave * ROWS + 16 * b + col, make_float2(m[b], l[b]));
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        float mm = NEVER;
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) mm = fmaxf(mm, get(ml + k * ROWS + 16 * b + col).x);
+        const float f = __builtin_amdgcn_exp2f(m[b] - mm);
+        RSFA_LDS float* const at = part + (wave * ROWS + 16 * b + col) * PITCH + 4 * grp;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *(RSFA_LDS f32x4*)(at + 16 * d) = acc[b][d] * f;
+    }
+    __syncthreads();
+    const int r = threadIdx.x / (D / E), d0 = threadIdx.x % (D / E) * E;
+    const int row = row0 + r;
+    if (row >= p.rows) return;
+    float mm = NEVER, ll = 0.0f;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) mm = fmaxf(mm, get(ml + k * ROWS + r).x);
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) {
+        const float2 v = get(ml + k * ROWS + r);
+        ll += v.y * __builtin_amdgcn_exp2f(v.x - mm);
+    }
+    float sum[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        sum[e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) sum[e] += part[(k * ROWS + r) * PITCH + d0 + e];
+    }
+    const int tok = row / p.group, head = row - tok * p.group;
+    const int64_t hq = h * p.group + head;
+    const int64_t out = (z * (int64_t)p.heads + hq) * p.t + tok;
+    if (p.splits > 1) {
+        const int64_t at = blockIdx.y * ((int64_t)p.bh * p.rows) + out;
+        if (d0 == 0) p.part_ml[at] = make_float2(mm, ll);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) *(float2*)(p.part_o + at * D + d0 + e) = make_float2(sum[e], sum[e + 1]);
+        return;
+    }
+    const float inv = len == 0 ? 0.0f : 1.0f / ll;
+    elem* const dst = (elem*)p.o + z * p.o_st[0] + hq * p.o_st[1] + tok * p.o_st[2] + d0;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+        typename T::x2 v = {(elem)(sum[e] * inv), (elem)(sum[e + 1] * inv)};
+        *(typename T::x2*)(dst + e) = v;
+    }
+    if (d0 == 0 && p.lse) p.lse[out] = len == 0 ? -INFINITY : (mm + __builtin_amdgcn_logf(ll)) * LN2;
+}
+
+// Sums of the rows' parts: D / 4 lanes hold a row, four values each, and `pp` such groups of a
+// workgroup take every pp-th part of it, so that the loads of a row's parts do not wait for each other.
+struct JoinParams {
+    const float* part_o;
+    const float2* part_ml;
+    void* o;
+    float* lse;
+    int64_t o_st[3];
+    const int32_t* lengths;
+    int32_t heads, t, n, splits, pp;
+    int64_t rows;  // Z * heads * t
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(256) cross_join_kernel(JoinParams p) {
+    constexpr int G = D / 4, GROUPS = 256 / G;
+    __shared__ f32x4 part[256];
+    __shared__ float2 ml[GROUPS];
+    const int lane = threadIdx.x % G, grp = threadIdx.x / G;
+    const int64_t id = (int64_t)blockIdx.x * (GROUPS / p.pp) + grp / p.pp;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o = {0, 0, 0, 0};
+    auto add = [&](float2 v, f32x4 x) {
+        const float now = fmaxf(m, v.x);
+        const float f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now), g = v.x == now ? 1.0f : __builtin_amdgcn_exp2f(v.x - now);
+        m = now;
+        l = l * f + v.y * g;
+        o = o * f + x * g;
+    };
+    if (id < p.rows) {
+        constexpr int U = 8;  // parts whose loads are under way together
+        for (int s0 = grp % p.pp; s0 < p.splits; s0 += U * p.pp) {
+            float2 v[U];
+            f32x4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int s = min(s0 + u * p.pp, p.splits - 1);
+                v[u] = p.part_ml[s * p.rows + id];
+                x[u] = *(const f32x4*)(p.part_o + (s * p.rows + id) * D + 4 * lane);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s0 + u * p.pp < p.splits) add(v[u], x[u]);
+        }
+    }
+    if (p.pp > 1) {
+        part[threadIdx.x] = o;
+        if (lane == 0) ml[grp] = make_float2(m, l);
+        __syncthreads();
+        if (grp % p.pp != 0) return;
+        for (int i = 1; i < p.pp; ++i) add(ml[grp + i], part[threadIdx.x + i * G]);
+    }
+    if (id >= p.rows) return;
+    const int64_t zh = id / p.t;
+    const int tok = (int)(id - zh * p.t), z = (int)(zh / p.heads), hq = (int)(zh - (int64_t)z * p.heads);
+    const bool none = p.lengths ? p.lengths[z] <= 0 : false;
+    const float inv = none ? 0.0f : 1.0f / l;
+    typedef typename T::elem elem;
+    elem* const dst = (elem*)p.o + z * p.o_st[0] + hq * p.o_st[1] + tok * p.o_st[2] + 4 * lane;
+    typename T::x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (elem)(o[i] * inv);
+    *(typename T::x4*)dst = w;
+    if (lane == 0 && p.lse) p.lse[id] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+struct Plan {
+    bool few;
+    int nb;                // few: blocks of 16 rows a workgroup
+    int64_t tiles;         // few: row tiles of a key head
+    const KernelEntry* e;  // many
+    int splits;
+    uint64_t part_o, part_ml, bytes;
+};
+
+template <class T, int NB>
+const void* few_fn(int64_t d) {
+    switch (d) {
+        case 32: return (const void*)&cross_few_kernel<T, 32, NB>;
+        case 64: return (const void*)&cross_few_kernel<T, 64, NB>;
+        case 128: return (const void*)&cross_few_kernel<T, 128, NB>;
+        default: return (const void*)&cross_few_kernel<T, 256, NB>;
+    }
+}
+
+template <class T>
+const void* join_fn(int64_t d) {
+    switch (d) {
+        case 32: return (const void*)&cross_join_kernel<T, 32>;
+        case 64: return (const void*)&cross_join_kernel<T, 64>;
+        case 128: return (const void*)&cross_join_kernel<T, 128>;
+        default: return (const void*)&cross_join_kernel<T, 256>;
+    }
+}
+
+int few_waves(int64_t d) { return d == 256 ? Few<256>::WAVES : Few<128>::WAVES; }
+
+const KernelEntry* find(const rsfa_cross_args* a, int nw, int bn) {
+    const KernelList l = a->dtype == RSFA_DTYPE_BF16 ? kernels_cross_bf16() : kernels_cross_f16();
+    for (int i = 0; i < l.count; ++i)
+        if (l.entries[i].d == a->head_dim && l.entries[i].nw == nw && (!bn || l.entries[i].bn == bn)) return &l.entries[i];
+    return nullptr;
+}
+
+Plan make_plan(const rsfa_cross_args* a) {
+    Plan p{};
+    const int cus = cross_cus();
+    const int64_t group = a->heads / a->key_heads, rows = group * a->t, bh = a->z * a->key_heads;
+    p.few = rows <= 32 || a->t <= 16;
+    int64_t able = 1, want = 1;
+    if (p.few) {
+        p.nb = rows <= 16 ? 1 : 2;
+        p.tiles = (rows + 16 * p.nb - 1) / (16 * p.nb);
+        const int64_t step = 32 * few_waves(a->head_dim);
+        const int64_t full = 4 * (int64_t)cus;
+        want = (full + bh * p.tiles - 1) / (bh * p.tiles);
+        able = (a->n + 2 * step - 1) / (2 * step);
+    } else {
+        const int64_t heads = a->z * a->heads;
+        const bool large = a->head_dim > 32 && a->t > 128 && heads * ((a->t + 255) / 256) >= cus;
+        p.e = a->head_dim == 32 ? find(a, 4, a->n >= 1024 ? 128 : 64) : find(a, large ? 8 : 4, 0);
+        const int64_t tasks = heads * ((a->t + p.e->bm - 1) / p.e->bm);
+        const int64_t full = p.e->nw == 8 ? cus : 2 * cus;
+        want = full / tasks;
+        able = a->n / 512;
+    }
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, able), 256));
+    if (p.splits > 1) {
+        const uint64_t all = (uint64_t)a->z * a->heads * a->t;
+        p.part_ml = 0;
+        p.part_o = (p.splits * all * 8 + 255) / 256 * 256;
+        p.bytes = p.part_o + p.splits * all * a->head_dim * 4;
+    }
+    return p;
+}
+
+int check(const rsfa_cross_args* a) {
+    if (!a) return RSFA_E_NULL;
+    if (a->struct_size != sizeof(rsfa_cross_args)) return RSFA_E_ABI;
+    return cross_check(a->dtype, a->z, a->heads, a->key_heads, a->t, a->n, a->head_dim);
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t rsfa_cross_fwd_workspace_bytes(const rsfa_cross_args* a) { return check(a) == RSFA_OK ? make_plan(a).bytes : 0; }
+
+int rsfa_cross_fwd(const rsfa_cross_args* a, void* stream) {
+    int st = check(a);
+    if (st != RSFA_OK) return st;
+    if (!a->q || !a->k || !a->v || !a->o) return RSFA_E_NULL;
+    for (auto [ptr, strides] : {std::pair(a->q, a->q_stride), std::pair(a->k, a->k_stride), std::pair(a->v, a->v_stride),
+                                std::pair((const void*)a->o, a->o_stride)})
+        if ((st = cross_check_rows(ptr, strides)) != RSFA_OK) return st;
+    if (((uintptr_t)a->lse | (uintptr_t)a->lengths) & 3) return RSFA_E_ALIGN;
+    const Plan plan = make_plan(a);
+    if (plan.bytes) {
+        if (!a->workspace || a->workspace_bytes < plan.bytes) return RSFA_E_WORKSPACE;
+        if ((uintptr_t)a->workspace & 15) return RSFA_E_ALIGN;
+    }
+    const bool bf16 = a->dtype == RSFA_DTYPE_BF16;
+    // (a scale of 0 would make a hidden score -inf * 0; at FLT_MIN the others still have weights of 1)
+    const float c = std::max(std::fabs(a->sm_scale) * LOG2E, FLT_MIN);
+    float2* const part_ml = plan.bytes ? (float2*)((char*)a->workspace + plan.part_ml) : nullptr;
+    float* const part_o = plan.bytes ? (float*)((char*)a->workspace + plan.part_o) : nullptr;
+    if (plan.few) {
+        FewParams p{};
+        p.q = a->q, p.k = a->k, p.v = a->v, p.o = a->o, p.lse = a->lse;
+        for (int i = 0; i < 3; ++i) p.q_st[i] = a->q_stride[i], p.k_st[i] = a->k_stride[i], p.v_st[i] = a->v_stride[i], p.o_st[i] = a->o_stride[i];
+        p.lengths = a->lengths;
+        p.heads = (int32_t)a->heads, p.key_heads = (int32_t)a->key_heads, p.group = (int32_t)(a->heads / a->key_heads);
+        p.t = (int32_t)a->t, p.n = (int32_t)a->n, p.bh = (int32_t)(a->z * a->key_heads), p.rows = p.group * p.t;
+        p.splits = plan.splits, p.c = c, p.neg = a->sm_scale < 0.0f ? 0x80008000u : 0u;
+        p.part_o = part_o, p.part_ml = part_ml;
+        const int64_t grid = p.bh * plan.tiles;
+        if (grid > 0x7fffffff) return RSFA_E_CROSS;
+        void* args[] = {&p};
+        const void* fn = bf16 ? (plan.nb == 1 ? few_fn<TypeBF16, 1>(a->head_dim) : few_fn<TypeBF16, 2>(a->head_dim))
+                              : (plan.nb == 1 ? few_fn<TypeF16, 1>(a->head_dim) : few_fn<TypeF16, 2>(a->head_dim));
+        if (hipLaunchKernel(fn, dim3((unsigned)grid, (unsigned)plan.splits), dim3(64 * few_waves(a->head_dim)), args, 0, (hipStream_t)stream) != hipSuccess)
+            return RSFA_E_LAUNCH;
+    } else {
+        FwdParams p{};
+        p.q = a->q, p.k = a->k, p.v = a->v, p.o = a->o, p.lse = a->lse;
+        p.q_sz = a->q_stride[0], p.q_sh = a->q_stride[1], p.q_sm = a->q_stride[2];
+        p.k_sz = a->k_stride[0], p.k_sh = a->k_stride[1], p.k_sn = a->k_stride[2];
+        p.v_sz = a->v_stride[0], p.v_sh = a->v_stride[1], p.v_sn = a->v_stride[2];
+        p.o_sz = a->o_stride[0], p.o_sh = a->o_stride[1], p.o_sm = a->o_stride[2];
+        p.H = (int32_t)a->key_heads;
+        p.num_heads = (int32_t)(a->z * a->key_heads);
+        p.group = (int32_t)(a->heads / a->key_heads);
+        p.n_ctx = (int32_t)a->t, p.n_keys = (int32_t)a->n, p.k_lengths = a->lengths;
+        p.splits = plan.splits;
+        p.q_blocks = (int32_t)((a->t + plan.e->bm - 1) / plan.e->bm);
+        const int64_t nmb = (int64_t)p.q_blocks * p.group * p.splits;
+        if (nmb * p.num_heads > (int64_t(1) << 30)) return RSFA_E_CROSS;
+        p.nmb = (int32_t)nmb;
+        p.num_tasks = p.num_heads * p.nmb;
+        p.c = c, p.neg = a->sm_scale < 0.0f ? 1u : 0u;
+        p.part_o = part_o, p.part_ml = part_ml;
+        if (plan.splits > 1) p.lse = nullptr;
+        if ((st = launch_cross(*plan.e, p, stream)) != RSFA_OK) return st;
+    }
+    if (plan.splits == 1) return RSFA_OK;
+    JoinParams j{};
+    j.part_o = part_o, j.part_ml = part_ml, j.o = a->o, j.lse = a->lse, j.lengths = a->lengths;
+    for (int i = 0; i < 3; ++i) j.o_st[i] = a->o_stride[i];
+    j.heads = (int32_t)a->heads, j.t = (int32_t)a->t, j.n = (int32_t)a->n, j.splits = plan.splits;
+    j.rows = a->z * a->heads * a->t;
+    const int groups = 256 / (int)(a->head_dim / 4);
+    j.pp = 1;
+    while (j.pp < groups && j.pp * 8 < plan.splits) j.pp *= 2;
+    const int64_t per = groups / j.pp, blocks = (j.rows + per - 1) / per;
+    if (blocks > 0x7fffffff) return RSFA_E_CROSS;
+    void* args[] = {&j};
+    return hipLaunchKernel(bf16 ? join_fn<TypeBF16>(a->head_dim) : join_fn<TypeF16>(a->head_dim), dim3((unsigned)blocks), dim3(256), args, 0,
+                           (hipStream_t)stream) == hipSuccess ? RSFA_OK : RSFA_E_LAUNCH;
+}
+
+}  // extern "C"

@@ -1,0 +1,580 @@
+// Gradients of cross attention (rsfa_cross_bwd, declared in include/rsfa.h).
+//
+//   P = exp(s q k^T - lse),  dV = P^T dO,  dS = P (dO V^T - delta),  dQ = s dS K,  dK = s dS^T Q
+//   delta = rowsum(dO o) - dlse
+//
+// Three kernels: the rows' statistics; dK and dV, whose workgroups hold a block of keys and pass over the rows of
+// their key head (all query heads of its group, so shared heads need no second sum); dQ, whose workgroups hold a block
+// of rows and pass over the keys.  Both pass kernels form S and dO V^T, which makes seven matrix products where
+// one kernel would have five, but every sum has one owner and one order: no atomics, the same bits in each call,
+// and no traffic for dQ's partial sums, which one kernel would add up in memory once per key block.
+// Where blocks are too few for the chip each pass is cut into parts, which sum_parts_kernel adds up.
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/rsfa.h"
+#include "cross.hpp"
+
+using namespace rsfa;
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+// Scores are multiplied by c = |sm_scale| * log2 e within the exponential; a smaller c than this changes no weight
+// (finite scores are below 2^40) and would make lse / c overflow.
+constexpr float LEAST_C = 7.888609052210118e-31f;  // 2^-100
+constexpr int ROWS = 64;  // rows are padded to whole tiles of 64 in the statistics
+
+struct BwdParams {
+    const void *q, *k, *v, *o, *go;
+    const float *lse, *glse;
+    void *gq, *gk, *gv;
+    int64_t q_st[3], k_st[3], v_st[3], o_st[3], go_st[3], gq_st[3], gk_st[3], gv_st[3];  // elements, of (Z, heads, rows)
+    const int32_t* lengths;
+    int32_t z, heads, key_heads, group, t, n;
+    int32_t tp;        // t in whole tiles
+    int32_t blocks;    // blocks of a key head (dK, dV) or of a query head (dQ)
+    int32_t splits;    // parts of the pass
+    float c, scale;
+    uint32_t neg;      // sign of sm_scale, as a mask for a pair of values
+    float *nl, *nd;    // [Z * heads][tp]: -lse / (c ln 2), -delta; rows past t: -inf, 0
+    float* part[2];    // splits > 1: [splits][rows][D] of dK and dV, or of dQ
+};
+
+__device__ __forceinline__ int keys_of(const BwdParams& p, int z) {
+    return __builtin_amdgcn_readfirstlane(p.lengths ? max(0, min(p.lengths[z], p.n)) : p.n);
+}
+
+// The head and block of a workgroup.  Workgroups go to the 8 XCDs in turn; the blocks of a head stay on
+// one (where heads divide evenly) and are neighbours in time, so that what all of them pass over is fetched into its L2 once.
+__device__ __forceinline__ void head_block(int heads, int blocks, int& head, int& block) {
+    int i = blockIdx.x, x = 0, step = 1;
+    if (heads % 8 == 0) x = i & 7, i >>= 3, step = 8;
+    const int local = i / blocks;
+    block = i - local * blocks;
+    head = local * step + x;
+}
+
+// One wave's direct load of 64 dwords into LDS (dma16's smaller sibling; see there for the s_nop).
+__device__ __forceinline__ void dma4(const void* sbase, uint32_t voff_bytes, uint32_t lds_addr) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1"
+                 :
+                 : "v"(voff_bytes), "s"(sbase), "{m0}"(lds_addr)
+                 : "memory");
+}
+
+// Statistics of the rows: D / 8 lanes a row.  Bound by memory: 4 D bytes a row.
+template <class T, int D>
+__global__ void __launch_bounds__(256) cross_stats_kernel(BwdParams p) {
+    typedef typename T::x8 x8;
+    typedef typename T::elem elem;
+    constexpr int LANES = D / 8;
+    const int64_t id = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES;
+    const int64_t zh = id / p.tp;
+    if (zh >= (int64_t)p.z * p.heads) return;
+    const int row = (int)(id - zh * p.tp), z = (int)(zh / p.heads), h = (int)(zh - (int64_t)z * p.heads);
+    float sum = 0.0f;
+    if (row < p.t) {
+        const x8 a = *(const x8*)((const elem*)p.o + z * p.o_st[0] + h * p.o_st[1] + row * p.o_st[2] + 8 * lane);
+        const x8 b = *(const x8*)((const elem*)p.go + z * p.go_st[0] + h * p.go_st[1] + row * p.go_st[2] + 8 * lane);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf((float)a[i], (float)b[i], sum);
+    }
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) sum += __shfl_xor(sum, d);
+    if (lane) return;
+    float nl = -INFINITY, nd = 0.0f;
+    if (row < p.t) {
+        const int64_t at = zh * p.t + row;
+        nl = -(p.lse[at] * LOG2E) / p.c;
+        nd = (p.glse ? p.glse[at] : 0.0f) - sum;
+    }
+    p.nl[id] = nl;
+    p.nd[id] = nd;
+}
+
+// Tiles of rows in LDS have the forward kernel's layout (fa_fwd_kernel.hpp): 16-row blocks of planes of 32 columns,
+// read as rows (A operand of S = Q K^T) and as transposes (A operand of dV^T = dO^T P) without bank conflicts.
+struct Lane {
+    int lane, hh, l32, l16;
+    uint32_t koff[2], voff[2];
+    int ld_row, ld_col;
+    template <int D>
+    __device__ __forceinline__ void set(int tid) {
+        constexpr int BLK = 32 * D;
+        lane = tid & 63, hh = lane >> 5, l32 = lane & 31, l16 = lane & 15;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) koff[e] = (l32 >> 4) * BLK + l16 * 64 + ((2 * e + hh) ^ row_swz(l16)) * 16;
+        const int vcc = 2 * ((lane >> 4) & 1) + ((l16 >> 1) & 1);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int r = 8 * u + 4 * hh + (l16 >> 2);
+            voff[u] = r * 64 + (vcc ^ row_swz(r)) * 16 + 8 * (l16 & 1);
+        }
+        ld_row = lane >> 2, ld_col = ((lane & 3) ^ row_swz(ld_row)) * 8;
+    }
+};
+
+// acc += A B over the D values of a row: A 32 rows of a tile in LDS, B in registers.
+template <class T, int D>
+__device__ __forceinline__ void rows_product(const RSFA_LDS char* tile, const Lane& w, const typename T::x8 (&b)[D / 16], f32x16& acc) {
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+        const typename T::x8 a = *(const RSFA_LDS typename T::x8*)(tile + w.koff[s & 1] + (s >> 1) * 1024);
+        acc = T::mfma(a, b[s], acc);
+    }
+}
+
+// acc[d] += A B over 32 rows of a tile: A the transpose of the tile's columns 32 d .., B in registers.
+template <class T, int D>
+__device__ __forceinline__ void columns_product(const RSFA_LDS char* tile, const Lane& w, const typename T::x8 (&b)[2], f32x16 (&acc)[D / 32]) {
+    typedef typename T::x8 x8;
+    constexpr int BLK = 32 * D;
+#pragma unroll
+    for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d) {
+            const RSFA_LDS char* const at = tile + h2 * BLK + d * 1024;
+            const i32x2 lo = __builtin_bit_cast(i32x2, T::tr_read(at + w.voff[0]));
+            const i32x2 hi = __builtin_bit_cast(i32x2, T::tr_read(at + w.voff[1]));
+            acc[d] = T::mfma(__builtin_bit_cast(x8, (i32x4){lo[0], lo[1], hi[0], hi[1]}), b[h2], acc[d]);
+        }
+}
+
+template <class T>
+__device__ __forceinline__ void pack(const f32x16& x, typename T::x8 (&b)[2]) {
+#pragma unroll
+    for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const typename T::x2 pr = T::cvt2(x[8 * h2 + 2 * i], x[8 * h2 + 2 * i + 1]);
+            b[h2][2 * i] = pr[0], b[h2][2 * i + 1] = pr[1];
+        }
+}
+
+// A row of a transposed accumulator: lane l holds row l % 32, values 32 d + 8 a + 4 (l / 32) + e.
+template <class T, int D>
+__device__ __forceinline__ void store_row(typename T::elem* dst, const f32x16 (&acc)[D / 32], float f, int hh) {
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            typename T::x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (typename T::elem)(acc[d][4 * a + e] * f);
+            *(typename T::x4*)(dst + 32 * d + 8 * a + 4 * hh) = v;
+        }
+}
+
+template <int D>
+__device__ __forceinline__ void store_part(float* dst, const f32x16 (&acc)[D / 32], int hh) {
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+            *(float4*)(dst + 32 * d + 8 * a + 4 * hh) = make_float4(acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]);
+}
+
+// dK and dV of 128 keys, 32 of each wave, held transposed (dK^T = Q^T dS, dV^T = dO^T P): with keys in the lanes S
+// and dS leave the matrix unit as the operands that the next products take.  K and V of the wave stay in registers;
+// tiles of rows of Q and dO pass through LDS, two buffers.
+template <int D>
+struct Bwd {
+    static constexpr int TILE_ROWS = D == 256 ? 32 : 64;
+    static constexpr int OCC = D == 256 ? 1 : D == 32 ? 4 : 2;  // waves of a SIMD
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Bwd<D>::OCC, Bwd<D>::OCC)))
+cross_dkv_kernel(BwdParams p) {
+    typedef typename T::x8 x8;
+    typedef typename T::elem elem;
+    constexpr int QB = Bwd<D>::TILE_ROWS, BLK = 32 * D, TILE = QB * D * 2, STATS = 512, BUF = 2 * TILE + STATS;
+    constexpr int DT = D / 32, KST = D / 16;
+    __shared__ __attribute__((aligned(1024))) char smem_raw[2 * BUF];
+    RSFA_LDS char* const smem = (RSFA_LDS char*)smem_raw;
+    const uint32_t smem_addr = (uint32_t)(uintptr_t)smem;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Lane w;
+    w.set<D>(threadIdx.x);
+    int kh, block;
+    head_block(p.z * p.key_heads, p.blocks, kh, block);
+    const int z = kh / p.key_heads, h = kh - z * p.key_heads;
+    const int nk = keys_of(p, z);
+    const int key = block * 128 + wave * 32 + w.l32;
+
+    const int tiles = (p.t + QB - 1) / QB, all = tiles * p.group;
+    const int each = (all + p.splits - 1) / p.splits;
+    int i = min((int)blockIdx.y * each, all);
+    const int end = block * 128 < nk ? min(i + each, all) : i;  // (no key: no pass)
+    const bool mine = block * 128 + wave * 32 < nk;             // the wave has a key
+
+    x8 kf[KST], vf[KST];
+    {
+        const int row = max(0, min(key, nk - 1));
+        const elem* kp = (const elem*)p.k + z * p.k_st[0] + h * p.k_st[1] + row * p.k_st[2] + 8 * w.hh;
+        const elem* vp = (const elem*)p.v + z * p.v_st[0] + h * p.v_st[1] + row * p.v_st[2] + 8 * w.hh;
+#pragma unroll
+        for (int s = 0; s < KST; ++s) {
+            kf[s] = __builtin_bit_cast(x8, *(const u32x4*)(kp + 16 * s) ^ p.neg);
+            vf[s] = *(const x8*)(vp + 16 * s);
+        }
+#pragma unroll
+        for (int s = 0; s < KST; ++s) asm volatile("" : "+v"(kf[s]), "+v"(vf[s]));  // (here, ahead of the direct loads)
+    }
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
+
+    auto load = [&](int it, int buf) {
+        const int g = it / tiles, row0 = (it - g * tiles) * QB;
+        const int hq = h * p.group + g;
+        const uint32_t dst = smem_addr + buf * BUF;
+        const elem* qb = (const elem*)p.q + z * p.q_st[0] + hq * p.q_st[1];
+        const elem* gb = (const elem*)p.go + z * p.go_st[0] + hq * p.go_st[1];
+        const int last = p.t - 1;  // rows past it repeat it: their statistics make P 0
+        auto rows = [&](const elem* base, int64_t st, int blk, uint32_t to) {
+            const int r0 = min(row0 + 16 * blk, last);
+            const uint32_t off = (uint32_t)(((min(r0 + w.ld_row, last) - r0) * st + w.ld_col) * 2);
+            const elem* at = base + r0 * st;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) dma16(at + 32 * c, off, to + blk * BLK + c * 1024);
+        };
+        if constexpr (QB == 64) {
+            rows(qb, p.q_st[2], wave, dst);
+            rows(gb, p.go_st[2], wave, dst + TILE);
+        } else if (wave < 2) {
+            rows(qb, p.q_st[2], wave, dst);
+        } else {
+            rows(gb, p.go_st[2], wave - 2, dst + TILE);
+        }
+        // (32-row tiles load 64 dwords too: the statistics have room behind the last)
+        if (wave < 2) {
+            const int64_t at = (int64_t)(z * p.heads + hq) * p.tp + row0;
+            dma4((wave ? p.nd : p.nl) + at, 4 * w.lane, dst + 2 * TILE + wave * 256);
+        }
+    };
+    auto stats = [&](const RSFA_LDS char* at, f32x16& x) {
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const f32x4 v = *(const RSFA_LDS f32x4*)(at + (8 * a + 4 * w.hh) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * a + e] = v[e];
+        }
+    };
+
+    if (i < end) load(i, 0);
+    for (int buf = 0; i < end; ++i, buf ^= 1) {
+        wait_loads_and_sync();
+        if (i + 1 < end) load(i + 1, buf ^ 1);
+        if (!mine) continue;
+        const RSFA_LDS char* const qt = smem + buf * BUF;
+        const RSFA_LDS char* const gt = qt + TILE;
+#pragma unroll
+        for (int st = 0; st < QB / 32; ++st) {
+            f32x16 s, x;
+            x8 b[2];
+            stats(gt + TILE + st * 128, s);
+            rows_product<T, D>(qt + st * 2 * BLK, w, kf, s);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * p.c);
+            pack<T>(s, b);
+            columns_product<T, D>(gt + st * 2 * BLK, w, b, dv);
+            stats(gt + TILE + 256 + st * 128, x);
+            rows_product<T, D>(gt + st * 2 * BLK, w, vf, x);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= x[r];
+            pack<T>(s, b);
+            columns_product<T, D>(qt + st * 2 * BLK, w, b, dk);
+        }
+    }
+    if (key >= p.n) return;
+    if (p.splits > 1) {
+        if (key >= nk) return;  // (the sum of the parts writes 0 there)
+        const int64_t at = (((int64_t)blockIdx.y * p.z * p.key_heads + kh) * p.n + key) * D;
+        if (p.gk) store_part<D>(p.part[0] + at, dk, w.hh);
+        if (p.gv) store_part<D>(p.part[1] + at, dv, w.hh);
+        return;
+    }
+    if (key >= nk) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
+    }
+    if (p.gk) store_row<T, D>((elem*)p.gk + z * p.gk_st[0] + h * p.gk_st[1] + key * p.gk_st[2], dk, p.scale, w.hh);
+    if (p.gv) store_row<T, D>((elem*)p.gv + z * p.gv_st[0] + h * p.gv_st[1] + key * p.gv_st[2], dv, 1.0f, w.hh);
+}
+
+// dQ of 128 rows, 32 of each wave, held transposed (dQ^T = K^T dS^T), rows in the lanes: a row's
+// statistics are one register each.  Q and dO of the wave stay in registers; tiles of K and V pass through LDS.
+template <class T, int D>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Bwd<D>::OCC, Bwd<D>::OCC)))
+cross_dq_kernel(BwdParams p) {
+    typedef typename T::x8 x8;
+    typedef typename T::elem elem;
+    constexpr int KB = Bwd<D>::TILE_ROWS, BLK = 32 * D, TILE = KB * D * 2, BUF = 2 * TILE;
+    constexpr int DT = D / 32, KST = D / 16;
+    __shared__ __attribute__((aligned(1024))) char smem_raw[2 * BUF];
+    RSFA_LDS char* const smem = (RSFA_LDS char*)smem_raw;
+    const uint32_t smem_addr = (uint32_t)(uintptr_t)smem;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Lane w;
+    w.set<D>(threadIdx.x);
+    int kh, block;
+    head_block(p.z * p.key_heads, p.blocks * p.group, kh, block);
+    const int z = kh / p.key_heads, h = kh - z * p.key_heads;
+    const int g = block / p.blocks, hq = h * p.group + g;
+    block -= g * p.blocks;
+    const int nk = keys_of(p, z);
+    const int row = block * 128 + wave * 32 + w.l32;
+    const bool mine = block * 128 + wave * 32 < p.t;
+
+    const int all = (nk + KB - 1) / KB, each = (all + p.splits - 1) / p.splits;
+    int i = min((int)blockIdx.y * each, all);
+    const int end = min(i + each, all);
+
+    x8 qf[KST], gf[KST];
+    float l2, nd;
+    {
+        const int r = min(row, p.t - 1);
+        const elem* qp = (const elem*)p.q + z * p.q_st[0] + hq * p.q_st[1] + r * p.q_st[2] + 8 * w.hh;
+        const elem* gp = (const elem*)p.go + z * p.go_st[0] + hq * p.go_st[1] + r * p.go_st[2] + 8 * w.hh;
+#pragma unroll
+        for (int s = 0; s < KST; ++s) {
+            qf[s] = __builtin_bit_cast(x8, *(const u32x4*)(qp + 16 * s) ^ p.neg);
+            gf[s] = *(const x8*)(gp + 16 * s);
+        }
+        const int64_t at = (int64_t)z * p.heads + hq;
+        l2 = p.lse[at * p.t + r] * LOG2E;
+        nd = p.nd[at * p.tp + r];
+#pragma unroll
+        for (int s = 0; s < KST; ++s) asm volatile("" : "+v"(qf[s]), "+v"(gf[s]));
+        asm volatile("" : "+v"(l2), "+v"(nd));
+    }
+    f32x16 dq[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dq[d][r] = 0.0f;
+
+    const elem* const kb = (const elem*)p.k + z * p.k_st[0] + h * p.k_st[1];
+    const elem* const vb = (const elem*)p.v + z * p.v_st[0] + h * p.v_st[1];
+    auto load = [&](int it, int buf) {
+        const int row0 = it * KB, last = nk - 1;
+        const uint32_t dst = smem_addr + buf * BUF;
+        auto rows = [&](const elem* base, int64_t st, int blk, uint32_t to) {
+            const int r0 = min(row0 + 16 * blk, last);
+            const uint32_t off = (uint32_t)(((min(r0 + w.ld_row, last) - r0) * st + w.ld_col) * 2);
+            const elem* at = base + r0 * st;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) dma16(at + 32 * c, off, to + blk * BLK + c * 1024);
+        };
+        if constexpr (KB == 64) {
+            rows(kb, p.k_st[2], wave, dst);
+            rows(vb, p.v_st[2], wave, dst + TILE);
+        } else if (wave < 2) {
+            rows(kb, p.k_st[2], wave, dst);
+        } else {
+            rows(vb, p.v_st[2], wave - 2, dst + TILE);
+        }
+    };
+    if (i < end) load(i, 0);
+    for (int buf = 0; i < end; ++i, buf ^= 1) {
+        wait_loads_and_sync();
+        if (i + 1 < end) load(i + 1, buf ^ 1);
+        if (!mine) continue;
+        const RSFA_LDS char* const kt = smem + buf * BUF;
+        const RSFA_LDS char* const vt = kt + TILE;
+#pragma unroll
+        for (int st = 0; st < KB / 32; ++st) {
+            f32x16 s = {}, x = {};
+            rows_product<T, D>(kt + st * 2 * BLK, w, qf, s);
+            rows_product<T, D>(vt + st * 2 * BLK, w, gf, x);
+            const int left = nk - i * KB - 32 * st - 4 * w.hh;  // keys of the sub-tile, from the lane's first on
+            if (i * KB + 32 * st + 32 > nk) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (8 * (r / 4) + r % 4 >= left) s[r] = -INFINITY;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -l2)) * (x[r] + nd);
+            x8 b[2];
+            pack<T>(s, b);
+            columns_product<T, D>(kt + st * 2 * BLK, w, b, dq);
+        }
+    }
+    if (row >= p.t) return;
+    if (p.splits > 1) {
+        const int64_t rows = (int64_t)p.z * p.heads * p.t;
+        store_part<D>(p.part[0] + (blockIdx.y * rows + ((int64_t)z * p.heads + hq) * p.t + row) * D, dq, w.hh);
+        return;
+    }
+    store_row<T, D>((elem*)p.gq + z * p.gq_st[0] + hq * p.gq_st[1] + row * p.gq_st[2], dq, p.scale, w.hh);
+}
+
+// Sums of parts: D / 4 lanes a row; rows past their sequence's length (dK, dV) become 0.
+struct SumParams {
+    const float* part;
+    void* out;
+    int64_t st[3];
+    const int32_t* lengths;  // or null
+    int32_t heads, n, splits;
+    int64_t rows;            // Z * heads * n
+    float f;
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(256) sum_parts_kernel(SumParams a, SumParams b) {
+    typedef typename T::elem elem;
+    const SumParams& p = blockIdx.y ? b : a;
+    constexpr int G = D / 4;
+    const int lane = threadIdx.x % G;
+    const int64_t id = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (id >= p.rows) return;
+    const int64_t zh = id / p.n;
+    const int row = (int)(id - zh * p.n), z = (int)(zh / p.heads), h = (int)(zh - (int64_t)z * p.heads);
+    f32x4 sum = {0, 0, 0, 0};
+    if (!p.lengths || row < p.lengths[z]) {
+#pragma unroll 4
+        for (int s = 0; s < p.splits; ++s) sum += *(const f32x4*)(p.part + (s * p.rows + id) * D + 4 * lane);
+    }
+    typename T::x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (elem)(sum[i] * p.f);
+    *(typename T::x4*)((elem*)p.out + z * p.st[0] + h * p.st[1] + row * p.st[2] + 4 * lane) = v;
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+struct Functions {
+    const void *stats, *dkv, *dq, *sum;
+};
+
+template <class T>
+Functions functions(int64_t d) {
+    switch (d) {
+        case 32: return {(const void*)&cross_stats_kernel<T, 32>, (const void*)&cross_dkv_kernel<T, 32>, (const void*)&cross_dq_kernel<T, 32>, (const void*)&sum_parts_kernel<T, 32>};
+        case 64: return {(const void*)&cross_stats_kernel<T, 64>, (const void*)&cross_dkv_kernel<T, 64>, (const void*)&cross_dq_kernel<T, 64>, (const void*)&sum_parts_kernel<T, 64>};
+        case 128: return {(const void*)&cross_stats_kernel<T, 128>, (const void*)&cross_dkv_kernel<T, 128>, (const void*)&cross_dq_kernel<T, 128>, (const void*)&sum_parts_kernel<T, 128>};
+        default: return {(const void*)&cross_stats_kernel<T, 256>, (const void*)&cross_dkv_kernel<T, 256>, (const void*)&cross_dq_kernel<T, 256>, (const void*)&sum_parts_kernel<T, 256>};
+    }
+}
+
+struct Plan {
+    int64_t tp, key_blocks, row_blocks;
+    int dkv_splits, dq_splits;
+    uint64_t nl, nd, dkv[2], dq, bytes;
+};
+
+Plan make_plan(const rsfa_cross_bwd_args* a) {
+    Plan p{};
+    const int64_t d = a->head_dim, group = a->heads / a->key_heads, kh = a->z * a->key_heads, qh = a->z * a->heads;
+    const int64_t tile = d == 256 ? 32 : 64, full = (int64_t)cross_cus() * (d == 256 ? 1 : d == 32 ? 4 : 2);
+    p.tp = (a->t + ROWS - 1) / ROWS * ROWS;
+    p.key_blocks = (a->n + 127) / 128;
+    p.row_blocks = (a->t + 127) / 128;
+    auto parts = [&](int64_t blocks, int64_t tiles) {
+        return (int)std::max<int64_t>(1, std::min<int64_t>({full / blocks, tiles / 4, 64}));
+    };
+    p.dkv_splits = parts(kh * p.key_blocks, group * ((a->t + tile - 1) / tile));
+    p.dq_splits = parts(qh * p.row_blocks, (a->n + tile - 1) / tile);
+    uint64_t at = 0;
+    auto take = [&](uint64_t n) {
+        const uint64_t here = at;
+        at += (n + 255) / 256 * 256;
+        return here;
+    };
+    p.nl = take((uint64_t)qh * p.tp * 4 + 256);
+    p.nd = take((uint64_t)qh * p.tp * 4 + 256);
+    if (p.dkv_splits > 1)
+        for (int i = 0; i < 2; ++i) p.dkv[i] = take((uint64_t)p.dkv_splits * kh * a->n * d * 4);
+    if (p.dq_splits > 1) p.dq = take((uint64_t)p.dq_splits * qh * a->t * d * 4);
+    p.bytes = at;
+    return p;
+}
+
+int check(const rsfa_cross_bwd_args* a) {
+    if (!a) return RSFA_E_NULL;
+    if (a->struct_size != sizeof(rsfa_cross_bwd_args)) return RSFA_E_ABI;
+    return cross_check(a->dtype, a->z, a->heads, a->key_heads, a->t, a->n, a->head_dim);
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t rsfa_cross_bwd_workspace_bytes(const rsfa_cross_bwd_args* a) { return check(a) == RSFA_OK ? make_plan(a).bytes : 0; }
+
+int rsfa_cross_bwd(const rsfa_cross_bwd_args* a, void* stream) {
+    int st = check(a);
+    if (st != RSFA_OK) return st;
+    if (!a->q || !a->k || !a->v || !a->o || !a->lse || !a->grad_o) return RSFA_E_NULL;
+    struct {
+        const void* at;
+        const int64_t* st;
+    } rows[] = {{a->q, a->q_stride}, {a->k, a->k_stride}, {a->v, a->v_stride}, {a->o, a->o_stride}, {a->grad_o, a->grad_o_stride},
+                {a->grad_q, a->grad_q_stride}, {a->grad_k, a->grad_k_stride}, {a->grad_v, a->grad_v_stride}};
+    for (auto& r : rows)
+        if (r.at && (st = cross_check_rows(r.at, r.st)) != RSFA_OK) return st;
+    if (((uintptr_t)a->lse | (uintptr_t)a->grad_lse | (uintptr_t)a->lengths) & 3) return RSFA_E_ALIGN;
+    const Plan plan = make_plan(a);
+    if (!a->workspace || a->workspace_bytes < plan.bytes) return RSFA_E_WORKSPACE;
+    if ((uintptr_t)a->workspace & 15) return RSFA_E_ALIGN;
+    char* const ws = (char*)a->workspace;
+    BwdParams p{};
+    p.q = a->q, p.k = a->k, p.v = a->v, p.o = a->o, p.go = a->grad_o, p.lse = a->lse, p.glse = a->grad_lse;
+    p.gq = a->grad_q, p.gk = a->grad_k, p.gv = a->grad_v;
+    for (int i = 0; i < 3; ++i) {
+        p.q_st[i] = a->q_stride[i], p.k_st[i] = a->k_stride[i], p.v_st[i] = a->v_stride[i], p.o_st[i] = a->o_stride[i];
+        p.go_st[i] = a->grad_o_stride[i], p.gq_st[i] = a->grad_q_stride[i], p.gk_st[i] = a->grad_k_stride[i], p.gv_st[i] = a->grad_v_stride[i];
+    }
+    p.lengths = a->lengths;
+    p.z = (int32_t)a->z, p.heads = (int32_t)a->heads, p.key_heads = (int32_t)a->key_heads, p.group = p.heads / p.key_heads;
+    p.t = (int32_t)a->t, p.n = (int32_t)a->n, p.tp = (int32_t)plan.tp;
+    p.scale = a->sm_scale;
+    p.c = std::max(std::fabs(a->sm_scale) * LOG2E, LEAST_C);
+    p.neg = a->sm_scale < 0.0f ? 0x80008000u : 0u;
+    p.nl = (float*)(ws + plan.nl), p.nd = (float*)(ws + plan.nd);
+    const int64_t d = a->head_dim, kh = a->z * a->key_heads, qh = a->z * a->heads;
+    const Functions fn = a->dtype == RSFA_DTYPE_BF16 ? functions<TypeBF16>(d) : functions<TypeF16>(d);
+    const int64_t stat_blocks = (qh * plan.tp + 2048 / d - 1) / (2048 / d);
+    const int64_t dkv_blocks = kh * plan.key_blocks, dq_blocks = qh * plan.row_blocks;
+    const int64_t per = 1024 / d, sum_k = (kh * a->n + per - 1) / per, sum_q = (qh * a->t + per - 1) / per;
+    if (std::max({stat_blocks, dkv_blocks, dq_blocks, sum_k, sum_q}) > 0x7fffffff) return RSFA_E_CROSS;
+    auto launch = [&](const void* f, int64_t x, int y, void** args) {
+        return hipLaunchKernel(f, dim3((unsigned)x, (unsigned)y), dim3(256), args, 0, (hipStream_t)stream) == hipSuccess;
+    };
+    void* args[] = {&p};
+    if (!launch(fn.stats, stat_blocks, 1, args)) return RSFA_E_LAUNCH;
+    if (p.gk || p.gv) {
+        p.blocks = (int32_t)plan.key_blocks, p.splits = plan.dkv_splits;
+        for (int i = 0; i < 2; ++i) p.part[i] = (float*)(ws + plan.dkv[i]);
+        if (!launch(fn.dkv, dkv_blocks, p.splits, args)) return RSFA_E_LAUNCH;
+        if (p.splits > 1) {
+            SumParams s[2] = {};
+            int n = 0;
+            if (p.gk) s[n++] = {p.part[0], p.gk, {p.gk_st[0], p.gk_st[1], p.gk_st[2]}, p.lengths, p.key_heads, p.n, p.splits, kh * a->n, p.scale};
+            if (p.gv) s[n++] = {p.part[1], p.gv, {p.gv_st[0], p.gv_st[1], p.gv_st[2]}, p.lengths, p.key_heads, p.n, p.splits, kh * a->n, 1.0f};
+            void* sum_args[] = {&s[0], &s[1]};
+            if (!launch(fn.sum, sum_k, n, sum_args)) return RSFA_E_LAUNCH;
+        }
+    }
+    if (p.gq) {
+        p.blocks = (int32_t)plan.row_blocks, p.splits = plan.dq_splits;
+        p.part[0] = (float*)(ws + plan.dq);
+        if (!launch(fn.dq, dq_blocks, p.splits, args)) return RSFA_E_LAUNCH;
+        if (p.splits > 1) {
+            SumParams s[2] = {{p.part[0], p.gq, {p.gq_st[0], p.gq_st[1], p.gq_st[2]}, nullptr, p.heads, p.t, p.splits, qh * a->t, p.scale}, {}};
+            void* sum_args[] = {&s[0], &s[1]};
+            if (!launch(fn.sum, sum_q, 1, sum_args)) return RSFA_E_LAUNCH;
+        }
+    }
+    return RSFA_OK;
+}
+
+}  // extern "C"

@@ -142,7 +142,10 @@ struct TypeF16V8 : TypeF16 {
 // causal prefix with the mask-free body, the diagonal with the masked body).
 // MODE_PREFIX / MODE_DIAG are the reference's two-launch causal split
 // (STAGE 4 / STAGE 5, flash_attention_forward.py:338-368).
-enum { MODE_FUSED = 0, MODE_PREFIX = 1, MODE_DIAG = 2 };
+// MODE_CROSS: keys of another length than the queries', of their own number of
+// heads, each sequence's first k_lengths[b] of them, in `splits` parts of whole
+// key tiles; several parts leave their rows' state in part_ml and part_o.
+enum { MODE_FUSED = 0, MODE_PREFIX = 1, MODE_DIAG = 2, MODE_CROSS = 3 };
 
 struct FwdParams {
     const void* q;
@@ -167,6 +170,15 @@ struct FwdParams {
     uint32_t neg;       // 1 when sm_scale < 0: q is negated (exact) and c = |c|
     uint32_t* ticket;   // dynamic queue counters (nq of them, 16 words apart; each returns
                         // to 0 at kernel end) or null for the static schedule
+    // MODE_CROSS: H and num_heads count key heads; a key head's nmb tasks are
+    // those of its group's query heads and parts, query blocks first
+    const int32_t* k_lengths;  // [Z], or null: n_keys of all
+    int32_t n_keys;
+    int32_t group;    // query heads per key head
+    int32_t splits;   // parts of the keys
+    int32_t q_blocks; // query blocks per query head
+    float* part_o;    // splits > 1: [splits][Z * query heads * n_ctx][D], un-normalised
+    float2* part_ml;  // ... [splits][Z * query heads * n_ctx]: maximum (log2 units), sum
 };
 
 // Queues.  Workgroups are dispatched to the 8 XCDs of an MI355X round robin,
@@ -261,6 +273,16 @@ __device__ __forceinline__ void decode_task(const FwdParams& p, const Queue& q, 
         }
     }
     bh = lh * p.nq + q.x;
+}
+
+// MODE_CROSS: block mb of a key head's tasks is query block mb % q_blocks of query
+// head h (given: the key head) and a part of the keys; the parts last, so that
+// the tasks under way together read the same keys.
+__device__ __forceinline__ void cross_task(const FwdParams& p, int& mb, int& h, int& part) {
+    const int rest = mb / p.q_blocks;
+    mb -= rest * p.q_blocks;
+    part = rest / p.group;
+    h = h * p.group + (rest - part * p.group);
 }
 
 // One wave's direct global->LDS load: each lane fetches 16 bytes from
@@ -405,7 +427,7 @@ __device__ __forceinline__ void wait_loads_and_sync() {
 // (bias blocks there spilled 164 bytes per lane inside the loop): +3 % on
 // B=64 S=1024 against the one-phase loop.
 constexpr bool uses_pingpong(int d, int bn, int nw, bool causal, int mode) {
-    return RSFA_PINGPONG && nw == 8 && mode == MODE_FUSED && (d <= 128 || d == 256) &&
+    return RSFA_PINGPONG && nw == 8 && (mode == MODE_FUSED || mode == MODE_CROSS) && (d <= 128 || d == 256) &&
            3 * (2 * bn * (d < 32 ? 32 : d) * 2) <= 160 * 1024 - 64;
 }
 
@@ -467,7 +489,9 @@ fa_fwd_kernel(FwdParams p) {
     static_assert(BN % 32 == 0 && BN >= 32, "BN must be a multiple of 32");
     static_assert(D % 16 == 0, "D must be a multiple of 16");
     static_assert((BN * CPR) % 64 == 0, "tile must be whole 1-KB load slices");
-    static_assert(MODE == MODE_FUSED || CAUSAL, "split modes are causal only");
+    constexpr bool CROSS = MODE == MODE_CROSS;
+    static_assert(MODE == MODE_FUSED || CROSS || CAUSAL, "split modes are causal only");
+    static_assert(!CROSS || !(CAUSAL || V8), "cross attention has no causal mask and two-byte values");
     // Ping-pong schedule for 8-wave workgroups (two waves per SIMD): the key
     // tiles every row of the workgroup sees unmasked run with waves 4-7 one
     // phase behind waves 0-3, so one wave of each SIMD runs its softmax (VALU)
@@ -695,7 +719,12 @@ fa_fwd_kernel(FwdParams p) {
         int bh, mb;
         decode_task<CAUSAL>(p, qu, t, bh, mb);
         const int b = bh / p.H;
-        const int h = bh - b * p.H;
+        const int hk = bh - b * p.H;  // key head
+        int h = hk, part = 0;
+        if constexpr (CROSS) {
+            cross_task(p, mb, h, part);
+            bh = b * p.H * p.group + h;  // (from here on the query head's)
+        }
         // REG_TIGHT: opaque per task, so values derived from n stay inside the
         // task instead of being hoisted out of the task loop and spilled
         int n = p.n_ctx;
@@ -704,13 +733,23 @@ fa_fwd_kernel(FwdParams p) {
         const int qrow = m0 + wave * 32 + l32;
 
         const elem* qb = qg + b * p.q_sz + h * p.q_sh;
-        const elem* kh = kg + b * p.k_sz + h * p.k_sh;
-        const velem* vh = vgp + b * p.v_sz + h * p.v_sh;
+        const elem* kh = kg + b * p.k_sz + hk * p.k_sh;
+        const velem* vh = vgp + b * p.v_sz + hk * p.v_sh;
         elem* ob = og + b * p.o_sz + h * p.o_sh;
 
+        int nk = n;  // keys
+        if constexpr (CROSS) {
+            nk = p.n_keys;
+            if (p.k_lengths) nk = max(0, min(__builtin_amdgcn_readfirstlane(p.k_lengths[b]), nk));
+        }
         // key tiles of this task
-        const int kv_end = CAUSAL ? min(n, m0 + BM) : n;
+        const int kv_end = CAUSAL ? min(nk, m0 + BM) : nk;
         int j0 = 0, j1 = (kv_end + BN - 1) / BN;
+        if constexpr (CROSS) {
+            const int each = (j1 + p.splits - 1) / p.splits;
+            j0 = min(part * each, j1);
+            j1 = min(j0 + each, j1);
+        }
         if (MODE == MODE_PREFIX) j1 = m0 / BN;
         if (MODE == MODE_DIAG) j0 = m0 / BN;
 
@@ -719,7 +758,7 @@ fa_fwd_kernel(FwdParams p) {
             const elem* kt0 = kh + (int64_t)kbase * p.k_sn;
             const velem* vt0 = vh + (int64_t)kbase * p.v_sn;
             const uint32_t dst0 = smem_addr + buf * BUF;
-            if (kbase + BN <= n) {
+            if (kbase + BN <= nk) {
                 // whole tile: one uniform base per tensor, per-slice offsets precomputed
 #pragma unroll
                 for (int sl = 0; sl < NSL; ++sl) {
@@ -741,7 +780,7 @@ fa_fwd_kernel(FwdParams p) {
                 }
                 return;
             }
-            const int last = n - 1 - kbase;  // last row of the tile inside the sequence
+            const int last = nk - 1 - kbase;  // last row of the tile inside the sequence
             if constexpr (V8) {
                 // rows past the sequence re-read its last row (masked later)
 #pragma unroll
@@ -808,7 +847,7 @@ fa_fwd_kernel(FwdParams p) {
         // [j0, jpp): ping-pong tiles (whole tiles no row of the workgroup masks).
         // The first loads go out before the Q loads, so their latencies overlap.
         int jpp = j0;
-        if constexpr (PP) jpp = min(j1, (CAUSAL ? m0 : n) / BN);
+        if constexpr (PP) jpp = min(j1, (CAUSAL ? m0 : nk) / BN);
         if constexpr (DIAG_PP || DIAG_VM) {
             if (m0 + BM <= n) jpp = j1;  // the diagonal tiles too (whole tiles only)
         }
@@ -1005,9 +1044,9 @@ fa_fwd_kernel(FwdParams p) {
 
         const int wq_lo = m0 + wave * 32;  // smallest query row of this wave
         const int wq_hi = wq_lo + 31;      // largest
-        const int lim = CAUSAL ? min(qrow, n - 1) : n - 1;     // last key this lane sees
-        const int vis_lo = CAUSAL ? min(wq_lo, n - 1) : n - 1;  // last key every lane of the wave sees
-        const int vis_hi = CAUSAL ? min(wq_hi, n - 1) : n - 1;  // last key any lane of the wave sees
+        const int lim = CAUSAL ? min(qrow, nk - 1) : nk - 1;     // last key this lane sees
+        const int vis_lo = CAUSAL ? min(wq_lo, nk - 1) : nk - 1;  // last key every lane of the wave sees
+        const int vis_hi = CAUSAL ? min(wq_hi, nk - 1) : nk - 1;  // last key any lane of the wave sees
 
         // S^T = K Q^T for the key tile whose K sits at LDS byte offset kofs.
         // Masked: keys past each row's last visible key become -inf, and 32-key
@@ -1109,7 +1148,9 @@ fa_fwd_kernel(FwdParams p) {
                 l_sum += p0 + p1;  // the reference sums the unrounded P for an e5m2 V
             } else {
                 const x2 pr = T::cvt2(p0, p1);
-                l_sum = T::dot2(pr, T::ones2(), l_sum);
+                // (cross attention's caller may want the logsumexp to 32 bits, its gradient does: P unrounded)
+                if constexpr (CROSS) l_sum += p0 + p1;
+                else l_sum = T::dot2(pr, T::ones2(), l_sum);
                 pk[kt][h2][2 * i] = pr[0];
                 pk[kt][h2][2 * i + 1] = pr[1];
             }
@@ -1425,10 +1466,16 @@ fa_fwd_kernel(FwdParams p) {
                                                             : ticket_of_task(qu, t) + qu.nwg);
                     if (ctr) t_next = tn;
                     if (tn < qu.ntask && jpp - j0 >= 4) {
-                        int nbh, nmb;
+                        int nbh, nmb, nhq = 0, npart = 0;
                         decode_task<CAUSAL>(p, qu, tn, nbh, nmb);
+                        if constexpr (CROSS) {
+                            nhq = nbh % p.H;
+                            cross_task(p, nmb, nhq, npart);
+                        }
                         if ((nmb + 1) * BM <= n) {
-                            const int nb = nbh / p.H, nh = nbh - nb * p.H;
+                            const int nb = nbh / p.H;
+                            int nh = nbh - nb * p.H;
+                            if constexpr (CROSS) nh = nhq;
                             qpf_do = true;
                             qnext = qg + nb * p.q_sz + nh * p.q_sh + (int64_t)nmb * BM * p.q_sm;
                         }
@@ -1594,7 +1641,22 @@ fa_fwd_kernel(FwdParams p) {
         // publishes them)
         if constexpr (QPF) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         const float lt = swap_sum(l_sum);
-        const float inv = 1.0f / lt;
+        float inv = 1.0f / lt;
+        if constexpr (CROSS) inv = nk == 0 ? 0.0f : inv;  // (no key: 0, and not 0 / 0)
+        bool whole = true;  // the rows' keys are all in this task
+        if constexpr (CROSS) {
+            whole = p.splits == 1;
+            if (!whole && qrow < n) {
+                const int64_t at = ((int64_t)part * p.num_heads * p.group + bh) * n + qrow;
+                if (hh == 0) p.part_ml[at] = make_float2(m_use, lt);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int a = 0; a < 4; ++a)
+                        *(float4*)(p.part_o + at * D + 32 * d + 8 * a + 4 * hh) =
+                            make_float4(o[d][4 * a + 0], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]);
+            }
+        }
         // O leaves through LDS: in the accumulator layout a lane holds 8 bytes
         // of a row per (d, a), so a direct store instruction writes 32 rows x
         // 16 bytes, and a CU needs ~64 cycles per such instruction (measured:
@@ -1626,38 +1688,40 @@ fa_fwd_kernel(FwdParams p) {
                             make_float4(o[d][4 * a + 0], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]);
                 }
         } else if constexpr (OSTAGE) {
-            __syncthreads();  // every wave is done with the K/V tiles
-            // a wave's own region: its reads of one round precede (in LDS
-            // order) its writes of the next, so rounds need no barrier
-            RSFA_LDS char* const ow = smem + wave * (32 * OROW);
-            constexpr int CH = OCOLS / 8;  // 16-byte chunks per staged row
-            constexpr int RPI = 64 / CH;   // rows per store instruction
-            const int rr = lane / CH, cc = (lane % CH) * 8;
-            const int row0 = m0 + wave * 32;
-#pragma unroll
-            for (int hf = 0; hf < D / OCOLS; ++hf) {
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) {
-                        const int col = 32 * d + 8 * a + 4 * hh;
-                        if (col < D && col / OCOLS == hf) {
-                            x4 v4;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v4[e] = (elem)(o[d][4 * a + e] * inv);
-                            *(RSFA_LDS x4*)(ow + l32 * OROW + (col - hf * OCOLS) * 2) = v4;
+            if (whole) {
+                __syncthreads();  // every wave is done with the K/V tiles
+                // a wave's own region: its reads of one round precede (in LDS
+                // order) its writes of the next, so rounds need no barrier
+                RSFA_LDS char* const ow = smem + wave * (32 * OROW);
+                constexpr int CH = OCOLS / 8;  // 16-byte chunks per staged row
+                constexpr int RPI = 64 / CH;   // rows per store instruction
+                const int rr = lane / CH, cc = (lane % CH) * 8;
+                const int row0 = m0 + wave * 32;
+    #pragma unroll
+                for (int hf = 0; hf < D / OCOLS; ++hf) {
+    #pragma unroll
+                    for (int d = 0; d < DT; ++d)
+    #pragma unroll
+                        for (int a = 0; a < 4; ++a) {
+                            const int col = 32 * d + 8 * a + 4 * hh;
+                            if (col < D && col / OCOLS == hf) {
+                                x4 v4;
+    #pragma unroll
+                                for (int e = 0; e < 4; ++e) v4[e] = (elem)(o[d][4 * a + e] * inv);
+                                *(RSFA_LDS x4*)(ow + l32 * OROW + (col - hf * OCOLS) * 2) = v4;
+                            }
                         }
+    #pragma unroll
+                    for (int it = 0; it < 32 / RPI; ++it) {
+                        const int r = it * RPI + rr;
+                        const x8 v = *(const RSFA_LDS x8*)(ow + r * OROW + cc * 2);
+                        if (row0 + r < n) *(x8*)(ob + (int64_t)(row0 + r) * p.o_sm + hf * OCOLS + cc) = v;
                     }
-#pragma unroll
-                for (int it = 0; it < 32 / RPI; ++it) {
-                    const int r = it * RPI + rr;
-                    const x8 v = *(const RSFA_LDS x8*)(ow + r * OROW + cc * 2);
-                    if (row0 + r < n) *(x8*)(ob + (int64_t)(row0 + r) * p.o_sm + hf * OCOLS + cc) = v;
                 }
+                if (p.lse && hh == 0 && qrow < n)
+                    p.lse[(int64_t)bh * n + qrow] = (m_use + __log2f(lt)) * 0.69314718055994530942f;
             }
-            if (p.lse && hh == 0 && qrow < n)
-                p.lse[(int64_t)bh * n + qrow] = (m_use + __log2f(lt)) * 0.69314718055994530942f;
-        } else if (qrow < n) {
+        } else if (qrow < n && whole) {
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll

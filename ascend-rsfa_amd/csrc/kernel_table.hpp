@@ -33,6 +33,12 @@ KernelList kernels_d32();
 KernelList kernels_d64();
 KernelList kernels_d128();
 KernelList kernels_d256();
+KernelList kernels_cross_f16();   // (called by cross_attention.hip alone)
+KernelList kernels_cross_bf16();
+
+// Launches a MODE_CROSS kernel for `p`, whose queues and counters it fills in (rsfa_api.hip).
+struct FwdParams;
+int launch_cross(const KernelEntry& e, FwdParams& p, void* stream);
 
 }  // namespace rsfa
 

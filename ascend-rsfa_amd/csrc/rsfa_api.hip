@@ -41,6 +41,7 @@ constexpr int kLdsPerCu = 160 * 1024;   // gfx950
 constexpr int kMaxKernels = 512;        // instantiations in all kernel lists
 
 KernelList all_lists[] = {kernels_d16(), kernels_d32(), kernels_d64(), kernels_d128(), kernels_d256()};
+KernelList cross_lists[] = {kernels_cross_f16(), kernels_cross_bf16()};
 
 template <class F>
 void for_each_kernel(F&& f) {
@@ -202,12 +203,14 @@ bool queue_needed(const FwdParams& p, int64_t grid, bool equal, int wgs) {
 
 // Position of an instantiation in the kernel lists (a fixed-size cache index).
 int kernel_index(const KernelEntry& e) {
-    int base = 0;
-    for (const KernelList& l : all_lists) {
-        if (&e >= l.entries && &e < l.entries + l.count) return base + (int)(&e - l.entries);
+    int base = 0, index = -1;
+    auto look = [&](const KernelList& l) {
+        if (&e >= l.entries && &e < l.entries + l.count) index = base + (int)(&e - l.entries);
         base += l.count;
-    }
-    return -1;
+    };
+    for (const KernelList& l : all_lists) look(l);
+    for (const KernelList& l : cross_lists) look(l);
+    return index;
 }
 
 // Resident workgroups per CU of an instantiation, queried once per device
@@ -486,6 +489,22 @@ __global__ void __launch_bounds__(64) clear_words(uint32_t* __restrict__ p, int 
 }
 
 }  // namespace
+
+int launch_cross(const KernelEntry& e, FwdParams& p, void* stream) {
+    int dev = 0, num_cus = 0, st;
+    if ((st = current_device(&dev)) != RSFA_OK) return st;
+    DeviceState& ds = g_dev[dev];
+    if ((st = device_cus(ds, dev, &num_cus)) != RSFA_OK) return st;
+    const int wgs = resident_wgs(ds, e);
+    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>((int64_t)num_cus * wgs, p.num_tasks));
+    p.nq = queue_count(p.num_heads, grid);
+    p.pairs = 0;
+    p.ticket = queue_needed(p, grid, !p.k_lengths, wgs) && dynamic_schedule_allowed(stream) ? stream_ticket(ds, stream) : nullptr;
+    void* args[] = {&p};
+    return hipLaunchKernel(e.fn, dim3((unsigned)grid), dim3((unsigned)(e.nw * 64)), args, 0, (hipStream_t)stream) == hipSuccess
+               ? RSFA_OK : RSFA_E_LAUNCH;
+}
+
 }  // namespace rsfa
 
 using namespace rsfa;
@@ -523,6 +542,9 @@ const char* rsfa_strerror(int status) {
         case RSFA_E_BUDGET:
             return "claim and evict need 0 <= recent + sinks <= budget <= capacity and n >= 1; evict a target of "
                    "the cache's shape with room for the budget";
+        case RSFA_E_CROSS:
+            return "cross attention needs head_dim 32, 64, 128 or 256, sizes of at least 1 within 32-bit counts, and query "
+                   "heads that are a multiple of the key heads";
         case RSFA_E_DRAFT:
             return "drafted tokens: 1 to 512 (RSFA_DRAFT_TOKENS) of them; attention of a tree takes no accumulate "
                    "and no first positions";

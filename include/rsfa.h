@@ -70,6 +70,7 @@ typedef enum rsfa_status {
     RSFA_E_CACHE     = -13, /* a cache or a call on one is out of its range: see
                                rsfa_cache4                                      */
     RSFA_E_BUDGET    = -14, /* claim / evict: budget, recent, sinks or n         */
+    RSFA_E_CROSS     = -16, /* cross attention: sizes or heads                  */
     RSFA_E_DRAFT     = -15  /* drafted tokens: more than RSFA_DRAFT_TOKENS, or
                                an option that a tree does not go with           */
 } rsfa_status;
@@ -375,6 +376,62 @@ typedef struct rsfa_cache4_evict_args {
 int rsfa_cache4_claim(const rsfa_cache4_evict_args *args, void *stream);
 int rsfa_cache4_evict(const rsfa_cache4_evict_args *args, void *stream);
 uint64_t rsfa_cache4_evict_workspace_bytes(const rsfa_cache4_evict_args *args, int32_t evict);
+
+/* ------------------------------------------------------------------------
+ * Cross attention: o = softmax(q k^T sm_scale) v over keys of another length.
+ *
+ * q, o [z, heads, t, head_dim], k, v [z, key_heads, n, head_dim] of one dtype (float16 or
+ * bfloat16); query head i reads key head i / (heads / key_heads).  With `lengths` (device, int32 [z];
+ * values outside [0, n] are taken as its ends) a sequence has its first lengths[z] keys; the others
+ * are not read.  A sequence without keys gives 0 (lse -inf).  Strides as everywhere;
+ * a stride of 0 repeats q, k or v.  Scores, sums, lse and accumulators are in 32 bits; softmax
+ * weights are rounded to the dtype for the product with v, as o is.
+ * Workspace: rsfa_cross_fwd_workspace_bytes of the same arguments (its contents need not outlive the
+ * call's kernels).
+ * ------------------------------------------------------------------------ */
+typedef struct rsfa_cross_args {
+    uint32_t       struct_size; /* = sizeof(rsfa_cross_args)                   */
+    int32_t        dtype;       /* RSFA_DTYPE_F16 or _BF16                      */
+    const void    *q, *k, *v;
+    void          *o;
+    float         *lse;         /* [z, heads, t], dense, or NULL: natural log   */
+    int64_t        z, heads, key_heads, t, n, head_dim; /* head_dim: 32, 64, 128, 256 */
+    int64_t        q_stride[4], k_stride[4], v_stride[4], o_stride[4];
+    const int32_t *lengths;     /* or NULL: n keys of all                      */
+    float          sm_scale;
+    uint32_t       reserved;    /* 0 */
+    void          *workspace;   /* 16-byte aligned */
+    uint64_t       workspace_bytes;
+} rsfa_cross_args;
+
+int rsfa_cross_fwd(const rsfa_cross_args *args, void *stream);
+uint64_t rsfa_cross_fwd_workspace_bytes(const rsfa_cross_args *args);
+
+/* Its gradients, from o and lse of the forward call, the gradient of o and, or NULL, of lse
+ * ([z, heads, t], dense).  A gradient whose pointer is NULL is not computed.  Gradients are whole:
+ * those of k and v are summed over the query heads of a group, and 0 for keys past a length.  Softmax weights
+ * and their gradients are rounded to the dtype for the products with rows; sums are in 32 bits, each in one order, so
+ * that a call gives the same bits each time.  The gradients' rows must not meet each other or an input. */
+typedef struct rsfa_cross_bwd_args {
+    uint32_t       struct_size; /* = sizeof(rsfa_cross_bwd_args)               */
+    int32_t        dtype;
+    const void    *q, *k, *v, *o;
+    const float   *lse;
+    const void    *grad_o;
+    const float   *grad_lse;
+    void          *grad_q, *grad_k, *grad_v;
+    int64_t        z, heads, key_heads, t, n, head_dim;
+    int64_t        q_stride[4], k_stride[4], v_stride[4], o_stride[4];
+    int64_t        grad_o_stride[4], grad_q_stride[4], grad_k_stride[4], grad_v_stride[4];
+    const int32_t *lengths;
+    float          sm_scale;
+    uint32_t       reserved;    /* 0 */
+    void          *workspace;   /* 16-byte aligned */
+    uint64_t       workspace_bytes;
+} rsfa_cross_bwd_args;
+
+int rsfa_cross_bwd(const rsfa_cross_bwd_args *args, void *stream);
+uint64_t rsfa_cross_bwd_workspace_bytes(const rsfa_cross_bwd_args *args);
 
 /* ------------------------------------------------------------------------
  * Drafted tokens.

@@ -1,0 +1,89 @@
+"""CPU tests of cross attention: refusals of the package and of the C ABI, the definition's gradients.
+
+Nothing here launches a kernel: every call is refused by its argument checks."""
+import ctypes
+
+import pytest
+import torch
+
+from ascend_rsfa import _native
+from ascend_rsfa.cross import cross_attention
+from oracle import cross as O
+
+
+def test_struct_layouts():
+    assert ctypes.sizeof(_native.CrossArgs) == 8 + 40 + 48 + 128 + 8 + 8 + 16
+    assert ctypes.sizeof(_native.CrossBwdArgs) == 8 + 80 + 48 + 256 + 8 + 8 + 16
+    assert "cross" in _native.strerror(_native.E_CROSS)
+
+
+def _args(kind=_native.CrossArgs, **over):
+    a = kind()
+    a.struct_size = ctypes.sizeof(a)
+    for name, _ in kind._fields_:
+        if name.endswith("_stride"):
+            getattr(a, name)[:] = (1024, 256, 64, 1)
+            setattr(a, name[:-7], 0x1000)
+    a.z, a.heads, a.key_heads, a.t, a.n, a.head_dim, a.sm_scale = 2, 4, 2, 4, 40, 64, 1.0
+    if kind is _native.CrossBwdArgs:
+        a.lse = 0x1000
+    for k, v in over.items():
+        setattr(a, k, v)
+    return a
+
+
+CALLS = [("rsfa_cross_fwd", _native.CrossArgs), ("rsfa_cross_bwd", _native.CrossBwdArgs)]
+
+
+@pytest.mark.parametrize("name,kind", CALLS)
+def test_abi_refusals(name, kind):
+    lib = _native.lib()
+    f = lambda **k: getattr(lib, name)(ctypes.byref(_args(kind, **k)), None)  # noqa: E731
+    size = lambda **k: getattr(lib, name + "_workspace_bytes")(ctypes.byref(_args(kind, **k)))  # noqa: E731
+    assert getattr(lib, name)(None, None) == _native.E_NULL
+    assert f(struct_size=8) == _native.E_ABI and size(struct_size=8) == 0
+    assert f(dtype=2) == f(dtype=3) == f(dtype=-1) == _native.E_DTYPE
+    for over in ({"z": 0}, {"heads": 0}, {"heads": 3}, {"key_heads": 0}, {"t": 0}, {"n": 0}, {"t": 1 << 29}, {"n": 1 << 31}, {"head_dim": 16},
+                 {"head_dim": 96}, {"z": 1 << 25}, {"heads": 1 << 24}, {"t": -1}, {"heads": 256, "key_heads": 1, "t": 1 << 21}):
+        assert f(**over) == _native.E_CROSS and size(**over) == 0, over
+    for p in ("q", "k", "v", "o"):
+        assert f(**{p: None}) == _native.E_NULL and f(**{p: 0x1008}) == _native.E_ALIGN
+        for st in ((1024, 256, 64, 2), (1024, 256, 65, 1), (-1024, 256, 64, 1), (1024, 4, 64, 1), (1024, 256, 1 << 25, 1)):
+            assert f(**{p + "_stride": (ctypes.c_int64 * 4)(*st)}) == _native.E_ALIGN
+    assert f(lse=0x1002) == f(lengths=0x1001) == _native.E_ALIGN
+    need = size(z=1, heads=1, key_heads=1, t=4, n=100000)
+    assert need > 0
+    small = {"z": 1, "heads": 1, "key_heads": 1, "t": 4, "n": 100000}
+    assert f(**small) == f(**small, workspace=0x1000, workspace_bytes=need - 1) == _native.E_WORKSPACE
+    assert f(**small, workspace=0x1008, workspace_bytes=need) == _native.E_ALIGN
+
+
+def test_backward_abi_refusals():
+    f = lambda **k: _native.lib().rsfa_cross_bwd(ctypes.byref(_args(_native.CrossBwdArgs, **k)), None)  # noqa: E731
+    assert f(lse=None) == f(grad_o=None) == _native.E_NULL
+    assert f(grad_lse=0x1002) == f(grad_o=0x1008) == f(grad_q=0x1008) == f(grad_k=0x1004) == f(grad_v=0x1001) == _native.E_ALIGN
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros((1, 1, 4, 64), dtype=torch.float16)
+    with pytest.raises(ValueError, match="GPU"):
+        cross_attention(x, x, x, 1.0)
+
+
+def test_the_definitions_gradients_against_differences():
+    g = torch.Generator().manual_seed(0)
+    q, k, v, go = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((2, 4, 3, 4), (2, 2, 5, 4), (2, 2, 5, 4), (2, 4, 3, 4)))
+    glse = torch.randn((2, 4, 3), generator=g, dtype=torch.float64)
+    lengths = [5, 3]
+    want = O.expect(q, k, v, lengths, 0.7, go, glse)
+    for i, name in enumerate(("dq", "dk", "dv")):
+        for at in range(0, (q, k, v)[i].numel(), 3):
+            def value(step):
+                x = [q, k, v]
+                x[i] = x[i].clone()
+                x[i].view(-1)[at] += step
+                o, lse = O.attend(*x, lengths, 0.7)
+                return float((o * go).sum() + (lse * glse).sum())
+
+            slope = (value(1e-5) - value(-1e-5)) / 2e-5
+            assert abs(slope - float(want[name][0].view(-1)[at])) < 1e-8
