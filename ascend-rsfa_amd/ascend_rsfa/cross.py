@@ -23,11 +23,14 @@ __all__ = ["cross_attention"]
 _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16}
 _HEAD_DIMS = (32, 64, 128, 256)
 
-# The argument struct is joined from a part that the tensors' shapes settle, kept by them, and packed addresses.
-_SIZES, _LENGTHS, _PTRS = (getattr(_native.CrossArgs, f).offset for f in ("z", "lengths", "q"))
+# An argument struct is joined from a part that the tensors' shapes settle, kept by them (`_PLANS`), and packed addresses:
+# a call's checks and sizes are then one lookup.
+_F, _B = _native.CrossArgs, _native.CrossBwdArgs
 _FWD_PTRS = struct.Struct("=5Q")  # q, k, v, o, lse
-_FWD_TAIL = struct.Struct("=QfIQQ")  # lengths, sm_scale, reserved, workspace, its bytes
-assert _SIZES - _PTRS == _FWD_PTRS.size and ctypes.sizeof(_native.CrossArgs) - _LENGTHS == _FWD_TAIL.size
+_BWD_PTRS = struct.Struct("=10Q")  # q, k, v, o, lse, grad_o, grad_lse, grad_q, grad_k, grad_v
+_TAIL = struct.Struct("=QfIQQ")  # lengths, sm_scale, reserved, workspace, its bytes
+assert _F.z.offset - _F.q.offset == _FWD_PTRS.size and ctypes.sizeof(_F) - _F.lengths.offset == _TAIL.size
+assert _B.z.offset - _B.q.offset == _BWD_PTRS.size and ctypes.sizeof(_B) - _B.lengths.offset == _TAIL.size
 _PLANS = {}
 _FUNCTIONS = {}
 
@@ -40,15 +43,18 @@ def _function(name):
     return fn
 
 
-def _on_device(device, fn, *args):
-    if device.index == torch.cuda.current_device():
+def _on_device(index, fn, *args):
+    if index == torch.cuda.current_device():
         return fn(*args)
-    with torch.cuda.device(device):
+    with torch.cuda.device(index):
         return fn(*args)
 
 
-def _call(device, name, args):
-    _raise_for(_on_device(device, _function(name), args, torch._C._cuda_getCurrentRawStream(device.index)))
+def _keep(key, plan):
+    if len(_PLANS) > 4096:
+        _PLANS.clear()
+    _PLANS[key] = plan
+    return plan
 
 
 def _empty_rows(t):
@@ -57,65 +63,78 @@ def _empty_rows(t):
     return o if _meets_contract(o) else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
+def _sizes(args, q, k):
+    args.struct_size, args.dtype = ctypes.sizeof(args), _DTYPES[q.dtype]
+    args.z, args.heads, args.t, args.head_dim = q.shape
+    args.key_heads, args.n = k.shape[1], k.shape[2]
+
+
 def _forward(q, k, v, scale, lengths, want_lse):
     """(o, lse or None) of checked tensors in the kernels' layout."""
-    o = _empty_rows(q)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
-    if o.numel() == 0:
-        return o, lse
-    if k.shape[2] == 0:
-        return o.zero_(), lse.fill_(-math.inf) if want_lse else None
     key = (q.shape, k.shape, q.stride(), k.stride(), v.stride(), q.dtype, q.device)
     plan = _PLANS.get(key)
     if plan is None:
-        args = _native.CrossArgs()
-        args.struct_size, args.dtype = ctypes.sizeof(args), _DTYPES[q.dtype]
-        args.z, args.heads, args.t, args.head_dim = q.shape
-        args.key_heads, args.n = k.shape[1], k.shape[2]
+        o = _empty_rows(q)
+        if o.numel() == 0 or k.shape[2] == 0:
+            o.zero_()
+            return o, torch.full(q.shape[:3], -math.inf, dtype=torch.float32, device=q.device) if want_lse else None
+        args = _F()
+        _sizes(args, q, k)
         for name, t in (("q_stride", q), ("k_stride", k), ("v_stride", v), ("o_stride", o)):
             getattr(args, name)[:] = t.stride()
-        nbytes = _on_device(q.device, _native.lib().rsfa_cross_fwd_workspace_bytes, ctypes.byref(args))
+        nbytes = _on_device(q.device.index, _native.lib().rsfa_cross_fwd_workspace_bytes, ctypes.byref(args))
         b = bytes(args)
-        if len(_PLANS) > 4096:
-            _PLANS.clear()
-        plan = _PLANS[key] = (b[:_PTRS], b[_SIZES:_LENGTHS], nbytes)
-    head, sizes, nbytes = plan
+        plan = _keep(key, (b[:_F.q.offset], b[_F.z.offset:_F.lengths.offset], nbytes, o.stride() == torch.empty_like(q).stride()))
+    else:
+        o = torch.empty_like(q) if plan[3] else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    head, sizes, nbytes, _ = plan
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _call(q.device, "rsfa_cross_fwd", b"".join((
-        head, _FWD_PTRS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if want_lse else 0), sizes,
-        _FWD_TAIL.pack(0 if lengths is None else lengths.data_ptr(), scale, 0, ws.data_ptr() if nbytes else 0, nbytes))))
+    args = b"".join((head, _FWD_PTRS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if want_lse else 0),
+                     sizes, _TAIL.pack(0 if lengths is None else lengths.data_ptr(), scale, 0, ws.data_ptr() if nbytes else 0, nbytes)))
+    dev = q.device.index
+    _raise_for(_on_device(dev, _function("rsfa_cross_fwd"), args, torch._C._cuda_getCurrentRawStream(dev)))
     return o, lse
 
 
 def _backward(q, k, v, o, lse, go, glse, scale, lengths, needs):
     """The gradients of q, k and v, those that ``needs`` names (None for the others)."""
-    grads = [_empty_rows(t) if need else None for t, need in zip((q, k, v), needs)]
     if q.numel() == 0 or k.shape[2] == 0:
-        return [g if g is None else g.zero_() for g in grads]
-    go = torch.zeros_like(o) if go is None else _as_kernel_layout(go)
+        return [torch.zeros_like(t) if need else None for t, need in zip((q, k, v), needs)]
+    if go is None:
+        go = torch.zeros_like(o)
     if glse is not None:
         glse = glse.contiguous()
-    args = _native.CrossBwdArgs()
-    args.struct_size, args.dtype = ctypes.sizeof(args), _DTYPES[q.dtype]
-    args.z, args.heads, args.t, args.head_dim = q.shape
-    args.key_heads, args.n = k.shape[1], k.shape[2]
-    for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("grad_o", go), ("grad_q", grads[0]), ("grad_k", grads[1]), ("grad_v", grads[2])):
-        if t is not None:
-            setattr(args, name, t.data_ptr())
-            getattr(args, name + "_stride")[:] = t.stride()
-    args.lse = lse.data_ptr()
-    args.grad_lse = None if glse is None else glse.data_ptr()
-    args.lengths = None if lengths is None else lengths.data_ptr()
-    args.sm_scale = scale
-    nbytes = _on_device(q.device, _native.lib().rsfa_cross_bwd_workspace_bytes, ctypes.byref(args))
+    key = (q.shape, k.shape, q.stride(), k.stride(), v.stride(), go.stride(), q.dtype, q.device, needs)
+    plan = _PLANS.get(key)
+    if plan is None or go.data_ptr() & 15:
+        go_ = _as_kernel_layout(go)
+        grads = [_empty_rows(t) if need else None for t, need in zip((q, k, v), needs)]
+        args = _B()
+        _sizes(args, q, k)
+        for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("grad_o", go_), ("grad_q", grads[0]), ("grad_k", grads[1]),
+                        ("grad_v", grads[2])):
+            if t is not None:
+                getattr(args, name + "_stride")[:] = t.stride()
+        nbytes = _on_device(q.device.index, _native.lib().rsfa_cross_bwd_workspace_bytes, ctypes.byref(args))
+        b = bytes(args)
+        plan = (b[:_B.q.offset], b[_B.z.offset:_B.lengths.offset], nbytes)
+        if go_ is go and all(g is None or g.stride() == torch.empty_like(t).stride() for g, t in zip(grads, (q, k, v))):
+            _keep(key, plan)
+        go = go_
+    else:
+        grads = [torch.empty_like(t) if need else None for t, need in zip((q, k, v), needs)]
+    head, sizes, nbytes = plan
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    args.workspace, args.workspace_bytes = ws.data_ptr(), nbytes
-    _raise_for(_on_device(q.device, _native.lib().rsfa_cross_bwd, ctypes.byref(args),
-                          torch._C._cuda_getCurrentRawStream(q.device.index)))
+    ptrs = [0 if t is None else t.data_ptr() for t in (q, k, v, o, lse, go, glse, *grads)]
+    args = b"".join((head, _BWD_PTRS.pack(*ptrs), sizes,
+                     _TAIL.pack(0 if lengths is None else lengths.data_ptr(), scale, 0, ws.data_ptr(), nbytes)))
+    dev = q.device.index
+    _raise_for(_on_device(dev, _function("rsfa_cross_bwd"), args, torch._C._cuda_getCurrentRawStream(dev)))
     return grads
 
 
-def _check(q, k, v, sm_scale, lengths):
+def _check(q, k, v, lengths):
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
         raise ValueError(f"q must be [Z, heads, T, D], k and v [Z, key heads, N, D]; got {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")
@@ -129,8 +148,6 @@ def _check(q, k, v, sm_scale, lengths):
         raise TypeError(f"unsupported dtype {q.dtype}; float16 and bfloat16 are supported")
     if not q.is_cuda or not (q.device == k.device == v.device):
         raise ValueError("q, k and v must be GPU tensors on one device")
-    if math.isnan(sm_scale):
-        raise ValueError("sm_scale is NaN")
     if lengths is not None:
         if not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or lengths.shape != q.shape[:1]:
             raise TypeError(f"lengths must be an int32 tensor [{q.shape[0]}]")
@@ -175,11 +192,20 @@ def cross_attention(q, k, v, sm_scale, lengths=None, *, return_lse=False):
     have gradients of 0.
     """
     sm_scale = float(sm_scale)
-    _check(q, k, v, sm_scale, lengths)
-    if lengths is not None:
-        lengths = lengths.contiguous()
-    q, k, v = (t if t.numel() == 0 else _as_kernel_layout(t) for t in (q, k, v))
-    if _has_tangent(q, k, v) or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+    if math.isnan(sm_scale):
+        raise ValueError("sm_scale is NaN")
+    # tensors with a key that is kept have passed the checks, and only their addresses may differ
+    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device, v.device,
+           (lengths.shape, lengths.stride(), lengths.dtype, lengths.device) if isinstance(lengths, torch.Tensor) else lengths is None)
+    if key not in _PLANS or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        _check(q, k, v, lengths)
+        if lengths is not None:
+            lengths = lengths.contiguous()
+        tensors = [t if t.numel() == 0 else _as_kernel_layout(t) for t in (q, k, v)]
+        if tensors[0] is q and tensors[1] is k and tensors[2] is v and (lengths is None or lengths.stride() == key[-1][1]):
+            _keep(key, True)
+        q, k, v = tensors
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _has_tangent(q, k, v):
         o, lse = _CrossAttention.apply(q, k, v, sm_scale, lengths)
     else:
         o, lse = _forward(q, k, v, sm_scale, lengths, return_lse)

@@ -3,9 +3,9 @@
 //   P = exp(s q k^T - lse),  dV = P^T dO,  dS = P (dO V^T - delta),  dQ = s dS K,  dK = s dS^T Q
 //   delta = rowsum(dO o) - dlse
 //
-// Three kernels: the rows' statistics; dK and dV, whose workgroups hold a block of keys and pass over the rows of
-// their key head (all query heads of its group, so shared heads need no second sum); dQ, whose workgroups hold a block
-// of rows and pass over the keys.  Both pass kernels form S and dO V^T, which makes seven matrix products where
+// Two kernels: dQ, whose workgroups hold a block of rows, form its delta and pass over the keys; then dK and dV, whose
+// workgroups hold a block of keys and pass over the rows of their key head (all query heads of its group, so
+// shared heads need no second sum).  Both form S and dO V^T, which makes seven matrix products where
 // one kernel would have five, but every sum has one owner and one order: no atomics, the same bits in each call,
 // and no traffic for dQ's partial sums, which one kernel would add up in memory once per key block.
 // Where blocks are too few for the chip each pass is cut into parts, which sum_parts_kernel adds up.
@@ -61,37 +61,6 @@ __device__ __forceinline__ void dma4(const void* sbase, uint32_t voff_bytes, uin
                  :
                  : "v"(voff_bytes), "s"(sbase), "{m0}"(lds_addr)
                  : "memory");
-}
-
-// Statistics of the rows: D / 8 lanes a row.  Bound by memory: 4 D bytes a row.
-template <class T, int D>
-__global__ void __launch_bounds__(256) cross_stats_kernel(BwdParams p) {
-    typedef typename T::x8 x8;
-    typedef typename T::elem elem;
-    constexpr int LANES = D / 8;
-    const int64_t id = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const int lane = threadIdx.x % LANES;
-    const int64_t zh = id / p.tp;
-    if (zh >= (int64_t)p.z * p.heads) return;
-    const int row = (int)(id - zh * p.tp), z = (int)(zh / p.heads), h = (int)(zh - (int64_t)z * p.heads);
-    float sum = 0.0f;
-    if (row < p.t) {
-        const x8 a = *(const x8*)((const elem*)p.o + z * p.o_st[0] + h * p.o_st[1] + row * p.o_st[2] + 8 * lane);
-        const x8 b = *(const x8*)((const elem*)p.go + z * p.go_st[0] + h * p.go_st[1] + row * p.go_st[2] + 8 * lane);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf((float)a[i], (float)b[i], sum);
-    }
-#pragma unroll
-    for (int d = 1; d < LANES; d <<= 1) sum += __shfl_xor(sum, d);
-    if (lane) return;
-    float nl = -INFINITY, nd = 0.0f;
-    if (row < p.t) {
-        const int64_t at = zh * p.t + row;
-        nl = -(p.lse[at] * LOG2E) / p.c;
-        nd = (p.glse ? p.glse[at] : 0.0f) - sum;
-    }
-    p.nl[id] = nl;
-    p.nd[id] = nd;
 }
 
 // Tiles of rows in LDS have the forward kernel's layout (fa_fwd_kernel.hpp): 16-row blocks of planes of 32 columns,
@@ -153,18 +122,53 @@ __device__ __forceinline__ void pack(const f32x16& x, typename T::x8 (&b)[2]) {
         }
 }
 
-// A row of a transposed accumulator: lane l holds row l % 32, values 32 d + 8 a + 4 (l / 32) + e.
+// A wave's 32 rows from `base` on into LDS of its own (rows behind the last of `left` repeat it), by direct loads of 16 rows x 64 bytes.
+template <int D, class E>
+__device__ __forceinline__ void load_rows(const E* base, int64_t st, int left, const Lane& w, uint32_t to) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const int r0 = min(16 * b, left - 1);
+        const uint32_t off = (uint32_t)(((min(r0 + w.ld_row, left - 1) - r0) * st + w.ld_col) * 2);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) dma16(base + r0 * st + 32 * c, off, to + b * (32 * D) + c * 1024);
+    }
+}
+
+// Those rows as operands: lane l has row l % 32, values 16 s + 8 (l / 32) ...
 template <class T, int D>
-__device__ __forceinline__ void store_row(typename T::elem* dst, const f32x16 (&acc)[D / 32], float f, int hh) {
+__device__ __forceinline__ void fragments(const RSFA_LDS char* at, const Lane& w, typename T::x8 (&f)[D / 16]) {
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d)
+    for (int s = 0; s < D / 16; ++s) f[s] = *(const RSFA_LDS typename T::x8*)(at + w.koff[s & 1] + (s >> 1) * 1024);
+}
+
+// The 32 rows of a wave's transposed accumulator (lane l holds row l % 32, values 32 d + 8 a + 4 (l / 32) + e), times f, to
+// memory, through LDS of its own: stored from the accumulator, every instruction would write 32 rows x 16 bytes, at 64 cycles
+// of the address unit each; so a row's chunks of 16 bytes lie side by side.  Rows from `left` on are not written.
+template <class T, int D>
+__device__ __forceinline__ void store_rows(typename T::elem* dst, int64_t st, int left, const f32x16 (&acc)[D / 32], float f,
+                                           const Lane& w, RSFA_LDS char* at) {
+    typedef typename T::x8 x8;
+    constexpr int COLS = D == 256 ? 128 : D;  // at once (all of D = 256 would not fit the wave's share)
+    constexpr int PITCH = 2 * COLS + 16, CH = COLS / 8, EACH = 64 / CH;
+    const int r0 = w.lane / CH, c = w.lane % CH;
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            typename T::x4 v;
+    for (int part = 0; part < D / COLS; ++part) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (typename T::elem)(acc[d][4 * a + e] * f);
-            *(typename T::x4*)(dst + 32 * d + 8 * a + 4 * hh) = v;
+        for (int d = 0; d < COLS / 32; ++d)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                typename T::x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (typename T::elem)(acc[part * (COLS / 32) + d][4 * a + e] * f);
+                *(RSFA_LDS typename T::x4*)(at + w.l32 * PITCH + (32 * d + 8 * a + 4 * w.hh) * 2) = v;
+            }
+#pragma unroll
+        for (int i = 0; i < 32 / EACH; ++i) {
+            const int r = i * EACH + r0;
+            const x8 v = *(const RSFA_LDS x8*)(at + r * PITCH + c * 16);
+            if (r < left) *(x8*)(dst + r * st + part * COLS + 8 * c) = v;
         }
+    }
 }
 
 template <int D>
@@ -182,15 +186,17 @@ __device__ __forceinline__ void store_part(float* dst, const f32x16 (&acc)[D / 3
 template <int D>
 struct Bwd {
     static constexpr int TILE_ROWS = D == 256 ? 32 : 64;
-    static constexpr int OCC = D == 256 ? 1 : D == 32 ? 4 : 2;  // waves of a SIMD
+    static constexpr int DKV_OCC = D == 256 ? 1 : D == 32 ? 4 : D == 64 ? 3 : 2;  // waves of a SIMD
+    static constexpr int DQ_OCC = D == 256 ? 1 : D <= 64 ? 4 : 2;
 };
 
 template <class T, int D>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Bwd<D>::OCC, Bwd<D>::OCC)))
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Bwd<D>::DKV_OCC, Bwd<D>::DKV_OCC)))
 cross_dkv_kernel(BwdParams p) {
     typedef typename T::x8 x8;
     typedef typename T::elem elem;
     constexpr int QB = Bwd<D>::TILE_ROWS, BLK = 32 * D, TILE = QB * D * 2, STATS = 512, BUF = 2 * TILE + STATS;
+    constexpr int TWO = QB == 64 ? 64 * D : 0;  // where a wave's second 32 rows lie in the LDS of its prologue
     constexpr int DT = D / 32, KST = D / 16;
     __shared__ __attribute__((aligned(1024))) char smem_raw[2 * BUF];
     RSFA_LDS char* const smem = (RSFA_LDS char*)smem_raw;
@@ -208,21 +214,25 @@ cross_dkv_kernel(BwdParams p) {
     const int each = (all + p.splits - 1) / p.splits;
     int i = min((int)blockIdx.y * each, all);
     const int end = block * 128 < nk ? min(i + each, all) : i;  // (no key: no pass)
-    const bool mine = block * 128 + wave * 32 < nk;             // the wave has a key
-
+    const bool mine = i < end && block * 128 + wave * 32 < nk;  // the wave has work
+    const int first = block * 128 + wave * 32;  // the wave's first key
+    RSFA_LDS char* const own = smem + wave * TILE;
     x8 kf[KST], vf[KST];
-    {
-        const int row = max(0, min(key, nk - 1));
-        const elem* kp = (const elem*)p.k + z * p.k_st[0] + h * p.k_st[1] + row * p.k_st[2] + 8 * w.hh;
-        const elem* vp = (const elem*)p.v + z * p.v_st[0] + h * p.v_st[1] + row * p.v_st[2] + 8 * w.hh;
-#pragma unroll
-        for (int s = 0; s < KST; ++s) {
-            kf[s] = __builtin_bit_cast(x8, *(const u32x4*)(kp + 16 * s) ^ p.neg);
-            vf[s] = *(const x8*)(vp + 16 * s);
+    if (mine) {
+        load_rows<D>((const elem*)p.k + z * p.k_st[0] + h * p.k_st[1] + first * p.k_st[2], p.k_st[2], nk - first, w, smem_addr + wave * TILE);
+        if constexpr (TWO == 0) {  // (one after the other through the same place)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            fragments<T, D>(own, w, kf);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
+        load_rows<D>((const elem*)p.v + z * p.v_st[0] + h * p.v_st[1] + first * p.v_st[2], p.v_st[2], nk - first, w, smem_addr + wave * TILE + TWO);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (TWO != 0) fragments<T, D>(own, w, kf);
+        fragments<T, D>(own + TWO, w, vf);
 #pragma unroll
-        for (int s = 0; s < KST; ++s) asm volatile("" : "+v"(kf[s]), "+v"(vf[s]));  // (here, ahead of the direct loads)
+        for (int s = 0; s < KST; ++s) kf[s] = __builtin_bit_cast(x8, __builtin_bit_cast(u32x4, kf[s]) ^ p.neg);
     }
+    __syncthreads();  // (the tiles go where these rows were)
     f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -291,7 +301,6 @@ cross_dkv_kernel(BwdParams p) {
             columns_product<T, D>(qt + st * 2 * BLK, w, b, dk);
         }
     }
-    if (key >= p.n) return;
     if (p.splits > 1) {
         if (key >= nk) return;  // (the sum of the parts writes 0 there)
         const int64_t at = (((int64_t)blockIdx.y * p.z * p.key_heads + kh) * p.n + key) * D;
@@ -305,18 +314,20 @@ cross_dkv_kernel(BwdParams p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
     }
-    if (p.gk) store_row<T, D>((elem*)p.gk + z * p.gk_st[0] + h * p.gk_st[1] + key * p.gk_st[2], dk, p.scale, w.hh);
-    if (p.gv) store_row<T, D>((elem*)p.gv + z * p.gv_st[0] + h * p.gv_st[1] + key * p.gv_st[2], dv, 1.0f, w.hh);
+    __syncthreads();  // (every wave is done with the tiles)
+    if (p.gk) store_rows<T, D>((elem*)p.gk + z * p.gk_st[0] + h * p.gk_st[1] + first * p.gk_st[2], p.gk_st[2], p.n - first, dk, p.scale, w, own);
+    if (p.gv) store_rows<T, D>((elem*)p.gv + z * p.gv_st[0] + h * p.gv_st[1] + first * p.gv_st[2], p.gv_st[2], p.n - first, dv, 1.0f, w, own);
 }
 
 // dQ of 128 rows, 32 of each wave, held transposed (dQ^T = K^T dS^T), rows in the lanes: a row's
 // statistics are one register each.  Q and dO of the wave stay in registers; tiles of K and V pass through LDS.
 template <class T, int D>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Bwd<D>::OCC, Bwd<D>::OCC)))
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Bwd<D>::DQ_OCC, Bwd<D>::DQ_OCC)))
 cross_dq_kernel(BwdParams p) {
     typedef typename T::x8 x8;
     typedef typename T::elem elem;
     constexpr int KB = Bwd<D>::TILE_ROWS, BLK = 32 * D, TILE = KB * D * 2, BUF = 2 * TILE;
+    constexpr int TWO = KB == 64 ? 64 * D : 0;  // where a wave's second 32 rows lie in the LDS of its prologue
     constexpr int DT = D / 32, KST = D / 16;
     __shared__ __attribute__((aligned(1024))) char smem_raw[2 * BUF];
     RSFA_LDS char* const smem = (RSFA_LDS char*)smem_raw;
@@ -335,26 +346,62 @@ cross_dq_kernel(BwdParams p) {
 
     const int all = (nk + KB - 1) / KB, each = (all + p.splits - 1) / p.splits;
     int i = min((int)blockIdx.y * each, all);
-    const int end = min(i + each, all);
+    const int end = p.gq ? min(i + each, all) : i;  // (without dQ the statistics are all there is to do)
 
+    const int first = block * 128 + wave * 32;  // the wave's first row
+    RSFA_LDS char* const own = smem + wave * TILE;
     x8 qf[KST], gf[KST];
-    float l2, nd;
-    {
-        const int r = min(row, p.t - 1);
-        const elem* qp = (const elem*)p.q + z * p.q_st[0] + hq * p.q_st[1] + r * p.q_st[2] + 8 * w.hh;
-        const elem* gp = (const elem*)p.go + z * p.go_st[0] + hq * p.go_st[1] + r * p.go_st[2] + 8 * w.hh;
-#pragma unroll
-        for (int s = 0; s < KST; ++s) {
-            qf[s] = __builtin_bit_cast(x8, *(const u32x4*)(qp + 16 * s) ^ p.neg);
-            gf[s] = *(const x8*)(gp + 16 * s);
+    float l2 = 0.0f, nd = 0.0f;
+    if (mine) {
+        const int64_t head = (int64_t)z * p.heads + hq;
+        const int left = p.t - first;
+        load_rows<D>((const elem*)p.q + z * p.q_st[0] + hq * p.q_st[1] + first * p.q_st[2], p.q_st[2], left, w, smem_addr + wave * TILE);
+        if constexpr (TWO == 0) {  // (one after the other through the same place)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            fragments<T, D>(own, w, qf);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        const int64_t at = (int64_t)z * p.heads + hq;
-        l2 = p.lse[at * p.t + r] * LOG2E;
-        nd = p.nd[at * p.tp + r];
+        load_rows<D>((const elem*)p.go + z * p.go_st[0] + hq * p.go_st[1] + first * p.go_st[2], p.go_st[2], left, w, smem_addr + wave * TILE + TWO);
+        // o comes as the direct loads bring dO: lane l has chunk l % 4 (swizzled) of row l / 4 of a plane
+        const elem* ob = (const elem*)p.o + z * p.o_st[0] + hq * p.o_st[1] + first * p.o_st[2] + w.ld_col;
+        x8 o[2][D / 32];
 #pragma unroll
-        for (int s = 0; s < KST; ++s) asm volatile("" : "+v"(qf[s]), "+v"(gf[s]));
-        asm volatile("" : "+v"(l2), "+v"(nd));
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) o[b][c] = *(const x8*)(ob + min(16 * b + w.ld_row, left - 1) * p.o_st[2] + 32 * c);
+        const int row_c = min(row, p.t - 1);
+        l2 = p.lse[head * p.t + row_c] * LOG2E;
+        const float gl = p.glse ? p.glse[head * p.t + row_c] : 0.0f;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (TWO != 0) fragments<T, D>(own, w, qf);
+        fragments<T, D>(own + TWO, w, gf);
+#pragma unroll
+        for (int s = 0; s < KST; ++s) qf[s] = __builtin_bit_cast(x8, __builtin_bit_cast(u32x4, qf[s]) ^ p.neg);
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                const x8 gr = *(const RSFA_LDS x8*)(own + TWO + b * BLK + c * 1024 + w.lane * 16);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[b] = __builtin_fmaf((float)o[b][c][e], (float)gr[e], sum[b]);
+            }
+            sum[b] += __shfl_xor(sum[b], 1);
+            sum[b] += __shfl_xor(sum[b], 2);
+        }
+        const float s0 = __shfl(sum[0], 4 * w.l16), s1 = __shfl(sum[1], 4 * w.l16);
+        nd = gl - (w.l32 < 16 ? s0 : s1);
+        // for dK and dV: rows behind the last have weights of 0
+        if (blockIdx.y == 0 && w.hh == 0 && row < p.tp) {
+            p.nl[head * p.tp + row] = row < p.t ? -l2 / p.c : -INFINITY;
+            p.nd[head * p.tp + row] = row < p.t ? nd : 0.0f;
+        }
+    } else if (blockIdx.y == 0 && w.hh == 0 && row < p.tp) {
+        p.nl[((int64_t)z * p.heads + hq) * p.tp + row] = -INFINITY;
+        p.nd[((int64_t)z * p.heads + hq) * p.tp + row] = 0.0f;
     }
+    if (!p.gq) return;
+    __syncthreads();  // (the tiles go where these rows were)
     f32x16 dq[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -407,13 +454,14 @@ cross_dq_kernel(BwdParams p) {
             columns_product<T, D>(kt + st * 2 * BLK, w, b, dq);
         }
     }
-    if (row >= p.t) return;
     if (p.splits > 1) {
+        if (row >= p.t) return;
         const int64_t rows = (int64_t)p.z * p.heads * p.t;
         store_part<D>(p.part[0] + (blockIdx.y * rows + ((int64_t)z * p.heads + hq) * p.t + row) * D, dq, w.hh);
         return;
     }
-    store_row<T, D>((elem*)p.gq + z * p.gq_st[0] + hq * p.gq_st[1] + row * p.gq_st[2], dq, p.scale, w.hh);
+    __syncthreads();  // (every wave is done with the tiles)
+    store_rows<T, D>((elem*)p.gq + z * p.gq_st[0] + hq * p.gq_st[1] + first * p.gq_st[2], p.gq_st[2], p.t - first, dq, p.scale, w, own);
 }
 
 // Sums of parts: D / 4 lanes a row; rows past their sequence's length (dK, dV) become 0.
@@ -452,16 +500,16 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(SumParams a, SumParams b
 // Host
 // ---------------------------------------------------------------------------
 struct Functions {
-    const void *stats, *dkv, *dq, *sum;
+    const void *dkv, *dq, *sum;
 };
 
 template <class T>
 Functions functions(int64_t d) {
     switch (d) {
-        case 32: return {(const void*)&cross_stats_kernel<T, 32>, (const void*)&cross_dkv_kernel<T, 32>, (const void*)&cross_dq_kernel<T, 32>, (const void*)&sum_parts_kernel<T, 32>};
-        case 64: return {(const void*)&cross_stats_kernel<T, 64>, (const void*)&cross_dkv_kernel<T, 64>, (const void*)&cross_dq_kernel<T, 64>, (const void*)&sum_parts_kernel<T, 64>};
-        case 128: return {(const void*)&cross_stats_kernel<T, 128>, (const void*)&cross_dkv_kernel<T, 128>, (const void*)&cross_dq_kernel<T, 128>, (const void*)&sum_parts_kernel<T, 128>};
-        default: return {(const void*)&cross_stats_kernel<T, 256>, (const void*)&cross_dkv_kernel<T, 256>, (const void*)&cross_dq_kernel<T, 256>, (const void*)&sum_parts_kernel<T, 256>};
+        case 32: return {(const void*)&cross_dkv_kernel<T, 32>, (const void*)&cross_dq_kernel<T, 32>, (const void*)&sum_parts_kernel<T, 32>};
+        case 64: return {(const void*)&cross_dkv_kernel<T, 64>, (const void*)&cross_dq_kernel<T, 64>, (const void*)&sum_parts_kernel<T, 64>};
+        case 128: return {(const void*)&cross_dkv_kernel<T, 128>, (const void*)&cross_dq_kernel<T, 128>, (const void*)&sum_parts_kernel<T, 128>};
+        default: return {(const void*)&cross_dkv_kernel<T, 256>, (const void*)&cross_dq_kernel<T, 256>, (const void*)&sum_parts_kernel<T, 256>};
     }
 }
 
@@ -542,37 +590,32 @@ int rsfa_cross_bwd(const rsfa_cross_bwd_args* a, void* stream) {
     p.nl = (float*)(ws + plan.nl), p.nd = (float*)(ws + plan.nd);
     const int64_t d = a->head_dim, kh = a->z * a->key_heads, qh = a->z * a->heads;
     const Functions fn = a->dtype == RSFA_DTYPE_BF16 ? functions<TypeBF16>(d) : functions<TypeF16>(d);
-    const int64_t stat_blocks = (qh * plan.tp + 2048 / d - 1) / (2048 / d);
     const int64_t dkv_blocks = kh * plan.key_blocks, dq_blocks = qh * plan.row_blocks;
     const int64_t per = 1024 / d, sum_k = (kh * a->n + per - 1) / per, sum_q = (qh * a->t + per - 1) / per;
-    if (std::max({stat_blocks, dkv_blocks, dq_blocks, sum_k, sum_q}) > 0x7fffffff) return RSFA_E_CROSS;
+    if (std::max({dkv_blocks, dq_blocks, sum_k, sum_q}) > 0x7fffffff) return RSFA_E_CROSS;
     auto launch = [&](const void* f, int64_t x, int y, void** args) {
         return hipLaunchKernel(f, dim3((unsigned)x, (unsigned)y), dim3(256), args, 0, (hipStream_t)stream) == hipSuccess;
     };
     void* args[] = {&p};
-    if (!launch(fn.stats, stat_blocks, 1, args)) return RSFA_E_LAUNCH;
-    if (p.gk || p.gv) {
-        p.blocks = (int32_t)plan.key_blocks, p.splits = plan.dkv_splits;
-        for (int i = 0; i < 2; ++i) p.part[i] = (float*)(ws + plan.dkv[i]);
-        if (!launch(fn.dkv, dkv_blocks, p.splits, args)) return RSFA_E_LAUNCH;
-        if (p.splits > 1) {
-            SumParams s[2] = {};
-            int n = 0;
-            if (p.gk) s[n++] = {p.part[0], p.gk, {p.gk_st[0], p.gk_st[1], p.gk_st[2]}, p.lengths, p.key_heads, p.n, p.splits, kh * a->n, p.scale};
-            if (p.gv) s[n++] = {p.part[1], p.gv, {p.gv_st[0], p.gv_st[1], p.gv_st[2]}, p.lengths, p.key_heads, p.n, p.splits, kh * a->n, 1.0f};
-            void* sum_args[] = {&s[0], &s[1]};
-            if (!launch(fn.sum, sum_k, n, sum_args)) return RSFA_E_LAUNCH;
-        }
+    p.blocks = (int32_t)plan.row_blocks, p.splits = p.gq ? plan.dq_splits : 1;
+    p.part[0] = (float*)(ws + plan.dq);
+    if (!launch(fn.dq, dq_blocks, p.splits, args)) return RSFA_E_LAUNCH;
+    if (p.splits > 1) {
+        SumParams s[2] = {{p.part[0], p.gq, {p.gq_st[0], p.gq_st[1], p.gq_st[2]}, nullptr, p.heads, p.t, p.splits, qh * a->t, p.scale}, {}};
+        void* sum_args[] = {&s[0], &s[1]};
+        if (!launch(fn.sum, sum_q, 1, sum_args)) return RSFA_E_LAUNCH;
     }
-    if (p.gq) {
-        p.blocks = (int32_t)plan.row_blocks, p.splits = plan.dq_splits;
-        p.part[0] = (float*)(ws + plan.dq);
-        if (!launch(fn.dq, dq_blocks, p.splits, args)) return RSFA_E_LAUNCH;
-        if (p.splits > 1) {
-            SumParams s[2] = {{p.part[0], p.gq, {p.gq_st[0], p.gq_st[1], p.gq_st[2]}, nullptr, p.heads, p.t, p.splits, qh * a->t, p.scale}, {}};
-            void* sum_args[] = {&s[0], &s[1]};
-            if (!launch(fn.sum, sum_q, 1, sum_args)) return RSFA_E_LAUNCH;
-        }
+    if (!p.gk && !p.gv) return RSFA_OK;
+    p.blocks = (int32_t)plan.key_blocks, p.splits = plan.dkv_splits;
+    for (int i = 0; i < 2; ++i) p.part[i] = (float*)(ws + plan.dkv[i]);
+    if (!launch(fn.dkv, dkv_blocks, p.splits, args)) return RSFA_E_LAUNCH;
+    if (p.splits > 1) {
+        SumParams s[2] = {};
+        int n = 0;
+        if (p.gk) s[n++] = {p.part[0], p.gk, {p.gk_st[0], p.gk_st[1], p.gk_st[2]}, p.lengths, p.key_heads, p.n, p.splits, kh * a->n, p.scale};
+        if (p.gv) s[n++] = {p.part[1], p.gv, {p.gv_st[0], p.gv_st[1], p.gv_st[2]}, p.lengths, p.key_heads, p.n, p.splits, kh * a->n, 1.0f};
+        void* sum_args[] = {&s[0], &s[1]};
+        if (!launch(fn.sum, sum_k, n, sum_args)) return RSFA_E_LAUNCH;
     }
     return RSFA_OK;
 }
