@@ -16,6 +16,16 @@ __device__ __forceinline__ f32x4 mfma16(TypeBF16::x8 a, TypeBF16::x8 b, f32x4 c)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// The head and block of a workgroup.  Workgroups go to the 8 XCDs in turn; the blocks of a head stay on
+// one (where heads divide evenly) and are neighbours in time, so that what all of them pass over is fetched into its L2 once.
+__device__ __forceinline__ void head_block(int heads, int blocks, int& head, int& block) {
+    int i = blockIdx.x, x = 0, step = 1;
+    if (heads % 8 == 0) x = i & 7, i >>= 3, step = 8;
+    const int local = i / blocks;
+    block = i - local * blocks;
+    head = local * step + x;
+}
+
 // Few rows: waves of a workgroup, whose tiles of 32 keys take 256 D bytes of LDS each, and waves of a SIMD.
 template <int D>
 struct Few {

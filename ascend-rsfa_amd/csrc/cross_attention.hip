@@ -32,6 +32,7 @@ struct FewParams {
     const int32_t* lengths;
     int32_t heads, key_heads, group, t, n, bh;   // bh = Z * key heads
     int32_t rows;                                // group * t: row = token * group + head of the group
+    int32_t tiles;                               // row tiles of a key head
     int32_t splits;
     float c;                                     // |sm_scale| * log2 e
     uint32_t neg;                                // sign of sm_scale, as a mask for a pair of q's values
@@ -62,8 +63,9 @@ __global__ void __launch_bounds__(64 * Few<D>::WAVES, Few<D>::OCC) cross_few_ker
     RSFA_LDS char* const smem = (RSFA_LDS char*)smem_raw;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, grp = lane >> 4;
-    const int bh = blockIdx.x % p.bh;  // with a multiple of 8, a head's row tiles meet in one XCD's L2
-    const int row0 = blockIdx.x / p.bh * ROWS;
+    int bh, block;
+    head_block(p.bh, p.tiles, bh, block);
+    const int row0 = block * ROWS;
     const int z = bh / p.key_heads, h = bh - z * p.key_heads;
     const int len = __builtin_amdgcn_readfirstlane(p.lengths ? max(0, min(p.lengths[z], p.n)) : p.n);
     const int chunk = ((len + p.splits - 1) / p.splits + STEP - 1) / STEP * STEP;
@@ -346,14 +348,16 @@ struct Plan {
     uint64_t part_o, part_ml, bytes;
 };
 
-template <class T, int NB>
-const void* few_fn(int64_t d) {
-    switch (d) {
-        case 32: return (const void*)&cross_few_kernel<T, 32, NB>;
-        case 64: return (const void*)&cross_few_kernel<T, 64, NB>;
-        case 128: return (const void*)&cross_few_kernel<T, 128, NB>;
-        default: return (const void*)&cross_few_kernel<T, 256, NB>;
-    }
+template <class T, int D>
+const void* few_fn(int nb) {
+    if constexpr (D < 256)
+        if (nb == 4) return (const void*)&cross_few_kernel<T, D, 4>;
+    return nb == 1 ? (const void*)&cross_few_kernel<T, D, 1> : (const void*)&cross_few_kernel<T, D, 2>;
+}
+
+template <class T>
+const void* few_fn(int64_t d, int nb) {
+    return d == 32 ? few_fn<T, 32>(nb) : d == 64 ? few_fn<T, 64>(nb) : d == 128 ? few_fn<T, 128>(nb) : few_fn<T, 256>(nb);
 }
 
 template <class T>
@@ -368,41 +372,79 @@ const void* join_fn(int64_t d) {
 
 int few_waves(int64_t d) { return d == 256 ? Few<256>::WAVES : Few<128>::WAVES; }
 
-const KernelEntry* find(const rsfa_cross_args* a, int nw, int bn) {
-    const KernelList l = a->dtype == RSFA_DTYPE_BF16 ? kernels_cross_bf16() : kernels_cross_f16();
-    for (int i = 0; i < l.count; ++i)
-        if (l.entries[i].d == a->head_dim && l.entries[i].nw == nw && (!bn || l.entries[i].bn == bn)) return &l.entries[i];
-    return nullptr;
-}
+// What a call takes is read off a model, in microseconds, of launches that pass `steps` tiles of keys; the least of
+// all variants and numbers of parts runs.  Measured on an MI355X in bfloat16, states in turn so that none stays in the last-level cache:
+//   few rows, 16, 32, 64 of them a workgroup: 8 key heads of 8192 keys, D = 128, 16 rows: 51, 68, 107 us, in 16 parts
+//   13, 14, 16; 128 heads of 1531, D = 64: 64 tokens 19, 14, 18, 200 tokens 44, 32, 25, the forward kernel 27;
+//   512 heads of 1500, D = 64: 64 tokens 66, 44, 40, 128 tokens 105, 68, 50, the forward kernel 45.
+//   The forward kernel's 8 and 4 waves: 128 heads of 1024 tokens, 4096 keys, D = 128: 249, 280; 64 heads of 4096
+//   tokens, D = 64: 77 keys 32, 23, 512 keys 52, 46; 16 heads of 200 tokens, 4096 keys, D = 256: 160, 133, in 16 parts 56, 29.
+constexpr double START_US = 4.0, FEW_US = 1.0, JOIN_US = 3.5;
+constexpr double READ_US = 1.0 / 5.3e6, PART_US = 1.0 / 4.0e6;  // a byte of keys; a byte of parts, each way
+struct FewCost {
+    int d, keys, per_cu;  // keys of a step (all waves), workgroups of a CU
+    double step[3];       // 16, 32, 64 rows
+};
+constexpr FewCost few_costs[] = {{32, 128, 4, {0.38, 0.49, 0.82}}, {64, 128, 2, {0.65, 0.78, 1.13}},
+                                 {128, 128, 1, {0.82, 1.00, 1.65}}, {256, 64, 1, {1.30, 1.60, 0.0}}};
+struct ManyCost {
+    int d, nw, bn, per_cu;
+    double task, step, task_shared, step_shared;  // shared: with per_cu workgroups on the CU
+    double full;                                  // factor of a filled launch, at the board's power limit
+};
+constexpr ManyCost many_costs[] = {{32, 4, 64, 4, 0.23, 0.61, 1.25, 0.83, 1.5},  {32, 4, 128, 3, 0.23, 1.10, 1.25, 1.50, 1.5},
+                                   {64, 8, 128, 1, 3.03, 1.49, 3.03, 1.49, 1.5}, {64, 4, 64, 3, 1.07, 0.90, 3.60, 1.30, 1.0},
+                                   {128, 8, 64, 1, 3.00, 1.34, 3.00, 1.34, 1.5}, {128, 4, 64, 2, 2.04, 1.15, 3.44, 1.48, 1.5},
+                                   {256, 8, 32, 1, 4.00, 1.22, 4.00, 1.22, 1.5}, {256, 4, 32, 2, 3.00, 1.00, 4.50, 1.30, 1.5}};
 
 Plan make_plan(const rsfa_cross_args* a) {
     Plan p{};
     const int cus = cross_cus();
-    const int64_t group = a->heads / a->key_heads, rows = group * a->t, bh = a->z * a->key_heads;
-    p.few = rows <= 32 || a->t <= 16;
-    int64_t able = 1, want = 1;
-    if (p.few) {
-        p.nb = rows <= 16 ? 1 : 2;
-        p.tiles = (rows + 16 * p.nb - 1) / (16 * p.nb);
-        const int64_t step = 32 * few_waves(a->head_dim);
-        const int64_t full = 4 * (int64_t)cus;
-        want = (full + bh * p.tiles - 1) / (bh * p.tiles);
-        able = (a->n + 2 * step - 1) / (2 * step);
-    } else {
-        const int64_t heads = a->z * a->heads;
-        const bool large = a->head_dim > 32 && a->t > 128 && heads * ((a->t + 255) / 256) >= cus;
-        p.e = a->head_dim == 32 ? find(a, 4, a->n >= 1024 ? 128 : 64) : find(a, large ? 8 : 4, 0);
-        const int64_t tasks = heads * ((a->t + p.e->bm - 1) / p.e->bm);
-        const int64_t full = p.e->nw == 8 ? cus : 2 * cus;
-        want = full / tasks;
-        able = a->n / 512;
+    const int64_t d = a->head_dim, rows = a->heads / a->key_heads * a->t, bh = a->z * a->key_heads, all = a->z * a->heads * a->t;
+    const double read = 2.0 * 2.0 * (double)bh * a->n * d * READ_US;
+    double best = 0.0;
+    auto take = [&](double us, int64_t workgroups, int splits, bool few, int nb, const KernelEntry* e) {
+        // (some CUs alone do not draw all of the memory's rate; reading and computing overlap for the most part)
+        const double bytes = read / (0.6 + 0.4 * std::min(1.0, (double)workgroups / cus));
+        us = START_US + std::max(us, bytes) + 0.25 * std::min(us, bytes);
+        if (splits > 1) us += JOIN_US + 2.0 * 4.0 * splits * (double)all * d * PART_US;
+        if (best != 0.0 && us >= best) return;
+        best = us;
+        p.few = few, p.nb = nb, p.e = e, p.splits = splits;
+    };
+    const KernelList list = a->dtype == RSFA_DTYPE_BF16 ? kernels_cross_bf16() : kernels_cross_f16();
+    for (int splits = 1; splits <= 64; splits *= 2) {
+        if (splits > 1 && a->n < 128 * (int64_t)splits) break;  // (parts of whole steps)
+        const int64_t keys = (a->n + splits - 1) / splits;
+        for (const FewCost& c : few_costs) {
+            if (c.d != d) continue;
+            for (int i = 0; i < 3 && c.step[i] != 0.0; ++i) {
+                const int nb = 1 << i;
+                if (i && 8 * nb >= rows) break;
+                const int64_t workgroups = bh * ((rows + 16 * nb - 1) / (16 * nb)) * splits;
+                const double alone = FEW_US + c.step[i] * (double)((keys + c.keys - 1) / c.keys), per = (double)workgroups / cus;
+                // a CU's second workgroup and those after it add less than half of the first's time
+                const double shared = alone * (1.0 + 0.45 * (std::min<double>(std::max(per, 1.0), c.per_cu) - 1.0));
+                take(shared * std::max(1.0, std::ceil(per / c.per_cu - 1e-9)), workgroups, splits, true, nb, nullptr);
+            }
+        }
+        for (const ManyCost& c : many_costs) {
+            if (c.d != d) continue;
+            const int64_t tasks = a->z * a->heads * ((a->t + 32 * c.nw - 1) / (32 * c.nw)) * splits;
+            const int64_t conc = std::max<int64_t>(1, std::min<int64_t>(c.per_cu, (tasks + cus - 1) / cus)), slots = cus * conc;
+            const double w = c.per_cu > 1 ? (double)(conc - 1) / (c.per_cu - 1) : 0.0;
+            const double task = c.task + w * (c.task_shared - c.task) + (c.step + w * (c.step_shared - c.step)) * (double)((keys + c.bn - 1) / c.bn);
+            const double us = std::max(task * (double)((tasks + slots - 1) / slots), task * (double)tasks / (double)(cus * c.per_cu) * c.full);
+            for (int i = 0; i < list.count; ++i)
+                if (list.entries[i].d == d && list.entries[i].nw == c.nw && list.entries[i].bn == c.bn)
+                    take(us, tasks, splits, false, 0, &list.entries[i]);
+        }
     }
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, able), 256));
+    p.tiles = p.few ? (rows + 16 * p.nb - 1) / (16 * p.nb) : 0;
     if (p.splits > 1) {
-        const uint64_t all = (uint64_t)a->z * a->heads * a->t;
         p.part_ml = 0;
-        p.part_o = (p.splits * all * 8 + 255) / 256 * 256;
-        p.bytes = p.part_o + p.splits * all * a->head_dim * 4;
+        p.part_o = ((uint64_t)p.splits * all * 8 + 255) / 256 * 256;
+        p.bytes = p.part_o + (uint64_t)p.splits * all * d * 4;
     }
     return p;
 }
@@ -444,13 +486,13 @@ int rsfa_cross_fwd(const rsfa_cross_args* a, void* stream) {
         p.lengths = a->lengths;
         p.heads = (int32_t)a->heads, p.key_heads = (int32_t)a->key_heads, p.group = (int32_t)(a->heads / a->key_heads);
         p.t = (int32_t)a->t, p.n = (int32_t)a->n, p.bh = (int32_t)(a->z * a->key_heads), p.rows = p.group * p.t;
+        p.tiles = (int32_t)plan.tiles;
         p.splits = plan.splits, p.c = c, p.neg = a->sm_scale < 0.0f ? 0x80008000u : 0u;
         p.part_o = part_o, p.part_ml = part_ml;
         const int64_t grid = p.bh * plan.tiles;
         if (grid > 0x7fffffff) return RSFA_E_CROSS;
         void* args[] = {&p};
-        const void* fn = bf16 ? (plan.nb == 1 ? few_fn<TypeBF16, 1>(a->head_dim) : few_fn<TypeBF16, 2>(a->head_dim))
-                              : (plan.nb == 1 ? few_fn<TypeF16, 1>(a->head_dim) : few_fn<TypeF16, 2>(a->head_dim));
+        const void* fn = bf16 ? few_fn<TypeBF16>(a->head_dim, plan.nb) : few_fn<TypeF16>(a->head_dim, plan.nb);
         if (hipLaunchKernel(fn, dim3((unsigned)grid, (unsigned)plan.splits), dim3(64 * few_waves(a->head_dim)), args, 0, (hipStream_t)stream) != hipSuccess)
             return RSFA_E_LAUNCH;
     } else {

@@ -45,16 +45,6 @@ __device__ __forceinline__ int keys_of(const BwdParams& p, int z) {
     return __builtin_amdgcn_readfirstlane(p.lengths ? max(0, min(p.lengths[z], p.n)) : p.n);
 }
 
-// The head and block of a workgroup.  Workgroups go to the 8 XCDs in turn; the blocks of a head stay on
-// one (where heads divide evenly) and are neighbours in time, so that what all of them pass over is fetched into its L2 once.
-__device__ __forceinline__ void head_block(int heads, int blocks, int& head, int& block) {
-    int i = blockIdx.x, x = 0, step = 1;
-    if (heads % 8 == 0) x = i & 7, i >>= 3, step = 8;
-    const int local = i / blocks;
-    block = i - local * blocks;
-    head = local * step + x;
-}
-
 // One wave's direct load of 64 dwords into LDS (dma16's smaller sibling; see there for the s_nop).
 __device__ __forceinline__ void dma4(const void* sbase, uint32_t voff_bytes, uint32_t lds_addr) {
     asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1"

@@ -816,8 +816,13 @@ fa_fwd_kernel(FwdParams p) {
             }
         };
 
-        // Ping-pong buffers: tile jj of K and V in buffer jj % NBUF.
-        auto bofs = [&](int jj) { return (uint32_t)((jj % NBUF) * BUF); };
+        // Ping-pong buffers: tile jj of K and V in buffer jj % NBUF.  (Cross
+        // attention counts from its part's first tile: the third buffer holds the
+        // ticket slot, or Q on its way, until the loop's first loads into it.)
+        auto bofs = [&](int jj) {
+            if constexpr (CROSS) jj -= j0;
+            return (uint32_t)((jj % NBUF) * BUF);
+        };
         // slice sl of this wave's share of tile jj of K (or V)
         // (the tile's first row at tp)
         auto pp_dma_at = [&](const elem* tp, const uint32_t(&go)[NSL], uint32_t dst0, int sl) {
