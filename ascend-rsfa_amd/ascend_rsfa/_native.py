@@ -321,6 +321,7 @@ SIGNATURES = {
     "rsfa_cross_bwd_workspace_bytes": (ctypes.c_uint64, [ctypes.POINTER(CrossBwdArgs)]),
     "rsfa_draft_tree": (ctypes.c_int, [ctypes.POINTER(DraftTreeArgs), ctypes.c_void_p]),
     "rsfa_cache4_attend_tree": (ctypes.c_int, [ctypes.POINTER(Cache4AttendArgs), ctypes.c_void_p, _I64, ctypes.c_void_p]),
+    "rsfa_cache4_attend_tree_workspace_bytes": (ctypes.c_uint64, [ctypes.POINTER(Cache4AttendArgs)]),
     "rsfa_cache4_keep": (ctypes.c_int, [ctypes.POINTER(Cache4KeepArgs), ctypes.c_void_p]),
     "rsfa_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "rsfa_abi_version": (ctypes.c_int, []),

@@ -397,13 +397,15 @@ class Cache4:
             return (o, lse) if return_lse else o
         accumulate = int(bool(accumulate))
         head = b"".join((parts[0], _AT_QO.pack(q_.data_ptr(), o.data_ptr(), lse.data_ptr() if return_lse else 0), parts[1]))
-        nbytes = parts[2].get((max_length, accumulate))
+        size = (max_length, accumulate, tree is not None)
+        nbytes = parts[2].get(size)
         if nbytes is None:
             tail = _AT_TAIL.pack(at, length, max_length, counts, positions, 0.0, accumulate, 0, 0)
             args = _native.Cache4AttendArgs.from_buffer_copy(head + tail)
-            nbytes = self._on_device(_native.lib().rsfa_cache4_attend_workspace_bytes, ctypes.byref(args))
+            fn = "rsfa_cache4_attend_workspace_bytes" if tree is None else "rsfa_cache4_attend_tree_workspace_bytes"
+            nbytes = self._on_device(getattr(_native.lib(), fn), ctypes.byref(args))
             if at:  # (an int's bound changes from call to call)
-                parts[2][max_length, accumulate] = nbytes
+                parts[2][size] = nbytes
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
         args = head + _AT_TAIL.pack(at, length, max_length, counts, positions, scale, accumulate, ws.data_ptr() if nbytes else 0, nbytes)
         if tree is None:

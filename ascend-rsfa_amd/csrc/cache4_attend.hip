@@ -521,16 +521,17 @@ __global__ void __launch_bounds__(256, 2) attend_kernel(AttendParams p) {
 // without LDS, 32 rows a wave: 1107.  Halves of a tile whose softmax and products alternate,
 // raised wave priority around the products, LDS reads two to eight MFMAs ahead:
 // no gain with four waves.)
-template <int D, int W>
+// With G = 2 the waves w and w + W / 2 have the same rows and a half of each tile's keys each, and add up at the end.
+template <int D, int W, int G = 1>
 struct Many {
-    static constexpr int PIECE = D == 256 ? 32 : 64;     // keys between two looks at the running maximum
-    static constexpr int PIECES = W / 4;
-    static constexpr int KEYS = PIECE * PIECES;          // of a tile: its fragments take 8 KB a wave at D = 128, 256
+    static constexpr int KEYS = (D == 256 ? 8 : 16) * W; // of a tile: its fragments take 8 KB a wave at D = 128, 256
+    static constexpr int PIECE = G > 1 ? KEYS / G : D == 256 ? 32 : 64;  // keys between two looks at the running maximum
+    static constexpr int PIECES = G > 1 ? 1 : W / 4;     // of a tile, that a wave computes with
     static constexpr int KF = KEYS / 32 * (D / 16) / W;  // K fragments a wave converts
     static constexpr int VF = KEYS / 16 * (D / 32) / W;  // V fragments
     static constexpr int KFRAGS = W * KF, FRAGS = W * (KF + VF);
     static constexpr int PER_BLOCK = W / (KEYS / 32);    // waves that share a block of 32 keys' K
-    static constexpr int ROWS = 32 * W;
+    static constexpr int ROWS = 32 * W / G;
 };
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -542,10 +543,10 @@ __device__ __forceinline__ f32x16 mfma32(BF16::x8 a, BF16::x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-template <class T, int D, int MASK, int W>
+template <class T, int D, int MASK, int W, int G = 1>
 __global__ void __launch_bounds__(64 * W, 2) attend_many_kernel(AttendParams p) {
     constexpr bool CAUSAL = MASK == MASK_POSITION, TREE = MASK == MASK_TREE;
-    typedef Many<D, W> M;
+    typedef Many<D, W, G> M;
     typedef typename T::x8 x8;
     typedef typename T::elem elem;
     constexpr int QS = D / 16, DT = D / 32, KEYS = M::KEYS, PIECE = M::PIECE, SB = PIECE / 32;
@@ -558,7 +559,8 @@ __global__ void __launch_bounds__(64 * W, 2) attend_many_kernel(AttendParams p) 
     const int z = bh / (int)p.c.h, h = bh - z * (int)p.c.h;
     const int len = __builtin_amdgcn_readfirstlane(length_of(p.lengths, p.length, z, p.most));
     const int count = p.counts ? max(0, min(p.counts[z], p.t)) : p.t;
-    const int row = blockIdx.x / p.bh * M::ROWS + 32 * wave + col;
+    const int part = wave / (W / G);  // of a tile's keys, the wave's own (G > 1)
+    const int row = blockIdx.x / p.bh * M::ROWS + 32 * (G > 1 ? wave % (W / G) : wave) + col;
     const int tok = row / p.group, head = row - tok * p.group;
     const bool valid = tok < count;  // (row < rows follows)
     const int64_t cb = z * p.c.code_stride[0] + h * p.c.code_stride[1];
@@ -807,10 +809,12 @@ __global__ void __launch_bounds__(64 * W, 2) attend_many_kernel(AttendParams p) 
         int buf = 0;
         for (int tile = start; tile < end; tile += KEYS, buf ^= 1) {
             __syncthreads();  // this tile is in LDS, and nobody reads the other buffer any more
-            if (late) compute(buf, tile, 0);
+            const int mine = G > 1 ? part : 0;
+            const bool there = G == 1 || tile + mine * PIECE < end;
+            if (late && there) compute(buf, tile, mine);
             if (tile + KEYS < end) convert(buf ^ 1);
             if (tile + 2 * KEYS < end) load(tile + 2 * KEYS);
-            if (!late) compute(buf, tile, 0);
+            if (!late && there) compute(buf, tile, mine);
 #pragma unroll
             for (int i = 1; i < M::PIECES; ++i)
                 if (tile + i * PIECE < end) compute(buf, tile, i);
@@ -818,6 +822,40 @@ __global__ void __launch_bounds__(64 * W, 2) attend_many_kernel(AttendParams p) 
     }
     l += __shfl_xor(l, 32);
     if (!valid) m = NEVER, l = 0.0f;  // past the count (q was taken as 0)
+    if constexpr (G > 1) {
+        // the waves of a row add up their parts of the keys, through the tiles' LDS
+        constexpr int RW = W / G;
+        static_assert(sizeof(frag) >= (W - RW) * 64 * DT * 64, "the sums fit the tiles' LDS");
+        f32x4* const sums = (f32x4*)&frag[0][0][0];  // [wave - RW][DT * 4][64]
+        __shared__ float2 ml[(W - RW) * 64];
+        __syncthreads();
+        if (part) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int a = 0; a < 4; ++a)
+                    sums[((wave - RW) * DT * 4 + d * 4 + a) * 64 + lane] = (f32x4){acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]};
+            ml[(wave - RW) * 64 + lane] = make_float2(m, l);
+        }
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int g = 0; g < G - 1; ++g) {
+            const float2 v = ml[(g * RW + wave) * 64 + lane];
+            const float now = fmaxf(m, v.x);
+            const float f = __builtin_amdgcn_exp2f(m - now), x = __builtin_amdgcn_exp2f(v.x - now);
+            m = now;
+            l = l * f + v.y * x;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const f32x4 o = sums[((g * RW + wave) * DT * 4 + d * 4 + a) * 64 + lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[d][4 * a + e] = acc[d][4 * a + e] * f + o[e] * x;
+                }
+        }
+    }
     if (row >= p.rows) return;
     if (p.splits > 1) {
         const int64_t at = ((int64_t)blockIdx.y * p.bh + bh) * p.rows + row;
@@ -1185,13 +1223,14 @@ struct Plan {
     bool few;          // attend_kernel, with nb blocks of 16 rows
     int nb;
     int waves, tiles, splits;
+    int groups;        // attend_many_kernel: parts of a tile's keys
     bool scores;       // weights from stored scores
     int weight_tiles, weight_parts;
     uint64_t part_w;
     uint64_t part_o, part_ml, scores_at, row_lse, bytes;  // offsets into the workspace
 };
 
-Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
+Plan make_plan(const rsfa_cache4_attend_args* a, int cus, bool tree) {
     Plan p{};
     const int64_t group = a->heads / a->cache.h, rows = group * a->t;
     const int64_t bh = a->cache.z * a->cache.h;
@@ -1199,13 +1238,19 @@ Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
     // (32 key heads of 8192 slots, bf16, causal, caches in turn, few and many rows' kernel at D = 64, 128, 256: 32 rows 17
     // and 26 us, 20 and 29, 38 and 55; 64 rows 24 and 27, 32 and 31, 63 and 66; 128 rows 36 and 31, 53 and 37, 94 and 92:
     // up to 64 rows the few rows' kernel would still be ahead at D = 64 and 256)
-    const bool few = rows <= 32;
+    // A tree's rows stay with it for longer: 8 or 16 sequences of 8 key heads, D = 64 and 128, 4096 and 8192 slots, bf16, caches in
+    // turn, 48 and 64 rows 25 and 35 us, 33 and 37, with many rows' kernel 49 and 35, 66 and 68 (its waves in two groups,
+    // below, 35, 47, 49); 32 sequences of up to 4096 slots, 100 rows, 86, 111 and 76; D = 256, 8000 slots, 120 rows 45, 58 and 53.
+    const bool few = rows <= (tree ? a->cache.head_dim == 256 ? 128 : 64 : 32);
     p.few = few;
     p.nb = rows <= 16 || a->cache.head_dim == 256 ? 1 : 2;
     // (D = 256, four and eight waves: 128 rows of the same 92 and 96 us, 192 rows 115 and 107; below 256 they are
     // the same within half a microsecond)
     p.waves = few || (a->cache.head_dim == 256 && rows <= 128) ? 4 : 8;
-    const int64_t tile_rows = few ? 16 * p.nb : 32 * p.waves;
+    // Up to 128 rows leave half of the eight waves without rows of their own: these take half of the others' keys.
+    // (Without a tree they idle, as they always have: sums in another order would be other bits.)
+    p.groups = tree && !few && rows <= 128 ? 2 : 1;
+    const int64_t tile_rows = few ? 16 * p.nb : 32 * p.waves / p.groups;
     p.tiles = (int)((rows + tile_rows - 1) / tile_rows);
     // Enough workgroups for the chip, of at least four steps each.  Few rows: eight
     // workgroups a CU even out lengths (64 sequences of 1024 to 4096 slots 46.6 -> 44.9 us
@@ -1213,7 +1258,10 @@ Plan make_plan(const rsfa_cache4_attend_args* a, int cus) {
     // 32768 slots: 13.1, 16.4 with two steps each, 22.9 with one).
     const int64_t step = few ? 4 * TILE : 16 * p.waves;
     const int64_t full = (few ? 8 : 8 / p.waves) * (int64_t)cus;
-    const int64_t want = (full + bh * p.tiles - 1) / (bh * p.tiles);
+    int64_t want = (full + bh * p.tiles - 1) / (bh * p.tiles);
+    // (a tree's parts are larger, for its rows, and so is the work of each step: 64 sequences of 8 key heads of up to 2048
+    // slots, 32 rows, 51 us with four parts, 31 with one; 16 of 4096, 40 rows, 35 with eight, 33)
+    if (tree && few) want = bh * p.tiles >= cus ? 1 : (2 * (int64_t)cus + bh * p.tiles - 1) / (bh * p.tiles);
     const int64_t able = (most + 4 * step - 1) / (4 * step);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, able), 256));
     // (computing the scores again instead, one token of 16 x 8 x 8192 slots at most, D = 128: 4
@@ -1255,6 +1303,8 @@ const void* attend_fn(const Plan& p) {
             if (p.nb == 2) return (const void*)&attend_kernel<T, D, 2, MASK>;
         return (const void*)&attend_kernel<T, D, 1, MASK>;
     }
+    if constexpr (MASK == MASK_TREE && D <= 128)
+        if (p.groups == 2) return (const void*)&attend_many_kernel<T, D, MASK, 8, 2>;
     if constexpr (D == 256)
         if (p.waves == 4) return (const void*)&attend_many_kernel<T, D, MASK, 4>;
     return (const void*)&attend_many_kernel<T, D, MASK, 8>;
@@ -1301,7 +1351,7 @@ int attend(const rsfa_cache4_attend_args* a, const int32_t* tree, int64_t tree_s
     if ((st = check_rows(a->q, a->q_stride)) != RSFA_OK || (st = check_rows(a->o, a->o_stride)) != RSFA_OK) return st;
     if (((uintptr_t)a->lse | (uintptr_t)a->lengths | (uintptr_t)a->counts | (uintptr_t)a->pos_start) & 3)
         return RSFA_E_ALIGN;
-    const Plan plan = make_plan(a, cus_of_current_device());
+    const Plan plan = make_plan(a, cus_of_current_device(), mask == MASK_TREE);
     if (plan.bytes) {
         if (!a->workspace || a->workspace_bytes < plan.bytes) return RSFA_E_WORKSPACE;
         if ((uintptr_t)a->workspace & 15) return RSFA_E_ALIGN;
@@ -1373,7 +1423,12 @@ extern "C" {
 
 uint64_t rsfa_cache4_attend_workspace_bytes(const rsfa_cache4_attend_args* a) {
     if (check_attend(a) != RSFA_OK) return 0;
-    return make_plan(a, cus_of_current_device()).bytes;
+    return make_plan(a, cus_of_current_device(), false).bytes;
+}
+
+uint64_t rsfa_cache4_attend_tree_workspace_bytes(const rsfa_cache4_attend_args* a) {
+    if (check_attend(a) != RSFA_OK) return 0;
+    return make_plan(a, cus_of_current_device(), true).bytes;
 }
 
 int rsfa_cache4_attend(const rsfa_cache4_attend_args* a, void* stream) {

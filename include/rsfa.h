@@ -463,9 +463,11 @@ int rsfa_draft_tree(const rsfa_draft_tree_args *args, void *stream);
  * t tokens (counts[z] of them) being the last slots in use.  Token i sees all slots before
  * them, and drafted token j < counts[z] where row i of `bits` has it; positions and `causal`
  * are not looked at.  `bits`: device, [t, words] for each sequence, bits_stride elements
- * apart (0: one for all).  accumulate must be 0 and pos_start NULL. */
+ * apart (0: one for all).  accumulate must be 0 and pos_start NULL.  Workspace:
+ * rsfa_cache4_attend_tree_workspace_bytes of the same arguments. */
 int rsfa_cache4_attend_tree(const rsfa_cache4_attend_args *args, const int32_t *bits,
                             int64_t bits_stride, void *stream);
+uint64_t rsfa_cache4_attend_tree_workspace_bytes(const rsfa_cache4_attend_args *args);
 
 /* keep: row j < counts[z] (NULL: n) of drafted token tokens[z, j] goes from slot
  * lengths[z] + tokens[z, j] to slot lengths[z] + j (lengths: the contexts), with its weight, and

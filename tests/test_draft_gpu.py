@@ -94,6 +94,7 @@ SHAPES = [
     (1, 2, 2, 1, [1], None), (2, 4, 2, 5, [5, 70], None), (3, 4, 1, 8, [40, 8, 1000], [8, 0, 3]),
     (2, 2, 2, 31, [500, 31], [31, 30]), (2, 4, 2, 16, [16, 4100], None), (1, 8, 1, 25, [2050], None),
     (2, 4, 4, 64, [64, 777], [64, 50]), (1, 2, 1, 97, [97 + 61], None), (1, 1, 1, 200, [3333], None), (1, 4, 2, 130, [9000], None),
+    (2, 4, 1, 25, [4100, 30], [25, 17]), (1, 2, 2, 128, [900], None), (1, 2, 1, 33, [333], None),
 ]
 
 
