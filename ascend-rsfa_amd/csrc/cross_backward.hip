@@ -9,8 +9,14 @@
 // one kernel would have five, but every sum has one owner and one order: no atomics, the same bits in each call,
 // and no traffic for dQ's partial sums, which one kernel would add up in memory once per key block.
 // Where blocks are too few for the chip each pass is cut into parts, which sum_parts_kernel adds up.
+//
+// P and dS are rounded to the type for the products with rows (half a step of each, as the matrix unit takes 16-bit
+// operands at sixteen times the rate of 32-bit ones); all else is in 32 bits.  float16 ends at 2^-14 where gradients
+// are often smaller still: P is scaled by 2^k there, with k from the largest |dO| and |dlse| of the row (dQ) or of the
+// key head's rows (dK, dV), so that dS lies in the middle of the type's range; it goes into the exponent and out at the end.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/rsfa.h"
 #include "cross.hpp"
@@ -38,6 +44,7 @@ struct BwdParams {
     float c, scale;
     uint32_t neg;      // sign of sm_scale, as a mask for a pair of values
     float *nl, *nd;    // [Z * heads][tp]: -lse / (c ln 2), -delta; rows past t: -inf, 0
+    float* top;        // [Z * heads][tp / 32]: largest |dO|, |dlse| of 32 rows (float16)
     float* part[2];    // splits > 1: [splits][rows][D] of dK and dV, or of dQ
 };
 
@@ -51,6 +58,13 @@ __device__ __forceinline__ void dma4(const void* sbase, uint32_t voff_bytes, uin
                  :
                  : "v"(voff_bytes), "s"(sbase), "{m0}"(lds_addr)
                  : "memory");
+}
+
+// k of the scale 2^k of float16 weights, for a largest |dO| and |dlse|: dS = P (dO v - delta) is then below 2^4 |v| of a few values'
+// sums, and P, at most 2^15, is whole down to 2^-18 (dO of 1) or less.
+__device__ __forceinline__ float weight_exponent(float top) {
+    const int e = (int)(__float_as_uint(top) >> 23 & 255) - 127;
+    return (float)max(0, min(3 - e, 15));
 }
 
 // Tiles of rows in LDS have the forward kernel's layout (fa_fwd_kernel.hpp): 16-row blocks of planes of 32 columns,
@@ -162,12 +176,12 @@ __device__ __forceinline__ void store_rows(typename T::elem* dst, int64_t st, in
 }
 
 template <int D>
-__device__ __forceinline__ void store_part(float* dst, const f32x16 (&acc)[D / 32], int hh) {
+__device__ __forceinline__ void store_part(float* dst, const f32x16 (&acc)[D / 32], float f, int hh) {
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int a = 0; a < 4; ++a)
-            *(float4*)(dst + 32 * d + 8 * a + 4 * hh) = make_float4(acc[d][4 * a], acc[d][4 * a + 1], acc[d][4 * a + 2], acc[d][4 * a + 3]);
+            *(float4*)(dst + 32 * d + 8 * a + 4 * hh) = make_float4(acc[d][4 * a] * f, acc[d][4 * a + 1] * f, acc[d][4 * a + 2] * f, acc[d][4 * a + 3] * f);
 }
 
 // dK and dV of 128 keys, 32 of each wave, held transposed (dK^T = Q^T dS, dV^T = dO^T P): with keys in the lanes S
@@ -188,6 +202,7 @@ cross_dkv_kernel(BwdParams p) {
     constexpr int QB = Bwd<D>::TILE_ROWS, BLK = 32 * D, TILE = QB * D * 2, STATS = 512, BUF = 2 * TILE + STATS;
     constexpr int TWO = QB == 64 ? 64 * D : 0;  // where a wave's second 32 rows lie in the LDS of its prologue
     constexpr int DT = D / 32, KST = D / 16;
+    constexpr bool F16 = std::is_same<T, TypeF16>::value;
     __shared__ __attribute__((aligned(1024))) char smem_raw[2 * BUF];
     RSFA_LDS char* const smem = (RSFA_LDS char*)smem_raw;
     const uint32_t smem_addr = (uint32_t)(uintptr_t)smem;
@@ -223,6 +238,16 @@ cross_dkv_kernel(BwdParams p) {
         for (int s = 0; s < KST; ++s) kf[s] = __builtin_bit_cast(x8, __builtin_bit_cast(u32x4, kf[s]) ^ p.neg);
     }
     __syncthreads();  // (the tiles go where these rows were)
+    float k2 = 0.0f;
+    if constexpr (F16) {
+        const int n = p.group * (p.tp / 32);
+        const float* top = p.top + (int64_t)kh * n;
+        float most = 0.0f;
+        for (int j = w.lane; j < n; j += 64) most = fmaxf(most, top[j]);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+        k2 = weight_exponent(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(most))));
+    }
     f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -280,7 +305,7 @@ cross_dkv_kernel(BwdParams p) {
             stats(gt + TILE + st * 128, s);
             rows_product<T, D>(qt + st * 2 * BLK, w, kf, s);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * p.c);
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(F16 ? __builtin_fmaf(s[r], p.c, k2) : s[r] * p.c);
             pack<T>(s, b);
             columns_product<T, D>(gt + st * 2 * BLK, w, b, dv);
             stats(gt + TILE + 256 + st * 128, x);
@@ -291,11 +316,12 @@ cross_dkv_kernel(BwdParams p) {
             columns_product<T, D>(qt + st * 2 * BLK, w, b, dk);
         }
     }
+    const float unscale = __builtin_amdgcn_exp2f(-k2);
     if (p.splits > 1) {
         if (key >= nk) return;  // (the sum of the parts writes 0 there)
         const int64_t at = (((int64_t)blockIdx.y * p.z * p.key_heads + kh) * p.n + key) * D;
-        if (p.gk) store_part<D>(p.part[0] + at, dk, w.hh);
-        if (p.gv) store_part<D>(p.part[1] + at, dv, w.hh);
+        if (p.gk) store_part<D>(p.part[0] + at, dk, unscale, w.hh);
+        if (p.gv) store_part<D>(p.part[1] + at, dv, unscale, w.hh);
         return;
     }
     if (key >= nk) {
@@ -305,8 +331,8 @@ cross_dkv_kernel(BwdParams p) {
             for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.0f;
     }
     __syncthreads();  // (every wave is done with the tiles)
-    if (p.gk) store_rows<T, D>((elem*)p.gk + z * p.gk_st[0] + h * p.gk_st[1] + first * p.gk_st[2], p.gk_st[2], p.n - first, dk, p.scale, w, own);
-    if (p.gv) store_rows<T, D>((elem*)p.gv + z * p.gv_st[0] + h * p.gv_st[1] + first * p.gv_st[2], p.gv_st[2], p.n - first, dv, 1.0f, w, own);
+    if (p.gk) store_rows<T, D>((elem*)p.gk + z * p.gk_st[0] + h * p.gk_st[1] + first * p.gk_st[2], p.gk_st[2], p.n - first, dk, p.scale * unscale, w, own);
+    if (p.gv) store_rows<T, D>((elem*)p.gv + z * p.gv_st[0] + h * p.gv_st[1] + first * p.gv_st[2], p.gv_st[2], p.n - first, dv, unscale, w, own);
 }
 
 // dQ of 128 rows, 32 of each wave, held transposed (dQ^T = K^T dS^T), rows in the lanes: a row's
@@ -319,6 +345,7 @@ cross_dq_kernel(BwdParams p) {
     constexpr int KB = Bwd<D>::TILE_ROWS, BLK = 32 * D, TILE = KB * D * 2, BUF = 2 * TILE;
     constexpr int TWO = KB == 64 ? 64 * D : 0;  // where a wave's second 32 rows lie in the LDS of its prologue
     constexpr int DT = D / 32, KST = D / 16;
+    constexpr bool F16 = std::is_same<T, TypeF16>::value;
     __shared__ __attribute__((aligned(1024))) char smem_raw[2 * BUF];
     RSFA_LDS char* const smem = (RSFA_LDS char*)smem_raw;
     const uint32_t smem_addr = (uint32_t)(uintptr_t)smem;
@@ -341,7 +368,7 @@ cross_dq_kernel(BwdParams p) {
     const int first = block * 128 + wave * 32;  // the wave's first row
     RSFA_LDS char* const own = smem + wave * TILE;
     x8 qf[KST], gf[KST];
-    float l2 = 0.0f, nd = 0.0f;
+    float l2 = 0.0f, nd = 0.0f, k2 = 0.0f;
     if (mine) {
         const int64_t head = (int64_t)z * p.heads + hq;
         const int left = p.t - first;
@@ -381,12 +408,26 @@ cross_dq_kernel(BwdParams p) {
         }
         const float s0 = __shfl(sum[0], 4 * w.l16), s1 = __shfl(sum[1], 4 * w.l16);
         nd = gl - (w.l32 < 16 ? s0 : s1);
+        if constexpr (F16) {
+            float most = __builtin_fabsf(gl);
+#pragma unroll
+            for (int s = 0; s < KST; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf((float)gf[s][e]));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            k2 = weight_exponent(most);
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+            if (blockIdx.y == 0 && w.lane == 0) p.top[head * (p.tp / 32) + first / 32] = most;
+        }
         // for dK and dV: rows behind the last have weights of 0
         if (blockIdx.y == 0 && w.hh == 0 && row < p.tp) {
             p.nl[head * p.tp + row] = row < p.t ? -l2 / p.c : -INFINITY;
             p.nd[head * p.tp + row] = row < p.t ? nd : 0.0f;
         }
+        l2 -= k2;
     } else if (blockIdx.y == 0 && w.hh == 0 && row < p.tp) {
+        if (F16 && w.lane == 0) p.top[((int64_t)z * p.heads + hq) * (p.tp / 32) + first / 32] = 0.0f;
         p.nl[((int64_t)z * p.heads + hq) * p.tp + row] = -INFINITY;
         p.nd[((int64_t)z * p.heads + hq) * p.tp + row] = 0.0f;
     }
@@ -447,11 +488,11 @@ cross_dq_kernel(BwdParams p) {
     if (p.splits > 1) {
         if (row >= p.t) return;
         const int64_t rows = (int64_t)p.z * p.heads * p.t;
-        store_part<D>(p.part[0] + (blockIdx.y * rows + ((int64_t)z * p.heads + hq) * p.t + row) * D, dq, w.hh);
+        store_part<D>(p.part[0] + (blockIdx.y * rows + ((int64_t)z * p.heads + hq) * p.t + row) * D, dq, __builtin_amdgcn_exp2f(-k2), w.hh);
         return;
     }
     __syncthreads();  // (every wave is done with the tiles)
-    store_rows<T, D>((elem*)p.gq + z * p.gq_st[0] + hq * p.gq_st[1] + first * p.gq_st[2], p.gq_st[2], p.t - first, dq, p.scale, w, own);
+    store_rows<T, D>((elem*)p.gq + z * p.gq_st[0] + hq * p.gq_st[1] + first * p.gq_st[2], p.gq_st[2], p.t - first, dq, p.scale * __builtin_amdgcn_exp2f(-k2), w, own);
 }
 
 // Sums of parts: D / 4 lanes a row; rows past their sequence's length (dK, dV) become 0.
@@ -506,7 +547,7 @@ Functions functions(int64_t d) {
 struct Plan {
     int64_t tp, key_blocks, row_blocks;
     int dkv_splits, dq_splits;
-    uint64_t nl, nd, dkv[2], dq, bytes;
+    uint64_t nl, nd, top, dkv[2], dq, bytes;
 };
 
 Plan make_plan(const rsfa_cross_bwd_args* a) {
@@ -529,6 +570,7 @@ Plan make_plan(const rsfa_cross_bwd_args* a) {
     };
     p.nl = take((uint64_t)qh * p.tp * 4 + 256);
     p.nd = take((uint64_t)qh * p.tp * 4 + 256);
+    if (a->dtype == RSFA_DTYPE_F16) p.top = take((uint64_t)qh * p.tp / 32 * 4);
     if (p.dkv_splits > 1)
         for (int i = 0; i < 2; ++i) p.dkv[i] = take((uint64_t)p.dkv_splits * kh * a->n * d * 4);
     if (p.dq_splits > 1) p.dq = take((uint64_t)p.dq_splits * qh * a->t * d * 4);
@@ -577,7 +619,7 @@ int rsfa_cross_bwd(const rsfa_cross_bwd_args* a, void* stream) {
     p.scale = a->sm_scale;
     p.c = std::max(std::fabs(a->sm_scale) * LOG2E, LEAST_C);
     p.neg = a->sm_scale < 0.0f ? 0x80008000u : 0u;
-    p.nl = (float*)(ws + plan.nl), p.nd = (float*)(ws + plan.nd);
+    p.nl = (float*)(ws + plan.nl), p.nd = (float*)(ws + plan.nd), p.top = (float*)(ws + plan.top);
     const int64_t d = a->head_dim, kh = a->z * a->key_heads, qh = a->z * a->heads;
     const Functions fn = a->dtype == RSFA_DTYPE_BF16 ? functions<TypeBF16>(d) : functions<TypeF16>(d);
     const int64_t dkv_blocks = kh * plan.key_blocks, dq_blocks = qh * plan.row_blocks;

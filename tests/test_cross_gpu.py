@@ -128,6 +128,19 @@ def test_scales(scale, T):
         _check(q, k, v, scale, _ints([150, 33]), _randn(q.shape, 4, dtype), _randn(q.shape[:3], 5, torch.float32))
 
 
+@pytest.mark.parametrize("std", [2.0 ** -20, 2.0 ** -12, 1.0, 2.0 ** 9])
+@pytest.mark.parametrize("T, D", [(3, 64), (90, 32), (200, 128), (70, 256)])
+def test_gradients_of_every_size(T, D, std):
+    # (rows of q and k large enough for gradients within float16's normal numbers, and a row of dO far above the others)
+    for dtype in (F16, BF16):
+        q, k, v = _inputs(2, 4, 2, T, 333, D, dtype)
+        go = _randn(q.shape, 4, dtype, std)
+        go[1, 3, T // 2] *= 64
+        up = 2.0 ** 7 if std < 1 else 1.0
+        _check(q * up, k * up, v, D ** -0.5 / up ** 2, _ints([333, 200]), go)
+        _check(q, k, v, D ** -0.5, None, go, _randn(q.shape[:3], 5, torch.float32, std))
+
+
 @pytest.mark.parametrize("T", [2, 90])
 def test_one_score_far_above_the_rest(T):
     # each row's weight on one key, anywhere along a long row, and rows of equal scores
