@@ -8,7 +8,9 @@ import torch
 
 from ascend_rsfa import _native
 from ascend_rsfa.cross import cross_attention
+from cross_launches import variants
 from oracle import cross as O
+from test_cross_gpu import SHAPES, VARIANTS
 
 
 def test_struct_layouts():
@@ -87,3 +89,26 @@ def test_the_definitions_gradients_against_differences():
 
             slope = (value(1e-5) - value(-1e-5)) / 2e-5
             assert abs(slope - float(want[name][0].view(-1)[at])) < 1e-8
+
+
+def test_the_shapes_of_the_variants_test_run_every_forward_variant(tmp_path):
+    seen = set()
+    for shape, launches in zip(VARIANTS, variants(VARIANTS, tmp_path)):
+        (name, numbers), *rest = launches
+        assert [x for x, _ in rest] in ([], ["cross_join_kernel"]) and numbers[0] == shape[5]
+        seen.add((name, numbers[:3] if name == "fa_fwd_kernel" else numbers[:2], bool(rest)))
+    few = [("cross_few_kernel", (d, nb)) for d in (32, 64, 128, 256) for nb in (1, 2, 4) if (d, nb) != (256, 4)]
+    many = [("fa_fwd_kernel", x) for x in ((32, 64, 4), (32, 128, 4), (64, 64, 4), (64, 128, 8), (128, 64, 4), (128, 64, 8),
+                                           (256, 32, 4), (256, 32, 8))]
+    assert seen == {(name, numbers, parts) for name, numbers in few + many for parts in (False, True)}
+
+
+def test_the_shapes_of_the_definitions_test_run_every_backward_variant(tmp_path):
+    for d in (32, 64, 128, 256):
+        seen = set()
+        for launches in variants([s[:5] + (d,) for s in SHAPES], tmp_path, "rsfa_cross_bwd"):
+            names = [x for x, _ in launches]
+            dq = names.index("cross_dkv_kernel")
+            assert names[0] == "cross_dq_kernel" and set(names[1:dq] + names[dq + 1:]) <= {"sum_parts_kernel"}
+            seen.add((dq > 1, len(names) > dq + 1))
+        assert {x for x, _ in seen} == {x for _, x in seen} == {False, True}

@@ -79,6 +79,32 @@ def test_matches_the_definition(shape, D, dtype):
     assert torch.equal(cross_attention(q, k, v, D ** -0.5, le), o)
 
 
+# every forward variant, whole and in parts (tests/test_cross_cpu.py holds them to it)
+VARIANTS = [
+    (46, 16, 2, 1, 1, 32), (1, 2, 1, 2, 4123, 32), (7, 128, 16, 7, 1, 32), (1, 8, 8, 34, 2123, 32), (59, 32, 4, 5, 1, 32),
+    (1, 32, 8, 9, 30654, 32), (1, 8, 8, 1, 2, 64), (2, 4, 2, 1, 927, 64), (4, 64, 8, 21, 1, 64), (2, 2, 2, 20, 8794, 64),
+    (8, 128, 16, 10, 1, 64), (1, 8, 8, 202, 1757, 64), (1, 2, 2, 1, 1, 128), (1, 2, 2, 1, 1078, 128), (21, 16, 8, 10, 1, 128),
+    (1, 64, 8, 9, 1702, 128), (5, 8, 8, 198, 1, 128), (2, 32, 8, 17, 3773, 128), (1, 1, 1, 5, 1, 256), (5, 1, 1, 2, 379, 256),
+    (3, 16, 16, 88, 1, 256), (4, 2, 1, 33, 2340, 256), (1, 2, 1, 3, 1, 32), (10, 1, 1, 66, 2529, 32), (2, 1, 1, 3, 111, 32),
+    (2, 2, 2, 142, 7000, 32), (17, 2, 1, 305, 1, 64), (7, 8, 4, 103, 4960, 64), (3, 4, 4, 3574, 345, 64), (11, 2, 2, 356, 3985, 64),
+    (5, 64, 8, 56, 1, 128), (1, 8, 8, 137, 10984, 128), (5, 32, 16, 140, 1, 128), (5, 8, 1, 231, 2676, 128), (38, 4, 4, 36, 1, 256),
+    (4, 4, 2, 65, 2605, 256), (74, 2, 2, 153, 1, 256), (20, 1, 1, 139, 4193, 256),
+]
+
+
+@pytest.mark.parametrize("shape", VARIANTS)
+def test_every_forward_variant(shape):
+    Z, Hq, H, T, N, D = shape
+    for dtype in (F16, BF16):
+        q, k, v = _inputs(Z, Hq, H, T, N, D, dtype)
+        for lengths in (None, [N - (z * 7919) % (N + 1) for z in range(Z)]):
+            le = None if lengths is None else _ints(lengths)
+            got = cross_attention(q, k, v, D ** -0.5, le, return_lse=True)
+            want = O.expect(q, k, v, lengths, D ** -0.5)
+            for name, x in zip(("o", "lse"), got):
+                _hold(name, x, want[name])
+
+
 @pytest.mark.parametrize("T", [1, 3, 40, 300])
 @pytest.mark.parametrize("D", [32, 64, 128, 256])
 def test_sequences_without_keys_and_lengths_outside(D, T):
