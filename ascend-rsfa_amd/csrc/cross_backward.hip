@@ -368,7 +368,7 @@ cross_dq_kernel(BwdParams p) {
     const int first = block * 128 + wave * 32;  // the wave's first row
     RSFA_LDS char* const own = smem + wave * TILE;
     x8 qf[KST], gf[KST];
-    float l2 = 0.0f, nd = 0.0f, k2 = 0.0f;
+    float l2 = 0.0f, nd = 0.0f, k2 = 0.0f, gl = 0.0f;
     if (mine) {
         const int64_t head = (int64_t)z * p.heads + hq;
         const int left = p.t - first;
@@ -388,7 +388,7 @@ cross_dq_kernel(BwdParams p) {
             for (int c = 0; c < D / 32; ++c) o[b][c] = *(const x8*)(ob + min(16 * b + w.ld_row, left - 1) * p.o_st[2] + 32 * c);
         const int row_c = min(row, p.t - 1);
         l2 = p.lse[head * p.t + row_c] * LOG2E;
-        const float gl = p.glse ? p.glse[head * p.t + row_c] : 0.0f;
+        if (p.glse) gl = p.glse[head * p.t + row_c];
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if constexpr (TWO != 0) fragments<T, D>(own, w, qf);
         fragments<T, D>(own + TWO, w, gf);
@@ -420,18 +420,8 @@ cross_dq_kernel(BwdParams p) {
             for (int d = 1; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
             if (blockIdx.y == 0 && w.lane == 0) p.top[head * (p.tp / 32) + first / 32] = most;
         }
-        // for dK and dV: rows behind the last have weights of 0
-        if (blockIdx.y == 0 && w.hh == 0 && row < p.tp) {
-            p.nl[head * p.tp + row] = row < p.t ? -l2 / p.c : -INFINITY;
-            p.nd[head * p.tp + row] = row < p.t ? nd : 0.0f;
-        }
         l2 -= k2;
-    } else if (blockIdx.y == 0 && w.hh == 0 && row < p.tp) {
-        if (F16 && w.lane == 0) p.top[((int64_t)z * p.heads + hq) * (p.tp / 32) + first / 32] = 0.0f;
-        p.nl[((int64_t)z * p.heads + hq) * p.tp + row] = -INFINITY;
-        p.nd[((int64_t)z * p.heads + hq) * p.tp + row] = 0.0f;
     }
-    if (!p.gq) return;
     __syncthreads();  // (the tiles go where these rows were)
     f32x16 dq[DT];
 #pragma unroll
@@ -460,24 +450,55 @@ cross_dq_kernel(BwdParams p) {
             rows(vb, p.v_st[2], wave - 2, dst + TILE);
         }
     };
-    if (i < end) load(i, 0);
+    // S^T and (dO V^T)^T of 32 keys of tile `it`
+    auto scores = [&](int it, int st, int buf, f32x16& s, f32x16& x) {
+        const RSFA_LDS char* const kt = smem + buf * BUF;
+        rows_product<T, D>(kt + st * 2 * BLK, w, qf, s);
+        rows_product<T, D>(kt + TILE + st * 2 * BLK, w, gf, x);
+        const int left = nk - it * KB - 32 * st - 4 * w.hh;  // keys of the sub-tile, from the lane's first on
+        if (it * KB + 32 * st + 32 > nk) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (8 * (r / 4) + r % 4 >= left) s[r] = -INFINITY;
+        }
+    };
+    // With few keys o is large and its rounding, in delta, would be as large as that of dS (8 keys, bfloat16: an error of dQ
+    // against 64 bits of 0.0026 relative to it, 0.0024 without, 0.0017 being its own rounding): delta is then rowsum(P (dO V^T)).
+    const bool once = all == 1 && i == 0;
+    if (once) {
+        load(0, 0);
+        wait_loads_and_sync();
+        if (mine) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int st = 0; st < KB / 32; ++st) {
+                f32x16 s = {}, x = {};
+                scores(0, st, 0, s, x);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -l2)), x[r], sum);
+            }
+            sum += __shfl_xor(sum, 32);
+            nd = gl - sum * __builtin_amdgcn_exp2f(-k2);
+        }
+    }
+    // for dK and dV: rows behind the last have weights of 0
+    if (blockIdx.y == 0 && w.hh == 0 && row < p.tp) {
+        const int64_t at = ((int64_t)z * p.heads + hq) * p.tp + row;
+        p.nl[at] = row < p.t ? -(l2 + k2) / p.c : -INFINITY;
+        p.nd[at] = row < p.t ? nd : 0.0f;
+        if (F16 && w.lane == 0 && !mine) p.top[((int64_t)z * p.heads + hq) * (p.tp / 32) + first / 32] = 0.0f;
+    }
+    if (!p.gq) return;
+    if (i < end && !once) load(i, 0);
     for (int buf = 0; i < end; ++i, buf ^= 1) {
         wait_loads_and_sync();
         if (i + 1 < end) load(i + 1, buf ^ 1);
         if (!mine) continue;
         const RSFA_LDS char* const kt = smem + buf * BUF;
-        const RSFA_LDS char* const vt = kt + TILE;
 #pragma unroll
         for (int st = 0; st < KB / 32; ++st) {
             f32x16 s = {}, x = {};
-            rows_product<T, D>(kt + st * 2 * BLK, w, qf, s);
-            rows_product<T, D>(vt + st * 2 * BLK, w, gf, x);
-            const int left = nk - i * KB - 32 * st - 4 * w.hh;  // keys of the sub-tile, from the lane's first on
-            if (i * KB + 32 * st + 32 > nk) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (8 * (r / 4) + r % 4 >= left) s[r] = -INFINITY;
-            }
+            scores(i, st, buf, s, x);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -l2)) * (x[r] + nd);
             x8 b[2];
