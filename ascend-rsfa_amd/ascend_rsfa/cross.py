@@ -23,8 +23,9 @@ __all__ = ["cross_attention"]
 _DTYPES = {torch.float16: _native.DTYPE_F16, torch.bfloat16: _native.DTYPE_BF16}
 _HEAD_DIMS = (32, 64, 128, 256)
 
-# An argument struct is joined from a part that the tensors' shapes settle, kept by them (`_PLANS`), and packed addresses:
-# a call's checks and sizes are then one lookup.
+# What a call does is settled by its tensors' shapes, strides, types and devices, and kept by them: a _Plan holds the
+# argument structs but for their addresses, so that a call is one lookup and a struct joined from bytes (a training step's
+# two passes run in two threads, each of which finds the other's objects far away).
 _F, _B = _native.CrossArgs, _native.CrossBwdArgs
 _FWD_PTRS = struct.Struct("=5Q")  # q, k, v, o, lse
 _BWD_PTRS = struct.Struct("=10Q")  # q, k, v, o, lse, grad_o, grad_lse, grad_q, grad_k, grad_v
@@ -50,87 +51,83 @@ def _on_device(index, fn, *args):
         return fn(*args)
 
 
-def _keep(key, plan):
-    if len(_PLANS) > 4096:
-        _PLANS.clear()
-    _PLANS[key] = plan
-    return plan
+def _launch(index, name, args):
+    status = _on_device(index, _function(name), args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _raise_for(status)
 
 
 def _empty_rows(t):
-    """An output like t, whose rows the kernels can write."""
+    """(an output like t, whose rows the kernels can write, whether empty_like gives it)."""
     o = torch.empty_like(t)
-    return o if _meets_contract(o) else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return (o, True) if _meets_contract(o) else (torch.empty(t.shape, dtype=t.dtype, device=t.device), False)
 
 
-def _sizes(args, q, k):
+def _struct(kind, tensors, q, k, workspace):
+    """(the struct's bytes before and after its addresses, workspace bytes) for {name: tensor}."""
+    args = kind()
     args.struct_size, args.dtype = ctypes.sizeof(args), _DTYPES[q.dtype]
     args.z, args.heads, args.t, args.head_dim = q.shape
     args.key_heads, args.n = k.shape[1], k.shape[2]
+    for name, t in tensors.items():
+        if t is not None:
+            getattr(args, name + "_stride")[:] = t.stride()
+    nbytes = _on_device(q.device.index, getattr(_native.lib(), workspace), ctypes.byref(args))
+    b = bytes(args)
+    return b[:kind.q.offset], b[kind.z.offset:kind.lengths.offset], nbytes
 
 
-def _forward(q, k, v, scale, lengths, want_lse):
-    """(o, lse or None) of checked tensors in the kernels' layout."""
-    key = (q.shape, k.shape, q.stride(), k.stride(), v.stride(), q.dtype, q.device)
-    plan = _PLANS.get(key)
-    if plan is None:
-        o = _empty_rows(q)
-        if o.numel() == 0 or k.shape[2] == 0:
-            o.zero_()
-            return o, torch.full(q.shape[:3], -math.inf, dtype=torch.float32, device=q.device) if want_lse else None
-        args = _F()
-        _sizes(args, q, k)
-        for name, t in (("q_stride", q), ("k_stride", k), ("v_stride", v), ("o_stride", o)):
-            getattr(args, name)[:] = t.stride()
-        nbytes = _on_device(q.device.index, _native.lib().rsfa_cross_fwd_workspace_bytes, ctypes.byref(args))
-        b = bytes(args)
-        plan = _keep(key, (b[:_F.q.offset], b[_F.z.offset:_F.lengths.offset], nbytes, o.stride() == torch.empty_like(q).stride()))
-    else:
-        o = torch.empty_like(q) if plan[3] else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    head, sizes, nbytes, _ = plan
+class _Plan:
+    """A call's argument structs, for tensors in the kernels' layout that are not empty."""
+
+    __slots__ = ("index", "head", "sizes", "nbytes", "like", "backward")
+
+    def __init__(self, q, k, v):
+        o, self.like = _empty_rows(q)
+        self.index = q.device.index
+        self.head, self.sizes, self.nbytes = _struct(_F, {"q": q, "k": k, "v": v, "o": o}, q, k, "rsfa_cross_fwd_workspace_bytes")
+        self.backward = {}
+
+
+def _forward(plan, q, k, v, scale, lengths, want_lse):
+    """(o, lse or None)."""
+    o = torch.empty_like(q) if plan.like else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
+    nbytes = plan.nbytes
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    args = b"".join((head, _FWD_PTRS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if want_lse else 0),
-                     sizes, _TAIL.pack(0 if lengths is None else lengths.data_ptr(), scale, 0, ws.data_ptr() if nbytes else 0, nbytes)))
-    dev = q.device.index
-    _raise_for(_on_device(dev, _function("rsfa_cross_fwd"), args, torch._C._cuda_getCurrentRawStream(dev)))
+    _launch(plan.index, "rsfa_cross_fwd", b"".join((
+        plan.head, _FWD_PTRS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr() if want_lse else 0), plan.sizes,
+        _TAIL.pack(0 if lengths is None else lengths.data_ptr(), scale, 0, ws.data_ptr() if nbytes else 0, nbytes))))
     return o, lse
 
 
-def _backward(q, k, v, o, lse, go, glse, scale, lengths, needs):
+def _backward(plan, q, k, v, o, lse, go, glse, scale, lengths, needs):
     """The gradients of q, k and v, those that ``needs`` names (None for the others)."""
-    if q.numel() == 0 or k.shape[2] == 0:
-        return [torch.zeros_like(t) if need else None for t, need in zip((q, k, v), needs)]
     if go is None:
         go = torch.zeros_like(o)
     if glse is not None:
         glse = glse.contiguous()
-    key = (q.shape, k.shape, q.stride(), k.stride(), v.stride(), go.stride(), q.dtype, q.device, needs)
-    plan = _PLANS.get(key)
-    if plan is None or go.data_ptr() & 15:
+    key = (go.stride(), needs)
+    kept = plan.backward.get(key)
+    if kept is None or go.data_ptr() & 15:
         go_ = _as_kernel_layout(go)
-        grads = [_empty_rows(t) if need else None for t, need in zip((q, k, v), needs)]
-        args = _B()
-        _sizes(args, q, k)
-        for name, t in (("q", q), ("k", k), ("v", v), ("o", o), ("grad_o", go_), ("grad_q", grads[0]), ("grad_k", grads[1]),
-                        ("grad_v", grads[2])):
-            if t is not None:
-                getattr(args, name + "_stride")[:] = t.stride()
-        nbytes = _on_device(q.device.index, _native.lib().rsfa_cross_bwd_workspace_bytes, ctypes.byref(args))
-        b = bytes(args)
-        plan = (b[:_B.q.offset], b[_B.z.offset:_B.lengths.offset], nbytes)
-        if go_ is go and all(g is None or g.stride() == torch.empty_like(t).stride() for g, t in zip(grads, (q, k, v))):
-            _keep(key, plan)
+        grads = [_empty_rows(t) if need else (None, True) for t, need in zip((q, k, v), needs)]
+        like = all(x for _, x in grads)
+        grads = [g for g, _ in grads]
+        kept = _struct(_B, {"q": q, "k": k, "v": v, "o": o, "grad_o": go_, "grad_q": grads[0], "grad_k": grads[1], "grad_v": grads[2]},
+                       q, k, "rsfa_cross_bwd_workspace_bytes")
+        if go_ is go and like:
+            if len(plan.backward) > 64:
+                plan.backward.clear()
+            plan.backward[key] = kept
         go = go_
     else:
         grads = [torch.empty_like(t) if need else None for t, need in zip((q, k, v), needs)]
-    head, sizes, nbytes = plan
+    head, sizes, nbytes = kept
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     ptrs = [0 if t is None else t.data_ptr() for t in (q, k, v, o, lse, go, glse, *grads)]
-    args = b"".join((head, _BWD_PTRS.pack(*ptrs), sizes,
-                     _TAIL.pack(0 if lengths is None else lengths.data_ptr(), scale, 0, ws.data_ptr(), nbytes)))
-    dev = q.device.index
-    _raise_for(_on_device(dev, _function("rsfa_cross_bwd"), args, torch._C._cuda_getCurrentRawStream(dev)))
+    _launch(plan.index, "rsfa_cross_bwd", b"".join((
+        head, _BWD_PTRS.pack(*ptrs), sizes, _TAIL.pack(0 if lengths is None else lengths.data_ptr(), scale, 0, ws.data_ptr(), nbytes))))
     return grads
 
 
@@ -158,10 +155,13 @@ def _check(q, k, v, lengths):
 class _CrossAttention(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, v, sm_scale, lengths):
-        o, lse = _forward(q, k, v, sm_scale, lengths, True)
+    def forward(ctx, q, k, v, plan, sm_scale, lengths):
+        if plan is None:
+            o, lse = _nothing(q)
+        else:
+            o, lse = _forward(plan, q, k, v, sm_scale, lengths, True)
         ctx.save_for_backward(q, k, v, o, lse, lengths)
-        ctx.sm_scale = sm_scale
+        ctx.plan, ctx.sm_scale = plan, sm_scale
         ctx.set_materialize_grads(False)
         return o, lse
 
@@ -170,8 +170,18 @@ class _CrossAttention(torch.autograd.Function):
     def backward(ctx, go, glse):
         q, k, v, o, lse, lengths = ctx.saved_tensors
         if go is None and glse is None:
-            return None, None, None, None, None
-        return (*_backward(q, k, v, o, lse, go, glse, ctx.sm_scale, lengths, ctx.needs_input_grad[:3]), None, None)
+            return None, None, None, None, None, None
+        needs = ctx.needs_input_grad[:3]
+        if ctx.plan is None:
+            grads = [torch.zeros_like(t) if need else None for t, need in zip((q, k, v), needs)]
+        else:
+            grads = _backward(ctx.plan, q, k, v, o, lse, go, glse, ctx.sm_scale, lengths, needs)
+        return (*grads, None, None, None)
+
+
+def _nothing(q):
+    """(o, lse) of rows that see no key, or of no rows."""
+    return torch.zeros(q.shape, dtype=q.dtype, device=q.device), torch.full(q.shape[:3], -math.inf, dtype=torch.float32, device=q.device)
 
 
 def cross_attention(q, k, v, sm_scale, lengths=None, *, return_lse=False):
@@ -197,16 +207,23 @@ def cross_attention(q, k, v, sm_scale, lengths=None, *, return_lse=False):
     # tensors with a key that is kept have passed the checks, and only their addresses may differ
     key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype, q.device, k.device, v.device,
            (lengths.shape, lengths.stride(), lengths.dtype, lengths.device) if isinstance(lengths, torch.Tensor) else lengths is None)
-    if key not in _PLANS or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+    plan = _PLANS.get(key)
+    if plan is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
         _check(q, k, v, lengths)
         if lengths is not None:
             lengths = lengths.contiguous()
-        tensors = [t if t.numel() == 0 else _as_kernel_layout(t) for t in (q, k, v)]
-        if tensors[0] is q and tensors[1] is k and tensors[2] is v and (lengths is None or lengths.stride() == key[-1][1]):
-            _keep(key, True)
-        q, k, v = tensors
+        if q.numel() and k.numel():
+            tensors = [_as_kernel_layout(t) for t in (q, k, v)]
+            plan = _Plan(*tensors)
+            if tensors[0] is q and tensors[1] is k and tensors[2] is v and (lengths is None or lengths.stride() == key[-1][1]):
+                if len(_PLANS) > 4096:
+                    _PLANS.clear()
+                _PLANS[key] = plan
+            q, k, v = tensors
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _has_tangent(q, k, v):
-        o, lse = _CrossAttention.apply(q, k, v, sm_scale, lengths)
+        o, lse = _CrossAttention.apply(q, k, v, plan, sm_scale, lengths)
+    elif plan is None:
+        o, lse = _nothing(q)
     else:
-        o, lse = _forward(q, k, v, sm_scale, lengths, return_lse)
+        o, lse = _forward(plan, q, k, v, sm_scale, lengths, return_lse)
     return (o, lse) if return_lse else o
