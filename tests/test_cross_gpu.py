@@ -190,6 +190,19 @@ def test_non_finite_values_of_visible_keys(T):
     assert torch.equal(torch.isnan(o), torch.isnan(want)) and torch.equal(torch.isinf(o), torch.isinf(want))
 
 
+@pytest.mark.parametrize("N", [40, 700])
+@pytest.mark.parametrize("T", [2, 150])
+def test_rows_whose_scores_are_all_minus_infinity_are_nan(T, N):
+    q, k, v = _inputs(2, 2, 1, T, N, 64, BF16)
+    k[..., 0] = 1.0 + k[..., 0].abs()
+    want = cross_attention(q, k, v, 0.125)
+    q[1, 0, T - 1, 0] = -math.inf
+    o = cross_attention(q, k, v, 0.125)
+    assert torch.isnan(o[1, 0, T - 1]).all()
+    o[1, 0, T - 1] = want[1, 0, T - 1]
+    assert torch.equal(o, want)
+
+
 def _strided(t, kind):
     Z, H, N, D = t.shape
     if kind == "bshd":
