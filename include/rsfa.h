@@ -23,8 +23,9 @@
  *   rsfa_strerror             -> (no counterpart: the reference raises Python
  *                                exceptions; codes map to them in the wrapper)
  *
- * rsfa_rotary and rsfa_cache4_* (below) have no counterpart in the reference:
- * they are what a program that serves with the operator runs around it.
+ * rsfa_rotary, rsfa_cache4_*, rsfa_cross_* and rsfa_draft_tree (below) have no
+ * counterpart in the reference: they are what a program that serves with the
+ * operator, or trains a decoder with an encoder, runs around it.
  *
  * Conventions
  *   - All tensor pointers are device pointers owned by the caller; the library
