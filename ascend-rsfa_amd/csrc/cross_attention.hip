@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(64 * Few<D>::WAVES, Few<D>::OCC) cross_few_ker
     const int ld_row = lane >> 2, ld_col = ((lane & 3) ^ row_swz(ld_row)) * 8;
     auto load = [&](int tile, int buf) {
         const uint32_t dst = lds0 + buf * (2 * TILE);
-        const int last = len - 1 - tile;  // rows behind the last key repeat it
+        const int last = len - 1 - tile;  // rows behind the last key repeat it (compute hides them)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const int row = min(16 * b + ld_row, last);
@@ -137,7 +137,8 @@ __global__ void __launch_bounds__(64 * Few<D>::WAVES, Few<D>::OCC) cross_few_ker
 
     auto compute = [&](int buf, int tile) {
         const RSFA_LDS char* const kt = smem + wave * (4 * TILE) + buf * (2 * TILE);
-        const RSFA_LDS char* const vt = kt + TILE;
+        RSFA_LDS char* const vt = smem + wave * (4 * TILE) + buf * (2 * TILE) + TILE;
+        if (__builtin_expect(tile + KEYS > end, 0)) hide_rows<D, KEYS>(vt, end - tile, lane);
         f32x4 s[NB][2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -279,7 +280,7 @@ struct JoinParams {
     float* lse;
     int64_t o_st[3];
     const int32_t* lengths;
-    int32_t heads, t, n, splits, pp;
+    int32_t heads, t, splits, pp;
     int64_t rows;  // Z * heads * t
 };
 
@@ -521,7 +522,7 @@ int rsfa_cross_fwd(const rsfa_cross_args* a, void* stream) {
     JoinParams j{};
     j.part_o = part_o, j.part_ml = part_ml, j.o = a->o, j.lse = a->lse, j.lengths = a->lengths;
     for (int i = 0; i < 3; ++i) j.o_st[i] = a->o_stride[i];
-    j.heads = (int32_t)a->heads, j.t = (int32_t)a->t, j.n = (int32_t)a->n, j.splits = plan.splits;
+    j.heads = (int32_t)a->heads, j.t = (int32_t)a->t, j.splits = plan.splits;
     j.rows = a->z * a->heads * a->t;
     const int groups = 256 / (int)(a->head_dim / 4);
     j.pp = 1;

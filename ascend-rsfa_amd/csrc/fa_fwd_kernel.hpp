@@ -419,6 +419,18 @@ __device__ __forceinline__ void wait_loads_and_sync() {
     __syncthreads();
 }
 
+// Zeroes the rows from `first` on of a tile of ROWS rows in LDS.  What fills a tile of V up has weights of 0, and 0 x inf
+// would be NaN.  (Every wave that reads the tile calls it: its own writes precede its reads, and all write the same.)
+template <int D, int ROWS>
+__device__ __forceinline__ void hide_rows(RSFA_LDS char* tile, int first, int lane) {
+#pragma unroll
+    for (int blk = 0; blk < ROWS / 16; ++blk)
+        if (16 * blk + (lane >> 2) >= first)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) *(RSFA_LDS i32x4*)(tile + blk * (32 * D) + c * 1024 + 16 * lane) = (i32x4){0, 0, 0, 0};
+    asm volatile("" ::: "memory");
+}
+
 // Whether an instantiation runs the ping-pong schedule (8-wave workgroups,
 // three K/V buffers within the 160 KB of LDS of a CU).  At D = 256 (32-key
 // tiles) O^T and Q^T take 192 of the 256 VGPRs: the loop still fits (+2 %
@@ -1278,9 +1290,9 @@ fa_fwd_kernel(FwdParams p) {
             x8 pk[NKT][2];
             qk_part((uint32_t)(buf * BUF), kbase, nkt_act, sacc, masked, std::false_type());
             softmax_part(sacc, pk, masked);
+            if constexpr (CROSS && decltype(masked)::value) hide_rows<D, BN>(smem + buf * BUF + TILE, nk - kbase, lane);
             pv_part((uint32_t)(buf * BUF + TILE), nkt_act, pk, masked);
         };
-
 
         int j = j0;
         if constexpr (PP) {
@@ -1702,21 +1714,21 @@ fa_fwd_kernel(FwdParams p) {
                 constexpr int RPI = 64 / CH;   // rows per store instruction
                 const int rr = lane / CH, cc = (lane % CH) * 8;
                 const int row0 = m0 + wave * 32;
-    #pragma unroll
+#pragma unroll
                 for (int hf = 0; hf < D / OCOLS; ++hf) {
-    #pragma unroll
+#pragma unroll
                     for (int d = 0; d < DT; ++d)
-    #pragma unroll
+#pragma unroll
                         for (int a = 0; a < 4; ++a) {
                             const int col = 32 * d + 8 * a + 4 * hh;
                             if (col < D && col / OCOLS == hf) {
                                 x4 v4;
-    #pragma unroll
+#pragma unroll
                                 for (int e = 0; e < 4; ++e) v4[e] = (elem)(o[d][4 * a + e] * inv);
                                 *(RSFA_LDS x4*)(ow + l32 * OROW + (col - hf * OCOLS) * 2) = v4;
                             }
                         }
-    #pragma unroll
+#pragma unroll
                     for (int it = 0; it < 32 / RPI; ++it) {
                         const int r = it * RPI + rr;
                         const x8 v = *(const RSFA_LDS x8*)(ow + r * OROW + cc * 2);

@@ -190,6 +190,19 @@ def test_non_finite_values_of_visible_keys(T):
     assert torch.equal(torch.isnan(o), torch.isnan(want)) and torch.equal(torch.isinf(o), torch.isinf(want))
 
 
+@pytest.mark.parametrize("N", [33, 97, 1001])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("T", [1, 50, 1500])
+def test_infinite_values_of_the_last_key(T, D, N):
+    # (what fills its tile up has no part in the sums)
+    q, k, v = _inputs(2, 4, 2, T, N, D, BF16)
+    n = _ints([N, N - 9])
+    v[0, 0, N - 1], v[1, 1, N - 10, 5] = math.inf, -math.inf
+    o = cross_attention(q, k, v, 0.01, n)
+    want, _ = O.attend(q, k, v, n, 0.01)
+    assert torch.equal(torch.isnan(o), torch.isnan(want)) and torch.equal(torch.isinf(o), torch.isinf(want))
+
+
 @pytest.mark.parametrize("N", [40, 700])
 @pytest.mark.parametrize("T", [2, 150])
 def test_rows_whose_scores_are_all_minus_infinity_are_nan(T, N):
