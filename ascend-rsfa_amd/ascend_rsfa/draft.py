@@ -45,9 +45,10 @@ class DraftTree:
             raise ValueError("bits must be a GPU tensor")
         if not 1 <= bits.shape[1] <= _native.DRAFT_TOKENS or bits.shape[0] < 1:
             raise ValueError(f"a tree has 1 to {_native.DRAFT_TOKENS} tokens; got {tuple(bits.shape)}")
-        if not bits[0].is_contiguous() or (bits.shape[0] > 1 and bits.stride(0) < 0):
+        if not bits[0].is_contiguous():
             raise ValueError("the rows of a tree's bits must lie densely")
-        if depths is not None and (depths.dtype != torch.int32 or depths.shape != bits.shape[:2] or depths.device != bits.device):
+        if depths is not None and (not isinstance(depths, torch.Tensor) or depths.dtype != torch.int32 or depths.shape != bits.shape[:2]
+                                   or depths.device != bits.device):
             raise ValueError(f"depths must be int32 {tuple(bits.shape[:2])} on the device of bits")
         self.bits, self.depths = bits, depths
         self.trees, self.tokens = bits.shape[:2]

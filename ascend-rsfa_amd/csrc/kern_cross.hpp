@@ -2,7 +2,8 @@
 // are those of the non-causal calls (kern_d*.hip): 8 waves, 256 query rows, and 4 waves, 128 rows; at head
 // dim 32 the two of 128 rows.  Head dim 64 has room for three waves a SIMD with 4 (135 registers): keys are often
 // few here, and a third workgroup hides the others' starts (64 heads of 4096 tokens: 77 keys 30 -> 23 us, 512 keys
-// 55 -> 46).
+// 55 -> 46).  Bound by the matrix unit at head dim 128, 8 x 16 heads of 1024 tokens, 4096 keys 238 us, 1155 TFLOP/s, 8 x 32
+// of 2048 tokens 888 us, 1238; by it and the vector unit at 64, as the non-causal calls are.
 #pragma once
 
 #include "fa_fwd_kernel.hpp"

@@ -166,6 +166,25 @@ def test_positions_do_not_hide_the_context():
     _check(cache, got, q, O.visible(O.seen(parents)[None], [60], None, 60), 0.125)
 
 
+@pytest.mark.parametrize("T", [6, 40, 130])
+def test_into_an_output_of_the_callers_with_a_bound_on_the_lengths(T):
+    cache, q = _filled(2, 2, 900, 64, BF16, 1), _randn((2, 4, T, 64), 2, BF16)
+    parents = _parents(T, 3)
+    wide = torch.full((2, T, 4, 80), 7.0, dtype=BF16, device="cuda")
+    out = wide[..., :64].transpose(1, 2)
+    o, lse = cache.attend(q, _ints([T + 300, T]), True, 0.1, tree=draft_tree(_ints(parents)), max_length=T + 300, out=out, return_lse=True)
+    assert o is out and (wide[..., 64:] == 7.0).all()
+    _check(cache, (o, lse), q, O.visible(O.seen(parents)[None].repeat(2, 1, 1), [T + 300, T], None, 900), 0.1)
+
+
+def test_keep_with_counts_outside_and_a_token_twice():
+    cache = _filled(3, 2, 60, 64, BF16, 4)
+    tokens, lengths, counts = [[4, 4, 4], [2, 2, 9], [0, 1, 2]], [20, 30, 40], [99, 3, -5]
+    want = _expect_kept(cache, tokens, lengths, [3, 3, 0], lengths)
+    cache.keep(_ints(tokens), _ints(lengths), counts=_ints(counts))
+    _same(cache, want)
+
+
 def test_a_chain_sees_what_causal_tokens_see():
     for T in (7, 60):
         cache = _filled(2, 2, 500, 128, BF16, 1)
@@ -290,7 +309,7 @@ def test_refusals():
                 lambda: cache.attend(q, n, True, 1.0, tree=tree, positions=n), lambda: cache.attend(q[:, :, :5], n, True, 1.0, tree=tree),
                 lambda: cache.attend(q, n, True, 1.0, tree=three), lambda: draft_tree(_ints([[]])), lambda: draft_tree(_ints([0] * 513)),
                 lambda: DraftTree(tree.bits.expand(1, 6, 1).transpose(0, 1).contiguous().transpose(0, 1)[:, ::2]),
-                lambda: DraftTree(tree.bits, tree.depths.long()), lambda: cache.keep(path.cpu(), n), lambda: cache.keep(path, 41),
+                lambda: DraftTree(tree.bits, tree.depths.long()), lambda: DraftTree(tree.bits, [[0] * 6]), lambda: cache.keep(path.cpu(), n), lambda: cache.keep(path, 41),
                 lambda: cache.keep(torch.zeros((2, 513), dtype=torch.int32).cuda(), n)):
         with pytest.raises(ValueError):
             bad()
