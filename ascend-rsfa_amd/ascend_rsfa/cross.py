@@ -52,7 +52,8 @@ def _on_device(index, fn, *args):
 
 
 def _launch(index, name, args):
-    status = _on_device(index, _function(name), args, torch._C._cuda_getCurrentRawStream(index))
+    fn, stream = _FUNCTIONS.get(name) or _function(name), torch._C._cuda_getCurrentRawStream(index)
+    status = fn(args, stream) if index == torch.cuda.current_device() else _on_device(index, fn, args, stream)
     if status:
         _raise_for(status)
 
@@ -155,28 +156,30 @@ def _check(q, k, v, lengths):
 class _CrossAttention(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, q, k, v, plan, sm_scale, lengths):
+    def forward(ctx, q, k, v, plan, sm_scale, lengths, return_lse):
         if plan is None:
             o, lse = _nothing(q)
         else:
             o, lse = _forward(plan, q, k, v, sm_scale, lengths, True)
         ctx.save_for_backward(q, k, v, o, lse, lengths)
         ctx.plan, ctx.sm_scale = plan, sm_scale
+        if not return_lse:
+            return o
         ctx.set_materialize_grads(False)
         return o, lse
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, go, glse):
+    def backward(ctx, go, glse=None):
         q, k, v, o, lse, lengths = ctx.saved_tensors
         if go is None and glse is None:
-            return None, None, None, None, None, None
+            return (None,) * 7
         needs = ctx.needs_input_grad[:3]
         if ctx.plan is None:
             grads = [torch.zeros_like(t) if need else None for t, need in zip((q, k, v), needs)]
         else:
             grads = _backward(ctx.plan, q, k, v, o, lse, go, glse, ctx.sm_scale, lengths, needs)
-        return (*grads, None, None, None)
+        return (*grads, None, None, None, None)
 
 
 def _nothing(q):
@@ -221,8 +224,8 @@ def cross_attention(q, k, v, sm_scale, lengths=None, *, return_lse=False):
                 _PLANS[key] = plan
             q, k, v = tensors
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _has_tangent(q, k, v):
-        o, lse = _CrossAttention.apply(q, k, v, plan, sm_scale, lengths)
-    elif plan is None:
+        return _CrossAttention.apply(q, k, v, plan, sm_scale, lengths, bool(return_lse))
+    if plan is None:
         o, lse = _nothing(q)
     else:
         o, lse = _forward(plan, q, k, v, sm_scale, lengths, return_lse)
