@@ -201,8 +201,9 @@ def cross_attention(q, k, v, sm_scale, lengths=None, *, return_lse=False):
     ``lse``: the natural logarithm of each row's sum of exponentials, float32 [Z, heads, T].
 
     Differentiable once in q, k and v, through o and lse; gradients do not change from call to call (no atomics).
-    For the gradients' products softmax weights and their gradients are rounded to the dtype.  Keys past a length
-    have gradients of 0.
+    For the gradients' products softmax weights and their gradients are rounded to the dtype, in float16 scaled by
+    a power of two first, which leaves room for states v of some thousands (beyond, gradients may overflow).  Keys
+    past a length have gradients of 0.
     """
     sm_scale = float(sm_scale)
     if math.isnan(sm_scale):

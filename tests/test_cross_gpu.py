@@ -167,6 +167,15 @@ def test_gradients_of_every_size(T, D, std):
         _check(q, k, v, D ** -0.5, None, go, _randn(q.shape[:3], 5, torch.float32, std))
 
 
+@pytest.mark.parametrize("std", [2.0 ** 4, 2.0 ** 7, 2.0 ** 9])
+@pytest.mark.parametrize("T, D", [(3, 64), (90, 32), (200, 128), (70, 256)])
+def test_gradients_over_large_states(T, D, std):
+    for dtype in (F16, BF16):
+        q, k, v = _inputs(2, 4, 2, T, 200, D, dtype)
+        for scale in (D ** -0.5, 1.0):  # (weights spread, and on few keys)
+            _check(q, k, (v * std).to(dtype), scale, _ints([200, 7]), _randn(q.shape, 4, dtype, 2.0 ** -10))
+
+
 @pytest.mark.parametrize("T", [2, 90])
 def test_one_score_far_above_the_rest(T):
     # each row's weight on one key, anywhere along a long row, and rows of equal scores
