@@ -494,13 +494,16 @@ cross_dq_kernel(BwdParams p) {
         if (F16 && w.lane == 0 && !mine) p.top[((int64_t)z * p.heads + hq) * (p.tp / 32) + first / 32] = 0.0f;
     }
     if (!p.gq) return;
-    // -delta is what the products dO V^T start from: 16 registers instead of an addition a score (bf16, eight sequences of
-    // 1500 keys, 1000 rows of 16 heads, D = 32 37.5 -> 35.0 us; four of 3000 keys, D = 64 57.5 -> 55.5, D = 128 95.5 -> 93.5; at D = 256 no
-    // difference.  With few keys, 77, D = 64, 30.0 -> 30.8)
-    f32x16 start;
+    // -delta is what the products dO V^T start from where there is room for it: 16 registers instead of an addition a score (bf16,
+    // eight sequences of 1500 keys, 1000 rows of 16 heads, D = 32 37.5 -> 35.0 us; four of 3000 keys, D = 128 95.5 -> 93.5; at D = 256
+    // no difference.  D = 64 has no room with four waves a SIMD: float16, 64 heads of 4096 rows, 77 keys 32.2 -> 37.4)
+    constexpr bool START = D == 32 || D == 128;
+    f32x16 start = {};
+    if constexpr (START) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) start[r] = nd;
-    asm volatile("" : "+v"(start));  // (kept, and not formed again for each tile)
+        for (int r = 0; r < 16; ++r) start[r] = nd;
+        asm volatile("" : "+v"(start));  // (kept, and not formed again for each tile)
+    }
     if (i < end && !once) load(i, 0);
     for (int buf = 0; i < end; ++i, buf ^= 1) {
         wait_loads_and_sync();
@@ -512,7 +515,7 @@ cross_dq_kernel(BwdParams p) {
             f32x16 s = {}, x = start;
             scores(i, st, buf, s, x);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -l2)) * x[r];
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -l2)) * (START ? x[r] : x[r] + nd);
             x8 b[2];
             pack<T>(s, b);
             columns_product<T, D>(kt + st * 2 * BLK, w, b, dq);
