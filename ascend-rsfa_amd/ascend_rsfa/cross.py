@@ -81,11 +81,12 @@ def _struct(kind, tensors, q, k, workspace):
 class _Plan:
     """A call's argument structs, for tensors in the kernels' layout that are not empty."""
 
-    __slots__ = ("index", "head", "sizes", "nbytes", "like", "backward")
+    __slots__ = ("index", "head", "sizes", "nbytes", "like", "kinds", "backward")
 
     def __init__(self, q, k, v):
         o, self.like = _empty_rows(q)
         self.index = q.device.index
+        self.kinds = tuple((t.shape, t.dtype, t.device) for t in (q, k, v, q, q))  # of q, k, v, o and the gradient of o
         self.head, self.sizes, self.nbytes = _struct(_F, {"q": q, "k": k, "v": v, "o": o}, q, k, "rsfa_cross_fwd_workspace_bytes")
         self.backward = {}
 
@@ -102,26 +103,42 @@ def _forward(plan, q, k, v, scale, lengths, want_lse):
     return o, lse
 
 
+def _check_saved(plan, rows, stats, lengths):
+    """q, k, v, o and the gradient of o; lse and its gradient; lengths: of the shapes, types and device that the kernels are told."""
+    shape, _, device = plan.kinds[0]
+    want = plan.kinds + (((shape[:3], torch.float32, device),) * 2) + ((shape[:1], torch.int32, device),)
+    for t, (of, dtype, on) in zip((*rows, *stats, lengths), want):
+        if t is not None and (t.shape != of or t.dtype != dtype or t.device != on):
+            raise RuntimeError(f"a saved tensor or a gradient of {dtype} {tuple(of)} on {on} came back as {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
 def _backward(plan, q, k, v, o, lse, go, glse, scale, lengths, needs):
     """The gradients of q, k and v, those that ``needs`` names (None for the others)."""
     if go is None:
         go = torch.zeros_like(o)
     if glse is not None:
         glse = glse.contiguous()
-    key = (go.stride(), needs)
+    # Saved tensors need not be those that were saved: a hook (one that offloads them, say) may bring back others, of other
+    # strides.  So all that the struct says of them is looked at, and tensors whose key is kept differ in their addresses only.
+    key = (needs, q.stride(), k.stride(), v.stride(), o.stride(), go.stride(), lse.stride(), q.shape, k.shape, v.shape, o.shape, go.shape,
+           lse.shape, q.dtype, k.dtype, v.dtype, o.dtype, go.dtype, lse.dtype, q.device, k.device, v.device, o.device, go.device, lse.device,
+           None if glse is None else (glse.shape, glse.dtype, glse.device),
+           None if lengths is None else (lengths.shape, lengths.stride(), lengths.dtype, lengths.device))
     kept = plan.backward.get(key)
-    if kept is None or go.data_ptr() & 15:
-        go_ = _as_kernel_layout(go)
+    if kept is None or (q.data_ptr() | k.data_ptr() | v.data_ptr() | o.data_ptr() | go.data_ptr()) & 15:
+        came = (q, k, v, o, go, lse, lengths)
+        _check_saved(plan, came[:5], (lse, glse), lengths)
+        q, k, v, o, go = (_as_kernel_layout(t) for t in came[:5])
+        lse, lengths = lse.contiguous(), None if lengths is None else lengths.contiguous()
         grads = [_empty_rows(t) if need else (None, True) for t, need in zip((q, k, v), needs)]
         like = all(x for _, x in grads)
         grads = [g for g, _ in grads]
-        kept = _struct(_B, {"q": q, "k": k, "v": v, "o": o, "grad_o": go_, "grad_q": grads[0], "grad_k": grads[1], "grad_v": grads[2]},
+        kept = _struct(_B, {"q": q, "k": k, "v": v, "o": o, "grad_o": go, "grad_q": grads[0], "grad_k": grads[1], "grad_v": grads[2]},
                        q, k, "rsfa_cross_bwd_workspace_bytes")
-        if go_ is go and like:
+        if like and all(a is b for a, b in zip(came, (q, k, v, o, go, lse, lengths))):
             if len(plan.backward) > 64:
                 plan.backward.clear()
             plan.backward[key] = kept
-        go = go_
     else:
         grads = [torch.empty_like(t) if need else None for t, need in zip((q, k, v), needs)]
     head, sizes, nbytes = kept

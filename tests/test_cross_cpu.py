@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from ascend_rsfa import _native
+from ascend_rsfa import _native, cross
 from ascend_rsfa.cross import cross_attention
 from cross_launches import variants
 from oracle import cross as O
@@ -112,3 +112,96 @@ def test_the_shapes_of_the_definitions_test_run_every_backward_variant(tmp_path)
             assert names[0] == "cross_dq_kernel" and set(names[1:dq] + names[dq + 1:]) <= {"sum_parts_kernel"}
             seen.add((dq > 1, len(names) > dq + 1))
         assert {x for x, _ in seen} == {x for _, x in seen} == {False, True}
+
+
+class _Calls:
+    """cross_attention on the CPU with its launches recorded: what each would read, by its addresses and strides."""
+
+    def __init__(self, monkeypatch):
+        self.tensors, self.calls = {}, []
+        monkeypatch.setattr(cross, "_PLANS", {})
+        monkeypatch.setattr(cross, "_check", lambda *a: None)
+        monkeypatch.setattr(cross, "_on_device", lambda index, fn, *a: fn(*a))
+        monkeypatch.setattr(cross, "_launch", self.launch)
+
+    def launch(self, index, name, args):
+        if name == "rsfa_cross_bwd":
+            self.calls.append(_native.CrossBwdArgs.from_buffer_copy(args))
+
+    def known(self, *tensors):
+        self.tensors.update({t.data_ptr(): t for t in tensors})
+
+    def last_reads_them(self):
+        """The last backward call's strides are those of the tensors at its addresses."""
+        a = self.calls[-1]
+        return all(tuple(getattr(a, n + "_stride")) == self.tensors[getattr(a, n)].stride() for n in ("q", "k", "v", "o") if getattr(a, n) in self.tensors)
+
+
+def _fused(Z, N, H, D):
+    """K and V, parts of one projection."""
+    big = torch.randn((Z, N, 2, H, D)).to(torch.bfloat16)
+    return big[:, :, 0].transpose(1, 2).requires_grad_(), big[:, :, 1].transpose(1, 2).requires_grad_()
+
+
+@pytest.mark.parametrize("order", ["kept first", "hook first"])
+def test_saved_tensors_that_a_hook_brings_back_in_another_layout(order, monkeypatch):
+    calls = _Calls(monkeypatch)
+    q = torch.randn((2, 7, 4, 64)).to(torch.bfloat16).transpose(1, 2).requires_grad_()
+    k, v = _fused(2, 5, 4, 64)
+    go = torch.ones((2, 4, 7, 64), dtype=torch.bfloat16)
+    back = []
+
+    def unpack(t):
+        back.append(t)
+        if t.dim() == 4:
+            calls.known(t)
+        return t
+
+    def step(hook):
+        if hook:
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(memory_format=torch.contiguous_format), unpack):
+                o = cross_attention(q, k, v, 0.125)
+        else:
+            o = cross_attention(q, k, v, 0.125)
+            calls.known(q, k, v, o)
+        torch.autograd.grad(o, (q, k, v), go)
+        assert calls.last_reads_them(), (order, hook)
+
+    for hook in (False, True, False) if order == "kept first" else (True, False, True):
+        step(hook)
+    assert len(calls.calls) == 3 and any(t.stride() != k.stride() for t in back if t.shape == k.shape)
+
+
+def test_saved_tensors_that_are_not_aligned_are_copied(monkeypatch):
+    calls = _Calls(monkeypatch)
+    q, k, v = (torch.randn((1, 2, n, 32)).to(torch.float16).requires_grad_() for n in (3, 6, 6))
+    go = torch.ones((1, 2, 3, 32), dtype=torch.float16)
+
+    def shifted(t):
+        big = torch.empty(t.numel() + 1, dtype=t.dtype)
+        return big[1:].view(t.shape).copy_(t)
+
+    for _ in range(2):
+        torch.autograd.grad(cross_attention(q, k, v, 1.0), (q, k, v), go)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, shifted):
+            o = cross_attention(q, k, v, 1.0)
+        torch.autograd.grad(o, (q, k, v), go)
+        a = calls.calls[-1]
+        assert not any(getattr(a, n) % 16 for n in ("q", "k", "v", "o"))
+
+
+@pytest.mark.parametrize("wrong", [lambda t: t[..., :t.shape[-1] // 2], lambda t: t.double(), lambda t: t.to("meta"), lambda t: t[:1]])
+def test_saved_tensors_that_come_back_as_others_are_refused(wrong, monkeypatch):
+    calls = _Calls(monkeypatch)
+    q, k, v = (torch.randn((2, 2, n, 32)).to(torch.float16).requires_grad_() for n in (3, 6, 6))
+    n = torch.tensor([6, 4], dtype=torch.int32)
+    for _ in range(2):
+        torch.autograd.grad(cross_attention(q, k, v, 1.0, n).sum(), (q, k, v))
+    done = len(calls.calls)
+    for which in range(6):  # of q, k, v, o, lse, lengths, in the order in which they come back
+        count = iter(range(6))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: wrong(t) if next(count) == which else t):
+            o = cross_attention(q, k, v, 1.0, n)
+        with pytest.raises(RuntimeError, match="came back as"):
+            torch.autograd.grad(o.sum(), (q, k, v))
+    assert len(calls.calls) == done

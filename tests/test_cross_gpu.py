@@ -414,3 +414,31 @@ def test_empty_calls():
     x = k.clone().requires_grad_()
     g, = torch.autograd.grad(cross_attention(q[:, :, :0], x, v, 1.0).sum(), x)
     assert (g == 0).all()
+
+
+@pytest.mark.parametrize("pin", [False, True])
+@pytest.mark.parametrize("order", ["kept first", "hook first"])
+@pytest.mark.parametrize("kind", ["bshd", "wide"])
+def test_saved_tensors_kept_on_the_host(kind, order, pin):
+    # a hook may bring saved tensors back in another layout; sizes of this test's own, so that nothing of them is kept before
+    T, N = 61 + 2 * pin, 131 + (order == "hook first") + 2 * (kind == "wide")
+    plain = _inputs(2, 4, 2, T, N, 64, BF16)
+    go, glse, n = _randn(plain[0].shape, 4, BF16), _randn(plain[0].shape[:3], 5, torch.float32), _ints([N, 77])
+    q, k, v = (_strided(t, kind).requires_grad_() for t in plain)
+
+    def step(hook):
+        if not hook:
+            return torch.autograd.grad(cross_attention(q, k, v, 0.125, n, return_lse=True), (q, k, v), (go, glse))
+        with torch.autograd.graph.save_on_cpu(pin_memory=pin):
+            o = cross_attention(q, k, v, 0.125, n, return_lse=True)
+        return torch.autograd.grad(o, (q, k, v), (go, glse))
+
+    want = None
+    for hook in (False, True, False, True) if order == "kept first" else (True, False, True, False):
+        got = step(hook)
+        if want is None:
+            bounds = O.expect(*plain, n.tolist(), 0.125, go, glse)
+            for name, g in zip(("dq", "dk", "dv"), got):
+                _hold(name, g, bounds[name])
+            want = got
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), (order, hook)
