@@ -35,6 +35,9 @@ class DraftTree:
     ``j // 32`` of row i is set.  ``depths``: int32 [trees, T], the number of a token's ancestors, or
     None.  One tree serves all sequences of a call, or there is one for each.  ``draft_tree`` makes one from parents;
     ``DraftTree(bits)`` takes a table of the caller's own (drafts that are not a tree).
+
+    A tree stays as it was made: its attributes are read-only, as the kernels read as many words as it had then.
+    Programs may write into ``bits`` (for another step of a captured graph, say).
     """
 
     def __init__(self, bits, depths=None):
@@ -50,8 +53,13 @@ class DraftTree:
         if depths is not None and (not isinstance(depths, torch.Tensor) or depths.dtype != torch.int32 or depths.shape != bits.shape[:2]
                                    or depths.device != bits.device):
             raise ValueError(f"depths must be int32 {tuple(bits.shape[:2])} on the device of bits")
-        self.bits, self.depths = bits, depths
-        self.trees, self.tokens = bits.shape[:2]
+        self._bits, self._depths = bits, depths
+        self._trees, self._tokens = bits.shape[:2]
+
+    bits = property(lambda self: self._bits)
+    depths = property(lambda self: self._depths)
+    trees = property(lambda self: self._trees)
+    tokens = property(lambda self: self._tokens)
 
 
 def draft_tree(parents):

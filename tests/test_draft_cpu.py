@@ -85,6 +85,13 @@ def test_cpu_tensors_are_refused():
         draft_tree(torch.zeros(4))
 
 
+@pytest.mark.parametrize("name", ["bits", "depths", "trees", "tokens"])
+def test_a_trees_attributes_are_read_only(name):
+    tree = DraftTree.__new__(DraftTree)
+    with pytest.raises(AttributeError):
+        setattr(tree, name, None)
+
+
 def test_the_definitions():
     parents = [-1, 0, 0, 2, -1]
     assert O.depths(parents) == [0, 1, 1, 2, 0]

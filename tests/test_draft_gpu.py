@@ -325,3 +325,13 @@ def test_refusals():
     cache.keep(torch.empty((2, 0), dtype=torch.int32).cuda(), n)
     _same(cache, want)
     assert cache.attend(q[:, :, :0], n, True, 1.0).shape == (2, 4, 0, 64)
+
+
+def test_a_tree_stays_as_it_was_made():
+    cache, q = _filled(2, 2, 90, 64, F16, 1), _randn((2, 4, 70, 64), 2, F16)
+    tree = draft_tree(_ints(_parents(70, 1)))
+    want = cache.attend(q, 90, True, 0.1, tree=tree)
+    for name, x in (("bits", tree.bits[:, :1, :1].clone()), ("depths", None), ("trees", 2), ("tokens", 3)):
+        with pytest.raises(AttributeError):
+            setattr(tree, name, x)
+    assert torch.equal(cache.attend(q, 90, True, 0.1, tree=tree), want)
