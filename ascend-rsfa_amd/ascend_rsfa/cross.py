@@ -219,7 +219,7 @@ def cross_attention(q, k, v, sm_scale, lengths=None, *, return_lse=False):
 
     Differentiable once in q, k and v, through o and lse; gradients do not change from call to call (no atomics).
     For the gradients' products softmax weights and their gradients are rounded to the dtype, in float16 scaled by
-    a power of two first, which leaves room for states v of some thousands (beyond, gradients may overflow).  Keys
+    powers of two first that keep them within the type, whatever the sizes of v and of o's gradient.  Keys
     past a length have gradients of 0.
     """
     sm_scale = float(sm_scale)

@@ -11,9 +11,13 @@
 // Where blocks are too few for the chip each pass is cut into parts, which sum_parts_kernel adds up.
 //
 // P and dS are rounded to the type for the products with rows (half a step of each, as the matrix unit takes 16-bit
-// operands at sixteen times the rate of 32-bit ones); all else is in 32 bits.  float16 ends at 2^-14 where gradients
-// are often smaller still: P is scaled by 2^k there, with k from the largest |dO| and |dlse| of the row (dQ) or of the
-// key head's rows (dK, dV), so that dS lies in the middle of the type's range; it goes into the exponent and out at the end.
+// operands at sixteen times the rate of 32-bit ones); all else is in 32 bits.  float16 ends at 2^-14 and at 2^16, where
+// gradients are often smaller or larger: P is scaled by 2^12 there, and dS by 2^k with a k for which it stays below 2^13 (so that
+// there is room for weights above 1, as the roundings of scores of some millions may give).  As P <= 1 and
+// |dO v| <= |dO| |v| (2-norms), |dS| of a key (dK) is at most |v| times the largest |dO| of the key head's rows plus
+// their largest |delta|, which the dQ kernel leaves per 32 rows.  For a row (dQ) the largest |v| is not known ahead: k goes by the
+// first 32 keys, with room for later ones 2^SPARE times as large; where that was not enough the sums are not finite, and the
+// workgroup finds the largest |v| and passes over its keys again.  2^k goes into the exponent and out at the end.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -44,7 +48,7 @@ struct BwdParams {
     float c, scale;
     uint32_t neg;      // sign of sm_scale, as a mask for a pair of values
     float *nl, *nd;    // [Z * heads][tp]: -lse / (c ln 2), -delta; rows past t: -inf, 0
-    float* top;        // [Z * heads][tp / 32]: largest |dO|, |dlse| of 32 rows (float16)
+    float2* top;       // float16: [Z * heads][tp / 32]: largest |dO| and |delta| of 32 rows
     float* part[2];    // splits > 1: [splits][rows][D] of dK and dV, or of dQ
 };
 
@@ -60,11 +64,23 @@ __device__ __forceinline__ void dma4(const void* sbase, uint32_t voff_bytes, uin
                  : "memory");
 }
 
-// k of the scale 2^k of float16 weights, for a largest |dO| and |dlse|: dS = P (dO v - delta) is then below 2^4 |v| of a few values'
-// sums, and P, at most 2^15, is whole down to 2^-18 (dO of 1) or less.
-__device__ __forceinline__ float weight_exponent(float top) {
-    const int e = (int)(__float_as_uint(top) >> 23 & 255) - 127;
-    return (float)max(0, min(3 - e, 15));
+// The greatest k for which 2^k x stays below 2^13, within -100 .. 40, where P 2^k and its sums are far from the ends of 32 bits.
+__device__ __forceinline__ float room(float x) {
+    const int e = (int)(__float_as_uint(x) >> 23 & 255) - 127;
+    return (float)max(-100, min(12 - e, 40));
+}
+
+constexpr float P_ROOM = 12.0f;  // of P itself
+constexpr float SPARE = 6.0f;
+
+template <class X8, int N>
+__device__ __forceinline__ float sum_of_squares(const X8 (&x)[N]) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < N; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)x[s][e], (float)x[s][e], sum);
+    return sum;
 }
 
 // Tiles of rows in LDS have the forward kernel's layout (fa_fwd_kernel.hpp): 16-row blocks of planes of 32 columns,
@@ -241,15 +257,18 @@ cross_dkv_kernel(BwdParams p) {
         for (int s = 0; s < KST; ++s) kf[s] = __builtin_bit_cast(x8, __builtin_bit_cast(u32x4, kf[s]) ^ p.neg);
     }
     __syncthreads();  // (the tiles go where these rows were)
-    float k2 = 0.0f;
+    float k2 = 0.0f, up = 1.0f;  // float16: of dS and, times up, of P
     if constexpr (F16) {
         const int n = p.group * (p.tp / 32);
-        const float* top = p.top + (int64_t)kh * n;
-        float most = 0.0f;
-        for (int j = w.lane; j < n; j += 64) most = fmaxf(most, top[j]);
+        const float2* const top = p.top + (int64_t)kh * n;
+        float go = 0.0f, delta = 0.0f;
+        for (int j = w.lane; j < n; j += 64) go = fmaxf(go, top[j].x), delta = fmaxf(delta, top[j].y);
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-        k2 = weight_exponent(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(most))));
+        for (int d = 1; d < 64; d <<= 1) go = fmaxf(go, __shfl_xor(go, d)), delta = fmaxf(delta, __shfl_xor(delta, d));
+        float v2 = mine ? sum_of_squares(vf) : 0.0f;
+        v2 += __shfl_xor(v2, 32);
+        k2 = room(go * __builtin_sqrtf(v2) + delta);
+        up = __builtin_amdgcn_exp2f(P_ROOM - k2);
     }
     f32x16 dk[DT], dv[DT];
 #pragma unroll
@@ -309,7 +328,14 @@ cross_dkv_kernel(BwdParams p) {
             rows_product<T, D>(qt + st * 2 * BLK, w, kf, s);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(F16 ? __builtin_fmaf(s[r], p.c, k2) : s[r] * p.c);
-            pack<T>(s, b);
+            if constexpr (F16) {
+                f32x16 x;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = s[r] * up;
+                pack<T>(x, b);
+            } else {
+                pack<T>(s, b);
+            }
             columns_product<T, D>(gt + st * 2 * BLK, w, b, dv);
             stats(gt + TILE + 256 + st * 128, x);
             rows_product<T, D>(gt + st * 2 * BLK, w, vf, x);
@@ -319,12 +345,12 @@ cross_dkv_kernel(BwdParams p) {
             columns_product<T, D>(qt + st * 2 * BLK, w, b, dk);
         }
     }
-    const float unscale = __builtin_amdgcn_exp2f(-k2);
+    const float unscale = __builtin_amdgcn_exp2f(-k2), unscale_p = F16 ? __builtin_amdgcn_exp2f(-P_ROOM) : 1.0f;
     if (p.splits > 1) {
         if (key >= nk) return;  // (the sum of the parts writes 0 there)
         const int64_t at = (((int64_t)blockIdx.y * p.z * p.key_heads + kh) * p.n + key) * D;
         if (p.gk) store_part<D>(p.part[0] + at, dk, unscale, w.hh);
-        if (p.gv) store_part<D>(p.part[1] + at, dv, unscale, w.hh);
+        if (p.gv) store_part<D>(p.part[1] + at, dv, unscale_p, w.hh);
         return;
     }
     if (key >= nk) {
@@ -335,7 +361,7 @@ cross_dkv_kernel(BwdParams p) {
     }
     __syncthreads();  // (every wave is done with the tiles)
     if (p.gk) store_rows<T, D>((elem*)p.gk + z * p.gk_st[0] + h * p.gk_st[1] + first * p.gk_st[2], p.gk_st[2], p.n - first, dk, p.scale * unscale, w, own);
-    if (p.gv) store_rows<T, D>((elem*)p.gv + z * p.gv_st[0] + h * p.gv_st[1] + first * p.gv_st[2], p.gv_st[2], p.n - first, dv, unscale, w, own);
+    if (p.gv) store_rows<T, D>((elem*)p.gv + z * p.gv_st[0] + h * p.gv_st[1] + first * p.gv_st[2], p.gv_st[2], p.n - first, dv, unscale_p, w, own);
 }
 
 // dQ of 128 rows, 32 of each wave, held transposed (dQ^T = K^T dS^T), rows in the lanes: a row's
@@ -373,7 +399,7 @@ cross_dq_kernel(BwdParams p) {
     const int first = block * 128 + wave * 32;  // the wave's first row
     RSFA_LDS char* const own = smem + wave * TILE;
     x8 qf[KST], gf[KST];
-    float l2 = 0.0f, nd = 0.0f, k2 = 0.0f, gl = 0.0f;
+    float l2 = 0.0f, nd = 0.0f, gl = 0.0f, go = 0.0f;
     if (mine) {
         const int64_t head = (int64_t)z * p.heads + hq;
         const int left = p.t - first;
@@ -414,18 +440,9 @@ cross_dq_kernel(BwdParams p) {
         const float s0 = __shfl(sum[0], 4 * w.l16), s1 = __shfl(sum[1], 4 * w.l16);
         nd = gl - (w.l32 < 16 ? s0 : s1);
         if constexpr (F16) {
-            float most = __builtin_fabsf(gl);
-#pragma unroll
-            for (int s = 0; s < KST; ++s)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, __builtin_fabsf((float)gf[s][e]));
-            most = fmaxf(most, __shfl_xor(most, 32));
-            k2 = weight_exponent(most);
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
-            if (blockIdx.y == 0 && w.lane == 0) p.top[head * (p.tp / 32) + first / 32] = most;
+            go = sum_of_squares(gf);
+            go = __builtin_sqrtf(go + __shfl_xor(go, 32));
         }
-        l2 -= k2;
     }
     __syncthreads();  // (the tiles go where these rows were)
     f32x16 dq[DT];
@@ -470,6 +487,7 @@ cross_dq_kernel(BwdParams p) {
     // With few keys o is large and its rounding, in delta, would be as large as that of dS (8 keys, bfloat16: an error of dQ
     // against 64 bits of 0.0026 relative to it, 0.0024 without, 0.0017 being its own rounding): delta is then rowsum(P (dO V^T)).
     const bool once = all == 1 && i == 0;
+    float most = 0.0f;  // float16: a bound on the row's |dO v|
     if (once) {
         load(0, 0);
         wait_loads_and_sync();
@@ -480,18 +498,29 @@ cross_dq_kernel(BwdParams p) {
                 f32x16 s = {}, x = {};
                 scores(0, st, 0, s, x);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sum = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -l2)), x[r], sum);
+                for (int r = 0; r < 16; ++r) {
+                    sum = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -l2)), x[r], sum);
+                    if (F16) most = fmaxf(most, __builtin_fabsf(x[r]));
+                }
             }
             sum += __shfl_xor(sum, 32);
-            nd = gl - sum * __builtin_amdgcn_exp2f(-k2);
+            nd = gl - sum;
+            most = fmaxf(most, __shfl_xor(most, 32));
         }
     }
     // for dK and dV: rows behind the last have weights of 0
     if (blockIdx.y == 0 && w.hh == 0 && row < p.tp) {
         const int64_t at = ((int64_t)z * p.heads + hq) * p.tp + row;
-        p.nl[at] = row < p.t ? -(l2 + k2) / p.c : -INFINITY;
+        p.nl[at] = row < p.t ? -l2 / p.c : -INFINITY;
         p.nd[at] = row < p.t ? nd : 0.0f;
-        if (F16 && w.lane == 0 && !mine) p.top[((int64_t)z * p.heads + hq) * (p.tp / 32) + first / 32] = 0.0f;
+    }
+    if constexpr (F16) {
+        if (blockIdx.y == 0) {
+            float a = go, b = __builtin_fabsf(nd);  // (0 for waves behind the last row)
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) a = fmaxf(a, __shfl_xor(a, d)), b = fmaxf(b, __shfl_xor(b, d));
+            if (w.lane == 0 && first < p.tp) p.top[((int64_t)z * p.heads + hq) * (p.tp / 32) + first / 32] = make_float2(a, b);
+        }
     }
     if (!p.gq) return;
     // -delta is what the products dO V^T start from where there is room for it: 16 registers instead of an addition a score (bf16,
@@ -505,21 +534,79 @@ cross_dq_kernel(BwdParams p) {
         asm volatile("" : "+v"(start));  // (kept, and not formed again for each tile)
     }
     if (i < end && !once) load(i, 0);
-    for (int buf = 0; i < end; ++i, buf ^= 1) {
-        wait_loads_and_sync();
-        if (i + 1 < end) load(i + 1, buf ^ 1);
-        if (!mine) continue;
-        const RSFA_LDS char* const kt = smem + buf * BUF;
+    float k2 = 0.0f;  // float16: dS is scaled by 2^k2
+    bool again = false;
+    if constexpr (F16) {
+        if (i < end && !once) {
+            wait_loads_and_sync();
+            if (mine) {
+                f32x16 x = {};
+                rows_product<T, D>(smem + TILE, w, gf, x);
 #pragma unroll
-        for (int st = 0; st < KB / 32; ++st) {
-            f32x16 s = {}, x = start;
-            scores(i, st, buf, s, x);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -l2)) * (START ? x[r] : x[r] + nd);
-            x8 b[2];
-            pack<T>(s, b);
-            columns_product<T, D>(kt + st * 2 * BLK, w, b, dq);
+                for (int r = 0; r < 16; ++r) most = fmaxf(most, __builtin_fabsf(x[r]));
+                most = fmaxf(most, __shfl_xor(most, 32));
+            }
         }
+        k2 = room(most + __builtin_fabsf(nd)) - (once ? 0.0f : SPARE);
+        l2 -= k2;
+    }
+    for (const int begin = i;; i = begin) {
+        for (int buf = 0; i < end; ++i, buf ^= 1) {
+            wait_loads_and_sync();
+            if (i + 1 < end) load(i + 1, buf ^ 1);
+            if (!mine) continue;
+            const RSFA_LDS char* const kt = smem + buf * BUF;
+#pragma unroll
+            for (int st = 0; st < KB / 32; ++st) {
+                f32x16 s = {}, x = start;
+                scores(i, st, buf, s, x);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], p.c, -l2)) * (START ? x[r] : x[r] + nd);
+                x8 b[2];
+                pack<T>(s, b);
+                columns_product<T, D>(kt + st * 2 * BLK, w, b, dq);
+            }
+        }
+        if constexpr (!F16) break;
+        if (once || again) break;
+        float test = 0.0f;  // NaN where a sum is not finite
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) test = __builtin_fmaf(dq[d][r], 0.0f, test);
+        const bool over = __any(test != 0.0f);
+        __syncthreads();  // (every wave is done with the tiles)
+        RSFA_LDS float* const found = (RSFA_LDS float*)smem;
+        if (w.lane == 0) found[wave] = over ? 1.0f : 0.0f;
+        __syncthreads();
+        again = found[0] + found[1] + found[2] + found[3] != 0.0f;
+        if (!again) break;
+        constexpr int G = D / 8;  // lanes of a key
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));  // (nothing of this is formed ahead of the loop)
+        float v2 = 0.0f;
+        for (int64_t key = (int64_t)begin * KB + tid / G, last = min((int64_t)end * KB, (int64_t)nk); key < last; key += 256 / G) {
+            const x8 v[1] = {*(const x8*)(vb + key * p.v_st[2] + 8 * (tid % G))};
+            float sum = sum_of_squares(v);
+#pragma unroll
+            for (int d = 1; d < G; d <<= 1) sum += __shfl_xor(sum, d);
+            v2 = fmaxf(v2, sum);
+        }
+#pragma unroll
+        for (int d = G; d < 64; d <<= 1) v2 = fmaxf(v2, __shfl_xor(v2, d));
+        __syncthreads();
+        if (w.lane == 0) found[wave] = v2;
+        __syncthreads();
+        v2 = fmaxf(fmaxf(found[0], found[1]), fmaxf(found[2], found[3]));
+        __syncthreads();
+        l2 += k2;
+        k2 = room(go * __builtin_sqrtf(v2) + __builtin_fabsf(nd));
+        l2 -= k2;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dq[d][r] = 0.0f;
+        load(begin, 0);
     }
     if (p.splits > 1) {
         if (row >= p.t) return;
@@ -607,7 +694,7 @@ Plan make_plan(const rsfa_cross_bwd_args* a) {
     };
     p.nl = take((uint64_t)qh * p.tp * 4 + 256);
     p.nd = take((uint64_t)qh * p.tp * 4 + 256);
-    if (a->dtype == RSFA_DTYPE_F16) p.top = take((uint64_t)qh * p.tp / 32 * 4);
+    if (a->dtype == RSFA_DTYPE_F16) p.top = take((uint64_t)qh * p.tp / 32 * 8);
     if (p.dkv_splits > 1)
         for (int i = 0; i < 2; ++i) p.dkv[i] = take((uint64_t)p.dkv_splits * kh * a->n * d * 4);
     if (p.dq_splits > 1) p.dq = take((uint64_t)p.dq_splits * qh * a->t * d * 4);
@@ -656,7 +743,7 @@ int rsfa_cross_bwd(const rsfa_cross_bwd_args* a, void* stream) {
     p.scale = a->sm_scale;
     p.c = std::max(std::fabs(a->sm_scale) * LOG2E, LEAST_C);
     p.neg = a->sm_scale < 0.0f ? 0x80008000u : 0u;
-    p.nl = (float*)(ws + plan.nl), p.nd = (float*)(ws + plan.nd), p.top = (float*)(ws + plan.top);
+    p.nl = (float*)(ws + plan.nl), p.nd = (float*)(ws + plan.nd), p.top = (float2*)(ws + plan.top);
     const int64_t d = a->head_dim, kh = a->z * a->key_heads, qh = a->z * a->heads;
     const Functions fn = a->dtype == RSFA_DTYPE_BF16 ? functions<TypeBF16>(d) : functions<TypeF16>(d);
     const int64_t dkv_blocks = kh * plan.key_blocks, dq_blocks = qh * plan.row_blocks;

@@ -40,8 +40,12 @@ def expect(q, k, v, lengths, scale, go=None, glse=None):
     * dv: (h + e + (rows + 16) 2 u) sum p |do| + h |dv|;
     * ds = p (do v - delta): do v is off by (D + 4) u sum |do||v|, delta by the bound of o times |do| (it is made from
       the rounded o) and (D + 6) u sum |o||do|; ds by those times p and (h + e + 4 u) |ds|;
-    * float16 weights and ds are scaled by 2^k before they are rounded, so that half a subnormal step is 2^(-25 - k): k is
-      3 - floor(log2 of the largest |do| and |dlse|), within 0 .. 15, of the row for dq, of all rows of the key head for dk and dv;
+    * float16 weights are scaled by 2^12 before they are rounded for dv, so that half a subnormal step is 2^-37; ds by 2^k, and it is
+      2^(-25 - k).  With |do|, |v| the 2-norms of rows, B = |do| max|v| + |delta| of a row for dq, and of a key, with the largest |do|
+      and |delta| of the key head's rows, for dk, bounds |ds|.  For dk k is 12 - floor(log2 B), at most 40, so that 2^-k <= 2^-12 B, one
+      binade more if B, as 32 bits have it, falls into the next: 2^-11 B.  For dq k may be that of a bound of the first 32 keys, at
+      most 2 B, less 6: 2^-4 B, or 2^-34.  Half a subnormal step is max(2^-36 B, 2^-65) for dk, max(2^-29 B, 2^-59) for dq;
+    * k, at most 100, in the exponent adds a rounding of (|lse| + 70) u to a weight of ds;
     * dq: scale times sum ds' bound |k|, (n + 16) 2 u scale sum |ds||k| for the sums, h |dq|; dk the same with rows and |q|.
     """
     Z, Hq, T, D = q.shape
@@ -53,11 +57,6 @@ def expect(q, k, v, lengths, scale, go=None, glse=None):
     bo, bl = _like(q.shape, q.shape[:3], device=dev)
     dq, dk, dv, bq, bk, bv = _like(q.shape, k.shape, k.shape, q.shape, k.shape, k.shape, device=dev)
     rows = Hq // H * T
-
-    def least(top):
-        """Half a subnormal step of the scaled weights, for the largest |do| and |dlse|."""
-        k = (3 - torch.floor(torch.log2(top.clamp(min=2.0 ** -126)))).clamp(0, 15)
-        return tiny * 2.0 ** -k
 
     for z in range(Z):
         n = N if lengths is None else max(0, min(N, int(lengths[z])))
@@ -79,22 +78,28 @@ def expect(q, k, v, lengths, scale, go=None, glse=None):
             e = e + bl[z, i][:, None] + 4 * u * m.abs()
             d = go[z, i].double()
             heads = slice(j * Hq // H, (j + 1) * Hq // H)
-            top, tops = d.abs().amax(-1, keepdim=True), go[z, heads].double().abs().max()
+            deltas = (go[z, heads].double() * o[z, heads]).sum(-1, keepdim=True)
             if glse is not None:
-                top, tops = torch.maximum(top, glse[z, i].double().abs()[:, None]), torch.maximum(tops, glse[z, heads].double().abs().max())
+                deltas = deltas - glse[z, heads].double()[..., None]
+            delta, norms = deltas[i - heads.start], c.norm(dim=-1)[None]
+            least_q = least_k = least_v = tiny
+            if q.dtype == torch.float16:
+                least_v = 2.0 ** -37
+                least_q = (2.0 ** -29 * (d.norm(dim=-1, keepdim=True) * norms.max() + delta.abs())).clamp(min=2.0 ** -59)
+                least_k = (2.0 ** -36 * (go[z, heads].double().norm(dim=-1).max() * norms + deltas.abs().max())).clamp(min=2.0 ** -65)
+                e = e + u * (m.abs() + 70)
             many = (rows + 16) * 2 * u
             dv[z, j, :n] += p.T @ d
-            bv[z, j, :n] += ((h + e + many) * p + least(tops)).T @ d.abs()
+            bv[z, j, :n] += ((h + e + many) * p + least_v).T @ d.abs()
             x = d @ c.T
-            delta = (d * o[z, i]).sum(-1, keepdim=True) - (0.0 if glse is None else glse[z, i].double()[:, None])
             ds = p * (x - delta)
             off = (D + 4) * u * (d.abs() @ c.abs().T) + (d.abs() * bo[z, i]).sum(-1, keepdim=True)
             off = off + (D + 6) * u * (d.abs() * o[z, i].abs()).sum(-1, keepdim=True) + 4 * u * (x.abs() + delta.abs())
             bs = p * off + (h + e + 4 * u) * ds.abs()
             dq[z, i] = scale * (ds @ b)
-            bq[z, i] = abs(scale) * ((bs + least(top) + sums * ds.abs()) @ b.abs())
+            bq[z, i] = abs(scale) * ((bs + least_q + sums * ds.abs()) @ b.abs())
             dk[z, j, :n] += scale * (ds.T @ a)
-            bk[z, j, :n] += abs(scale) * ((bs + least(tops) + many * ds.abs()).T @ a.abs())
+            bk[z, j, :n] += abs(scale) * ((bs + least_k + many * ds.abs()).T @ a.abs())
     out = {"o": (o, bo), "lse": (lse, bl)}
     if go is not None:
         for name, x, b in (("dq", dq, bq), ("dk", dk, bk), ("dv", dv, bv)):

@@ -442,3 +442,58 @@ def test_saved_tensors_kept_on_the_host(kind, order, pin):
                 _hold(name, g, bounds[name])
             want = got
         assert all(torch.equal(a, b) for a, b in zip(got, want)), (order, hook)
+
+
+@pytest.mark.parametrize("signs", ["alike", "random"])
+@pytest.mark.parametrize("states", [1.0, 64.0, 300.0, 1024.0])
+@pytest.mark.parametrize("grads", [2.0 ** -10, 1.0, 64.0, 512.0])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_float16_gradients_whose_sums_pass_the_type(D, grads, states, signs):
+    # dO v, of all signs alike D grads states, lies above 2^16, the gradients themselves do not
+    for T, N, lengths in ((3, 2, None), (3, 200, [200, 150]), (70, 64, None), (90, 333, [333, 30]), (5, 1500, None)):
+        q, k, v = _inputs(2, 2, 2, T, N, D, F16, seed=T)
+        go = _randn(q.shape, 4, F16)
+        if signs == "alike":
+            v = torch.sign(v[..., :1]).expand_as(v).contiguous()
+            go = torch.ones_like(go)
+        v, go = v * states, go * grads
+        # (dq is at most the scale times |ds| times a few keys' values, dk that times the rows')
+        scale = min(D ** -0.5, 2.0 ** 12 / (grads * states * (D if signs == "alike" else 8 * D ** 0.5) * max(1.0, T / N)))
+        le = None if lengths is None else _ints(lengths)
+        glse = _randn(q.shape[:3], 5, torch.float32, grads)
+        want = O.expect(q, k, v, lengths, scale, go, glse)
+        assert all(x.abs().max() < 2.0 ** 15.9 for x, _ in want.values())
+        got = _train(q, k, v, scale, le, go, glse)
+        for name, value in want.items():
+            _hold(name, got[name], value)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("T, N", [(3, 200), (90, 700), (2, 9000)])
+def test_float16_gradients_of_keys_far_above_the_first(T, N, D):
+    # the first keys' values, which the scale of dS goes by, are small or 0, some later ones' large; of the last rows' dO too
+    for small in (0.0, 2.0 ** -12):
+        for at in (33, N - 1):
+            q, k, v = _inputs(2, 2, 1, T, N, D, F16)
+            v *= small
+            v[:, :, at], v[0, 0, at - 1] = 512.0, -512.0
+            go = torch.ones_like(q)
+            go[1, 1, T - 1] = 8.0
+            _check(q, k, v, 2.0 ** -7, _ints([N, at + 1]), go)
+            # (equal weights of opposite values: delta is 0 and tells nothing of them; every second row like that)
+            v[:, :, at - 1] = -512.0
+            q[:, :, ::2] = 0.0
+            _check(q, k, v, 2.0 ** -7, _ints([N, at + 1]), go)
+
+
+def test_float16_rows_beside_one_that_is_not_finite():
+    # gradients of v and of q that a row's infinite dO does not reach are what they were
+    q, k, v = _inputs(2, 2, 2, 90, 150, 64, F16)
+    go = _randn(q.shape, 4, F16)
+    want = _train(q, k, v, 0.125, None, go)
+    go[1, 0, 40, 7] = math.inf
+    got = _train(q, k, v, 0.125, None, go)
+    assert torch.isnan(got["dq"][1, 0, 40]).all() and torch.isinf(got["dv"][1, 0, :, 7]).all()
+    for x, name in ((got["dq"], "dq"), (got["dv"], "dv")):
+        x[1, 0, 40 if name == "dq" else slice(None), slice(None) if name == "dq" else 7] = want[name][1, 0, 40 if name == "dq" else slice(None), slice(None) if name == "dq" else 7]
+        assert torch.allclose(x.double(), want[name].double(), rtol=2.0 ** -9, atol=2.0 ** -14)
