@@ -282,7 +282,7 @@ cross_dkv_kernel(BwdParams p) {
         const uint32_t dst = smem_addr + buf * BUF;
         const elem* qb = (const elem*)p.q + z * p.q_st[0] + hq * p.q_st[1];
         const elem* gb = (const elem*)p.go + z * p.go_st[0] + hq * p.go_st[1];
-        const int last = p.t - 1;  // rows past it repeat it: their statistics make P 0
+        const int last = p.t - 1;  // rows past it repeat it: their statistics make P 0 (and dO is hidden)
         auto rows = [&](const elem* base, int64_t st, int blk, uint32_t to) {
             const int r0 = min(row0 + 16 * blk, last);
             const uint32_t off = (uint32_t)(((min(r0 + w.ld_row, last) - r0) * st + w.ld_col) * 2);
@@ -313,13 +313,16 @@ cross_dkv_kernel(BwdParams p) {
         }
     };
 
+    int left = p.t - i % tiles * QB;  // rows from the tile's first on
     if (i < end) load(i, 0);
-    for (int buf = 0; i < end; ++i, buf ^= 1) {
+    for (int buf = 0; i < end; ++i, buf ^= 1, left = left > QB ? left - QB : p.t) {
         wait_loads_and_sync();
         if (i + 1 < end) load(i + 1, buf ^ 1);
         if (!mine) continue;
         const RSFA_LDS char* const qt = smem + buf * BUF;
-        const RSFA_LDS char* const gt = qt + TILE;
+        RSFA_LDS char* const gt = smem + buf * BUF + TILE;
+        // (P of the rows that fill a tile up is 0, and 0 times an infinite dO would be NaN)
+        if (__builtin_expect(left < QB, 0)) hide_rows<D, QB>(gt, left, w.lane);
 #pragma unroll
         for (int st = 0; st < QB / 32; ++st) {
             f32x16 s, x;

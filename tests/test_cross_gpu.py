@@ -497,3 +497,18 @@ def test_float16_rows_beside_one_that_is_not_finite():
     for x, name in ((got["dq"], "dq"), (got["dv"], "dv")):
         x[1, 0, 40 if name == "dq" else slice(None), slice(None) if name == "dq" else 7] = want[name][1, 0, 40 if name == "dq" else slice(None), slice(None) if name == "dq" else 7]
         assert torch.allclose(x.double(), want[name].double(), rtol=2.0 ** -9, atol=2.0 ** -14)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("T", [1, 31, 33, 90, 700])
+def test_an_infinite_gradient_of_the_last_row(T, D, dtype):
+    # (what fills its tile up has no part in the sums: dv is infinite where the row's dO is, not NaN)
+    q, k, v = _inputs(2, 4, 2, T, 200, D, dtype)
+    n, go = _ints([200, 77]), _randn(q.shape, 4, dtype)
+    want = O.expect(q, k, v, [200, 77], 0.01, go)["dv"]
+    go[0, 1, T - 1, 3], go[1, 2, T - 1, D - 1] = math.inf, -math.inf
+    got = _train(q, k, v, 0.01, n, go)["dv"]
+    assert (got[0, 0, :, 3] == math.inf).all() and (got[1, 1, :77, D - 1] == -math.inf).all()
+    got[0, 0, :, 3], got[1, 1, :77, D - 1] = want[0][0, 0, :, 3], want[0][1, 1, :77, D - 1]
+    _hold("dv", got, want)
