@@ -45,7 +45,7 @@ HIPCC_FLAGS = [
 # softmax then copies each score out of the AGPRs.  The kernels built for two
 # waves per SIMD use no AGPRs either way and compile to the same code.
 # cross_backward.hip: the same for its one-wave-per-SIMD kernels of head dim 256,
-# which spill 396 registers and more otherwise, 53 (36 in float16) so.
+# which spill 396 registers and more otherwise, 28 (36 in float16) so.
 FILE_FLAGS = {"kern_d256.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               "cross_backward.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
