@@ -20,8 +20,6 @@ namespace {
 
 constexpr float LN2 = 0.6931471805599453f;
 constexpr float LOG2E = 1.4426950408889634f;
-// A running maximum of scores starts below every finite score, and finite: a hidden score's exp2(-inf - m) is 0.
-constexpr float NEVER = -3.0e38f;
 constexpr float SLACK = 8.0f;  // how far (log2 units) a score may pass the running maximum: weights stay below 2^8
 
 struct FewParams {

@@ -76,6 +76,8 @@ __device__ __forceinline__ int row_swz(int r) { return 2 * ((r >> 2) & 1) + ((r 
 // slack means fewer rescales of O where the scores spread widely (sm_scale
 // 0.5 at D = 128: +1.9 % over a slack of 8).
 constexpr float RESCALE_SLACK = 15.0f;
+// Start of a running maximum that has to be finite: no score is less but -inf, whose exp2(-inf - NEVER) is 0.
+constexpr float NEVER = -3.40282347e38f;
 
 struct TypeF16 {
     static constexpr bool v8 = false;  // V tiles in LDS as float8 bytes
@@ -1002,7 +1004,9 @@ fa_fwd_kernel(FwdParams p) {
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
-        float m_use = -INFINITY;  // running max (exp2 domain) of this lane's query row
+        // running max (exp2 domain) of this lane's query row (cross attention: finite, so that a tile of keys
+        // whose scores are all -inf leaves a row at sums of 0, and not at -inf - -inf)
+        float m_use = CROSS ? NEVER : -INFINITY;
         float l_sum = 0.0f;       // this lane's half of the row sum
         // Bias blocks of the diagonal ping-pong tiles: sub-tile kt of tile tt
         // lies below (<0), on (0) or above (>0) this wave's 32 rows.

@@ -512,3 +512,23 @@ def test_an_infinite_gradient_of_the_last_row(T, D, dtype):
     assert (got[0, 0, :, 3] == math.inf).all() and (got[1, 1, :77, D - 1] == -math.inf).all()
     got[0, 0, :, 3], got[1, 1, :77, D - 1] = want[0][0, 0, :, 3], want[0][1, 1, :77, D - 1]
     _hold("dv", got, want)
+
+
+@pytest.mark.parametrize("hidden", [1, 130, 600])
+@pytest.mark.parametrize("shape", [(2, 4, 2, T, 700) for T in (1, 6, 50, 300)] + [(1, 8, 8, 137, 10984), (2, 32, 8, 17, 3773), (1, 2, 1, 1, 9000)])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_keys_whose_scores_are_minus_infinity(D, shape, hidden):
+    # the first keys, tiles and whole parts of them; then every second tile of 128: as if the others were all
+    Z, Hq, H, T, N = shape
+    hidden = hidden * N // 700
+    q, k, v = _inputs(Z, Hq, H, T, N, D, BF16)
+    q[..., 0] = 1.0 + q[..., 0].abs()
+    n = [N - 5 * z for z in range(Z)]
+    for gone in (torch.arange(N) < hidden, torch.arange(N) // 128 % 2 == (0 if hidden > 1 else 1)):
+        x = k.clone()
+        x[:, :, gone.cuda(), 0] = -math.inf
+        got = cross_attention(q, x, v, D ** -0.5, _ints(n), return_lse=True)
+        at = (~gone).cuda()
+        want = O.expect(q, k[:, :, at], v[:, :, at], [int((~gone)[:m].sum()) for m in n], D ** -0.5)
+        for name, y in zip(("o", "lse"), got):
+            _hold(name, y, want[name])
