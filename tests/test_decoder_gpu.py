@@ -7,11 +7,13 @@ from ascend_rsfa.cache4 import Cache4
 from ascend_rsfa.cross import cross_attention
 from ascend_rsfa.draft import draft_tree
 from ascend_rsfa.rotary import rotary, rotary_plan
+from oracle import cross as X64
+from oracle import draft as D64
 from oracle import serving as S
 
 pytestmark = pytest.mark.gpu
 
-BF16 = torch.bfloat16
+BF16, HALF = torch.bfloat16, 2.0 ** -8
 BUFFERS = ("k_codes", "k_scales", "v_codes", "v_scales", "positions", "weights")
 
 
@@ -90,3 +92,60 @@ def test_drafted_decoding_equals_decoding_token_by_token():
     assert torch.equal(lengths, at)
     for name in BUFFERS[:5]:
         assert torch.equal(getattr(one, name)[:, :, :n], getattr(cache, name)[:, :, :n]), name
+
+
+def _bounded(q, k, v, see, scale):
+    """Attention of drafted tokens in float64, and what the kernel may be off by: the tolerance of tests/test_draft_gpu.py for bfloat16."""
+    o, _, total, reach = D64.attend(q, k, v, see, scale)
+    r, sums = (q.shape[3] + 4) * 2.0 ** -24 * reach, (int(see.sum(-1).max()) + 16) * 2.0 ** -23
+    return o, total * (HALF + (2 * r + sums)[..., None]) * (1 + HALF) + o.abs() * HALF
+
+
+def test_drafted_decoding_equals_decoding_token_by_token_where_ancestors_weigh():
+    # Drafted tokens share a direction in the dims that rotary turns least, so that each token's weight lies on its ancestors and
+    # itself; outputs are held to the bounds of their own elements, which a tree that hides or shows other tokens is far outside of.
+    Z, H, D, T, group, steps, scale = 2, 2, 64, 9, 2, 5, 64 ** -0.5
+    plan = rotary_plan(D)
+    keys, values = _randn((Z, H, 77, D), 1, BF16), _randn((Z, H, 77, D), 2, BF16)
+    prompts = [_randn((Z, H, 130, D), 3, BF16), _randn((Z, H, 130, D), 4, BF16)]
+    way = torch.zeros(D)
+    way[[28, 29, 30, 31, 60, 61, 62, 63]] = 2.5
+    drafted, one = Cache4(Z, H, 300, D, BF16), Cache4(Z, H, 300, D, BF16)
+    lengths, at = _ints([0] * Z), _ints([0] * Z)
+    for c, n in ((drafted, lengths), (one, at)):
+        _, k = rotary(prompts[0], prompts[0], 0, plan)
+        c.append(k, prompts[1], n)
+        n += 130
+    told_apart = 0
+    for step in range(steps):
+        x = (0.5 * _randn((Z, H * group, T, D), 10 + step, torch.float32) + way.cuda()).to(BF16)
+        v = _randn((Z, H, T, D), 20 + step, BF16)
+        g = torch.Generator().manual_seed(step)
+        parents = [max(-1, i - 1 - int(torch.randint(0, 2, (1,), generator=g))) for i in range(T)]
+        path, i = [], T - 1
+        while i >= 0:
+            path, i = [i] + path, parents[i]
+        tree = draft_tree(_ints(parents))
+        q, k = rotary(x, x[:, ::group].contiguous(), lengths[:, None] + tree.depths, plan)
+        drafted.append(k, v, lengths)
+        got = (drafted.attend(q, lengths + T, True, scale, tree=tree) + cross_attention(x, keys, values, scale))[:, :, path]
+        # what it is, and what it would be if tokens saw themselves and the context alone, or all drafted tokens up to themselves
+        rows = S.values(drafted.k_codes, drafted.k_scales), S.values(drafted.v_codes, drafted.v_scales)
+        tables = D64.seen(parents), torch.eye(T, dtype=torch.bool), torch.ones((T, T), dtype=torch.bool).tril()
+        o, wrong, more = (_bounded(q, *rows, D64.visible(t.expand(Z, T, T), (lengths + T).tolist(), None, 300), scale) for t in tables)
+        c, bound = X64.expect(x, keys, values, None, scale)["o"]
+        off = 2 * ((o[1] + bound) * (1 + HALF) + HALF * (o[0] + c).abs())[:, :, path]
+        for other in (wrong, more):
+            told_apart += int(((other[0] - o[0])[:, :, path].abs() > off).sum())
+        for j, t in enumerate(path):
+            y = x[:, :, t:t + 1]
+            q, k = rotary(y, y[:, ::group].contiguous(), at[:, None], plan)
+            one.append(k, v[:, :, t:t + 1], at)
+            at += 1
+            want = one.attend(q, at, True, scale) + cross_attention(y, keys, values, scale)
+            assert ((want - got[:, :, j:j + 1]).double().abs() <= off[:, :, j:j + 1]).all(), (step, t)
+            assert ((want.double() - (o[0] + c)[:, :, t:t + 1]).abs() <= off[:, :, j:j + 1] / 2).all(), (step, t)
+        drafted.keep(_ints([path] * Z), lengths)
+        lengths += len(path)
+    compared = 2 * Z * H * group * D * int((lengths - 130)[0])
+    assert told_apart > compared // 2, (told_apart, compared)
