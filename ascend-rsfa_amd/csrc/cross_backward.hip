@@ -15,9 +15,10 @@
 // gradients are often smaller or larger: P is scaled by 2^12 there, and dS by 2^k with a k for which it stays below 2^13 (so that
 // there is room for weights above 1, as the roundings of scores of some millions may give).  As P <= 1 and
 // |dO v| <= |dO| |v| (2-norms), |dS| of a key (dK) is at most |v| times the largest |dO| of the key head's rows plus
-// their largest |delta|, which the dQ kernel leaves per 32 rows.  For a row (dQ) the largest |v| is not known ahead: k goes by the
-// first 32 keys, with room for later ones 2^SPARE times as large; where that was not enough the sums are not finite, and the
-// workgroup finds the largest |v| and passes over its keys again.  2^k goes into the exponent and out at the end.
+// their largest |delta|, which the dQ kernel leaves per 32 rows.  For a row (dQ) the largest |v| is not known ahead, but P |v| is about
+// |o| at most, unless large values cancel in o: k goes by |dO| |o| + |delta|, with room for 2^SPARE times as much; where that was not
+// enough the sums are not finite, and the workgroup finds the largest |v| and passes over its keys again.  2^k goes into the
+// exponent and out at the end.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -402,7 +403,8 @@ cross_dq_kernel(BwdParams p) {
     const int first = block * 128 + wave * 32;  // the wave's first row
     RSFA_LDS char* const own = smem + wave * TILE;
     x8 qf[KST], gf[KST];
-    float l2 = 0.0f, nd = 0.0f, gl = 0.0f, go = 0.0f;
+    float l2 = 0.0f, nd = 0.0f, gl = 0.0f;
+    float go = 0.0f, most = 0.0f;  // float16: |dO|; what |dO v| is taken to be at most
     if (mine) {
         const int64_t head = (int64_t)z * p.heads + hq;
         const int left = p.t - first;
@@ -428,7 +430,7 @@ cross_dq_kernel(BwdParams p) {
         fragments<T, D>(own + TWO, w, gf);
 #pragma unroll
         for (int s = 0; s < KST; ++s) qf[s] = __builtin_bit_cast(x8, __builtin_bit_cast(u32x4, qf[s]) ^ p.neg);
-        float sum[2] = {0.0f, 0.0f};
+        float sum[2] = {0.0f, 0.0f}, o2[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
 #pragma unroll
@@ -439,12 +441,19 @@ cross_dq_kernel(BwdParams p) {
             }
             sum[b] += __shfl_xor(sum[b], 1);
             sum[b] += __shfl_xor(sum[b], 2);
+            if constexpr (F16) {
+                o2[b] = sum_of_squares(o[b]);
+                o2[b] += __shfl_xor(o2[b], 1);
+                o2[b] += __shfl_xor(o2[b], 2);
+            }
         }
         const float s0 = __shfl(sum[0], 4 * w.l16), s1 = __shfl(sum[1], 4 * w.l16);
         nd = gl - (w.l32 < 16 ? s0 : s1);
         if constexpr (F16) {
             go = sum_of_squares(gf);
             go = __builtin_sqrtf(go + __shfl_xor(go, 32));
+            const float a = __shfl(o2[0], 4 * w.l16), b = __shfl(o2[1], 4 * w.l16);
+            most = go * __builtin_sqrtf(w.l32 < 16 ? a : b);
         }
     }
     __syncthreads();  // (the tiles go where these rows were)
@@ -490,12 +499,12 @@ cross_dq_kernel(BwdParams p) {
     // With few keys o is large and its rounding, in delta, would be as large as that of dS (8 keys, bfloat16: an error of dQ
     // against 64 bits of 0.0026 relative to it, 0.0024 without, 0.0017 being its own rounding): delta is then rowsum(P (dO V^T)).
     const bool once = all == 1 && i == 0;
-    float most = 0.0f;  // float16: a bound on the row's |dO v|
     if (once) {
         load(0, 0);
         wait_loads_and_sync();
         if (mine) {
             float sum = 0.0f;
+            most = 0.0f;
 #pragma unroll
             for (int st = 0; st < KB / 32; ++st) {
                 f32x16 s = {}, x = {};
@@ -540,16 +549,6 @@ cross_dq_kernel(BwdParams p) {
     float k2 = 0.0f;  // float16: dS is scaled by 2^k2
     bool again = false;
     if constexpr (F16) {
-        if (i < end && !once) {
-            wait_loads_and_sync();
-            if (mine) {
-                f32x16 x = {};
-                rows_product<T, D>(smem + TILE, w, gf, x);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) most = fmaxf(most, __builtin_fabsf(x[r]));
-                most = fmaxf(most, __shfl_xor(most, 32));
-            }
-        }
         k2 = room(most + __builtin_fabsf(nd)) - (once ? 0.0f : SPARE);
         l2 -= k2;
     }

@@ -43,8 +43,8 @@ def expect(q, k, v, lengths, scale, go=None, glse=None):
     * float16 weights are scaled by 2^12 before they are rounded for dv, so that half a subnormal step is 2^-37; ds by 2^k, and it is
       2^(-25 - k).  With |do|, |v| the 2-norms of rows, B = |do| max|v| + |delta| of a row for dq, and of a key, with the largest |do|
       and |delta| of the key head's rows, for dk, bounds |ds|.  For dk k is 12 - floor(log2 B), at most 40, so that 2^-k <= 2^-12 B, one
-      binade more if B, as 32 bits have it, falls into the next: 2^-11 B.  For dq k may be that of a bound of the first 32 keys, at
-      most 2 B, less 6: 2^-4 B, or 2^-34.  Half a subnormal step is max(2^-36 B, 2^-65) for dk, max(2^-29 B, 2^-59) for dq;
+      binade more if B, as 32 bits have it, falls into the next: 2^-11 B.  For dq k may be that of |do| |o| + |delta|, at most
+      B (and 2^-11 of it, as o is rounded), less 6, 2^-5 B, or of the largest |do v| + |delta|, at most 2 B: 2^-4 B is more, or 2^-34.  Half a subnormal step is max(2^-36 B, 2^-65) for dk, max(2^-29 B, 2^-59) for dq;
     * k, at most 100, in the exponent adds a rounding of (|lse| + 70) u to a weight of ds;
     * dq: scale times sum ds' bound |k|, (n + 16) 2 u scale sum |ds||k| for the sums, h |dq|; dk the same with rows and |q|.
     """
