@@ -31,9 +31,9 @@ using namespace rsfa;
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-// Scores are multiplied by c = |sm_scale| * log2 e within the exponential; a smaller c than this changes no weight
-// (finite scores are below 2^40) and would make lse / c overflow.
-constexpr float LEAST_C = 7.888609052210118e-31f;  // 2^-100
+// Scores are multiplied by c = |sm_scale| * log2 e within the exponential; with a smaller c than this the part of lse / c
+// that the number of keys makes up would overflow, and no weight is another but for scores q k above 2^100.
+constexpr float LEAST_C = 7.523163845262640e-37f;  // 2^-120
 constexpr int ROWS = 64;  // rows are padded to whole tiles of 64 in the statistics
 
 struct BwdParams {

@@ -532,3 +532,15 @@ def test_keys_whose_scores_are_minus_infinity(D, shape, hidden):
         want = O.expect(q, k[:, :, at], v[:, :, at], [int((~gone)[:m].sum()) for m in n], D ** -0.5)
         for name, y in zip(("o", "lse"), got):
             _hold(name, y, want[name])
+
+
+@pytest.mark.parametrize("T", [3, 70])
+def test_small_scales_of_large_values(T):
+    # scores of the usual size, of q and k 2^52 times as large: the same bits, but for the gradients' exponents
+    q, k, v = _inputs(2, 4, 2, T, 150, 64, BF16)
+    go, glse, n = _randn(q.shape, 4, BF16), _randn(q.shape[:3], 5, torch.float32), _ints([150, 33])
+    want = _train(q, k, v, 0.125, n, go, glse)
+    got = _train(q * 2.0 ** 52, k * 2.0 ** 52, v, 2.0 ** -107, n, go, glse)
+    for name in want:
+        up = 2.0 ** 52 if name in ("dq", "dk") else 1.0
+        assert torch.equal(got[name].double() * up, want[name].double()), name
