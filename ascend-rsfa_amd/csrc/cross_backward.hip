@@ -577,8 +577,7 @@ cross_dq_kernel(BwdParams p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) test = __builtin_fmaf(dq[d][r], 0.0f, test);
         const bool over = __any(test != 0.0f);
-        __syncthreads();  // (every wave is done with the tiles)
-        RSFA_LDS float* const found = (RSFA_LDS float*)smem;
+        __shared__ float found[4];
         if (w.lane == 0) found[wave] = over ? 1.0f : 0.0f;
         __syncthreads();
         again = found[0] + found[1] + found[2] + found[3] != 0.0f;
@@ -616,7 +615,7 @@ cross_dq_kernel(BwdParams p) {
         store_part<D>(p.part[0] + (blockIdx.y * rows + ((int64_t)z * p.heads + hq) * p.t + row) * D, dq, __builtin_amdgcn_exp2f(-k2), w.hh);
         return;
     }
-    __syncthreads();  // (every wave is done with the tiles)
+    if (!F16 || once || again) __syncthreads();  // (every wave is done with the tiles)
     store_rows<T, D>((elem*)p.gq + z * p.gq_st[0] + hq * p.gq_st[1] + first * p.gq_st[2], p.gq_st[2], p.t - first, dq, p.scale * __builtin_amdgcn_exp2f(-k2), w, own);
 }
 
