@@ -206,7 +206,8 @@ __device__ __forceinline__ void store_part(float* dst, const f32x16 (&acc)[D / 3
 // tiles of rows of Q and dO pass through LDS, two buffers.
 // Bound by the matrix unit at D = 128: 8 x 32 heads of 2048 rows, 4096 keys of 8, bf16, 1684 us, 1306 TFLOP/s of its four products, as many
 // as a large library product reaches; at D = 64 the vector unit, with an exponential, two products and half a conversion a score,
-// has more to do than the matrix unit: 16 x 16 heads of 447 rows, 1531 keys, 850 TFLOP/s.
+// has more to do than the matrix unit: 16 x 16 heads of 447 rows, 1531 keys, 850 TFLOP/s (float16, whose two scales are one more
+// product a score, 108 us where one scale took 104).
 template <int D>
 struct Bwd {
     static constexpr int TILE_ROWS = D == 256 ? 32 : 64;
@@ -371,7 +372,8 @@ cross_dkv_kernel(BwdParams p) {
 // dQ of 128 rows, 32 of each wave, held transposed (dQ^T = K^T dS^T), rows in the lanes: a row's
 // statistics are one register each.  Q and dO of the wave stay in registers; tiles of K and V pass through LDS.
 // Bound as dK and dV are: the same calls 1336 us, 1235 TFLOP/s of its three products, and 880 TFLOP/s; with few keys by memory:
-// 8 x 8 heads of 4096 rows, 77 keys, D = 64 32 us, 4.2 TB/s of q, o, dO and dQ.
+// 8 x 8 heads of 4096 rows, 19 to 77 keys, D = 64, bf16 31 us, 4.4 TB/s of q, o, dO and dQ, float16, which forms |dO|, |o| and looks
+// whether its sums are finite, 36, 3.7 TB/s.
 template <class T, int D>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Bwd<D>::DQ_OCC, Bwd<D>::DQ_OCC)))
 cross_dq_kernel(BwdParams p) {
