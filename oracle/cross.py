@@ -45,7 +45,7 @@ def expect(q, k, v, lengths, scale, go=None, glse=None):
       and |delta| of the key head's rows, for dk, bounds |ds|.  For dk k is 12 - floor(log2 B), at most 40, so that 2^-k <= 2^-12 B, one
       binade more if B, as 32 bits have it, falls into the next: 2^-11 B.  For dq k may be that of |do| |o| + |delta|, at most
       B (and 2^-11 of it, as o is rounded), less 6, 2^-5 B, or of the largest |do v| + |delta|, at most 2 B: 2^-4 B is more, or 2^-34.  Half a subnormal step is max(2^-36 B, 2^-65) for dk, max(2^-29 B, 2^-59) for dq;
-    * k, at most 100, in the exponent adds a rounding of (|lse| + 70) u to a weight of ds;
+    * k in the exponent, at most 40 where all is finite, adds up to three roundings of (|lse| + 0.7 k) u each to a weight of ds;
     * dq: scale times sum ds' bound |k|, (n + 16) 2 u scale sum |ds||k| for the sums, h |dq|; dk the same with rows and |q|.
     """
     Z, Hq, T, D = q.shape
@@ -87,7 +87,7 @@ def expect(q, k, v, lengths, scale, go=None, glse=None):
                 least_v = 2.0 ** -37
                 least_q = (2.0 ** -29 * (d.norm(dim=-1, keepdim=True) * norms.max() + delta.abs())).clamp(min=2.0 ** -59)
                 least_k = (2.0 ** -36 * (go[z, heads].double().norm(dim=-1).max() * norms + deltas.abs().max())).clamp(min=2.0 ** -65)
-                e = e + u * (m.abs() + 70)
+                e = e + u * 3 * (m.abs() + 28)
             many = (rows + 16) * 2 * u
             dv[z, j, :n] += p.T @ d
             bv[z, j, :n] += ((h + e + many) * p + least_v).T @ d.abs()
